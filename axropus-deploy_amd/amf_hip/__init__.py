@@ -33,11 +33,13 @@ ERR_RUNTIME = -7
 ERRFLAG_BLOCK_RANGE = 1
 ERRFLAG_CONTEXT = 2
 ERRFLAG_SYNC = 4
+ERRFLAG_FREE_LIST = 8
 
 # element types (same numbering as the AMFK header dtype tag)
 DTYPE_F16 = 0
 DTYPE_F32 = 1
 DTYPE_BF16 = 2
+DTYPE_E4M3 = 3  # K/V caches of the paged attention
 
 # codec formats
 FMT_FP8_E4M3 = 1
@@ -134,6 +136,30 @@ SIGNATURES = {
         _c_i32,
         [_c_ptr, _c_i32, _c_ptr, _c_i32, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_ptr, _c_i32,
          _c_ptr, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_f32, _c_i32, _c_ptr, _c_ptr],
+    ),
+    "amf_paged_decode_workspace_bytes": (_c_i64, [_c_i32, _c_i32, _c_i32]),
+    "amf_paged_decode_attn": (
+        _c_i32,
+        [_c_ptr, _c_i32, _c_i64, _c_i64, _c_ptr, _c_i32, _c_ptr, _c_ptr, _c_i32, _c_i64, _c_i64,
+         _c_i64, _c_i64, _c_ptr, _c_i64, _c_i32, _c_ptr, _c_ptr, _c_ptr, _c_i32, _c_i32, _c_i32,
+         _c_i32, _c_i32, _c_i32, _c_i32, _c_f32, _c_f32, _c_f32, _c_ptr, _c_i64, _c_ptr, _c_ptr],
+    ),
+    "amf_page_key_bounds": (
+        _c_i32,
+        [_c_ptr, _c_i32, _c_i64, _c_i64, _c_i64, _c_i64, _c_ptr, _c_i64, _c_i32, _c_ptr, _c_ptr,
+         _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_ptr, _c_i32, _c_ptr, _c_ptr],
+    ),
+    "amf_select_pages_workspace_bytes": (_c_i64, [_c_i32, _c_i32, _c_i32, _c_i32, _c_i32]),
+    "amf_select_pages": (
+        _c_i32,
+        [_c_ptr, _c_i32, _c_i64, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_i64, _c_i32, _c_ptr, _c_i32,
+         _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_ptr, _c_ptr, _c_ptr,
+         _c_i64, _c_ptr, _c_ptr],
+    ),
+    "amf_build_slot_maps": (
+        _c_i32,
+        [_c_ptr, _c_ptr, _c_i32, _c_ptr, _c_i64, _c_i32, _c_i32, _c_i64, _c_ptr, _c_i64, _c_ptr,
+         _c_i64, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr],
     ),
     "amf_fnv1a64": (ctypes.c_uint64, [_c_ptr, _c_i64, ctypes.c_uint64]),
     "amf_hash_tokens": (ctypes.c_uint64, [_c_ptr, _c_i64]),
@@ -245,6 +271,19 @@ def call(func: str, *args) -> None:
     rc = fn(*args)
     if rc != OK:
         check(func, rc)
+
+
+def call_on(device, func: str, *args) -> None:
+    """call() with `device`, which holds the tensors, as the current device
+    (the null stream and the launch belong to the current one)."""
+    import torch
+
+    idx = _device_index(device)
+    if torch.cuda.current_device() == idx:
+        call(func, *args)
+    else:
+        with torch.cuda.device(idx):
+            call(func, *args)
 
 
 # ---------------------------------------------------------------- helpers --

@@ -8,8 +8,9 @@ then to any kernel of the storage format, then to fallback_fp16_kernel.
 Every kernel registered here runs on the GPU through libamf_hip.so:
 
 * hip_decode_attention(q, k, v, scale=None, mask=None, *, block_tables=...,
-  context_lens=...) is the paged GQA INT4 decode (amf_int4_paged_decode_attn)
-  when a block table is given, and dense attention otherwise: straight from
+  context_lens=...) is a paged GQA decode when a block table is given, over an
+  INT4 pool (amf_int4_paged_decode_attn) or, where k is a tensor, over vLLM's
+  own cache (paged_decode_attention), and dense attention otherwise: straight from
   the codes for int4_sym CompressedKV K/V (amf_int4_sym_dense_attn), else
   over the restored K/V (amf_dense_attn).
 * fallback_fp16_kernel keeps the reference's name and signature
@@ -45,6 +46,7 @@ from ..codecs import (
     CompressedKV,
     get_codec,
 )
+from .paged import paged_decode_attention
 
 logger = logging.getLogger(__name__)
 
@@ -396,20 +398,37 @@ def hip_decode_attention(q: torch.Tensor, k: Any, v: Any = None, scale: Optional
                          max_context_len: Optional[int] = None,
                          out: Optional[torch.Tensor] = None,
                          out_dtype: Optional[torch.dtype] = None, algo: str = "auto",
-                         workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+                         workspace: Optional[torch.Tensor] = None,
+                         pages: Optional[torch.Tensor] = None,
+                         page_counts: Optional[torch.Tensor] = None, k_scale: float = 1.0,
+                         v_scale: float = 1.0) -> torch.Tensor:
     """The gfx950 decode kernel: positional arguments as the reference's
     (q, k, v, scale=None, mask=None); with block_tables/context_lens keywords,
-    k is the INT4 page pool (v unused) and the paged GQA kernel runs."""
+    a paged GQA kernel runs over k, an INT4 page pool (v unused) or a tensor:
+    a layer's cache, or its K plane with v the V plane (paged_decode_attention,
+    which takes pages, page_counts, k_scale and v_scale)."""
     if block_tables is not None or context_lens is not None:
         if block_tables is None or context_lens is None:
             raise ValueError("paged decode needs both block_tables and context_lens")
         if mask is not None:
             raise ValueError("paged decode takes no mask (causality is the context length)")
+        if isinstance(k, torch.Tensor):
+            if algo != "auto":
+                raise ValueError(f"algo {algo!r} is for INT4 pools")
+            return paged_decode_attention(
+                q, k, v, block_tables=block_tables, context_lens=context_lens, scale=scale,
+                max_context_len=max_context_len, pages=pages, page_counts=page_counts,
+                k_scale=k_scale, v_scale=v_scale, out=out, out_dtype=out_dtype,
+                workspace=workspace)
+        if pages is not None or page_counts is not None or k_scale != 1.0 or v_scale != 1.0:
+            raise ValueError("pages and scales are for a cache given as a tensor")
         if v is not None and v is not k:
             raise ValueError("paged decode reads K and V from the one page pool passed as k")
         return paged_int4_decode(q, k, block_tables, context_lens, scale=scale,
                                  max_context_len=max_context_len, out=out, out_dtype=out_dtype,
                                  algo=algo, workspace=workspace)
+    if pages is not None or page_counts is not None or k_scale != 1.0 or v_scale != 1.0:
+        raise ValueError("pages and scales need block_tables and context_lens")
     res = int4_sym_attention(q, k, v, scale, mask, out_dtype)
     if res is None:
         res = dense_attention(q, _to_tensor(k, q), _to_tensor(v, q), scale, mask, out_dtype)

@@ -67,6 +67,7 @@ extern "C" {
 /* bits ORed into *err_flag by kernels */
 #define AMF_ERRFLAG_BLOCK_RANGE 1    /* a block id was outside [0, pool_pages) */
 #define AMF_ERRFLAG_CONTEXT     2    /* a context length exceeded its block table */
+#define AMF_ERRFLAG_FREE_LIST   8    /* the free list does not hold a sequence's new pages */
 #define AMF_ERRFLAG_SYNC        4    /* a launch missed words its predecessor writes (that call's output is invalid) */
 
 /* ---- element types: same numbering as the AMFK header dtype field
@@ -74,6 +75,7 @@ extern "C" {
 #define AMF_DTYPE_F16   0
 #define AMF_DTYPE_F32   1
 #define AMF_DTYPE_BF16  2
+#define AMF_DTYPE_E4M3  3  /* FP8 e4m3fn: K/V caches of the paged attention only */
 
 /* ---- codec formats ------------------------------------------------------
  * Layouts are per plane; n_pages pages of one plane are contiguous.
@@ -362,6 +364,119 @@ int amf_int4_paged_decode_attn_noalloc(const void* q, int32_t q_dtype, void* out
                                        int32_t head_dim, int32_t block_size,
                                        int32_t max_context_len, float softmax_scale,
                                        int32_t algo, int32_t* err_flag, void* stream);
+
+/* ---- one decode step over a paged K/V cache ----------------------------------
+ * The cache is read as it is: element (page p, token t, KV head h, dim d) of K
+ * and of V at base + p * page_stride + t * token_stride + h * head_stride + d
+ * (strides in elements, the same for K and V), which covers vLLM's
+ * [pages][tokens][heads][dim] and [pages][heads][tokens][dim] orders.
+ * block_tables: int32 [num_seqs] rows of table_pages page ids, bt_stride
+ * entries apart; context_lens: int32 [num_seqs], below 1 = no tokens.  Tokens
+ * behind a context length are never used, whatever their pages hold.  Page ids
+ * outside [0, pool_pages) are skipped (AMF_ERRFLAG_BLOCK_RANGE); a context
+ * longer than its table row is cut to it (AMF_ERRFLAG_CONTEXT).
+ * No counterpart in the reference. */
+
+/* Attention of one new token per sequence:
+ *   out[s][h] = v_scale * softmax(q[s][h] . K^T * softmax_scale * k_scale) V
+ * over the first context_lens[s] tokens, in fp32, rounded once to out_dtype.
+ * q [num_seqs][num_q_heads][head_dim] with the given strides (elements, last
+ * dim contiguous); out contiguous.  Query head h reads KV head
+ * h / (num_q_heads / num_kv_heads).  kv_dtype AMF_DTYPE_BF16, _F16, _F32 (q of
+ * the same type) or _E4M3 (q bf16 or fp16); head_dim at most 256.
+ * pages: NULL, or int32 [num_seqs][num_kv_heads][max_pages], the places in the
+ * sequence's block table that the KV head attends to, of which the first
+ * page_counts[s][h] count; negative entries are skipped, a place listed twice
+ * counts twice.  A sequence without tokens gives zeros; scores that are all
+ * -inf, or hold a NaN or +inf, give NaN, as softmax does.
+ * softmax_scale <= 0 selects 1/sqrt(head_dim).  max_context_len: at least every
+ * context length (only a hint of how to cut the work).
+ * workspace: amf_paged_decode_workspace_bytes() bytes, 16-byte aligned; calls
+ * sharing one must be ordered on one stream. */
+int64_t amf_paged_decode_workspace_bytes(int32_t num_q_heads, int32_t num_kv_heads,
+                                         int32_t head_dim);
+
+int amf_paged_decode_attn(const void* q, int32_t q_dtype, int64_t q_seq_stride,
+                          int64_t q_head_stride, void* out, int32_t out_dtype,
+                          const void* k, const void* v, int32_t kv_dtype,
+                          int64_t page_stride, int64_t token_stride, int64_t head_stride,
+                          int64_t pool_pages, const int32_t* block_tables, int64_t bt_stride,
+                          int32_t table_pages, const int32_t* context_lens,
+                          const int32_t* pages, const int32_t* page_counts, int32_t max_pages,
+                          int32_t num_seqs, int32_t num_q_heads, int32_t num_kv_heads,
+                          int32_t head_dim, int32_t block_size, int32_t max_context_len,
+                          float softmax_scale, float k_scale, float v_scale,
+                          void* workspace, int64_t workspace_bytes,
+                          int32_t* err_flag, void* stream);
+
+/* bounds [pool_pages][num_kv_heads][2][head_dim] (16-byte aligned): the
+ * smallest, then the largest key of a page per channel, over the page's tokens
+ * inside the context, for the pages of each sequence from the one of token
+ * first_tokens[s] on (NULL: all).  max_new_tokens > 0 promises
+ * context_lens[s] - first_tokens[s] <= max_new_tokens and sizes the grid.  Of
+ * a page that sequences share, one sequence's bounds stay.  bounds_dtype is
+ * kv_dtype, or for _E4M3 keys (taken without k_scale) bf16 or fp16; fp32
+ * caches are AMF_ERR_UNSUPPORTED.  head_dim a multiple of 8 up to 256; keys and
+ * strides aligned to 8 elements.  NaN keys make NaN bounds. */
+int amf_page_key_bounds(const void* k, int32_t kv_dtype, int64_t page_stride,
+                        int64_t token_stride, int64_t head_stride, int64_t pool_pages,
+                        const int32_t* block_tables, int64_t bt_stride, int32_t table_pages,
+                        const int32_t* context_lens, const int32_t* first_tokens,
+                        int32_t max_new_tokens, int32_t num_seqs, int32_t num_kv_heads,
+                        int32_t head_dim, int32_t block_size, void* bounds,
+                        int32_t bounds_dtype, int32_t* err_flag, void* stream);
+
+/* The num_pages pages of each (sequence, KV head) with the largest
+ *   max over the KV head's query heads of sum_d max(q_d lo_d, q_d hi_d)
+ * over the bounds above, which no key of the page can exceed; summed in 64
+ * bits, the lower place first among equals, the sequence's first first_pages
+ * and last last_pages always among them.  pages int32
+ * [num_seqs][num_kv_heads][num_pages]: places in the block table in ascending
+ * order, -1 behind the page_counts[s][h] = min(num_pages, pages of s) of them.
+ * A page whose score is not finite ranks above all that are.  q, its strides
+ * and bounds 16-byte aligned, of one dtype (bf16 or fp16).
+ * max_context_len: at least every context length (longer ones are cut, flagged
+ * AMF_ERRFLAG_CONTEXT).  workspace: amf_select_pages_workspace_bytes() bytes, 8-byte
+ * aligned; calls sharing one must be ordered on one stream. */
+int64_t amf_select_pages_workspace_bytes(int32_t num_seqs, int32_t num_kv_heads,
+                                         int32_t table_pages, int32_t block_size,
+                                         int32_t max_context_len);
+
+int amf_select_pages(const void* q, int32_t dtype, int64_t q_seq_stride, int64_t q_head_stride,
+                     const void* bounds, int64_t pool_pages, const int32_t* block_tables,
+                     int64_t bt_stride, int32_t table_pages, const int32_t* context_lens,
+                     int32_t max_context_len, int32_t num_seqs, int32_t num_q_heads,
+                     int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
+                     int32_t num_pages, int32_t first_pages, int32_t last_pages,
+                     int32_t* pages, int32_t* page_counts, void* workspace,
+                     int64_t workspace_bytes, int32_t* err_flag, void* stream);
+
+/* The maps of a step in which sequence s, holding context_lens[s] tokens, gets
+ * new_tokens[s] more (values below 0 count as 0): its new pages are taken from
+ * free_pages[*free_used ..n_free) in sequence order and written behind its last
+ * page in block_tables; token j of sequence s is row query_start[s] + j of
+ *   slot_mapping (int64) = page id * block_size + place in the page, and
+ *   positions    (int64) = context_lens[s] + j.
+ * query_start int32 [num_seqs + 1] is the exclusive sum of new_tokens;
+ * context_out = context_lens + new_tokens; free_used_out (may be NULL) =
+ * *free_used + pages taken (free_used NULL = 0).  Outputs must not overlap
+ * inputs.  num_tokens: rows of slot_mapping and positions; rows behind the last
+ * token get slot -1 and position 0.
+ * A sequence whose pages its table row cannot hold (AMF_ERRFLAG_CONTEXT), or
+ * that the free list no longer holds (AMF_ERRFLAG_FREE_LIST; so do later ones
+ * that need pages), gets none: its context_out is context_lens, its slots are
+ * -1.  A page id outside [0, pool_pages) gives slots of -1
+ * (AMF_ERRFLAG_BLOCK_RANGE); more tokens than num_tokens are left out
+ * (AMF_ERRFLAG_CONTEXT).
+ * Replaces the slots of AMFReqMeta.make (amf_kv_connector.py:90-115), built on
+ * the host per request. */
+int amf_build_slot_maps(const int32_t* context_lens, const int32_t* new_tokens,
+                        int32_t num_seqs, int32_t* block_tables, int64_t bt_stride,
+                        int32_t table_pages, int32_t block_size, int64_t pool_pages,
+                        const int32_t* free_pages, int64_t n_free, const int32_t* free_used,
+                        int64_t num_tokens, int64_t* slot_mapping, int64_t* positions,
+                        int32_t* query_start, int32_t* context_out, int32_t* free_used_out,
+                        int32_t* err_flag, void* stream);
 
 /* ---- prefix keys (host functions, no device work) ---------------------------
  * FNV-1a over bytes, continuing from hash h (pass AMF_FNV_OFFSET to start).
