@@ -144,6 +144,38 @@ struct RawRow<DT, true> {
   }
 };
 
+// bf16 terms of a softmax weight.
+constexpr int kTerms = 3;
+
+// The terms of the weights p0 and p1 (low and high half of each word).  A
+// positive weight has only positive terms, a zero one only zeros: inf in V
+// then gives inf under a positive weight (mixed signs or a zero term would
+// make it NaN) and NaN under a zero one, as the product with the weight itself
+// does.  Each term is the top half of the bit pattern below the remainder's,
+// so the next remainder is positive and exact and the third fits 8 bits.
+__device__ __forceinline__ void weight_split(float p0, float p1, uint32_t (&w)[kTerms]) {
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const uint32_t a = __builtin_elementwise_sub_sat(f2u(p0), 1u) & 0xFFFF0000u;
+    const uint32_t b = __builtin_elementwise_sub_sat(f2u(p1), 1u) & 0xFFFF0000u;
+    w[k] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+    p0 -= u2f(a);
+    p1 -= u2f(b);
+  }
+  w[2] = __builtin_amdgcn_perm(f2u(p1), f2u(p0), 0x07060302u);
+}
+
+// A pair of fp16 V values as two bf16 pairs, hi + lo: the top 8 bits of each
+// value's 11 and the rest, below 2^8.  The clamp only meets the NaN of an
+// infinite value's remainder and makes it -256: hi alone is then infinite.
+__device__ __forceinline__ void v_split(uint32_t w, uint32_t& hi, uint32_t& lo) {
+  const uint32_t a = f2u(half_lo<false>(w)), b = f2u(half_hi<false>(w));
+  hi = __builtin_amdgcn_perm(b, a, 0x07060302u);
+  const float ra = __builtin_amdgcn_fmed3f(u2f(a) - u2f(a & 0xFFFF0000u), -256.0f, 256.0f);
+  const float rb = __builtin_amdgcn_fmed3f(u2f(b) - u2f(b & 0xFFFF0000u), -256.0f, 256.0f);
+  lo = __builtin_amdgcn_perm(f2u(rb), f2u(ra), 0x07060302u);
+}
+
 // Four consecutive outputs at element i (a multiple of 4), rounded to an
 // AMF_DTYPE_* output.
 __device__ __forceinline__ void store4(void* out, int out_dtype, int64_t i, f32x4 x) {

@@ -137,27 +137,98 @@ __device__ __forceinline__ Unit find_unit(const PagedArgs& a, int64_t groups, co
   }
 }
 
-// ---- tokens --------------------------------------------------------------------
+// ---- segments ------------------------------------------------------------------
 
-// Byte offset of token i of the list of (s, hkv) from the cache's start, -1 for
-// one that is not there.
-__device__ __forceinline__ int64_t token_offset(const PagedArgs& a, int s, int hkv, int64_t i,
-                                                int64_t ctx) {
-  int64_t j = a.block_shift >= 0 ? i >> a.block_shift : i / a.block_size;
-  const int at = (int)(i - j * a.block_size);
-  if (a.pages) {
-    const int64_t row = (int64_t)s * a.num_kv_heads + hkv;
-    if (j >= min(a.page_counts[row], a.max_pages)) return -1;
-    j = a.pages[row * a.max_pages + j];
-    if (j < 0) return -1;
+// The steps of one pair that lie in a workgroup's share.
+struct Segment {
+  int seq, hkv, heads;
+  int64_t head0;     // first query head, of the step's rows
+  int64_t st0, st1;  // steps
+  int64_t ctx;
+  bool whole;        // all steps of the pair
+  float* part;       // where the partial goes otherwise
+};
+
+// Walks a share, u in [u0, u1), pair by pair.
+template <int TILE>
+__device__ __forceinline__ Segment segment_at(const PagedArgs& a, const Unit& un, int64_t u,
+                                              int64_t u0, int64_t u1) {
+  Segment g;
+  const int64_t pair = (u - un.start) / un.steps;
+  g.st0 = (u - un.start) - pair * un.steps;
+  g.st1 = min(un.steps, g.st0 + (u1 - u));
+  g.seq = un.seq;
+  g.hkv = (int)(pair / a.tiles);
+  const int tile = (int)(pair - (int64_t)g.hkv * a.tiles);
+  g.heads = min(TILE, a.group - tile * TILE);
+  g.head0 = (int64_t)un.seq * a.num_q_heads + g.hkv * a.group + tile * TILE;
+  g.ctx = a.context_lens[un.seq];
+  g.whole = g.st0 == 0 && g.st1 == un.steps;
+  g.part = a.part + (2 * (int64_t)blockIdx.x + (u != u0)) * a.part_stride;
+  return g;
+}
+
+// Moves on to unit u, perhaps of the next sequence with tokens; u lies in the
+// launch.
+__device__ __forceinline__ void advance(const PagedArgs& a, Unit& un, int64_t u) {
+  if (u < un.start + (int64_t)a.num_kv_heads * a.tiles * un.steps) return;
+  un.start = u;
+  do {
+    ++un.seq;
+    un.steps = seq_steps(a, un.seq);
+  } while (un.steps == 0);
+}
+
+// The pages of a run of steps, looked up by the workgroup and kept in LDS: the
+// loads of K and V then depend on no load but their own.
+constexpr int kPageSlots = 1024;
+struct PageRun {
+  int32_t id[kPageSlots];
+  int32_t tokens[kPageSlots];  // of the page that count; 0 where there is none
+};
+
+// Steps that a run holds: kPageSlots pages, one of them begun before the run.
+__device__ __forceinline__ int64_t run_steps(const PagedArgs& a) {
+  return max((int64_t)1, (int64_t)(kPageSlots - 1) * a.block_size / kStep);
+}
+
+__device__ __forceinline__ int64_t page_of(const PagedArgs& a, int64_t t) {
+  return a.block_shift >= 0 ? t >> a.block_shift : t / a.block_size;
+}
+
+__device__ __forceinline__ void load_pages(const PagedArgs& a, const Segment& g, int64_t st0,
+                                           int64_t st1, PageRun& run) {
+  __syncthreads();  // the last run has been read
+  const int64_t j0 = page_of(a, st0 * kStep), j1 = page_of(a, st1 * kStep - 1);
+  const int64_t row = (int64_t)g.seq * a.num_kv_heads + g.hkv;
+  const int64_t count = a.pages ? min(a.page_counts[row], a.max_pages) : a.table_pages;
+  for (int64_t j = j0 + threadIdx.x; j <= j1; j += kThreads) {
+    int64_t p = -1, left = 0;
+    int32_t id = 0;
+    if (j < count) p = a.pages ? a.pages[row * a.max_pages + j] : j;
+    if (p >= 0) left = min(g.ctx - p * a.block_size, (int64_t)a.block_size);
+    if (left > 0) {
+      id = p < a.table_pages ? a.block_tables[g.seq * a.bt_stride + p] : -1;
+      if (id < 0 || id >= a.pool_pages) {
+        if (a.err_flag) atomicOr(a.err_flag, AMF_ERRFLAG_BLOCK_RANGE);
+        id = 0;
+        left = 0;
+      }
+    }
+    run.id[j - j0] = id;
+    run.tokens[j - j0] = (int32_t)max(left, (int64_t)0);
   }
-  if (j * a.block_size + at >= ctx) return -1;
-  const int64_t id = j < a.table_pages ? a.block_tables[s * a.bt_stride + j] : -1;
-  if (id < 0 || id >= a.pool_pages) {
-    if (a.err_flag) atomicOr(a.err_flag, AMF_ERRFLAG_BLOCK_RANGE);
-    return -1;
-  }
-  return id * a.page_stride + at * a.token_stride + hkv * a.head_stride;
+  __syncthreads();
+}
+
+// Byte offset of token t's row from the cache's start, -1 for a token that does
+// not count; the run begins with page j0.
+__device__ __forceinline__ int64_t token_offset(const PagedArgs& a, const Segment& g,
+                                                const PageRun& run, int64_t j0, int64_t t) {
+  const int64_t j = page_of(a, t);
+  const int at = (int)(t - j * a.block_size);
+  if (at >= run.tokens[j - j0]) return -1;
+  return run.id[j - j0] * a.page_stride + at * a.token_stride + g.hkv * a.head_stride;
 }
 
 // ---- joining -------------------------------------------------------------------
@@ -207,6 +278,7 @@ __global__ __launch_bounds__(kThreads) void paged_attn_general_kernel(PagedArgs 
   constexpr int ES = KDT == AMF_DTYPE_F32 ? 4 : KDT == AMF_DTYPE_E4M3 ? 1 : 2;
   constexpr int QS = QDT == AMF_DTYPE_F32 ? 4 : 2;
   constexpr int DI = kMaxDim / 64;
+  __shared__ PageRun run;
   __shared__ float q_lds[kGenHeads][kMaxDim];
   __shared__ float p_lds[kWaves][kGenHeads][kChunk];
   __shared__ float acc_lds[kWaves][kGenHeads][kMaxDim];
@@ -217,23 +289,18 @@ __global__ __launch_bounds__(kThreads) void paged_attn_general_kernel(PagedArgs 
   empty_seqs(a);
   Unit un = find_unit(a, gridDim.x, [](int64_t share) { return (int64_t)blockIdx.x * share; });
   if (un.seq < 0) return;
-  const int64_t pairs = (int64_t)a.num_kv_heads * a.tiles;
   const int64_t u0 = blockIdx.x * un.share, u1 = min(u0 + un.share, un.total);
   for (int64_t u = u0; u < u1;) {
-    const int64_t pair = (u - un.start) / un.steps;
-    const int64_t st0 = (u - un.start) % un.steps, st1 = min(un.steps, st0 + (u1 - u));
-    const int s = un.seq, hkv = (int)(pair / a.tiles), tile = (int)(pair % a.tiles);
-    const int heads = min(kGenHeads, a.group - tile * kGenHeads);
-    const int head0 = hkv * a.group + tile * kGenHeads;
-    const int64_t ctx = a.context_lens[s], len = seq_tokens(a, s);
-    __syncthreads();
+    advance(a, un, u);
+    const Segment sg = segment_at<kGenHeads>(a, un, u, u0, u1);
+    u += sg.st1 - sg.st0;
     for (int i = tid; i < kGenHeads * D; i += kThreads) {
       const int g = i / D, d = i - g * D;
-      q_lds[g][d] = g < heads ? kv_elem<QDT>(static_cast<const uint8_t*>(a.q) +
-                                             (s * a.q_seq + (head0 + g) * a.q_head + d) * QS)
-                              : 0.0f;
+      const int64_t head = sg.head0 - (int64_t)sg.seq * a.num_q_heads + g;
+      q_lds[g][d] = g < sg.heads ? kv_elem<QDT>(static_cast<const uint8_t*>(a.q) +
+                                                (sg.seq * a.q_seq + head * a.q_head + d) * QS)
+                                 : 0.0f;
     }
-    __syncthreads();
     float m[kGenHeads], l[kGenHeads], acc[kGenHeads][DI];
 #pragma unroll
     for (int g = 0; g < kGenHeads; ++g) {
@@ -242,53 +309,59 @@ __global__ __launch_bounds__(kThreads) void paged_attn_general_kernel(PagedArgs 
 #pragma unroll
       for (int i = 0; i < DI; ++i) acc[g][i] = 0.0f;
     }
-    for (int64_t st = st0; st < st1; ++st) {
-      const int64_t t = st * kStep + wave * kChunk + (lane & 31);
-      const int64_t off = t < len ? token_offset(a, s, hkv, t, ctx) : -1;
-      const bool ok = off >= 0;
-      if (!__any(ok)) continue;
-      float x[kGenHeads];
+    const int64_t hold = run_steps(a);
+    for (int64_t r0 = sg.st0; r0 < sg.st1; r0 += hold) {
+      const int64_t r1 = min(r0 + hold, sg.st1), j0 = page_of(a, r0 * kStep);
+      load_pages(a, sg, r0, r1, run);
+      for (int64_t st = r0; st < r1; ++st) {
+        const int64_t off =
+            token_offset(a, sg, run, j0, st * kStep + wave * kChunk + (lane & 31));
+        const bool ok = off >= 0;
+        if (!__any(ok)) continue;
+        float x[kGenHeads];
 #pragma unroll
-      for (int g = 0; g < kGenHeads; ++g) x[g] = 0.0f;
-      if (ok) {
-        for (int d = d0; d < d1; ++d) {
-          const float kd = kv_elem<KDT>(a.k + off + d * ES);
+        for (int g = 0; g < kGenHeads; ++g) x[g] = 0.0f;
+        if (ok) {
+          for (int d = d0; d < d1; ++d) {
+            const float kd = kv_elem<KDT>(a.k + off + d * ES);
 #pragma unroll
-          for (int g = 0; g < kGenHeads; ++g) x[g] = __builtin_fmaf(q_lds[g][d], kd, x[g]);
+            for (int g = 0; g < kGenHeads; ++g) x[g] = __builtin_fmaf(q_lds[g][d], kd, x[g]);
+          }
         }
-      }
 #pragma unroll
-      for (int g = 0; g < kGenHeads; ++g) {
-        x[g] += __shfl_xor(x[g], 32);
-        float top = ok ? x[g] * a.score_scale : -INFINITY;
-        for (int o = 16; o > 0; o >>= 1) top = max_nan(top, __shfl_xor(top, o));
-        const float mn = max_nan(m[g], top);
-        const float p = ok ? __builtin_amdgcn_exp2f(__builtin_fmaf(x[g], a.score_scale, -mn)) : 0.0f;
-        const float w = weight_to(m[g], mn);
-        m[g] = mn;
-        l[g] = l[g] * w + (half ? 0.0f : p);
+        for (int g = 0; g < kGenHeads; ++g) {
+          x[g] += __shfl_xor(x[g], 32);
+          float top = ok ? x[g] * a.score_scale : -INFINITY;
+          for (int o = 16; o > 0; o >>= 1) top = max_nan(top, __shfl_xor(top, o));
+          const float mn = max_nan(m[g], top);
+          const float p =
+              ok ? __builtin_amdgcn_exp2f(__builtin_fmaf(x[g], a.score_scale, -mn)) : 0.0f;
+          const float w = weight_to(m[g], mn);
+          m[g] = mn;
+          l[g] = l[g] * w + (half ? 0.0f : p);
 #pragma unroll
-        for (int i = 0; i < DI; ++i) acc[g][i] *= w;
-        if (!half) p_lds[wave][g][lane] = p;
-      }
-      __builtin_amdgcn_wave_barrier();
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      for (int j = 0; j < kChunk; ++j) {
-        const int64_t row = __shfl(off, j);
-        if (row < 0) continue;
-        float w[kGenHeads];
-#pragma unroll
-        for (int g = 0; g < kGenHeads; ++g) w[g] = p_lds[wave][g][j];
-#pragma unroll
-        for (int i = 0; i < DI; ++i) {
-          const int d = lane + 64 * i;
-          if (d >= D) continue;
-          const float vd = kv_elem<KDT>(a.v + row + d * ES);
-#pragma unroll
-          for (int g = 0; g < kGenHeads; ++g) acc[g][i] = __builtin_fmaf(w[g], vd, acc[g][i]);
+          for (int i = 0; i < DI; ++i) acc[g][i] *= w;
+          if (!half) p_lds[wave][g][lane] = p;
         }
+        __builtin_amdgcn_wave_barrier();
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        for (int j = 0; j < kChunk; ++j) {
+          const int64_t row = __shfl(off, j);
+          if (row < 0) continue;
+          float w[kGenHeads];
+#pragma unroll
+          for (int g = 0; g < kGenHeads; ++g) w[g] = p_lds[wave][g][j];
+#pragma unroll
+          for (int i = 0; i < DI; ++i) {
+            const int d = lane + 64 * i;
+            if (d >= D) continue;
+            const float vd = kv_elem<KDT>(a.v + row + d * ES);
+#pragma unroll
+            for (int g = 0; g < kGenHeads; ++g) acc[g][i] = __builtin_fmaf(w[g], vd, acc[g][i]);
+          }
+        }
+        __builtin_amdgcn_wave_barrier();
       }
-      __builtin_amdgcn_wave_barrier();
     }
 #pragma unroll
     for (int g = 0; g < kGenHeads; ++g) {
@@ -302,9 +375,7 @@ __global__ __launch_bounds__(kThreads) void paged_attn_general_kernel(PagedArgs 
       for (int i = 0; i < DI; ++i) acc_lds[wave][g][lane + 64 * i] = acc[g][i];
     }
     __syncthreads();
-    const bool whole = st0 == 0 && st1 == un.steps;
-    float* part = whole ? nullptr : a.part + (2 * (int64_t)blockIdx.x + (u != u0)) * a.part_stride;
-    for (int i = tid; i < heads * D; i += kThreads) {
+    for (int i = tid; i < sg.heads * D; i += kThreads) {
       const int g = i / D, d = i - g * D;
       float top = m_lds[0][g], sum = 0.0f, x = 0.0f;
       for (int w = 1; w < kWaves; ++w) top = max_nan(top, m_lds[w][g]);
@@ -313,25 +384,306 @@ __global__ __launch_bounds__(kThreads) void paged_attn_general_kernel(PagedArgs 
         sum = __builtin_fmaf(l_lds[w][g], f, sum);
         x = __builtin_fmaf(acc_lds[w][g][d], f, x);
       }
-      if (whole) {
-        store_out(a, ((int64_t)s * a.num_q_heads + head0 + g) * D + d,
-                  sum == 0.0f ? 0.0f : x * (a.v_scale / sum));
+      if (sg.whole) {
+        store_out(a, (sg.head0 + g) * D + d, sum == 0.0f ? 0.0f : x * (a.v_scale / sum));
       } else {
-        part[g * (D + kPartPad) + d] = x;
+        float* part = sg.part + g * (D + kPartPad);
+        part[d] = x;
         if (d == 0) {
-          part[g * (D + kPartPad) + D] = top;
-          part[g * (D + kPartPad) + D + 1] = sum;
+          part[D] = top;
+          part[D + 1] = sum;
         }
       }
     }
-    // the next pair, perhaps of the next sequence with tokens
-    u += st1 - st0;
-    if (u < u1 && u == un.start + pairs * un.steps) {
-      un.start = u;
-      do {
-        ++un.seq;
-        un.steps = seq_steps(a, un.seq);
-      } while (un.steps == 0);
+  }
+}
+
+// ---- matrix kernel -------------------------------------------------------------
+//
+// bf16 and fp16 queries, head_dim 64, 128 or 256, rows of whole 16-byte vectors.
+// A wave takes 32 tokens and up to 16 query heads on 16x16x32 tiles; lane
+// (lo, hi) = (lane % 16, lane / 16).
+//
+//   scores   S^T = K Q^T: K rows as the A operand straight from memory (16 bytes
+//            of row lo), the heads' q as B, kept in registers.  Lane (lo, hi)
+//            gets head lo's scores of tokens 4 hi + r and 16 + 4 hi + r, r < 4.
+//   weights  so a head's m and l are per-lane scalars (joined over hi), and its
+//            8 weights are the B operand of the second product as they are, its
+//            k slots taking those tokens.
+//   output   O^T = V^T P^T: the A operand holds, of tokens 4 hi + r and 16 + 4 hi
+//            + r, dims DP lo .. DP lo + DP - 1 (DP = head_dim / 16): 8 row pieces
+//            that lie side by side in memory for the lanes of a row, transposed
+//            in registers by byte permutes, and no K or V goes through LDS.
+//
+// Precision: products of 16-bit K and q are exact and summed in fp32.  Weights
+// are fp32 and enter as three bf16 terms whose sum is the weight; fp16 V enters
+// as two bf16 terms (11 bits), of which the lower meets the weight's first two
+// terms (the third's product is below 2^-24 of the whole).  FP8 elements are
+// exact in either 16-bit type.
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+
+template <int DT>
+__device__ __forceinline__ f32x4 mfma16(const u32x4& a, const u32x4& b, const f32x4& c) {
+  if constexpr (DT == AMF_DTYPE_BF16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a),
+                                                   __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a),
+                                                  __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
+}
+
+// Two of the four e4m3 codes of w (the low or the high two) as a pair of DT.
+template <int DT, bool HIGH>
+__device__ __forceinline__ uint32_t e4m3_pair(uint32_t w) {
+  if constexpr (DT == AMF_DTYPE_BF16)
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, HIGH));
+  else
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, HIGH));
+}
+
+constexpr int kTileHeads = 16;
+constexpr int matrix_waves(int D) { return D == 256 ? 1 : 2; }  // per SIMD, at least
+
+template <int QDT, int KDT, int D>
+__global__ __launch_bounds__(kThreads, matrix_waves(D)) void paged_attn_matrix_kernel(PagedArgs a) {
+  constexpr bool FP8 = KDT == AMF_DTYPE_E4M3;
+  constexpr bool V16 = KDT == AMF_DTYPE_F16;  // V in two terms
+  constexpr int ES = FP8 ? 1 : 2;
+  constexpr int KS = D / 32;          // k steps of a score tile
+  constexpr int KL = KS * ES / 2;     // 16-byte loads of a K row per lane
+  constexpr int DP = D / 16;          // dims of a V row per lane
+  constexpr int VW = DP * ES / 4;     // their words
+  constexpr int ROW = D + 4;          // LDS row of a head's output, 4 banks on
+  __shared__ PageRun run;
+  __shared__ __attribute__((aligned(16))) float acc_lds[kWaves][kTileHeads][ROW];
+  __shared__ float m_lds[kWaves][kTileHeads], l_lds[kWaves][kTileHeads];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int lo = lane & 15, hi = lane >> 4;
+  empty_seqs(a);
+  Unit un = find_unit(a, gridDim.x, [](int64_t share) { return (int64_t)blockIdx.x * share; });
+  if (un.seq < 0) return;
+  const int64_t u0 = blockIdx.x * un.share, u1 = min(u0 + un.share, un.total);
+  for (int64_t u = u0; u < u1;) {
+    advance(a, un, u);
+    const Segment sg = segment_at<kTileHeads>(a, un, u, u0, u1);
+    u += sg.st1 - sg.st0;
+    // q of head lo, dims 32 ks + 8 hi .. (FP8: the dims of the K bytes that the
+    // lane loads, 64 j + 16 hi .., two k steps)
+    u32x4 qf[KS];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      const int d = FP8 ? 64 * (ks / 2) + 16 * hi + 8 * (ks % 2) : 32 * ks + 8 * hi;
+      qf[ks] = u32x4{0, 0, 0, 0};
+      if (lo < sg.heads) {
+        const int64_t head = sg.head0 - (int64_t)sg.seq * a.num_q_heads + lo;
+        qf[ks] = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.q) +
+                                                 sg.seq * a.q_seq + head * a.q_head + d);
+      }
+    }
+    float m = -INFINITY, l = 0.0f;
+    f32x4 acc[DP];
+#pragma unroll
+    for (int j = 0; j < DP; ++j) acc[j] = f32x4{0, 0, 0, 0};
+    u32x4 kr[2][KL];
+    uint32_t vr[8][VW];
+    const int64_t head_off = sg.hkv * a.head_stride;
+    // rows of K: tokens 16 i + lo; tokens that do not count read page 0
+    auto load_k = [&](int64_t off) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int64_t o = __shfl(off, 16 * i + lo);
+        const uint8_t* p = a.k + (o < 0 ? head_off : o) + 16 * hi;
+#pragma unroll
+        for (int n = 0; n < KL; ++n)
+          kr[i][n] = ld_stream(reinterpret_cast<const u32x4*>(p + 64 * n));
+      }
+    };
+    auto load_v = [&](int64_t off) {
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        const int64_t o = __shfl(off, 16 * (r / 4) + 4 * hi + r % 4);
+        const uint8_t* p = a.v + (o < 0 ? head_off : o) + DP * ES * lo;
+        if constexpr (VW >= 4) {
+#pragma unroll
+          for (int n = 0; n < VW / 4; ++n) {
+            const u32x4 x = ld_stream(reinterpret_cast<const u32x4*>(p) + n);
+#pragma unroll
+            for (int w = 0; w < 4; ++w) vr[r][4 * n + w] = x[w];
+          }
+        } else if constexpr (VW == 2) {
+          const u32x2 x = ld_stream(reinterpret_cast<const u32x2*>(p));
+          vr[r][0] = x[0];
+          vr[r][1] = x[1];
+        } else {
+          vr[r][0] = ld_stream(reinterpret_cast<const uint32_t*>(p));
+        }
+      }
+    };
+    const int64_t hold = run_steps(a);
+    for (int64_t r0 = sg.st0; r0 < sg.st1; r0 += hold) {
+      const int64_t r1 = min(r0 + hold, sg.st1), j0 = page_of(a, r0 * kStep);
+      load_pages(a, sg, r0, r1, run);
+      const int64_t t = wave * kChunk + (lane & 31);
+      int64_t off = token_offset(a, sg, run, j0, r0 * kStep + t);
+      uint32_t seen = (uint32_t)__ballot(off >= 0);
+      if (seen) {
+        load_k(off);
+        load_v(off);
+      }
+      for (int64_t st = r0; st < r1; ++st) {
+        // the next step's rows
+        int64_t next = -1;
+        if (st + 1 < r1) next = token_offset(a, sg, run, j0, (st + 1) * kStep + t);
+        const uint32_t seen_next = (uint32_t)__ballot(next >= 0);
+        f32x4 s[2];
+        if (seen) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            s[i] = f32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+              u32x4 kf;
+              if constexpr (FP8) {
+                const uint32_t w0 = kr[i][ks / 2][2 * (ks % 2)], w1 = kr[i][ks / 2][2 * (ks % 2) + 1];
+                kf = u32x4{e4m3_pair<QDT, false>(w0), e4m3_pair<QDT, true>(w0),
+                           e4m3_pair<QDT, false>(w1), e4m3_pair<QDT, true>(w1)};
+              } else {
+                kf = kr[i][ks];
+              }
+              s[i] = mfma16<QDT>(kf, qf[ks], s[i]);
+            }
+          }
+        }
+        if (seen_next) load_k(next);
+        if (seen) {
+          const uint32_t mine = seen >> (4 * hi);  // bits r and 16 + r: this lane's tokens
+          const bool full = seen == 0xFFFFFFFFu;
+          float x[8], p[8], top = -INFINITY;
+#pragma unroll
+          for (int r = 0; r < 8; ++r) {
+            x[r] = s[r / 4][r % 4];
+            const float y = x[r] * a.score_scale;
+            top = max_nan(top, full || (mine >> (16 * (r / 4) + r % 4) & 1) ? y : -INFINITY);
+          }
+          top = max_nan(top, __shfl_xor(top, 16));
+          top = max_nan(top, __shfl_xor(top, 32));
+          const float mn = max_nan(m, top);
+          const float w = weight_to(m, mn);
+          m = mn;
+          float sum = 0.0f;
+#pragma unroll
+          for (int r = 0; r < 8; ++r) {
+            p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r], a.score_scale, -mn));
+            if (!full && !(mine >> (16 * (r / 4) + r % 4) & 1)) p[r] = 0.0f;
+            sum += p[r];
+          }
+          l = l * w + sum;
+          if (__any(w != 1.0f)) {
+#pragma unroll
+            for (int j = 0; j < DP; ++j) acc[j] *= w;
+          }
+          uint32_t pb[kTerms][4];
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            uint32_t t3[kTerms];
+            weight_split(p[2 * n], p[2 * n + 1], t3);
+#pragma unroll
+            for (int k = 0; k < kTerms; ++k) pb[k][n] = t3[k];
+          }
+          if (!full) {  // V rows that do not count: zeros, not what page 0 holds
+#pragma unroll
+            for (int r = 0; r < 8; ++r)
+              if (!(mine >> (16 * (r / 4) + r % 4) & 1)) {
+#pragma unroll
+                for (int n = 0; n < VW; ++n) vr[r][n] = 0;
+              }
+          }
+#pragma unroll
+          for (int j = 0; j < DP; j += 2) {  // dims j and j + 1 of each lane's piece
+            uint32_t v2[8];
+#pragma unroll
+            for (int r = 0; r < 8; ++r) {
+              if constexpr (FP8)
+                v2[r] = j % 4 ? e4m3_pair<AMF_DTYPE_BF16, true>(vr[r][j / 4])
+                              : e4m3_pair<AMF_DTYPE_BF16, false>(vr[r][j / 4]);
+              else
+                v2[r] = vr[r][j / 2];
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              u32x4 va, vl;
+#pragma unroll
+              for (int n = 0; n < 4; ++n) {
+                va[n] = __builtin_amdgcn_perm(v2[2 * n + 1], v2[2 * n],
+                                              e ? 0x07060302u : 0x05040100u);
+                if constexpr (V16) {
+                  uint32_t h2, l2;
+                  v_split(va[n], h2, l2);
+                  va[n] = h2;
+                  vl[n] = l2;
+                }
+              }
+#pragma unroll
+              for (int k = 0; k < kTerms; ++k) {
+                const u32x4 pk{pb[k][0], pb[k][1], pb[k][2], pb[k][3]};
+                acc[j + e] = mfma16<AMF_DTYPE_BF16>(va, pk, acc[j + e]);
+                if constexpr (V16) {
+                  if (k < 2) acc[j + e] = mfma16<AMF_DTYPE_BF16>(vl, pk, acc[j + e]);
+                }
+              }
+            }
+          }
+        }
+        if (seen_next) load_v(next);
+        seen = seen_next;
+      }
+    }
+    // the four waves' parts
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    __syncthreads();  // the last pair's parts have been read
+    if (lo < sg.heads) {
+      if (hi == 0) {
+        m_lds[wave][lo] = m;
+        l_lds[wave][lo] = l;
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        float* o = &acc_lds[wave][lo][DP * (4 * hi + r)];
+#pragma unroll
+        for (int j = 0; j < DP; j += 4)
+          *reinterpret_cast<f32x4*>(o + j) =
+              f32x4{acc[j][r], acc[j + 1][r], acc[j + 2][r], acc[j + 3][r]};
+      }
+    }
+    __syncthreads();
+    for (int i = tid; i < sg.heads * (D / 4); i += kThreads) {
+      const int g = i / (D / 4), d = 4 * (i - g * (D / 4));
+      float top = m_lds[0][g], sum = 0.0f;
+      f32x4 x{0, 0, 0, 0};
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w) top = max_nan(top, m_lds[w][g]);
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        const float f = weight_to(m_lds[w][g], top);
+        sum += l_lds[w][g] * f;
+        x += *reinterpret_cast<const f32x4*>(&acc_lds[w][g][d]) * f;
+      }
+      if (sg.whole) {
+        if (sum == 0.0f)
+          x = f32x4{0, 0, 0, 0};
+        else
+          x *= a.v_scale / sum;
+        store4(a.out, a.out_dtype, (sg.head0 + g) * D + d, x);
+      } else {
+        float* part = sg.part + g * (D + kPartPad);
+        *reinterpret_cast<f32x4*>(part + d) = x;
+        if (d == 0) {
+          part[D] = top;
+          part[D + 1] = sum;
+        }
+      }
     }
   }
 }
@@ -376,15 +728,26 @@ __global__ __launch_bounds__(kThreads) void paged_attn_merge_kernel(PagedArgs a,
 
 constexpr int64_t kGroups = 1024;  // workgroups of a launch
 
-int tile_heads(int32_t group) { return std::min<int32_t>(group, kGenHeads); }
-
+// Floats of a partial, for either kernel.
 int64_t part_floats(int32_t group, int32_t head_dim) {
-  return (int64_t)tile_heads(group) * (head_dim + kPartPad);
+  return (int64_t)std::min<int32_t>(group, kTileHeads) * (head_dim + kPartPad);
 }
 
 template <int QDT, int KDT>
-void launch_general(const PagedArgs& a, hipStream_t st) {
-  paged_attn_general_kernel<QDT, KDT><<<dim3((unsigned)kGroups), kThreads, 0, st>>>(a);
+void launch(const PagedArgs& a, bool matrix, hipStream_t st) {
+  const dim3 grid((unsigned)kGroups);
+  if constexpr (QDT != AMF_DTYPE_F32) {
+    if (matrix) {
+      if (a.head_dim == 64)
+        paged_attn_matrix_kernel<QDT, KDT, 64><<<grid, kThreads, 0, st>>>(a);
+      else if (a.head_dim == 128)
+        paged_attn_matrix_kernel<QDT, KDT, 128><<<grid, kThreads, 0, st>>>(a);
+      else
+        paged_attn_matrix_kernel<QDT, KDT, 256><<<grid, kThreads, 0, st>>>(a);
+      return;
+    }
+  }
+  paged_attn_general_kernel<QDT, KDT><<<grid, kThreads, 0, st>>>(a);
 }
 
 }  // namespace
@@ -462,7 +825,13 @@ extern "C" int amf_paged_decode_attn(
   a.block_size = block_size;
   a.block_shift = (block_size & (block_size - 1)) == 0 ? __builtin_ctz(block_size) : -1;
   a.group = num_q_heads / num_kv_heads;
-  a.tiles = (a.group + kGenHeads - 1) / kGenHeads;
+  // rows that 16-byte loads and stores reach
+  const int64_t bits = (int64_t)((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) |
+                       a.page_stride | a.token_stride | a.head_stride |
+                       (q_seq_stride * qs) | (q_head_stride * qs);
+  const bool matrix = qs == 2 && split_head_dim(head_dim) && aligned16(bits);
+  const int tile = matrix ? kTileHeads : kGenHeads;
+  a.tiles = (a.group + tile - 1) / tile;
   a.out_dtype = out_dtype;
   a.score_scale = (softmax_scale > 0.0f ? softmax_scale : 1.0f / sqrtf((float)head_dim)) *
                   k_scale * kLog2e;
@@ -472,16 +841,19 @@ extern "C" int amf_paged_decode_attn(
   a.err_flag = err_flag;
   hipStream_t st = as_stream(stream);
   if (kv_dtype == AMF_DTYPE_BF16)
-    launch_general<AMF_DTYPE_BF16, AMF_DTYPE_BF16>(a, st);
+    launch<AMF_DTYPE_BF16, AMF_DTYPE_BF16>(a, matrix, st);
   else if (kv_dtype == AMF_DTYPE_F16)
-    launch_general<AMF_DTYPE_F16, AMF_DTYPE_F16>(a, st);
+    launch<AMF_DTYPE_F16, AMF_DTYPE_F16>(a, matrix, st);
   else if (kv_dtype == AMF_DTYPE_F32)
-    launch_general<AMF_DTYPE_F32, AMF_DTYPE_F32>(a, st);
+    launch<AMF_DTYPE_F32, AMF_DTYPE_F32>(a, matrix, st);
   else if (q_dtype == AMF_DTYPE_BF16)
-    launch_general<AMF_DTYPE_BF16, AMF_DTYPE_E4M3>(a, st);
+    launch<AMF_DTYPE_BF16, AMF_DTYPE_E4M3>(a, matrix, st);
   else
-    launch_general<AMF_DTYPE_F16, AMF_DTYPE_E4M3>(a, st);
+    launch<AMF_DTYPE_F16, AMF_DTYPE_E4M3>(a, matrix, st);
   if (int rc = check_launch(who)) return rc;
-  paged_attn_merge_kernel<kGenHeads><<<dim3((unsigned)(kGroups - 1)), kThreads, 0, st>>>(a, kGroups);
+  if (matrix)
+    paged_attn_merge_kernel<kTileHeads><<<dim3((unsigned)(kGroups - 1)), kThreads, 0, st>>>(a, kGroups);
+  else
+    paged_attn_merge_kernel<kGenHeads><<<dim3((unsigned)(kGroups - 1)), kThreads, 0, st>>>(a, kGroups);
   return check_launch(who);
 }
