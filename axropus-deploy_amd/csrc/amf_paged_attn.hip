@@ -59,9 +59,20 @@ struct PagedArgs {
   int32_t out_dtype;
   float score_scale;    // softmax scale * k_scale * log2(e)
   float v_scale;
+  bool whole;           // a workgroup takes a whole pair
+  struct Cut* cuts;     // [workgroup]
   float* part;          // [workgroup][2][heads of a tile][head_dim + kPartPad]
   int64_t part_stride;  // floats of one partial
   int32_t* err_flag;
+};
+
+// The pair that begins in a workgroup's share and does not end there: its
+// partials are slot `slot` of this workgroup and slot 0 of the next, to `last`.
+struct Cut {
+  int32_t heads;  // 0: no such pair
+  int32_t head0;  // of the step's rows
+  int32_t last;
+  int32_t slot;
 };
 
 // ---- shares --------------------------------------------------------------------
@@ -93,15 +104,23 @@ struct Unit {
   int64_t steps;  // of each of its pairs
 };
 
-// The place of unit at(share), the same in every thread; seq is -1 behind the
-// last unit.
-template <typename At>
-__device__ __forceinline__ Unit find_unit(const PagedArgs& a, int64_t groups, const At& at) {
+// The place of the workgroup's first unit, the same in every thread; seq is -1
+// where it has none.
+__device__ __forceinline__ Unit find_unit(const PagedArgs& a) {
+  const int64_t groups = gridDim.x;
   __shared__ int64_t tmp[kWaves];
   __shared__ Unit found;
   const int64_t pairs = (int64_t)a.num_kv_heads * a.tiles;
   const int tid = threadIdx.x;
   Unit r{};
+  if (a.whole) {
+    r.seq = (int)(blockIdx.x / pairs);
+    r.steps = r.share = seq_steps(a, r.seq);
+    r.start = (int64_t)blockIdx.x * r.steps - blockIdx.x % pairs * r.steps;
+    r.total = r.start + pairs * r.steps;
+    if (r.steps == 0) r.seq = -1;
+    return r;
+  }
   int64_t steps = 0, before = 0;
   if (a.num_seqs <= kThreads) {  // one scan gives the total and the places
     if (tid < a.num_seqs) steps = seq_steps(a, tid);
@@ -112,7 +131,7 @@ __device__ __forceinline__ Unit find_unit(const PagedArgs& a, int64_t groups, co
     block_exclusive<kThreads>(mine, tmp, &r.total);
   }
   r.share = (r.total + groups - 1) / groups;
-  const int64_t u = at(r.share);
+  const int64_t u = blockIdx.x * r.share;
   if (u >= r.total) {
     r.seq = -1;
     return r;
@@ -165,6 +184,9 @@ __device__ __forceinline__ Segment segment_at(const PagedArgs& a, const Unit& un
   g.ctx = a.context_lens[un.seq];
   g.whole = g.st0 == 0 && g.st1 == un.steps;
   g.part = a.part + (2 * (int64_t)blockIdx.x + (u != u0)) * a.part_stride;
+  if (!g.whole && g.st0 == 0 && threadIdx.x == 0)
+    a.cuts[blockIdx.x] = Cut{g.heads, (int32_t)g.head0, (int32_t)((u + un.steps - 1) / un.share),
+                             u != u0};
   return g;
 }
 
@@ -287,7 +309,8 @@ __global__ __launch_bounds__(kThreads) void paged_attn_general_kernel(PagedArgs 
   const int D = a.head_dim, half = lane >> 5;
   const int d0 = half ? (D + 1) / 2 : 0, d1 = half ? D : (D + 1) / 2;
   empty_seqs(a);
-  Unit un = find_unit(a, gridDim.x, [](int64_t share) { return (int64_t)blockIdx.x * share; });
+  Unit un = find_unit(a);
+  if (!a.whole && tid == 0) a.cuts[blockIdx.x].heads = 0;
   if (un.seq < 0) return;
   const int64_t u0 = blockIdx.x * un.share, u1 = min(u0 + un.share, un.total);
   for (int64_t u = u0; u < u1;) {
@@ -461,7 +484,8 @@ __global__ __launch_bounds__(kThreads, matrix_waves(D)) void paged_attn_matrix_k
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int lo = lane & 15, hi = lane >> 4;
   empty_seqs(a);
-  Unit un = find_unit(a, gridDim.x, [](int64_t share) { return (int64_t)blockIdx.x * share; });
+  Unit un = find_unit(a);
+  if (!a.whole && tid == 0) a.cuts[blockIdx.x].heads = 0;
   if (un.seq < 0) return;
   const int64_t u0 = blockIdx.x * un.share, u1 = min(u0 + un.share, un.total);
   for (int64_t u = u0; u < u1;) {
@@ -690,43 +714,92 @@ __global__ __launch_bounds__(kThreads, matrix_waves(D)) void paged_attn_matrix_k
 
 // ---- merge ---------------------------------------------------------------------
 //
-// Workgroup b looks at the boundary between shares b and b + 1.  When it cuts a
-// pair, and is the first that does, the workgroup joins the pair's partials:
-// slot 1 of the workgroup the pair begins in (slot 0 if it begins the share),
-// slot 0 of the others.
-template <int TILE>
-__global__ __launch_bounds__(kThreads) void paged_attn_merge_kernel(PagedArgs a, int64_t groups) {
+// A workgroup per (cut pair, head): threads take W dims of every n-th partial,
+// several partials loaded ahead of their use, and are joined in LDS.
+template <int W>
+__global__ __launch_bounds__(kThreads) void paged_attn_merge_kernel(PagedArgs a) {
+  constexpr int kAhead = 4;
+  __shared__ float x_lds[kThreads][W], m_lds[kThreads], l_lds[kThreads];
   const int64_t b = blockIdx.x;
-  const Unit un = find_unit(a, groups, [b](int64_t share) { return (b + 1) * share; });
-  if (un.seq < 0) return;
-  const int64_t ub = (b + 1) * un.share;
-  const int64_t pair = (ub - un.start) / un.steps;
-  const int64_t begin = un.start + pair * un.steps, end = begin + un.steps;
-  if (begin == ub || begin < ub - un.share) return;
-  const int64_t last = (end - 1) / un.share;
-  const int hkv = (int)(pair / a.tiles), tile = (int)(pair % a.tiles);
-  const int heads = min(TILE, a.group - tile * TILE);
-  const int D = a.head_dim, row = D + kPartPad;
-  const int64_t head0 = (int64_t)un.seq * a.num_q_heads + hkv * a.group + tile * TILE;
-  for (int i = threadIdx.x; i < heads * D; i += kThreads) {
-    const int g = i / D, d = i - g * D;
-    float m = -INFINITY, l = 0.0f, acc = 0.0f;
-    for (int64_t w = b; w <= last; ++w) {
-      const int slot = w == b && begin != b * un.share;
-      const float* p = a.part + (2 * w + slot) * a.part_stride + g * row;
-      const float pm = p[D], top = max_nan(m, pm);
-      const float f = weight_to(m, top), pf = weight_to(pm, top);
-      l = l * f + p[D + 1] * pf;
-      acc = acc * f + p[d] * pf;
-      m = top;
+  const Cut cut = a.cuts[b];
+  const int g = blockIdx.y, tid = threadIdx.x;
+  if (g >= cut.heads) return;
+  const int D = a.head_dim, row = g * (D + kPartPad);
+  const int cols = (D + W - 1) / W, rows = kThreads / cols;
+  const int col = tid % cols, r = tid / cols;
+  float m = -INFINITY, l = 0.0f, x[W];
+#pragma unroll
+  for (int e = 0; e < W; ++e) x[e] = 0.0f;
+  if (r < rows) {
+    const int64_t n = cut.last - b + 1;
+    for (int64_t i0 = r; i0 < n; i0 += kAhead * rows) {
+      float pm[kAhead], pl[kAhead], px[kAhead][W];
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        const int64_t i = i0 + k * rows;
+        pm[k] = -INFINITY;
+        pl[k] = 0.0f;
+#pragma unroll
+        for (int e = 0; e < W; ++e) px[k][e] = 0.0f;
+        if (i < n) {
+          const float* p = a.part + (2 * (b + i) + (i == 0 ? cut.slot : 0)) * a.part_stride + row;
+          pm[k] = p[D];
+          pl[k] = p[D + 1];
+          if constexpr (W == 4) {
+            const f32x4 v = *reinterpret_cast<const f32x4*>(p + 4 * col);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) px[k][e] = v[e];
+          } else {
+            px[k][0] = p[col];
+          }
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        const float top = max_nan(m, pm[k]);
+        const float f = weight_to(m, top), pf = weight_to(pm[k], top);
+        l = l * f + pl[k] * pf;
+#pragma unroll
+        for (int e = 0; e < W; ++e) x[e] = x[e] * f + px[k][e] * pf;
+        m = top;
+      }
     }
-    store_out(a, (head0 + g) * D + d, l == 0.0f ? 0.0f : acc * (a.v_scale / l));
   }
+  m_lds[tid] = m;
+  l_lds[tid] = l;
+#pragma unroll
+  for (int e = 0; e < W; ++e) x_lds[tid][e] = x[e];
+  __syncthreads();
+  if (r > 0) return;
+  for (int k = 1; k < rows; ++k) {
+    const int o = tid + k * cols;
+    const float pm = m_lds[o], top = max_nan(m, pm);
+    const float f = weight_to(m, top), pf = weight_to(pm, top);
+    l = l * f + l_lds[o] * pf;
+#pragma unroll
+    for (int e = 0; e < W; ++e) x[e] = x[e] * f + x_lds[o][e] * pf;
+    m = top;
+  }
+  const float scale = l == 0.0f ? 0.0f : a.v_scale / l;
+  const int64_t at = (int64_t)(cut.head0 + g) * D + W * col;
+  if constexpr (W == 4)
+    store4(a.out, a.out_dtype, at,
+           l == 0.0f ? f32x4{0, 0, 0, 0}
+                     : f32x4{x[0] * scale, x[1] * scale, x[2] * scale, x[3] * scale});
+  else
+    store_out(a, at, l == 0.0f ? 0.0f : x[0] * scale);
 }
 
 // ---- launch --------------------------------------------------------------------
 
-constexpr int64_t kGroups = 1024;  // workgroups of a launch
+#ifndef PG_WHOLE
+#define PG_WHOLE 8
+#endif
+#ifndef PG_GROUPS
+#define PG_GROUPS 512
+#endif
+constexpr int64_t kGroups = 1024;  // most workgroups that share a launch's steps
+constexpr int64_t kWholeSteps = PG_WHOLE;
 
 // Floats of a partial, for either kernel.
 int64_t part_floats(int32_t group, int32_t head_dim) {
@@ -734,8 +807,8 @@ int64_t part_floats(int32_t group, int32_t head_dim) {
 }
 
 template <int QDT, int KDT>
-void launch(const PagedArgs& a, bool matrix, hipStream_t st) {
-  const dim3 grid((unsigned)kGroups);
+void launch(const PagedArgs& a, int64_t groups, bool matrix, hipStream_t st) {
+  const dim3 grid((unsigned)groups);
   if constexpr (QDT != AMF_DTYPE_F32) {
     if (matrix) {
       if (a.head_dim == 64)
@@ -757,7 +830,8 @@ extern "C" int64_t amf_paged_decode_workspace_bytes(int32_t num_q_heads, int32_t
   if (num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads != 0 || head_dim <= 0 ||
       head_dim > kMaxDim)
     return 0;
-  return 2 * kGroups * part_floats(num_q_heads / num_kv_heads, head_dim) * (int64_t)sizeof(float);
+  return kGroups * (int64_t)sizeof(Cut) +
+         2 * kGroups * part_floats(num_q_heads / num_kv_heads, head_dim) * (int64_t)sizeof(float);
 }
 
 extern "C" int amf_paged_decode_attn(
@@ -836,24 +910,36 @@ extern "C" int amf_paged_decode_attn(
   a.score_scale = (softmax_scale > 0.0f ? softmax_scale : 1.0f / sqrtf((float)head_dim)) *
                   k_scale * kLog2e;
   a.v_scale = v_scale;
-  a.part = static_cast<float*>(workspace);
+  // the most steps that a pair can have, as far as the host knows
+  const int64_t tokens = pages ? (int64_t)max_pages * block_size
+                               : std::min<int64_t>(max_context_len, (int64_t)table_pages * block_size);
+  const int64_t steps = std::max<int64_t>(1, (tokens + kStep - 1) / kStep);
+  const int64_t pairs = (int64_t)num_seqs * num_kv_heads * a.tiles;
+  if (pairs > 0x7FFFFFFF || (int64_t)num_seqs * num_q_heads > 0x7FFFFFFF)
+    return fail(AMF_ERR_UNSUPPORTED, "%s: %d sequences of %d heads", who, num_seqs, num_q_heads);
+  a.whole = steps <= kWholeSteps;
+  const int64_t groups = a.whole ? pairs : std::min(pairs * steps, (int64_t)PG_GROUPS);
+  a.cuts = static_cast<Cut*>(workspace);
+  a.part = reinterpret_cast<float*>(a.cuts + kGroups);
   a.part_stride = part_floats(a.group, head_dim);
   a.err_flag = err_flag;
   hipStream_t st = as_stream(stream);
   if (kv_dtype == AMF_DTYPE_BF16)
-    launch<AMF_DTYPE_BF16, AMF_DTYPE_BF16>(a, matrix, st);
+    launch<AMF_DTYPE_BF16, AMF_DTYPE_BF16>(a, groups, matrix, st);
   else if (kv_dtype == AMF_DTYPE_F16)
-    launch<AMF_DTYPE_F16, AMF_DTYPE_F16>(a, matrix, st);
+    launch<AMF_DTYPE_F16, AMF_DTYPE_F16>(a, groups, matrix, st);
   else if (kv_dtype == AMF_DTYPE_F32)
-    launch<AMF_DTYPE_F32, AMF_DTYPE_F32>(a, matrix, st);
+    launch<AMF_DTYPE_F32, AMF_DTYPE_F32>(a, groups, matrix, st);
   else if (q_dtype == AMF_DTYPE_BF16)
-    launch<AMF_DTYPE_BF16, AMF_DTYPE_E4M3>(a, matrix, st);
+    launch<AMF_DTYPE_BF16, AMF_DTYPE_E4M3>(a, groups, matrix, st);
   else
-    launch<AMF_DTYPE_F16, AMF_DTYPE_E4M3>(a, matrix, st);
+    launch<AMF_DTYPE_F16, AMF_DTYPE_E4M3>(a, groups, matrix, st);
   if (int rc = check_launch(who)) return rc;
+  if (a.whole) return ok();
+  const dim3 grid((unsigned)groups, (unsigned)std::min<int32_t>(a.group, tile));
   if (matrix)
-    paged_attn_merge_kernel<kTileHeads><<<dim3((unsigned)(kGroups - 1)), kThreads, 0, st>>>(a, kGroups);
+    paged_attn_merge_kernel<4><<<grid, kThreads, 0, st>>>(a);
   else
-    paged_attn_merge_kernel<kGenHeads><<<dim3((unsigned)(kGroups - 1)), kThreads, 0, st>>>(a, kGroups);
+    paged_attn_merge_kernel<1><<<grid, kThreads, 0, st>>>(a);
   return check_launch(who);
 }
