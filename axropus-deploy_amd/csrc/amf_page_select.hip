@@ -128,64 +128,129 @@ __device__ __forceinline__ uint64_t order_key(double x) {
 constexpr uint64_t kForced = ~0ull;  // first and last pages
 constexpr uint64_t kInfinite = 0xFFF0000000000000ull;  // order_key(inf)
 
-template <bool BF16>
-__device__ __forceinline__ float elem16(uint16_t w) {
-  return BF16 ? bf16_to_f32(w) : (float)__builtin_bit_cast(_Float16, w);
-}
+// A wave scores kTiles times 16 pages against SETS times 4 query heads with 4x4x4
+// products in 64 bits, four blocks side by side: lane (lo, hi) = (lane % 16,
+// lane / 16) holds page lo's bounds in dims 32 c + 8 hi + e as the A operand of
+// step (c, e), and as B head lo % 4's q in that dim, split as max(q, 0) against
+// hi and min(q, 0) against lo; D gives it page 4 (lo / 4) + hi of head lo % 4.
+// q waits in LDS as doubles.  (fp64 on the vector units took 95 us for 8
+// sequences x 65000 tokens, 64 / 8 heads of 128: a conversion, a choice and a
+// product per element and head, and a reduction over lanes.)
+constexpr int kTiles = 1;  // 1: 48.2 us, 2: 47.5 (13.9 / 14.3 for one sequence x 131072)
+constexpr int kScorePages = kThreads / 64 * 16 * kTiles;  // pages of a workgroup
+constexpr int kHeadSet = 4;
 
-// LP lanes share a page, 8 channels each.
-constexpr int kScorePages = 64;  // pages of a workgroup
+__device__ __forceinline__ double max64(double x, double y) { return x > y ? x : y; }
 
-template <bool BF16, int LP>
+// NC chunks of 32 dims; SETS of heads share a bound's conversion to a double.
+// The heads' workgroups of a page run side by side: their bounds lie together.
+template <bool BF16, int NC, int SETS>
 __global__ __launch_bounds__(kThreads) void page_score_kernel(SelectArgs a) {
-  const int s = blockIdx.z, h = blockIdx.y;
+  // [dim in step order][set][hi][head] -> (max(q, 0), min(q, 0))
+  __shared__ __attribute__((aligned(16))) double q_lds[NC * 8][SETS][4][kHeadSet][2];
+  const int s = blockIdx.z, h = blockIdx.x;
+  const int64_t p0 = (int64_t)blockIdx.y * kScorePages;
   const int64_t n = seq_pages(a, s);
-  const int64_t p0 = (int64_t)blockIdx.x * kScorePages;
   if (p0 >= n || n <= a.num_pages) return;
-  const int sub = threadIdx.x % LP, d = 8 * sub;
-  const bool live = d < a.head_dim;
-  const uint16_t* q0 = a.q + s * a.q_seq + (int64_t)h * a.group * a.q_head + d;
-  uint64_t* keys = a.keys + ((int64_t)s * a.num_kv_heads + h) * a.max_pages;
-  for (int64_t p = p0 + threadIdx.x / LP; p < min(p0 + kScorePages, n); p += kThreads / LP) {
-    const int64_t id = a.block_tables[s * a.bt_stride + p];
-    const bool ok = id >= 0 && id < a.pool_pages;
-    float lo[8], hi[8];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int lo = lane & 15, hi = lane >> 4;
+  const int64_t base = p0 + wave * 16 * kTiles;
+  u32x4 b[kTiles][2][NC];
+  bool ok[kTiles];
+  int64_t id[kTiles];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) lo[e] = hi[e] = 0.0f;
-    if (ok && live) {
-      const uint16_t* b = a.bounds + ((id * a.num_kv_heads + h) * 2) * a.head_dim + d;
-      unpack8<BF16>(ld_stream(reinterpret_cast<const u32x4*>(b)), lo);
-      unpack8<BF16>(ld_stream(reinterpret_cast<const u32x4*>(b + a.head_dim)), hi);
+  for (int t = 0; t < kTiles; ++t) {
+    const int64_t p = base + 16 * t + lo;
+    id[t] = p < n ? a.block_tables[s * a.bt_stride + p] : -1;
+    ok[t] = id[t] >= 0 && id[t] < a.pool_pages;
+  }
+#pragma unroll
+  for (int t = 0; t < kTiles; ++t) {
+    const uint16_t* src =
+        a.bounds + ((ok[t] ? id[t] : 0) * a.num_kv_heads + h) * 2 * a.head_dim + 8 * hi;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      b[t][0][c] = b[t][1][c] = u32x4{0, 0, 0, 0};
+      if (ok[t] && 32 * c + 8 * hi < a.head_dim) {
+        b[t][0][c] = ld_stream(reinterpret_cast<const u32x4*>(src + 32 * c));
+        b[t][1][c] = ld_stream(reinterpret_cast<const u32x4*>(src + a.head_dim + 32 * c));
+      }
     }
-    bool finite = true;
+  }
+  double best[kTiles];
+  int fin[kTiles];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) finite = finite && fabsf(lo[e]) < INFINITY && fabsf(hi[e]) < INFINITY;
-    double best = -INFINITY;
-    for (int g = 0; g < a.group; ++g) {
-      double u = 0.0;
-      if (live) {
-        float x[8];
-        unpack8<BF16>(*reinterpret_cast<const u32x4*>(q0 + g * a.q_head), x);
+  for (int t = 0; t < kTiles; ++t) {
+    best[t] = -INFINITY;
+    fin[t] = 1;
+  }
+  for (int g0 = 0; g0 < a.group; g0 += SETS * kHeadSet) {
+    __syncthreads();
+    for (int i = tid; i < NC * 32 * SETS * kHeadSet; i += kThreads) {
+      const int d = i % (NC * 32), g = i / (NC * 32);
+      float x = 0.0f;
+      if (d < a.head_dim && g0 + g < a.group)
+        x = half_lo<BF16>(a.q[s * a.q_seq + ((int64_t)h * a.group + g0 + g) * a.q_head + d]);
+      double* o = q_lds[8 * (d / 32) + d % 8][g / kHeadSet][d / 8 % 4][g % kHeadSet];
+      o[0] = x < 0.0f ? 0.0 : (double)x;  // a NaN stays one
+      o[1] = x < 0.0f ? (double)x : 0.0;
+    }
+    __syncthreads();
+    double u[kTiles][SETS];
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          u = __builtin_fma((double)x[e], (double)(x[e] >= 0.0f ? hi[e] : lo[e]), u);
+    for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+      for (int k = 0; k < SETS; ++k) u[t][k] = 0.0;
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        double l[kTiles], m[kTiles];
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) {
+          uint32_t wl = b[t][0][c][e / 2], wh = b[t][1][c][e / 2];
+          asm volatile("" : "+v"(wl), "+v"(wh));  // converted here, not before the loop
+          l[t] = e % 2 ? half_hi<BF16>(wl) : half_lo<BF16>(wl);
+          m[t] = e % 2 ? half_hi<BF16>(wh) : half_lo<BF16>(wh);
+        }
+#pragma unroll
+        for (int k = 0; k < SETS; ++k) {
+          const double* q = q_lds[8 * c + e][k][hi][lo % 4];
+          const double qp = q[0], qm = q[1];
+#pragma unroll
+          for (int t = 0; t < kTiles; ++t) {
+            u[t][k] = __builtin_amdgcn_mfma_f64_4x4x4f64(m[t], qp, u[t][k], 0, 0, 0);
+            u[t][k] = __builtin_amdgcn_mfma_f64_4x4x4f64(l[t], qm, u[t][k], 0, 0, 0);
+          }
+        }
       }
 #pragma unroll
-      for (int o = LP / 2; o > 0; o >>= 1) u += __shfl_xor(u, o, LP);
-      finite = finite && u - u == 0.0;
-      best = max(best, u);
-    }
-    // a NaN or an infinity anywhere: above every finite score
+    for (int t = 0; t < kTiles; ++t)
 #pragma unroll
-    for (int o = LP / 2; o > 0; o >>= 1) finite = __shfl_xor((int)finite, o, LP) && finite;
-    if (sub == 0) {
-      uint64_t key = finite ? order_key(best) : kInfinite;
-      if (!ok) {
+      for (int k = 0; k < SETS; ++k) {
+        fin[t] &= u[t][k] - u[t][k] == 0.0;
+        if (g0 + k * kHeadSet + lo % 4 < a.group) best[t] = max64(best[t], u[t][k]);
+      }
+  }
+  const int place = 4 * (lo / 4) + hi;
+#pragma unroll
+  for (int t = 0; t < kTiles; ++t) {
+    // the best of the heads, in the four lanes of a page
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) {
+      best[t] = max64(best[t], __shfl_xor(best[t], o));
+      fin[t] &= __shfl_xor(fin[t], o);
+    }
+    const int good = __shfl((int)ok[t], place);
+    const int64_t p = base + 16 * t + place;
+    if (lo % 4 == 0 && p < n) {
+      uint64_t key = fin[t] ? order_key(best[t]) : kInfinite;
+      if (!good) {
         key = 0;  // never scored: behind every page that can be read
         if (a.err_flag) atomicOr(a.err_flag, AMF_ERRFLAG_BLOCK_RANGE);
       }
       if (p < a.first_pages || p >= n - a.last_pages) key = kForced;
-      keys[p] = key;
+      a.keys[((int64_t)s * a.num_kv_heads + h) * a.max_pages + p] = key;
     }
   }
 }
@@ -193,17 +258,49 @@ __global__ __launch_bounds__(kThreads) void page_score_kernel(SelectArgs a) {
 // ---- choice --------------------------------------------------------------------
 
 constexpr int kPickThreads = 1024;
+constexpr int kPickKeys = 8;  // consecutive keys of a thread
+constexpr int kPickTile = kPickThreads * kPickKeys;
+constexpr int kDigit = 11;  // bits
+constexpr int kBins = 1 << kDigit;
+
+// Sum over the threads before this one, and over all in *total; tmp holds a
+// word per wave.  Starts and ends with a barrier.
+__device__ __forceinline__ uint32_t pick_exclusive(uint32_t v, uint32_t* tmp, uint32_t* total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  uint32_t x = v;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const uint32_t y = __shfl_up(x, o);
+    if (lane >= o) x += y;
+  }
+  __syncthreads();
+  if (lane == 63) tmp[wave] = x;
+  __syncthreads();
+  uint32_t before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < kPickThreads / 64; ++w) {
+    const uint32_t y = tmp[w];
+    if (w < wave) before += y;
+    all += y;
+  }
+  *total = all;
+  __syncthreads();
+  return before + x - v;
+}
 
 // The num_pages largest keys of one (sequence, KV head), the lower page first
 // among equals, in page order.  The key of the last one taken is found digit by
-// digit (8 bits, a histogram in LDS), then the pages above it and the first of
-// its equals are written at their ranks.
+// digit (a histogram in LDS each), from the first bit in which the keys differ,
+// so that one or two digits separate scores that share sign and exponent; then
+// the pages above it and the first of its equals are written at their ranks.
+// Forced pages are left out of the search.  Up to kPickTile keys stay in
+// registers (MANY: they are read again for each pass).
+template <bool MANY>
 __global__ __launch_bounds__(kPickThreads) void page_pick_kernel(SelectArgs a) {
-  __shared__ uint32_t hist[256];
-  __shared__ int64_t tmp[kPickThreads / 64];
-  __shared__ uint64_t s_prefix;
-  __shared__ int32_t s_left;
-  __shared__ int s_done;
+  __shared__ uint32_t hist[kBins];
+  __shared__ uint32_t tmp[kPickThreads / 64];
+  __shared__ uint64_t s_lo[kPickThreads / 64], s_hi[kPickThreads / 64];
+  __shared__ uint32_t s_digit, s_left, s_all;
   const int s = blockIdx.y, h = blockIdx.x, tid = threadIdx.x;
   const int64_t n = seq_pages(a, s);
   const int64_t row = (int64_t)s * a.num_kv_heads + h;
@@ -221,66 +318,141 @@ __global__ __launch_bounds__(kPickThreads) void page_pick_kernel(SelectArgs a) {
     return;
   }
   const uint64_t* keys = a.keys + row * a.max_pages;
-  uint64_t prefix = 0;  // the digits found, in place
-  int32_t left = K;     // of the keys with these digits, how many are taken
-  int shift = 56;
-  for (;; shift -= 8) {
-    for (int i = tid; i < 256; i += kPickThreads) hist[i] = 0;
-    __syncthreads();
-    for (int64_t i = tid; i < n; i += kPickThreads) {
-      const uint64_t k = keys[i];
-      if (shift == 56 || (k >> (shift + 8)) == (prefix >> (shift + 8)))
-        atomicAdd(&hist[(k >> shift) & 255], 1u);
+  uint64_t kept[kPickKeys];
+  auto load = [&](int64_t t0) {  // this thread's keys of a tile; 0 behind the last
+#pragma unroll
+    for (int e = 0; e < kPickKeys; ++e) {
+      const int64_t i = t0 + (int64_t)tid * kPickKeys + e;
+      kept[e] = i < n ? keys[i] : 0;
     }
-    __syncthreads();
-    if (tid < 64) {  // the digit below which `left` keys do not fit; lane l: digits 4l ..
-      uint32_t c[4], sum = 0;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) sum += c[i] = hist[4 * tid + i];
-      int64_t all;
-      int64_t above = wave_exclusive(sum, &all);
-      above = all - above - sum;  // keys with larger digits than this lane's
-#pragma unroll
-      for (int i = 3; i >= 0; --i) {
-        if (above < left && above + c[i] >= left) {
-          s_prefix = prefix | (uint64_t)(4 * tid + i) << shift;
-          s_left = left - (int32_t)above;
-          s_done = above + c[i] == left;  // all of them are taken
-        }
-        above += c[i];
+  };
+  auto each_tile = [&](auto&& body) {
+    if constexpr (MANY) {
+      for (int64_t t0 = 0; t0 < n; t0 += kPickTile) {
+        load(t0);
+        body(t0);
       }
+    } else {
+      body((int64_t)0);
+    }
+  };
+  if constexpr (!MANY) load(0);
+  auto searched = [&](int64_t t0, int e) {
+    return t0 + (int64_t)tid * kPickKeys + e < n && kept[e] != kForced;
+  };
+  // range of the keys searched, and how many are forced
+  uint64_t lo = ~0ull, hi = 0;
+  each_tile([&](int64_t t0) {
+#pragma unroll
+    for (int e = 0; e < kPickKeys; ++e)
+      if (searched(t0, e)) {
+        lo = min(lo, kept[e]);
+        hi = max(hi, kept[e]);
+      }
+  });
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    lo = min(lo, (uint64_t)__shfl_xor((unsigned long long)lo, o));
+    hi = max(hi, (uint64_t)__shfl_xor((unsigned long long)hi, o));
+  }
+  if ((tid & 63) == 0) {
+    s_lo[tid >> 6] = lo;
+    s_hi[tid >> 6] = hi;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kPickThreads / 64; ++w) {
+    lo = min(lo, s_lo[w]);
+    hi = max(hi, s_hi[w]);
+  }
+  uint32_t left = (uint32_t)(K - min((int64_t)a.first_pages + a.last_pages, n));
+  uint64_t cut = lo;  // keys of these digits: `left` of them are taken
+  int shift = lo < hi ? 64 - __builtin_clzll(lo ^ hi) : 0;  // bits not decided yet
+  if (left == 0) {  // nothing but the forced pages
+    cut = kForced;
+    shift = 0;
+  }
+  while (shift > 0 && left > 0) {
+    const int next = max(shift - kDigit, 0), bins = 1 << (shift - next);
+    for (int i = tid; i < bins; i += kPickThreads) hist[i] = 0;
+    __syncthreads();
+    const uint64_t above = shift == 64 ? 0 : cut >> shift;
+    each_tile([&](int64_t t0) {
+#pragma unroll
+      for (int e = 0; e < kPickKeys; ++e)
+        if (searched(t0, e) && (shift == 64 || kept[e] >> shift == above))
+          atomicAdd(&hist[(kept[e] >> next) & (bins - 1)], 1u);
+    });
+    __syncthreads();
+    // bins from the top, two a thread: the one in which `left` keys are reached
+    uint32_t c[kBins / kPickThreads], sum = 0, all;
+#pragma unroll
+    for (int k = 0; k < kBins / kPickThreads; ++k) {
+      const int bin = bins - 1 - (tid * (kBins / kPickThreads) + k);
+      sum += c[k] = bin >= 0 ? hist[bin] : 0;
+    }
+    uint32_t before = pick_exclusive(sum, tmp, &all);
+#pragma unroll
+    for (int k = 0; k < kBins / kPickThreads; ++k) {
+      if (before < left && before + c[k] >= left) {
+        s_digit = bins - 1 - (tid * (kBins / kPickThreads) + k);
+        s_left = left - before;
+        s_all = before + c[k] == left;
+      }
+      before += c[k];
     }
     __syncthreads();
-    prefix = s_prefix;
+    cut = (cut >> next >> (shift - next) << (shift - next) | s_digit) << next;
     left = s_left;
-    if (s_done || shift == 0) break;
+    shift = next;
+    if (s_all) break;
     __syncthreads();
   }
-  // taken: keys whose digits are above the prefix, and `left` of its equals
-  const uint64_t cut = prefix >> shift;
-  int64_t gt0 = 0, eq0 = 0;
-  for (int64_t i0 = 0; i0 < n; i0 += kPickThreads) {
-    const int64_t i = i0 + tid;
-    const uint64_t k = i < n ? keys[i] >> shift : 0;
-    const bool gt = i < n && k > cut, eq = i < n && k == cut;
-    int64_t all;
-    const int64_t both = block_exclusive<kPickThreads>((int64_t)gt << 32 | (int64_t)eq, tmp, &all);
-    const int64_t eq_before = eq0 + (both & 0xFFFFFFFF), gt_before = gt0 + (both >> 32);
-    if (gt || (eq && eq_before < left)) out[gt_before + min(eq_before, (int64_t)left)] = (int32_t)i;
-    gt0 += all >> 32;
-    eq0 += all & 0xFFFFFFFF;
-  }
+  // taken: keys whose digits are above the cut's, and `left` of its equals
+  cut >>= shift;
+  uint32_t gt0 = 0, eq0 = 0;
+  each_tile([&](int64_t t0) {
+    uint32_t gt = 0, eq = 0;
+#pragma unroll
+    for (int e = 0; e < kPickKeys; ++e) {
+      const bool in = t0 + (int64_t)tid * kPickKeys + e < n;
+      gt += in && (kept[e] == kForced || kept[e] >> shift > cut);
+      eq += in && kept[e] != kForced && kept[e] >> shift == cut;
+    }
+    uint32_t all;  // both below 2^14 in a tile
+    const uint32_t both = pick_exclusive(gt << 16 | eq, tmp, &all);
+    uint32_t g = gt0 + (both >> 16), q = eq0 + (both & 0xFFFFu);
+#pragma unroll
+    for (int e = 0; e < kPickKeys; ++e) {
+      const int64_t i = t0 + (int64_t)tid * kPickKeys + e;
+      if (i >= n) continue;
+      const bool above = kept[e] == kForced || kept[e] >> shift > cut;
+      const bool equal = kept[e] != kForced && kept[e] >> shift == cut;
+      if (above || (equal && q < left)) out[g + min(q, left)] = (int32_t)i;
+      g += above;
+      q += equal;
+    }
+    gt0 += all >> 16;
+    eq0 += all & 0xFFFFu;
+  });
+}
+
+template <bool BF16, int NC>
+void launch_score_sets(const SelectArgs& a, dim3 grid, hipStream_t st) {
+  if (a.group <= kHeadSet)
+    page_score_kernel<BF16, NC, 1><<<grid, kThreads, 0, st>>>(a);
+  else
+    page_score_kernel<BF16, NC, 2><<<grid, kThreads, 0, st>>>(a);
 }
 
 template <bool BF16>
 void launch_score(const SelectArgs& a, dim3 grid, hipStream_t st) {
-  const int lanes = a.head_dim / 8;
-  if (lanes <= 8)
-    page_score_kernel<BF16, 8><<<grid, kThreads, 0, st>>>(a);
-  else if (lanes <= 16)
-    page_score_kernel<BF16, 16><<<grid, kThreads, 0, st>>>(a);
+  if (a.head_dim <= 64)
+    launch_score_sets<BF16, 2>(a, grid, st);
+  else if (a.head_dim <= 128)
+    launch_score_sets<BF16, 4>(a, grid, st);
   else
-    page_score_kernel<BF16, 32><<<grid, kThreads, 0, st>>>(a);
+    launch_score_sets<BF16, 8>(a, grid, st);
 }
 
 int64_t select_max_pages(int32_t table_pages, int32_t block_size, int32_t max_context_len) {
@@ -406,14 +578,18 @@ extern "C" int amf_select_pages(const void* q, int32_t dtype, int64_t q_seq_stri
                      max_pages, static_cast<uint64_t*>(workspace), pages, page_counts, err_flag};
   hipStream_t st = as_stream(stream);
   if (scored) {
-    const dim3 grid((unsigned)((max_pages + kScorePages - 1) / kScorePages),
-                    (unsigned)num_kv_heads, (unsigned)num_seqs);
+    const unsigned chunks = (unsigned)((max_pages + kScorePages - 1) / kScorePages);
+    const dim3 grid((unsigned)num_kv_heads, chunks, (unsigned)num_seqs);
     if (dtype == AMF_DTYPE_BF16)
       launch_score<true>(a, grid, st);
     else
       launch_score<false>(a, grid, st);
     if (int rc = check_launch(who)) return rc;
   }
-  page_pick_kernel<<<dim3((unsigned)num_kv_heads, (unsigned)num_seqs), kPickThreads, 0, st>>>(a);
+  const dim3 rows((unsigned)num_kv_heads, (unsigned)num_seqs);
+  if (max_pages > kPickTile)
+    page_pick_kernel<true><<<rows, kPickThreads, 0, st>>>(a);
+  else
+    page_pick_kernel<false><<<rows, kPickThreads, 0, st>>>(a);
   return check_launch(who);
 }
