@@ -263,27 +263,19 @@ def check(func: str, rc: int) -> None:
 _FNS: dict = {}  # (name) -> bound entry point of the loaded library
 
 
-def call(func: str, *args) -> None:
-    """Call a status-returning entry point and raise on failure."""
+def entry(func: str):
+    """The bound entry point of the loaded library."""
     fn = _FNS.get(func)
     if fn is None:
         fn = _FNS[func] = getattr(load(), func)
-    rc = fn(*args)
+    return fn
+
+
+def call(func: str, *args) -> None:
+    """Call a status-returning entry point and raise on failure."""
+    rc = entry(func)(*args)
     if rc != OK:
         check(func, rc)
-
-
-def call_on(device, func: str, *args) -> None:
-    """call() with `device`, which holds the tensors, as the current device
-    (the null stream and the launch belong to the current one)."""
-    import torch
-
-    idx = _device_index(device)
-    if torch.cuda.current_device() == idx:
-        call(func, *args)
-    else:
-        with torch.cuda.device(idx):
-            call(func, *args)
 
 
 # ---------------------------------------------------------------- helpers --

@@ -29,19 +29,40 @@ import torch
 
 import amf_hip
 
-_KV_TAGS = {torch.float16: amf_hip.DTYPE_F16, torch.float32: amf_hip.DTYPE_F32,
-            torch.bfloat16: amf_hip.DTYPE_BF16, torch.float8_e4m3fn: amf_hip.DTYPE_E4M3}
+_TAGS = {torch.float16: amf_hip.DTYPE_F16, torch.float32: amf_hip.DTYPE_F32,
+         torch.bfloat16: amf_hip.DTYPE_BF16}
+_KV_TAGS = {**_TAGS, torch.float8_e4m3fn: amf_hip.DTYPE_E4M3}
 _HALVES = (torch.bfloat16, torch.float16)
+_I32 = torch.int32
 _I32_MAX = 0x7FFFFFFF
 _WS: dict = {}  # (entry point, sizes) -> workspace bytes
 
+# The checks below run on every call of a decode step, where the host's time is
+# what a small batch waits for: they compare in place and leave the words of an
+# error to a slow path.
+
+
+_current_device = getattr(torch._C, "_cuda_getDevice", None)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def _launch(idx: int, func: str, *args) -> None:
+    """A status-returning entry point with device idx, which holds the tensors,
+    as the current one (the null stream and the launch belong to it)."""
+    fn = amf_hip.entry(func)
+    if _current_device() == idx:
+        rc = fn(*args)
+    else:
+        with torch.cuda.device(idx):
+            rc = fn(*args)
+    if rc:
+        amf_hip.check(func, rc)
+
 
 def _workspace(name: str, sizes: tuple, given: Optional[torch.Tensor], dev: torch.device,
-               stream: int) -> Tuple[Optional[torch.Tensor], int]:
-    """(workspace, its bytes): the caller's, checked, or the scratch buffer of
-    this device and stream (a new one under graph capture)."""
-    from .dispatch import _check_buffer, _scratch
-
+               stream: int) -> Tuple[Optional[int], int]:
+    """(address of the workspace, its bytes): the caller's, checked, or the
+    scratch buffer of this device and stream (a new one under graph capture)."""
     key = (name, sizes)
     need = _WS.get(key)
     if need is None:
@@ -49,98 +70,93 @@ def _workspace(name: str, sizes: tuple, given: Optional[torch.Tensor], dev: torc
             _WS.clear()
         need = _WS[key] = int(getattr(amf_hip.load(), name)(*sizes))
     if given is not None:
-        _check_buffer(given, "workspace", dev)
+        _dispatch._check_buffer(given, "workspace", dev)
         have = given.numel() * given.element_size()
         if have < need:
             raise ValueError(f"workspace of {have} bytes, {need} needed")
-        return given, have
-    return (_scratch(dev, stream, need), need) if need else (None, 0)
+        return given.data_ptr(), have
+    return (_dispatch._scratch(dev, stream, need).data_ptr(), need) if need else (None, 0)
 
 
-class _Cache(NamedTuple):
-    """K and V of a layer as the C ABI takes them (strides in elements)."""
-
-    k: int
-    v: int
-    strides: Tuple[int, int, int]
-    pages: int
-    block: int
-    heads: int
-    dim: int
-    dtype: torch.dtype
-    device: torch.device
-
-
-def _cache(k: torch.Tensor, v: Optional[torch.Tensor]) -> _Cache:
-    """A layer [2, pages, block, heads, dim] (v None), or K and V planes
-    [pages, block, heads, dim] with the same strides; a plane alone holds both.
-    The last dim is contiguous, the others may be strided."""
+def _cache(k: torch.Tensor, v: Optional[torch.Tensor]) -> tuple:
+    """(device index, K address, V address, strides of page, token and head,
+    pages, block, heads, dim) of a layer [2, pages, block, heads, dim] (v
+    None), or of K and V planes [pages, block, heads, dim] with the same
+    strides; a plane alone holds both.  The last dim is contiguous, the others
+    may be strided."""
     if not isinstance(k, torch.Tensor):
         raise TypeError(f"a K/V cache is a tensor, got {type(k).__name__}")
-    amf_hip.require_device_tensor(k, "paged cache")
+    idx = k.get_device()
+    if idx < 0:
+        amf_hip.require_device_tensor(k, "paged cache")
     shape, st = k.shape, k.stride()
     kp = vp = k.data_ptr()
     if v is None and len(shape) == 5:
-        if shape[0] != 2:
+        planes, nb, bs, H, D = shape
+        plane, ps, ts, hs, ds = st
+        if planes != 2:
             raise ValueError(f"a layer's cache is [2, pages, block, heads, dim], got {tuple(shape)}")
-        vp = kp + st[0] * k.element_size()
-        shape, st = shape[1:], st[1:]
+        vp = kp + plane * k.element_size()
     elif len(shape) != 4:
         raise ValueError(f"K/V cache of shape {tuple(shape)}: expected [2, pages, block, heads, "
                          "dim], or planes [pages, block, heads, dim]")
-    elif v is not None and v is not k:
-        if not isinstance(v, torch.Tensor) or v.shape != shape or v.stride() != st:
-            raise ValueError("K and V planes differ in shape or strides")
-        if v.dtype != k.dtype or v.device != k.device:
-            raise ValueError("K and V planes differ in type or device")
-        vp = v.data_ptr()
+    else:
+        nb, bs, H, D = shape
+        ps, ts, hs, ds = st
+        if v is not None and v is not k:
+            if not isinstance(v, torch.Tensor) or v.shape != shape or v.stride() != st:
+                raise ValueError("K and V planes differ in shape or strides")
+            if v.dtype != k.dtype or v.device != k.device:
+                raise ValueError("K and V planes differ in type or device")
+            vp = v.data_ptr()
     if k.dtype not in _KV_TAGS:
         raise TypeError(f"paged cache of {k.dtype}: bf16, fp16, fp32 or float8_e4m3fn")
-    nb, bs, H, D = shape
-    if st[3] != 1 and D != 1:
+    if ds != 1 and D != 1:
         raise ValueError("the cache's last dim must be contiguous")
-    if nb == 0 or bs == 0 or H == 0 or D == 0:
+    if not (nb and bs and H and D):
         raise ValueError(f"empty K/V cache {tuple(shape)}")
-    return _Cache(kp, vp, (st[0], st[1], st[2]), nb, bs, H, D, k.dtype, k.device)
+    return idx, kp, vp, ps, ts, hs, nb, bs, H, D
 
 
-def _int32(t: Any, what: str, dev: torch.device, shape: tuple) -> torch.Tensor:
-    """t, checked to be a contiguous int32 tensor of `shape` on dev."""
-    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32:
+def _int32(t: Any, what: str, idx: int, shape: tuple) -> int:
+    """The address of t, which has to be a contiguous int32 tensor of `shape` on
+    device idx."""
+    if (isinstance(t, torch.Tensor) and t.dtype is _I32 and t.get_device() == idx
+            and t.shape == shape and t.is_contiguous()):
+        return t.data_ptr()
+    if not isinstance(t, torch.Tensor) or t.dtype != _I32:
         raise TypeError(f"{what} must be an int32 tensor, got "
                         f"{getattr(t, 'dtype', type(t).__name__)}")
-    if t.device != dev:
-        raise ValueError(f"{what} is on {t.device}, the call's tensors on {dev}")
-    if tuple(t.shape) != shape or not t.is_contiguous():
-        raise ValueError(f"{what} must be contiguous {shape}, got {tuple(t.shape)}")
-    return t
+    if t.get_device() != idx:
+        raise ValueError(f"{what} is on {t.device}, the call's tensors on device {idx}")
+    raise ValueError(f"{what} must be contiguous {tuple(shape)}, got {tuple(t.shape)}")
 
 
-def _table(t: Any, dev: torch.device, seqs: Optional[int]) -> torch.Tensor:
-    """A block table: int32 [seqs, pages] on dev, rows contiguous."""
-    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32:
+def _table(t: Any, idx: int, seqs: Optional[int]) -> Tuple[int, int, int, int]:
+    """(address, row stride, sequences, pages of a row) of a block table: int32
+    [seqs, pages] on device idx, rows contiguous and apart."""
+    if not isinstance(t, torch.Tensor) or t.dtype is not _I32:
         raise TypeError(f"block_tables must be an int32 tensor, got "
                         f"{getattr(t, 'dtype', type(t).__name__)}")
-    if t.device != dev:
-        raise ValueError(f"block_tables is on {t.device}, the call's tensors on {dev}")
-    if t.dim() != 2 or (seqs is not None and t.shape[0] != seqs):
-        raise ValueError(f"block_tables {tuple(t.shape)} does not match {seqs} sequences")
-    if (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+    if t.get_device() != idx:
+        raise ValueError(f"block_tables is on {t.device}, the call's tensors on device {idx}")
+    shape = t.shape
+    if len(shape) != 2 or (seqs is not None and shape[0] != seqs):
+        raise ValueError(f"block_tables {tuple(shape)} does not match {seqs} sequences")
+    S, n = shape
+    row, one = t.stride()
+    if (n > 1 and one != 1) or (S > 1 and row < n):
         raise ValueError("block_tables rows must be contiguous and apart")
-    return t
+    return t.data_ptr(), row if row > n else n, S, n
 
 
-def _row_stride(t: torch.Tensor) -> int:
-    return max(t.stride(0), t.shape[1])
+def _flag(err_flag: Optional[torch.Tensor], idx: int) -> Optional[int]:
+    return None if err_flag is None else _int32(err_flag, "err_flag", idx, (1,))
 
 
-def _flag(err_flag: Optional[torch.Tensor], dev: torch.device) -> Optional[int]:
-    return None if err_flag is None else _int32(err_flag, "err_flag", dev, (1,)).data_ptr()
-
-
-def _query(q: Any, dev: torch.device, dim: int) -> torch.Tensor:
-    """q as [seqs, heads, dim] on dev with contiguous, 16-byte aligned heads (a
-    copy where they are not)."""
+def _query(q: Any, idx: int, dim: int) -> torch.Tensor:
+    """q as [seqs, heads, dim] on device idx with contiguous, 16-byte aligned
+    heads (a copy where they are not)."""
     if not isinstance(q, torch.Tensor):
         raise TypeError(f"q must be a tensor, got {type(q).__name__}")
     if q.dim() == 4:
@@ -150,8 +166,8 @@ def _query(q: Any, dev: torch.device, dim: int) -> torch.Tensor:
     if q.dim() != 3 or q.shape[2] != dim:
         raise ValueError(f"q must be [seqs, heads, {dim}] or [seqs, heads, 1, {dim}], got "
                          f"{tuple(q.shape)}")
-    if q.device != dev:
-        raise ValueError(f"q is on {q.device}, the cache on {dev}")
+    if q.get_device() != idx:
+        raise ValueError(f"q is on {q.device}, the call's tensors on device {idx}")
     if not q.is_contiguous():
         st, n = q.stride(), 16 // q.element_size()
         if st[2] != 1 or st[0] % n or st[1] % n or q.data_ptr() % 16:
@@ -183,52 +199,52 @@ def paged_decode_attention(q: torch.Tensor, k_cache: torch.Tensor,
     int32 [seqs, Hkv, n] with page_counts int32 [seqs, Hkv] limits each KV head
     to the listed places of the block table (select_pages makes them).  out:
     contiguous, q's shape; otherwise one of out_dtype (q's type)."""
-    c = _cache(k_cache, v_cache)
-    dev = c.device
-    q3 = _query(q, dev, c.dim)
-    S, Hq, D = q3.shape
-    if q3.dtype != c.dtype and not (c.dtype == torch.float8_e4m3fn and q3.dtype in _HALVES):
-        raise TypeError(f"paged decode: q is {q3.dtype}, the cache {c.dtype}")
-    if Hq == 0 or Hq % c.heads:
-        raise ValueError(f"{Hq} query heads is not a multiple of {c.heads} KV heads")
-    bt = _table(block_tables, dev, S)
-    cl = _int32(context_lens, "context_lens", dev, (S,))
-    if scale is not None and not scale > 0.0:
+    idx, kp, vp, ps, ts, hs, nb, bs, H, D = _cache(k_cache, v_cache)
+    q3 = _query(q, idx, D)
+    S, Hq, _ = q3.shape
+    kdt, qdt = k_cache.dtype, q3.dtype
+    if qdt is not kdt and not (kdt is torch.float8_e4m3fn and qdt in _HALVES):
+        raise TypeError(f"paged decode: q is {qdt}, the cache {kdt}")
+    if Hq == 0 or Hq % H:
+        raise ValueError(f"{Hq} query heads is not a multiple of {H} KV heads")
+    bt, row, _, width = _table(block_tables, idx, S)
+    cl = _int32(context_lens, "context_lens", idx, (S,))
+    if scale is None:
+        scale = 0.0
+    elif not scale > 0.0:
         raise ValueError(f"scale must be positive, got {scale}")
-    if (pages is None) != (page_counts is None):
-        raise ValueError("pages and page_counts come together")
+    pg = pc = None
     max_pages = 0
     if pages is not None:
+        if page_counts is None:
+            raise ValueError("pages and page_counts come together")
         if not isinstance(pages, torch.Tensor) or pages.dim() != 3:
             raise ValueError("pages must be an int32 tensor [seqs, KV heads, n]")
         max_pages = pages.shape[2]
-        _int32(pages, "pages", dev, (S, c.heads, max_pages))
-        _int32(page_counts, "page_counts", dev, (S, c.heads))
-    if max_context_len is None:
-        max_context_len = bt.shape[1] * c.block
+        pg = _int32(pages, "pages", idx, (S, H, max_pages))
+        pc = _int32(page_counts, "page_counts", idx, (S, H))
+    elif page_counts is not None:
+        raise ValueError("pages and page_counts come together")
+    most = width * bs if max_context_len is None else int(max_context_len)
+    dev = q.device
     if out is None:
-        out = torch.empty(q.shape, dtype=out_dtype or q3.dtype, device=dev)
+        out = torch.empty(q.shape, dtype=out_dtype or qdt, device=dev)
     else:
-        from .dispatch import _check_buffer
-
-        _check_buffer(out, "out", dev)
+        _dispatch._check_buffer(out, "out", dev)
         if out.shape != q.shape and tuple(out.shape) != (S, Hq, D):
             raise ValueError(f"paged decode: out has shape {tuple(out.shape)}, q {tuple(q.shape)}")
         if out_dtype is not None and out.dtype != out_dtype:
             raise ValueError(f"paged decode: out is {out.dtype}, out_dtype asks for {out_dtype}")
-    stream = amf_hip.stream_handle(dev)
-    ws, wsb = _workspace("amf_paged_decode_workspace_bytes", (Hq, c.heads, D), workspace, dev,
-                         stream)
-    qs = q3.stride()
-    amf_hip.call_on(
-        dev, "amf_paged_decode_attn", q3.data_ptr(), amf_hip.dtype_tag(q3.dtype), qs[0], qs[1],
-        out.data_ptr(), amf_hip.dtype_tag(out.dtype), c.k, c.v, _KV_TAGS[c.dtype], *c.strides,
-        c.pages, bt.data_ptr(), _row_stride(bt), bt.shape[1], cl.data_ptr(),
-        None if pages is None else pages.data_ptr(),
-        None if pages is None else page_counts.data_ptr(), max_pages, S, Hq, c.heads, D, c.block,
-        min(int(max_context_len), _I32_MAX), 0.0 if scale is None else float(scale),
-        float(k_scale), float(v_scale), None if ws is None else ws.data_ptr(), wsb,
-        _flag(err_flag, dev), stream)
+    if out.dtype not in _TAGS:
+        raise ValueError(f"paged decode: output dtype {out.dtype} is not bf16/fp16/fp32")
+    stream = _raw_stream(idx)
+    ws, wsb = _workspace("amf_paged_decode_workspace_bytes", (Hq, H, D), workspace, dev, stream)
+    qs, qh, _ = q3.stride()
+    _launch(
+        idx, "amf_paged_decode_attn", q3.data_ptr(), _TAGS[qdt], qs, qh, out.data_ptr(),
+        _TAGS[out.dtype], kp, vp, _KV_TAGS[kdt], ps, ts, hs, nb, bt, row, width, cl, pg, pc,
+        max_pages, S, Hq, H, D, bs, most if most < _I32_MAX else _I32_MAX, scale, k_scale, v_scale,
+        ws, wsb, _flag(err_flag, idx), stream)
     return out
 
 
@@ -247,38 +263,36 @@ def page_key_bounds(k_cache: torch.Tensor, block_tables: torch.Tensor,
     got more).  bounds [pages, Hkv, 2, D] of the cache's type (FP8: dtype, bf16
     by default) is updated in place, or made (zeros where nothing is written).
     Returns bounds."""
-    c = _cache(k_cache, None)
-    dev = c.device
-    if c.dtype not in _KV_TAGS or c.dtype == torch.float32 or c.dim % 8 or c.dim > 256:
+    idx, kp, _, ps, ts, hs, nb, bs, H, D = _cache(k_cache, None)
+    kdt = k_cache.dtype
+    if kdt is torch.float32 or D % 8 or D > 256:
         raise ValueError(f"page bounds need a bf16, fp16 or FP8 cache with head_dim a multiple of "
-                         f"8 up to 256, got {c.dtype}, {c.dim}")
-    bt = _table(block_tables, dev, None)
-    S = bt.shape[0]
-    cl = _int32(context_lens, "context_lens", dev, (S,))
-    ft = None
-    if first_tokens is not None:
-        ft = _int32(first_tokens, "first_tokens", dev, (S,)).data_ptr()
-    if max_new_tokens is not None and (max_new_tokens <= 0 or ft is None):
+                         f"8 up to 256, got {kdt}, {D}")
+    bt, row, S, width = _table(block_tables, idx, None)
+    cl = _int32(context_lens, "context_lens", idx, (S,))
+    ft = None if first_tokens is None else _int32(first_tokens, "first_tokens", idx, (S,))
+    if max_new_tokens is None:
+        max_new_tokens = 0
+    elif max_new_tokens <= 0 or ft is None:
         raise ValueError("max_new_tokens is positive and comes with first_tokens")
-    if c.dtype == torch.float8_e4m3fn:
+    if kdt is torch.float8_e4m3fn:
         bdt = dtype or (torch.bfloat16 if bounds is None else bounds.dtype)
     else:
-        bdt = dtype or c.dtype
-        if bdt != c.dtype:
-            raise ValueError(f"bounds of a {c.dtype} cache have its type, not {bdt}")
+        bdt = dtype or kdt
+        if bdt != kdt:
+            raise ValueError(f"bounds of a {kdt} cache have its type, not {bdt}")
     if bdt not in _HALVES:
         raise ValueError(f"page bounds are bf16 or fp16, not {bdt}")
-    shape = (c.pages, c.heads, 2, c.dim)
+    shape = (nb, H, 2, D)
     if bounds is None:
-        bounds = torch.zeros(shape, dtype=bdt, device=dev)
-    elif (not isinstance(bounds, torch.Tensor) or tuple(bounds.shape) != shape
-          or bounds.dtype != bdt or bounds.device != dev or not bounds.is_contiguous()):
-        raise ValueError(f"bounds must be contiguous {shape} of {bdt} on {dev}")
-    amf_hip.call_on(
-        dev, "amf_page_key_bounds", c.k, _KV_TAGS[c.dtype], *c.strides, c.pages, bt.data_ptr(),
-        _row_stride(bt), bt.shape[1], cl.data_ptr(), ft,
-        min(int(max_new_tokens or 0), _I32_MAX), S, c.heads, c.dim, c.block, bounds.data_ptr(),
-        amf_hip.dtype_tag(bdt), _flag(err_flag, dev), amf_hip.stream_handle(dev))
+        bounds = torch.zeros(shape, dtype=bdt, device=k_cache.device)
+    elif (not isinstance(bounds, torch.Tensor) or bounds.shape != shape or bounds.dtype != bdt
+          or bounds.get_device() != idx or not bounds.is_contiguous()):
+        raise ValueError(f"bounds must be contiguous {shape} of {bdt} on device {idx}")
+    _launch(
+        idx, "amf_page_key_bounds", kp, _KV_TAGS[kdt], ps, ts, hs, nb, bt, row, width, cl, ft,
+        min(int(max_new_tokens), _I32_MAX), S, H, D, bs, bounds.data_ptr(), _TAGS[bdt],
+        _flag(err_flag, idx), _raw_stream(idx))
     return bounds
 
 
@@ -302,45 +316,47 @@ def select_pages(q: torch.Tensor, bounds: torch.Tensor, block_tables: torch.Tens
     workspace."""
     if not isinstance(bounds, torch.Tensor) or bounds.dim() != 4 or bounds.shape[2] != 2:
         raise ValueError("bounds must be [pages, KV heads, 2, head_dim]")
-    amf_hip.require_device_tensor(bounds, "page bounds")
-    if bounds.dtype not in _HALVES or not bounds.is_contiguous():
-        raise ValueError(f"bounds must be contiguous bf16 or fp16, got {bounds.dtype}")
-    dev = bounds.device
+    idx = bounds.get_device()
+    if idx < 0:
+        amf_hip.require_device_tensor(bounds, "page bounds")
+    dt = bounds.dtype
+    if dt not in _HALVES or not bounds.is_contiguous():
+        raise ValueError(f"bounds must be contiguous bf16 or fp16, got {dt}")
     nb, H, _, D = bounds.shape
-    q3 = _query(q, dev, D)
+    q3 = _query(q, idx, D)
     S, Hq, _ = q3.shape
-    if q3.dtype != bounds.dtype:
-        raise TypeError(f"select_pages: q is {q3.dtype}, the bounds {bounds.dtype}")
+    if q3.dtype is not dt:
+        raise TypeError(f"select_pages: q is {q3.dtype}, the bounds {dt}")
     if Hq == 0 or Hq % H:
         raise ValueError(f"{Hq} query heads is not a multiple of {H} KV heads")
-    bt = _table(block_tables, dev, S)
-    cl = _int32(context_lens, "context_lens", dev, (S,))
+    bt, row, _, width = _table(block_tables, idx, S)
+    cl = _int32(context_lens, "context_lens", idx, (S,))
     if num_pages <= 0 or first_pages < 0 or last_pages < 0 or first_pages + last_pages > num_pages:
         raise ValueError(f"num_pages {num_pages} has to hold first_pages {first_pages} and "
                          f"last_pages {last_pages}")
     if block_size <= 0:
         raise ValueError(f"block_size must be positive, got {block_size}")
-    if max_context_len is None:
-        max_context_len = bt.shape[1] * block_size
-    elif max_context_len < 0:
+    most = width * block_size if max_context_len is None else int(max_context_len)
+    if most < 0:
         raise ValueError(f"max_context_len must not be negative, got {max_context_len}")
-    max_context_len = min(int(max_context_len), _I32_MAX)
+    most = min(most, _I32_MAX)
+    dev = bounds.device
     if out is None:
-        pages = torch.empty((S, H, num_pages), dtype=torch.int32, device=dev)
-        counts = torch.empty((S, H), dtype=torch.int32, device=dev)
+        pages = torch.empty((S, H, num_pages), dtype=_I32, device=dev)
+        counts = torch.empty((S, H), dtype=_I32, device=dev)
+        pg, pc = pages.data_ptr(), counts.data_ptr()
     else:
-        pages = _int32(out[0], "pages", dev, (S, H, num_pages))
-        counts = _int32(out[1], "page counts", dev, (S, H))
-    stream = amf_hip.stream_handle(dev)
-    ws, wsb = _workspace("amf_select_pages_workspace_bytes",
-                         (S, H, bt.shape[1], block_size, max_context_len), workspace, dev, stream)
-    qs = q3.stride()
-    amf_hip.call_on(
-        dev, "amf_select_pages", q3.data_ptr(), amf_hip.dtype_tag(q3.dtype), qs[0], qs[1],
-        bounds.data_ptr(), nb, bt.data_ptr(), _row_stride(bt), bt.shape[1], cl.data_ptr(),
-        max_context_len, S, Hq, H, D, block_size, num_pages, first_pages, last_pages,
-        pages.data_ptr(), counts.data_ptr(), None if ws is None else ws.data_ptr(), wsb,
-        _flag(err_flag, dev), stream)
+        pages, counts = out
+        pg = _int32(pages, "pages", idx, (S, H, num_pages))
+        pc = _int32(counts, "page counts", idx, (S, H))
+    stream = _raw_stream(idx)
+    ws, wsb = _workspace("amf_select_pages_workspace_bytes", (S, H, width, block_size, most),
+                         workspace, dev, stream)
+    qs, qh, _ = q3.stride()
+    _launch(
+        idx, "amf_select_pages", q3.data_ptr(), _TAGS[dt], qs, qh, bounds.data_ptr(), nb, bt, row,
+        width, cl, most, S, Hq, H, D, block_size, num_pages, first_pages, last_pages, pg, pc, ws,
+        wsb, _flag(err_flag, idx), stream)
     return pages, counts
 
 
@@ -376,48 +392,50 @@ def build_slot_maps(context_lens: torch.Tensor, new_tokens: torch.Tensor,
     err_flag), as do page ids outside [0, pool_pages)."""
     if not isinstance(block_tables, torch.Tensor):
         raise TypeError("block_tables must be an int32 tensor")
-    amf_hip.require_device_tensor(block_tables, "block_tables")
-    dev = block_tables.device
-    bt = _table(block_tables, dev, None)
-    S = bt.shape[0]
-    cl = _int32(context_lens, "context_lens", dev, (S,))
-    nt = _int32(new_tokens, "new_tokens", dev, (S,))
+    idx = block_tables.get_device()
+    if idx < 0:
+        amf_hip.require_device_tensor(block_tables, "block_tables")
+    bt, row, S, width = _table(block_tables, idx, None)
+    cl = _int32(context_lens, "context_lens", idx, (S,))
+    nt = _int32(new_tokens, "new_tokens", idx, (S,))
     if block_size <= 0 or num_tokens < 0:
         raise ValueError(f"bad block_size {block_size} or num_tokens {num_tokens}")
-    if pool_pages is not None and pool_pages <= 0:
+    if pool_pages is None:
+        pool_pages = _I32_MAX
+    elif pool_pages <= 0:
         raise ValueError(f"pool_pages must be positive, got {pool_pages}")
-    n_free = 0
+    n_free, fp = 0, None
     if free_pages is not None:
         if not isinstance(free_pages, torch.Tensor) or free_pages.dim() != 1:
             raise ValueError("free_pages must be an int32 tensor [n]")
         n_free = free_pages.shape[0]
-        _int32(free_pages, "free_pages", dev, (n_free,))
-    if free_used is not None:
-        _int32(free_used, "free_used", dev, (1,))
+        fp = _int32(free_pages, "free_pages", idx, (n_free,))
+    fu = None if free_used is None else _int32(free_used, "free_used", idx, (1,))
     if out is None:
-        wide = torch.empty((2, num_tokens), dtype=torch.int64, device=dev)
-        out = SlotMaps(wide[0], wide[1], torch.empty(S + 1, dtype=torch.int32, device=dev),
-                       torch.empty(S, dtype=torch.int32, device=dev),
-                       torch.empty(1, dtype=torch.int32, device=dev))
+        dev = block_tables.device
+        slots, pos = torch.empty((2, num_tokens), dtype=torch.int64, device=dev).unbind(0)
+        start, lens, used = torch.empty(2 * S + 2, dtype=_I32, device=dev).split_with_sizes(
+            (S + 1, S, 1))
+        out = SlotMaps(slots, pos, start, lens, used)
+        ptrs = (slots.data_ptr(), pos.data_ptr(), start.data_ptr(), lens.data_ptr(),
+                used.data_ptr())
     else:
         for t, name in ((out.slot_mapping, "slot_mapping"), (out.positions, "positions")):
-            if (t.dtype != torch.int64 or t.device != dev or tuple(t.shape) != (num_tokens,)
+            if (t.dtype != torch.int64 or t.get_device() != idx or t.shape != (num_tokens,)
                     or not t.is_contiguous()):
-                raise ValueError(f"out.{name} must be contiguous int64 ({num_tokens},) on {dev}")
-        _int32(out.query_start, "out.query_start", dev, (S + 1,))
-        _int32(out.context_lens, "out.context_lens", dev, (S,))
-        _int32(out.free_used, "out.free_used", dev, (1,))
-        for t, name in ((cl, "context_lens"), (nt, "new_tokens"), (free_used, "free_used")):
-            if t is not None and any(t.numel() and t.data_ptr() == o.data_ptr() for o in out):
+                raise ValueError(f"out.{name} must be contiguous int64 ({num_tokens},) on "
+                                 f"device {idx}")
+        ptrs = (out.slot_mapping.data_ptr(), out.positions.data_ptr(),
+                _int32(out.query_start, "out.query_start", idx, (S + 1,)),
+                _int32(out.context_lens, "out.context_lens", idx, (S,)),
+                _int32(out.free_used, "out.free_used", idx, (1,)))
+        for p, name in ((cl, "context_lens"), (nt, "new_tokens"), (fu, "free_used")):
+            if p and p in ptrs:
                 raise ValueError(f"{name} must not be one of the outputs")
-    amf_hip.call_on(
-        dev, "amf_build_slot_maps", cl.data_ptr(), nt.data_ptr(), S, bt.data_ptr(),
-        _row_stride(bt), bt.shape[1], block_size, _I32_MAX if pool_pages is None else pool_pages,
-        free_pages.data_ptr() if n_free else None, n_free,
-        None if free_used is None else free_used.data_ptr(), num_tokens,
-        out.slot_mapping.data_ptr(), out.positions.data_ptr(), out.query_start.data_ptr(),
-        out.context_lens.data_ptr(), out.free_used.data_ptr(), _flag(err_flag, dev),
-        amf_hip.stream_handle(dev))
+    _launch(
+        idx, "amf_build_slot_maps", cl, nt, S, bt, row, width, block_size, pool_pages,
+        fp if n_free else None, n_free, fu, num_tokens, *ptrs, _flag(err_flag, idx),
+        _raw_stream(idx))
     return out
 
 
@@ -428,3 +446,5 @@ __all__ = [
     "paged_decode_attention",
     "select_pages",
 ]
+
+from . import dispatch as _dispatch  # noqa: E402  (it imports this module's attention)
