@@ -9,14 +9,15 @@
 // for its KV head.  Each K and V element is read once, for all query heads that
 // share it, and meets the running maximum m and sum l of each head's softmax.
 //
-// Work.  Steps of NW waves x 32 tokens; the steps of all (sequence, KV head,
-// head tile) pairs, sequence-major, are cut into equal shares, one per
-// workgroup of a grid that is resident as a whole, so every workgroup reads
-// about the same number of tokens whatever the mix of context lengths.  A
-// workgroup finds its share by summing the lengths itself (they are on the
-// device), its waves take 32 tokens of a step each and are joined in LDS.  A
-// pair inside one share is finished there; one that several
-// share leaves a partial (acc, m, l) per workgroup, and a second launch joins
+// Work.  Steps of 4 waves x 32 or 64 tokens; the steps of all sequences, one
+// after the other, are cut into equal shares, and each share is taken by as many
+// workgroups as there are (KV head, head tile) pairs, side by side: they read the
+// same pages at the same time, and the grid is resident as a whole, so every
+// workgroup reads about the same number of tokens whatever the mix of context
+// lengths.  A workgroup finds its share by summing the lengths itself (they are
+// on the device), its waves take a quarter of a step each and are joined in LDS.
+// What of a sequence lies inside one share is finished there; where several share
+// it, each workgroup leaves a partial (acc, m, l), and a second launch joins
 // those.
 #include <algorithm>
 
@@ -31,10 +32,8 @@ namespace {
 
 using namespace amf;
 
-constexpr int kChunk = 32;  // tokens of a wave's step
 constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
-constexpr int kStep = kWaves * kChunk;
 constexpr int kMaxDim = 256;
 
 struct PagedArgs {
@@ -54,6 +53,7 @@ struct PagedArgs {
   int32_t max_pages;
   int32_t num_seqs, num_q_heads, num_kv_heads, head_dim, block_size;
   int32_t block_shift;  // log2(block_size), or -1
+  int32_t step_shift;   // log2 of the tokens of a step (of all waves)
   int32_t group;        // query heads of a KV head
   int32_t tiles;        // head tiles of a group
   int32_t out_dtype;
@@ -67,11 +67,12 @@ struct PagedArgs {
 };
 
 // The pair that begins in a workgroup's share and does not end there: its
-// partials are slot `slot` of this workgroup and slot 0 of the next, to `last`.
+// partials are slot `slot` of this workgroup and slot 0 of the `more` next
+// shares' workgroups of that (KV head, head tile).
 struct Cut {
   int32_t heads;  // 0: no such pair
   int32_t head0;  // of the step's rows
-  int32_t last;
+  int32_t more;
   int32_t slot;
 };
 
@@ -92,67 +93,70 @@ __device__ __forceinline__ int64_t seq_tokens(const PagedArgs& a, int s) {
 }
 
 __device__ __forceinline__ int64_t seq_steps(const PagedArgs& a, int s) {
-  return (seq_tokens(a, s) + kStep - 1) / kStep;
+  return (seq_tokens(a, s) + (1 << a.step_shift) - 1) >> a.step_shift;
 }
 
-// Where a unit (a step of a pair) lies.
+// The step at which a workgroup's share begins, counted over the sequences.
 struct Unit {
-  int64_t total;  // units of the launch
-  int64_t share;  // units of a workgroup
-  int seq;
-  int64_t start;  // first unit of that sequence
-  int64_t steps;  // of each of its pairs
+  int64_t total;  // steps of the launch
+  int64_t share;  // steps of a workgroup
+  int64_t first;  // of this workgroup
+  int seq;        // the sequence it lies in, -1: there is none
+  int64_t start;  // first step of that sequence
+  int64_t steps;  // its steps
 };
 
-// The place of the workgroup's first unit, the same in every thread; seq is -1
-// where it has none.
+__device__ __forceinline__ int pairs_of(const PagedArgs& a) { return a.num_kv_heads * a.tiles; }
+
+// The same in every thread.
 __device__ __forceinline__ Unit find_unit(const PagedArgs& a) {
-  const int64_t groups = gridDim.x;
   __shared__ int64_t tmp[kWaves];
-  __shared__ Unit found;
-  const int64_t pairs = (int64_t)a.num_kv_heads * a.tiles;
+  __shared__ int found_seq;
+  __shared__ int64_t found_start, found_steps;
+  const int pairs = pairs_of(a);
+  const int64_t shares = gridDim.x / pairs, mine = blockIdx.x / pairs;
   const int tid = threadIdx.x;
   Unit r{};
   if (a.whole) {
-    r.seq = (int)(blockIdx.x / pairs);
-    r.steps = r.share = seq_steps(a, r.seq);
-    r.start = (int64_t)blockIdx.x * r.steps - blockIdx.x % pairs * r.steps;
-    r.total = r.start + pairs * r.steps;
+    r.seq = (int)mine;
+    r.total = r.share = r.steps = seq_steps(a, r.seq);
     if (r.steps == 0) r.seq = -1;
     return r;
   }
   int64_t steps = 0, before = 0;
   if (a.num_seqs <= kThreads) {  // one scan gives the total and the places
     if (tid < a.num_seqs) steps = seq_steps(a, tid);
-    before = block_exclusive<kThreads>(steps * pairs, tmp, &r.total);
+    before = block_exclusive<kThreads>(steps, tmp, &r.total);
   } else {
-    int64_t mine = 0;
-    for (int s = tid; s < a.num_seqs; s += kThreads) mine += seq_steps(a, s) * pairs;
-    block_exclusive<kThreads>(mine, tmp, &r.total);
+    int64_t sum = 0;
+    for (int s = tid; s < a.num_seqs; s += kThreads) sum += seq_steps(a, s);
+    block_exclusive<kThreads>(sum, tmp, &r.total);
   }
-  r.share = (r.total + groups - 1) / groups;
-  const int64_t u = blockIdx.x * r.share;
-  if (u >= r.total) {
+  r.share = (r.total + shares - 1) / shares;
+  r.first = mine * r.share;
+  if (r.first >= r.total) {
     r.seq = -1;
     return r;
   }
-  if (a.num_seqs <= kThreads) {
-    if (before <= u && u < before + steps * pairs) found = Unit{r.total, r.share, tid, before, steps};
-    __syncthreads();
-    return found;
-  }
   int64_t base = 0;
   for (int s0 = 0;; s0 += kThreads) {
-    const int s = s0 + tid;
-    int64_t all;
-    steps = s < a.num_seqs ? seq_steps(a, s) : 0;
-    before = base + block_exclusive<kThreads>(steps * pairs, tmp, &all);
-    if (u < base + all) {  // uniform; u < total, so this comes
-      if (before <= u && u < before + steps * pairs) found = Unit{r.total, r.share, s, before, steps};
-      __syncthreads();
-      return found;
+    if (a.num_seqs > kThreads) {
+      int64_t all;
+      steps = s0 + tid < a.num_seqs ? seq_steps(a, s0 + tid) : 0;
+      before = base + block_exclusive<kThreads>(steps, tmp, &all);
+      base += all;
+      if (r.first >= base) continue;  // uniform; first < total, so this ends
     }
-    base += all;
+    if (before <= r.first && r.first < before + steps) {
+      found_seq = s0 + tid;
+      found_start = before;
+      found_steps = steps;
+    }
+    __syncthreads();
+    r.seq = found_seq;
+    r.start = found_start;
+    r.steps = found_steps;
+    return r;
   }
 }
 
@@ -168,32 +172,33 @@ struct Segment {
   float* part;       // where the partial goes otherwise
 };
 
-// Walks a share, u in [u0, u1), pair by pair.
+// The segment from step u of sequence un.seq on; the share ends at u1.
 template <int TILE>
 __device__ __forceinline__ Segment segment_at(const PagedArgs& a, const Unit& un, int64_t u,
-                                              int64_t u0, int64_t u1) {
+                                              int64_t u1) {
   Segment g;
-  const int64_t pair = (u - un.start) / un.steps;
-  g.st0 = (u - un.start) - pair * un.steps;
+  const int pairs = pairs_of(a), pair = blockIdx.x % pairs;
+  g.st0 = u - un.start;
   g.st1 = min(un.steps, g.st0 + (u1 - u));
   g.seq = un.seq;
-  g.hkv = (int)(pair / a.tiles);
-  const int tile = (int)(pair - (int64_t)g.hkv * a.tiles);
+  g.hkv = pair / a.tiles;
+  const int tile = pair - g.hkv * a.tiles;
   g.heads = min(TILE, a.group - tile * TILE);
   g.head0 = (int64_t)un.seq * a.num_q_heads + g.hkv * a.group + tile * TILE;
   g.ctx = a.context_lens[un.seq];
   g.whole = g.st0 == 0 && g.st1 == un.steps;
-  g.part = a.part + (2 * (int64_t)blockIdx.x + (u != u0)) * a.part_stride;
+  g.part = a.part + (2 * (int64_t)blockIdx.x + (u != un.first)) * a.part_stride;
   if (!g.whole && g.st0 == 0 && threadIdx.x == 0)
-    a.cuts[blockIdx.x] = Cut{g.heads, (int32_t)g.head0, (int32_t)((u + un.steps - 1) / un.share),
-                             u != u0};
+    a.cuts[blockIdx.x] = Cut{g.heads, (int32_t)g.head0,
+                             (int32_t)((u + un.steps - 1) / un.share - blockIdx.x / pairs),
+                             u != un.first};
   return g;
 }
 
-// Moves on to unit u, perhaps of the next sequence with tokens; u lies in the
+// Moves on to step u, perhaps of the next sequence with tokens; u lies in the
 // launch.
 __device__ __forceinline__ void advance(const PagedArgs& a, Unit& un, int64_t u) {
-  if (u < un.start + (int64_t)a.num_kv_heads * a.tiles * un.steps) return;
+  if (u < un.start + un.steps) return;
   un.start = u;
   do {
     ++un.seq;
@@ -211,7 +216,7 @@ struct PageRun {
 
 // Steps that a run holds: kPageSlots pages, one of them begun before the run.
 __device__ __forceinline__ int64_t run_steps(const PagedArgs& a) {
-  return max((int64_t)1, (int64_t)(kPageSlots - 1) * a.block_size / kStep);
+  return max((int64_t)1, (int64_t)(kPageSlots - 1) * a.block_size >> a.step_shift);
 }
 
 __device__ __forceinline__ int64_t page_of(const PagedArgs& a, int64_t t) {
@@ -221,7 +226,8 @@ __device__ __forceinline__ int64_t page_of(const PagedArgs& a, int64_t t) {
 __device__ __forceinline__ void load_pages(const PagedArgs& a, const Segment& g, int64_t st0,
                                            int64_t st1, PageRun& run) {
   __syncthreads();  // the last run has been read
-  const int64_t j0 = page_of(a, st0 * kStep), j1 = page_of(a, st1 * kStep - 1);
+  const int64_t j0 = page_of(a, st0 << a.step_shift);
+  const int64_t j1 = page_of(a, (st1 << a.step_shift) - 1);
   const int64_t row = (int64_t)g.seq * a.num_kv_heads + g.hkv;
   const int64_t count = a.pages ? min(a.page_counts[row], a.max_pages) : a.table_pages;
   for (int64_t j = j0 + threadIdx.x; j <= j1; j += kThreads) {
@@ -294,6 +300,7 @@ __device__ __forceinline__ void empty_seqs(const PagedArgs& a) {
 // A lane scores one token of the chunk (two lanes share its dims) and, for PV,
 // owns dims lane, lane + 64, ...
 constexpr int kGenHeads = 4;  // query heads of a tile
+constexpr int kChunk = 32;     // tokens of a wave's step
 
 template <int QDT, int KDT>
 __global__ __launch_bounds__(kThreads) void paged_attn_general_kernel(PagedArgs a) {
@@ -312,10 +319,10 @@ __global__ __launch_bounds__(kThreads) void paged_attn_general_kernel(PagedArgs 
   Unit un = find_unit(a);
   if (!a.whole && tid == 0) a.cuts[blockIdx.x].heads = 0;
   if (un.seq < 0) return;
-  const int64_t u0 = blockIdx.x * un.share, u1 = min(u0 + un.share, un.total);
-  for (int64_t u = u0; u < u1;) {
+  const int64_t u1 = min(un.first + un.share, un.total);
+  for (int64_t u = un.first; u < u1;) {
     advance(a, un, u);
-    const Segment sg = segment_at<kGenHeads>(a, un, u, u0, u1);
+    const Segment sg = segment_at<kGenHeads>(a, un, u, u1);
     u += sg.st1 - sg.st0;
     for (int i = tid; i < kGenHeads * D; i += kThreads) {
       const int g = i / D, d = i - g * D;
@@ -334,11 +341,11 @@ __global__ __launch_bounds__(kThreads) void paged_attn_general_kernel(PagedArgs 
     }
     const int64_t hold = run_steps(a);
     for (int64_t r0 = sg.st0; r0 < sg.st1; r0 += hold) {
-      const int64_t r1 = min(r0 + hold, sg.st1), j0 = page_of(a, r0 * kStep);
+      const int64_t r1 = min(r0 + hold, sg.st1), j0 = page_of(a, r0 << a.step_shift);
       load_pages(a, sg, r0, r1, run);
       for (int64_t st = r0; st < r1; ++st) {
         const int64_t off =
-            token_offset(a, sg, run, j0, st * kStep + wave * kChunk + (lane & 31));
+            token_offset(a, sg, run, j0, (st << a.step_shift) + wave * kChunk + (lane & 31));
         const bool ok = off >= 0;
         if (!__any(ok)) continue;
         float x[kGenHeads];
@@ -424,7 +431,7 @@ __global__ __launch_bounds__(kThreads) void paged_attn_general_kernel(PagedArgs 
 // ---- matrix kernel -------------------------------------------------------------
 //
 // bf16 and fp16 queries, head_dim 64, 128 or 256, rows of whole 16-byte vectors.
-// A wave takes 32 tokens and up to 16 query heads on 16x16x32 tiles; lane
+// A wave takes blocks of 32 tokens and up to 16 query heads on 16x16x32 tiles; lane
 // (lo, hi) = (lane % 16, lane / 16).
 //
 //   scores   S^T = K Q^T: K rows as the A operand straight from memory (16 bytes
@@ -467,12 +474,16 @@ __device__ __forceinline__ uint32_t e4m3_pair(uint32_t w) {
 
 constexpr int kTileHeads = 16;
 constexpr int matrix_waves(int D) { return D == 256 ? 1 : 2; }  // per SIMD, at least
+// Tokens of a wave's step: 64 where their K and V are at most 16 KB, the bytes
+// that a wave keeps in flight.
+constexpr int matrix_chunk(int D, int es) { return D * es <= 128 ? 64 : 32; }
 
 template <int QDT, int KDT, int D>
 __global__ __launch_bounds__(kThreads, matrix_waves(D)) void paged_attn_matrix_kernel(PagedArgs a) {
   constexpr bool FP8 = KDT == AMF_DTYPE_E4M3;
   constexpr bool V16 = KDT == AMF_DTYPE_F16;  // V in two terms
   constexpr int ES = FP8 ? 1 : 2;
+  constexpr int CH = matrix_chunk(D, ES), NB = CH / 32;
   constexpr int KS = D / 32;          // k steps of a score tile
   constexpr int KL = KS * ES / 2;     // 16-byte loads of a K row per lane
   constexpr int DP = D / 16;          // dims of a V row per lane
@@ -487,10 +498,10 @@ __global__ __launch_bounds__(kThreads, matrix_waves(D)) void paged_attn_matrix_k
   Unit un = find_unit(a);
   if (!a.whole && tid == 0) a.cuts[blockIdx.x].heads = 0;
   if (un.seq < 0) return;
-  const int64_t u0 = blockIdx.x * un.share, u1 = min(u0 + un.share, un.total);
-  for (int64_t u = u0; u < u1;) {
+  const int64_t u1 = min(un.first + un.share, un.total);
+  for (int64_t u = un.first; u < u1;) {
     advance(a, un, u);
-    const Segment sg = segment_at<kTileHeads>(a, un, u, u0, u1);
+    const Segment sg = segment_at<kTileHeads>(a, un, u, u1);
     u += sg.st1 - sg.st0;
     // q of head lo, dims 32 ks + 8 hi .. (FP8: the dims of the K bytes that the
     // lane loads, 64 j + 16 hi .., two k steps)
@@ -509,23 +520,22 @@ __global__ __launch_bounds__(kThreads, matrix_waves(D)) void paged_attn_matrix_k
     f32x4 acc[DP];
 #pragma unroll
     for (int j = 0; j < DP; ++j) acc[j] = f32x4{0, 0, 0, 0};
-    u32x4 kr[2][KL];
-    uint32_t vr[8][VW];
+    u32x4 kr[2 * NB][KL];
+    uint32_t vr[8 * NB][VW];
     const int64_t head_off = sg.hkv * a.head_stride;
     // rows of K: tokens 16 i + lo; tokens that do not count read page 0
     auto load_k = [&](int64_t off) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < 2 * NB; ++i) {
         const int64_t o = __shfl(off, 16 * i + lo);
         const uint8_t* p = a.k + (o < 0 ? head_off : o) + 16 * hi;
 #pragma unroll
-        for (int n = 0; n < KL; ++n)
-          kr[i][n] = ld_stream(reinterpret_cast<const u32x4*>(p + 64 * n));
+        for (int n = 0; n < KL; ++n) kr[i][n] = *reinterpret_cast<const u32x4*>(p + 64 * n);
       }
     };
     auto load_v = [&](int64_t off) {
 #pragma unroll
-      for (int r = 0; r < 8; ++r) {
+      for (int r = 0; r < 8 * NB; ++r) {
         const int64_t o = __shfl(off, 16 * (r / 4) + 4 * hi + r % 4);
         const uint8_t* p = a.v + (o < 0 ? head_off : o) + DP * ES * lo;
         if constexpr (VW >= 4) {
@@ -546,11 +556,11 @@ __global__ __launch_bounds__(kThreads, matrix_waves(D)) void paged_attn_matrix_k
     };
     const int64_t hold = run_steps(a);
     for (int64_t r0 = sg.st0; r0 < sg.st1; r0 += hold) {
-      const int64_t r1 = min(r0 + hold, sg.st1), j0 = page_of(a, r0 * kStep);
+      const int64_t r1 = min(r0 + hold, sg.st1), j0 = page_of(a, r0 << a.step_shift);
       load_pages(a, sg, r0, r1, run);
-      const int64_t t = wave * kChunk + (lane & 31);
-      int64_t off = token_offset(a, sg, run, j0, r0 * kStep + t);
-      uint32_t seen = (uint32_t)__ballot(off >= 0);
+      const int64_t t = wave * CH + (lane & (CH - 1));
+      int64_t off = token_offset(a, sg, run, j0, (r0 << a.step_shift) + t);
+      uint64_t seen = __ballot(off >= 0);
       if (seen) {
         load_k(off);
         load_v(off);
@@ -558,12 +568,12 @@ __global__ __launch_bounds__(kThreads, matrix_waves(D)) void paged_attn_matrix_k
       for (int64_t st = r0; st < r1; ++st) {
         // the next step's rows
         int64_t next = -1;
-        if (st + 1 < r1) next = token_offset(a, sg, run, j0, (st + 1) * kStep + t);
-        const uint32_t seen_next = (uint32_t)__ballot(next >= 0);
-        f32x4 s[2];
+        if (st + 1 < r1) next = token_offset(a, sg, run, j0, ((st + 1) << a.step_shift) + t);
+        const uint64_t seen_next = __ballot(next >= 0);
+        f32x4 s[2 * NB];
         if (seen) {
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
+          for (int i = 0; i < 2 * NB; ++i) {
             s[i] = f32x4{0, 0, 0, 0};
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
@@ -581,15 +591,19 @@ __global__ __launch_bounds__(kThreads, matrix_waves(D)) void paged_attn_matrix_k
         }
         if (seen_next) load_k(next);
         if (seen) {
-          const uint32_t mine = seen >> (4 * hi);  // bits r and 16 + r: this lane's tokens
-          const bool full = seen == 0xFFFFFFFFu;
-          float x[8], p[8], top = -INFINITY;
+          const bool full = seen == ~0ull;
+          // whether this lane's token r of block b counts
+          auto counts = [&](int b, int r) {
+            return full || ((uint32_t)(seen >> (32 * b)) >> (4 * hi) >> (16 * (r / 4) + r % 4) & 1);
+          };
+          float x[NB][8], p[NB][8], top = -INFINITY;
 #pragma unroll
-          for (int r = 0; r < 8; ++r) {
-            x[r] = s[r / 4][r % 4];
-            const float y = x[r] * a.score_scale;
-            top = max_nan(top, full || (mine >> (16 * (r / 4) + r % 4) & 1) ? y : -INFINITY);
-          }
+          for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int r = 0; r < 8; ++r) {
+              x[b][r] = s[2 * b + r / 4][r % 4];
+              top = max_nan(top, counts(b, r) ? x[b][r] * a.score_scale : -INFINITY);
+            }
           top = max_nan(top, __shfl_xor(top, 16));
           top = max_nan(top, __shfl_xor(top, 32));
           const float mn = max_nan(m, top);
@@ -597,63 +611,68 @@ __global__ __launch_bounds__(kThreads, matrix_waves(D)) void paged_attn_matrix_k
           m = mn;
           float sum = 0.0f;
 #pragma unroll
-          for (int r = 0; r < 8; ++r) {
-            p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r], a.score_scale, -mn));
-            if (!full && !(mine >> (16 * (r / 4) + r % 4) & 1)) p[r] = 0.0f;
-            sum += p[r];
-          }
+          for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int r = 0; r < 8; ++r) {
+              p[b][r] = counts(b, r) ? __builtin_amdgcn_exp2f(
+                                           __builtin_fmaf(x[b][r], a.score_scale, -mn))
+                                     : 0.0f;
+              sum += p[b][r];
+            }
           l = l * w + sum;
           if (__any(w != 1.0f)) {
 #pragma unroll
             for (int j = 0; j < DP; ++j) acc[j] *= w;
           }
-          uint32_t pb[kTerms][4];
 #pragma unroll
-          for (int n = 0; n < 4; ++n) {
-            uint32_t t3[kTerms];
-            weight_split(p[2 * n], p[2 * n + 1], t3);
+          for (int b = 0; b < NB; ++b) {
+            u32x4 pb[kTerms];
 #pragma unroll
-            for (int k = 0; k < kTerms; ++k) pb[k][n] = t3[k];
-          }
-          if (!full) {  // V rows that do not count: zeros, not what page 0 holds
+            for (int n = 0; n < 4; ++n) {
+              uint32_t t3[kTerms];
+              weight_split(p[b][2 * n], p[b][2 * n + 1], t3);
 #pragma unroll
-            for (int r = 0; r < 8; ++r)
-              if (!(mine >> (16 * (r / 4) + r % 4) & 1)) {
+              for (int k = 0; k < kTerms; ++k) pb[k][n] = t3[k];
+            }
+            if (!full) {  // V rows that do not count: zeros, not what page 0 holds
 #pragma unroll
-                for (int n = 0; n < VW; ++n) vr[r][n] = 0;
-              }
-          }
+              for (int r = 0; r < 8; ++r)
+                if (!counts(b, r)) {
 #pragma unroll
-          for (int j = 0; j < DP; j += 2) {  // dims j and j + 1 of each lane's piece
-            uint32_t v2[8];
-#pragma unroll
-            for (int r = 0; r < 8; ++r) {
-              if constexpr (FP8)
-                v2[r] = j % 4 ? e4m3_pair<AMF_DTYPE_BF16, true>(vr[r][j / 4])
-                              : e4m3_pair<AMF_DTYPE_BF16, false>(vr[r][j / 4]);
-              else
-                v2[r] = vr[r][j / 2];
+                  for (int n = 0; n < VW; ++n) vr[8 * b + r][n] = 0;
+                }
             }
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              u32x4 va, vl;
+            for (int j = 0; j < DP; j += 2) {  // dims j and j + 1 of each lane's piece
+              uint32_t v2[8];
 #pragma unroll
-              for (int n = 0; n < 4; ++n) {
-                va[n] = __builtin_amdgcn_perm(v2[2 * n + 1], v2[2 * n],
-                                              e ? 0x07060302u : 0x05040100u);
-                if constexpr (V16) {
-                  uint32_t h2, l2;
-                  v_split(va[n], h2, l2);
-                  va[n] = h2;
-                  vl[n] = l2;
-                }
+              for (int r = 0; r < 8; ++r) {
+                if constexpr (FP8)
+                  v2[r] = j % 4 ? e4m3_pair<AMF_DTYPE_BF16, true>(vr[8 * b + r][j / 4])
+                                : e4m3_pair<AMF_DTYPE_BF16, false>(vr[8 * b + r][j / 4]);
+                else
+                  v2[r] = vr[8 * b + r][j / 2];
               }
 #pragma unroll
-              for (int k = 0; k < kTerms; ++k) {
-                const u32x4 pk{pb[k][0], pb[k][1], pb[k][2], pb[k][3]};
-                acc[j + e] = mfma16<AMF_DTYPE_BF16>(va, pk, acc[j + e]);
-                if constexpr (V16) {
-                  if (k < 2) acc[j + e] = mfma16<AMF_DTYPE_BF16>(vl, pk, acc[j + e]);
+              for (int e = 0; e < 2; ++e) {
+                u32x4 va, vl;
+#pragma unroll
+                for (int n = 0; n < 4; ++n) {
+                  va[n] = __builtin_amdgcn_perm(v2[2 * n + 1], v2[2 * n],
+                                                e ? 0x07060302u : 0x05040100u);
+                  if constexpr (V16) {
+                    uint32_t h2, l2;
+                    v_split(va[n], h2, l2);
+                    va[n] = h2;
+                    vl[n] = l2;
+                  }
+                }
+#pragma unroll
+                for (int k = 0; k < kTerms; ++k) {
+                  acc[j + e] = mfma16<AMF_DTYPE_BF16>(va, pb[k], acc[j + e]);
+                  if constexpr (V16) {
+                    if (k < 2) acc[j + e] = mfma16<AMF_DTYPE_BF16>(vl, pb[k], acc[j + e]);
+                  }
                 }
               }
             }
@@ -731,18 +750,20 @@ __global__ __launch_bounds__(kThreads) void paged_attn_merge_kernel(PagedArgs a)
 #pragma unroll
   for (int e = 0; e < W; ++e) x[e] = 0.0f;
   if (r < rows) {
-    const int64_t n = cut.last - b + 1;
-    for (int64_t i0 = r; i0 < n; i0 += kAhead * rows) {
+    const int n = cut.more + 1, pairs = pairs_of(a);
+    for (int i0 = r; i0 < n; i0 += kAhead * rows) {
       float pm[kAhead], pl[kAhead], px[kAhead][W];
 #pragma unroll
       for (int k = 0; k < kAhead; ++k) {
-        const int64_t i = i0 + k * rows;
+        const int i = i0 + k * rows;
         pm[k] = -INFINITY;
         pl[k] = 0.0f;
 #pragma unroll
         for (int e = 0; e < W; ++e) px[k][e] = 0.0f;
         if (i < n) {
-          const float* p = a.part + (2 * (b + i) + (i == 0 ? cut.slot : 0)) * a.part_stride + row;
+          const float* p = a.part +
+                           (2 * (b + (int64_t)i * pairs) + (i == 0 ? cut.slot : 0)) * a.part_stride +
+                           row;
           pm[k] = p[D];
           pl[k] = p[D + 1];
           if constexpr (W == 4) {
@@ -798,12 +819,19 @@ __global__ __launch_bounds__(kThreads) void paged_attn_merge_kernel(PagedArgs a)
 #ifndef PG_GROUPS
 #define PG_GROUPS 512
 #endif
-constexpr int64_t kGroups = 1024;  // most workgroups that share a launch's steps
+constexpr int64_t kGroups = PG_GROUPS;  // workgroups that share a launch's steps
 constexpr int64_t kWholeSteps = PG_WHOLE;
 
 // Floats of a partial, for either kernel.
 int64_t part_floats(int32_t group, int32_t head_dim) {
   return (int64_t)std::min<int32_t>(group, kTileHeads) * (head_dim + kPartPad);
+}
+
+// Workgroups that may leave partials: at least one share of every (KV head, head
+// tile).
+int64_t part_groups(int32_t num_kv_heads, int32_t group) {
+  return std::max<int64_t>(kGroups,
+                           (int64_t)num_kv_heads * ((group + kGenHeads - 1) / kGenHeads));
 }
 
 template <int QDT, int KDT>
@@ -830,8 +858,9 @@ extern "C" int64_t amf_paged_decode_workspace_bytes(int32_t num_q_heads, int32_t
   if (num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads != 0 || head_dim <= 0 ||
       head_dim > kMaxDim)
     return 0;
-  return kGroups * (int64_t)sizeof(Cut) +
-         2 * kGroups * part_floats(num_q_heads / num_kv_heads, head_dim) * (int64_t)sizeof(float);
+  const int32_t group = num_q_heads / num_kv_heads;
+  return part_groups(num_kv_heads, group) *
+         ((int64_t)sizeof(Cut) + 2 * part_floats(group, head_dim) * (int64_t)sizeof(float));
 }
 
 extern "C" int amf_paged_decode_attn(
@@ -913,14 +942,18 @@ extern "C" int amf_paged_decode_attn(
   // the most steps that a pair can have, as far as the host knows
   const int64_t tokens = pages ? (int64_t)max_pages * block_size
                                : std::min<int64_t>(max_context_len, (int64_t)table_pages * block_size);
-  const int64_t steps = std::max<int64_t>(1, (tokens + kStep - 1) / kStep);
+  const int chunk = matrix ? matrix_chunk(head_dim, es) : kChunk;
+  a.step_shift = __builtin_ctz(chunk * kWaves);
+  const int64_t steps = std::max<int64_t>(1, (tokens + chunk * kWaves - 1) / (chunk * kWaves));
   const int64_t pairs = (int64_t)num_seqs * num_kv_heads * a.tiles;
   if (pairs > 0x7FFFFFFF || (int64_t)num_seqs * num_q_heads > 0x7FFFFFFF)
     return fail(AMF_ERR_UNSUPPORTED, "%s: %d sequences of %d heads", who, num_seqs, num_q_heads);
   a.whole = steps <= kWholeSteps;
-  const int64_t groups = a.whole ? pairs : std::min(pairs * steps, (int64_t)PG_GROUPS);
+  const int64_t heads = (int64_t)num_kv_heads * a.tiles;
+  const int64_t shares = std::min(std::max<int64_t>(kGroups / heads, 1), num_seqs * steps);
+  const int64_t groups = a.whole ? pairs : shares * heads;
   a.cuts = static_cast<Cut*>(workspace);
-  a.part = reinterpret_cast<float*>(a.cuts + kGroups);
+  a.part = reinterpret_cast<float*>(a.cuts + part_groups(num_kv_heads, a.group));
   a.part_stride = part_floats(a.group, head_dim);
   a.err_flag = err_flag;
   hipStream_t st = as_stream(stream);
