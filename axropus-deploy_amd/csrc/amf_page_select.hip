@@ -257,14 +257,14 @@ __global__ __launch_bounds__(kThreads) void page_score_kernel(SelectArgs a) {
 
 // ---- choice --------------------------------------------------------------------
 
-constexpr int kPickThreads = 1024;
 constexpr int kPickKeys = 8;  // consecutive keys of a thread
-constexpr int kPickTile = kPickThreads * kPickKeys;
-constexpr int kDigit = 11;  // bits
+constexpr int kDigit = 11;    // bits
 constexpr int kBins = 1 << kDigit;
 
 // Sum over the threads before this one, and over all in *total; tmp holds a
-// word per wave.  Starts and ends with a barrier.
+// word per wave and is not used again before the next barrier but one.  One
+// barrier.
+template <int NT>
 __device__ __forceinline__ uint32_t pick_exclusive(uint32_t v, uint32_t* tmp, uint32_t* total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   uint32_t x = v;
@@ -273,18 +273,16 @@ __device__ __forceinline__ uint32_t pick_exclusive(uint32_t v, uint32_t* tmp, ui
     const uint32_t y = __shfl_up(x, o);
     if (lane >= o) x += y;
   }
-  __syncthreads();
   if (lane == 63) tmp[wave] = x;
   __syncthreads();
   uint32_t before = 0, all = 0;
 #pragma unroll
-  for (int w = 0; w < kPickThreads / 64; ++w) {
+  for (int w = 0; w < NT / 64; ++w) {
     const uint32_t y = tmp[w];
     if (w < wave) before += y;
     all += y;
   }
   *total = all;
-  __syncthreads();
   return before + x - v;
 }
 
@@ -293,13 +291,17 @@ __device__ __forceinline__ uint32_t pick_exclusive(uint32_t v, uint32_t* tmp, ui
 // digit (a histogram in LDS each), from the first bit in which the keys differ,
 // so that one or two digits separate scores that share sign and exponent; then
 // the pages above it and the first of its equals are written at their ranks.
-// Forced pages are left out of the search.  Up to kPickTile keys stay in
+// Forced pages are left out of the search.  Up to NT * kPickKeys keys stay in
 // registers (MANY: they are read again for each pass).
-template <bool MANY>
-__global__ __launch_bounds__(kPickThreads) void page_pick_kernel(SelectArgs a) {
-  __shared__ uint32_t hist[kBins];
-  __shared__ uint32_t tmp[kPickThreads / 64];
-  __shared__ uint64_t s_lo[kPickThreads / 64], s_hi[kPickThreads / 64];
+//
+// Bound by its barriers: three a digit, on 16 waves or, for up to 2048 pages, 4.
+template <int NT, bool MANY>
+__global__ __launch_bounds__(NT) void page_pick_kernel(SelectArgs a) {
+  constexpr int kTile = NT * kPickKeys;
+  constexpr int kMine = kBins / NT;  // bins of a thread
+  __shared__ uint32_t hist[2][kBins];
+  __shared__ uint32_t tmp[2][NT / 64];
+  __shared__ uint64_t s_lo[NT / 64], s_hi[NT / 64];
   __shared__ uint32_t s_digit, s_left, s_all;
   const int s = blockIdx.y, h = blockIdx.x, tid = threadIdx.x;
   const int64_t n = seq_pages(a, s);
@@ -312,9 +314,9 @@ __global__ __launch_bounds__(kPickThreads) void page_pick_kernel(SelectArgs a) {
     if (h == 0 && a.err_flag && (int64_t)a.context_lens[s] > a.max_pages * a.block_size)
       atomicOr(a.err_flag, AMF_ERRFLAG_CONTEXT);
   }
-  for (int i = count + tid; i < K; i += kPickThreads) out[i] = -1;
+  for (int i = count + tid; i < K; i += NT) out[i] = -1;
   if (n <= K) {
-    for (int i = tid; i < count; i += kPickThreads) out[i] = i;
+    for (int i = tid; i < count; i += NT) out[i] = i;
     return;
   }
   const uint64_t* keys = a.keys + row * a.max_pages;
@@ -328,7 +330,7 @@ __global__ __launch_bounds__(kPickThreads) void page_pick_kernel(SelectArgs a) {
   };
   auto each_tile = [&](auto&& body) {
     if constexpr (MANY) {
-      for (int64_t t0 = 0; t0 < n; t0 += kPickTile) {
+      for (int64_t t0 = 0; t0 < n; t0 += kTile) {
         load(t0);
         body(t0);
       }
@@ -340,7 +342,9 @@ __global__ __launch_bounds__(kPickThreads) void page_pick_kernel(SelectArgs a) {
   auto searched = [&](int64_t t0, int e) {
     return t0 + (int64_t)tid * kPickKeys + e < n && kept[e] != kForced;
   };
-  // range of the keys searched, and how many are forced
+#pragma unroll
+  for (int k = 0; k < kMine; ++k) hist[0][tid + k * NT] = 0;
+  // range of the keys searched
   uint64_t lo = ~0ull, hi = 0;
   each_tile([&](int64_t t0) {
 #pragma unroll
@@ -361,41 +365,42 @@ __global__ __launch_bounds__(kPickThreads) void page_pick_kernel(SelectArgs a) {
   }
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kPickThreads / 64; ++w) {
+  for (int w = 0; w < NT / 64; ++w) {
     lo = min(lo, s_lo[w]);
     hi = max(hi, s_hi[w]);
   }
-  uint32_t left = (uint32_t)(K - min((int64_t)a.first_pages + a.last_pages, n));
+  // n > K, so first_pages + last_pages pages are forced
+  uint32_t left = (uint32_t)(K - a.first_pages - a.last_pages);
   uint64_t cut = lo;  // keys of these digits: `left` of them are taken
   int shift = lo < hi ? 64 - __builtin_clzll(lo ^ hi) : 0;  // bits not decided yet
   if (left == 0) {  // nothing but the forced pages
     cut = kForced;
     shift = 0;
   }
-  while (shift > 0 && left > 0) {
+  int now = 0;
+  while (shift > 0) {  // uniform
     const int next = max(shift - kDigit, 0), bins = 1 << (shift - next);
-    for (int i = tid; i < bins; i += kPickThreads) hist[i] = 0;
-    __syncthreads();
     const uint64_t above = shift == 64 ? 0 : cut >> shift;
     each_tile([&](int64_t t0) {
 #pragma unroll
       for (int e = 0; e < kPickKeys; ++e)
         if (searched(t0, e) && (shift == 64 || kept[e] >> shift == above))
-          atomicAdd(&hist[(kept[e] >> next) & (bins - 1)], 1u);
+          atomicAdd(&hist[now][(kept[e] >> next) & (bins - 1)], 1u);
     });
     __syncthreads();
-    // bins from the top, two a thread: the one in which `left` keys are reached
-    uint32_t c[kBins / kPickThreads], sum = 0, all;
+    // bins from the top, kMine a thread: the one in which `left` keys are reached
+    uint32_t c[kMine], sum = 0, all;
 #pragma unroll
-    for (int k = 0; k < kBins / kPickThreads; ++k) {
-      const int bin = bins - 1 - (tid * (kBins / kPickThreads) + k);
-      sum += c[k] = bin >= 0 ? hist[bin] : 0;
+    for (int k = 0; k < kMine; ++k) {
+      const int bin = bins - 1 - (tid * kMine + k);
+      sum += c[k] = bin >= 0 ? hist[now][bin] : 0;
+      hist[now ^ 1][tid + k * NT] = 0;
     }
-    uint32_t before = pick_exclusive(sum, tmp, &all);
+    uint32_t before = pick_exclusive<NT>(sum, tmp[now], &all);
 #pragma unroll
-    for (int k = 0; k < kBins / kPickThreads; ++k) {
+    for (int k = 0; k < kMine; ++k) {
       if (before < left && before + c[k] >= left) {
-        s_digit = bins - 1 - (tid * (kBins / kPickThreads) + k);
+        s_digit = bins - 1 - (tid * kMine + k);
         s_left = left - before;
         s_all = before + c[k] == left;
       }
@@ -405,8 +410,8 @@ __global__ __launch_bounds__(kPickThreads) void page_pick_kernel(SelectArgs a) {
     cut = (cut >> next >> (shift - next) << (shift - next) | s_digit) << next;
     left = s_left;
     shift = next;
-    if (s_all) break;
-    __syncthreads();
+    now ^= 1;
+    if (s_all) break;  // s_*: written again after the next histogram's barrier
   }
   // taken: keys whose digits are above the cut's, and `left` of its equals
   cut >>= shift;
@@ -420,7 +425,8 @@ __global__ __launch_bounds__(kPickThreads) void page_pick_kernel(SelectArgs a) {
       eq += in && kept[e] != kForced && kept[e] >> shift == cut;
     }
     uint32_t all;  // both below 2^14 in a tile
-    const uint32_t both = pick_exclusive(gt << 16 | eq, tmp, &all);
+    const uint32_t both = pick_exclusive<NT>(gt << 16 | eq, tmp[now], &all);
+    now ^= 1;
     uint32_t g = gt0 + (both >> 16), q = eq0 + (both & 0xFFFFu);
 #pragma unroll
     for (int e = 0; e < kPickKeys; ++e) {
@@ -587,9 +593,11 @@ extern "C" int amf_select_pages(const void* q, int32_t dtype, int64_t q_seq_stri
     if (int rc = check_launch(who)) return rc;
   }
   const dim3 rows((unsigned)num_kv_heads, (unsigned)num_seqs);
-  if (max_pages > kPickTile)
-    page_pick_kernel<true><<<rows, kPickThreads, 0, st>>>(a);
+  if (max_pages <= 256 * kPickKeys)
+    page_pick_kernel<256, false><<<rows, 256, 0, st>>>(a);
+  else if (max_pages <= 1024 * kPickKeys)
+    page_pick_kernel<1024, false><<<rows, 1024, 0, st>>>(a);
   else
-    page_pick_kernel<false><<<rows, kPickThreads, 0, st>>>(a);
+    page_pick_kernel<1024, true><<<rows, 1024, 0, st>>>(a);
   return check_launch(who);
 }
