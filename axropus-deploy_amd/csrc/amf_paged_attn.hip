@@ -56,24 +56,25 @@ struct PagedArgs {
   int32_t step_shift;   // log2 of the tokens of a step (of all waves)
   int32_t group;        // query heads of a KV head
   int32_t tiles;        // head tiles of a group
+  int32_t side;         // (KV head, head tile) pairs of a workgroup: 1, 2 or 4
   int32_t out_dtype;
   float score_scale;    // softmax scale * k_scale * log2(e)
   float v_scale;
-  bool whole;           // a workgroup takes a whole pair
-  struct Cut* cuts;     // [workgroup]
-  float* part;          // [workgroup][2][heads of a tile][head_dim + kPartPad]
+  bool whole;           // a share is a whole sequence
+  bool by_seq;          // cuts are kept by sequence (fewer than shares), else by share
+  struct Cut* cuts;     // [sequence or share][pair]
+  float* part;          // [share][pair][2][heads of a tile][head_dim + kPartPad]
   int64_t part_stride;  // floats of one partial
   int32_t* err_flag;
 };
 
-// The pair that begins in a workgroup's share and does not end there: its
-// partials are slot `slot` of this workgroup and slot 0 of the `more` next
-// shares' workgroups of that (KV head, head tile).
+// A pair that does not end in the share where it begins: its partials are slot
+// `slot` of that share's place and slot 0 of the `more` next shares' for the pair.
 struct Cut {
   int32_t heads;  // 0: no such pair
   int32_t head0;  // of the step's rows
   int32_t more;
-  int32_t slot;
+  int32_t place;  // 2 * place + slot
 };
 
 // ---- shares --------------------------------------------------------------------
@@ -107,14 +108,16 @@ struct Unit {
 };
 
 __device__ __forceinline__ int pairs_of(const PagedArgs& a) { return a.num_kv_heads * a.tiles; }
+// Workgroups of a share.
+__device__ __forceinline__ int teams_of(const PagedArgs& a) { return pairs_of(a) / a.side; }
 
 // The same in every thread.
 __device__ __forceinline__ Unit find_unit(const PagedArgs& a) {
   __shared__ int64_t tmp[kWaves];
   __shared__ int found_seq;
   __shared__ int64_t found_start, found_steps;
-  const int pairs = pairs_of(a);
-  const int64_t shares = gridDim.x / pairs, mine = blockIdx.x / pairs;
+  const int teams = teams_of(a);
+  const int64_t shares = gridDim.x / teams, mine = blockIdx.x / teams;
   const int tid = threadIdx.x;
   Unit r{};
   if (a.whole) {
@@ -162,7 +165,7 @@ __device__ __forceinline__ Unit find_unit(const PagedArgs& a) {
 
 // ---- segments ------------------------------------------------------------------
 
-// The steps of one pair that lie in a workgroup's share.
+// The steps of one pair that lie in a share.
 struct Segment {
   int seq, hkv, heads;
   int64_t head0;     // first query head, of the step's rows
@@ -172,12 +175,14 @@ struct Segment {
   float* part;       // where the partial goes otherwise
 };
 
-// The segment from step u of sequence un.seq on; the share ends at u1.
+// The segment from step u of sequence un.seq on, for pair n of the workgroup; the
+// share ends at u1.
 template <int TILE>
 __device__ __forceinline__ Segment segment_at(const PagedArgs& a, const Unit& un, int64_t u,
-                                              int64_t u1) {
+                                              int64_t u1, int n) {
   Segment g;
-  const int pairs = pairs_of(a), pair = blockIdx.x % pairs;
+  const int teams = teams_of(a), pair = (blockIdx.x % teams) * a.side + n;
+  const int64_t share = blockIdx.x / teams, place = share * pairs_of(a) + pair;
   g.st0 = u - un.start;
   g.st1 = min(un.steps, g.st0 + (u1 - u));
   g.seq = un.seq;
@@ -187,12 +192,20 @@ __device__ __forceinline__ Segment segment_at(const PagedArgs& a, const Unit& un
   g.head0 = (int64_t)un.seq * a.num_q_heads + g.hkv * a.group + tile * TILE;
   g.ctx = a.context_lens[un.seq];
   g.whole = g.st0 == 0 && g.st1 == un.steps;
-  g.part = a.part + (2 * (int64_t)blockIdx.x + (u != un.first)) * a.part_stride;
-  if (!g.whole && g.st0 == 0 && threadIdx.x == 0)
-    a.cuts[blockIdx.x] = Cut{g.heads, (int32_t)g.head0,
-                             (int32_t)((u + un.steps - 1) / un.share - blockIdx.x / pairs),
-                             u != un.first};
+  g.part = a.part + (2 * place + (u != un.first)) * a.part_stride;
   return g;
+}
+
+// Notes whether the pair of a segment that begins it is cut.
+__device__ __forceinline__ void note_cut(const PagedArgs& a, const Unit& un, const Segment& g,
+                                         int64_t u, int n) {
+  if (a.whole || g.st0 != 0 || (g.whole && !a.by_seq)) return;
+  const int teams = teams_of(a), pairs = pairs_of(a), pair = (blockIdx.x % teams) * a.side + n;
+  const int64_t share = blockIdx.x / teams;
+  a.cuts[(a.by_seq ? g.seq : share) * pairs + pair] =
+      Cut{g.whole ? 0 : g.heads, (int32_t)g.head0,
+          (int32_t)((u + un.steps - 1) / un.share - share),
+          (int32_t)(2 * (share * pairs + pair) + (u != un.first))};
 }
 
 // Moves on to step u, perhaps of the next sequence with tokens; u lies in the
@@ -282,12 +295,18 @@ __device__ __forceinline__ void store_out(const PagedArgs& a, int64_t i, float x
 }
 
 // Zeros for the sequences without tokens, and the flag of contexts that their
-// block tables do not hold; the workgroups take turns.
+// block tables do not hold (the workgroups take turns); no cut, until one is noted.
 __device__ __forceinline__ void empty_seqs(const PagedArgs& a) {
   const int64_t row = (int64_t)a.num_q_heads * a.head_dim;
+  if (!a.whole && !a.by_seq && threadIdx.x < a.side)  // until a cut is found
+    a.cuts[(int64_t)blockIdx.x * a.side + threadIdx.x].heads = 0;
   for (int64_t s = blockIdx.x; s < a.num_seqs; s += gridDim.x) {
-    if (seq_tokens(a, (int)s) == 0)
+    if (seq_tokens(a, (int)s) == 0) {
       for (int64_t i = threadIdx.x; i < row; i += kThreads) store_out(a, s * row + i, 0.0f);
+      if (!a.whole && a.by_seq)
+        for (int i = threadIdx.x; i < pairs_of(a); i += kThreads)
+          a.cuts[s * pairs_of(a) + i].heads = 0;
+    }
     if (threadIdx.x == 0 && a.err_flag &&
         (int64_t)a.context_lens[s] > (int64_t)a.table_pages * a.block_size)
       atomicOr(a.err_flag, AMF_ERRFLAG_CONTEXT);
@@ -317,12 +336,12 @@ __global__ __launch_bounds__(kThreads) void paged_attn_general_kernel(PagedArgs 
   const int d0 = half ? (D + 1) / 2 : 0, d1 = half ? D : (D + 1) / 2;
   empty_seqs(a);
   Unit un = find_unit(a);
-  if (!a.whole && tid == 0) a.cuts[blockIdx.x].heads = 0;
   if (un.seq < 0) return;
   const int64_t u1 = min(un.first + un.share, un.total);
   for (int64_t u = un.first; u < u1;) {
     advance(a, un, u);
-    const Segment sg = segment_at<kGenHeads>(a, un, u, u1);
+    const Segment sg = segment_at<kGenHeads>(a, un, u, u1, 0);
+    if (tid == 0) note_cut(a, un, sg, u, 0);
     u += sg.st1 - sg.st0;
     for (int i = tid; i < kGenHeads * D; i += kThreads) {
       const int g = i / D, d = i - g * D;
@@ -492,16 +511,18 @@ __global__ __launch_bounds__(kThreads, matrix_waves(D)) void paged_attn_matrix_k
   __shared__ PageRun run;
   __shared__ __attribute__((aligned(16))) float acc_lds[kWaves][kTileHeads][ROW];
   __shared__ float m_lds[kWaves][kTileHeads], l_lds[kWaves][kTileHeads];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lo = lane & 15, hi = lane >> 4;
   empty_seqs(a);
   Unit un = find_unit(a);
-  if (!a.whole && tid == 0) a.cuts[blockIdx.x].heads = 0;
   if (un.seq < 0) return;
   const int64_t u1 = min(un.first + un.share, un.total);
   for (int64_t u = un.first; u < u1;) {
     advance(a, un, u);
-    const Segment sg = segment_at<kTileHeads>(a, un, u, u1);
+    const Segment sg = segment_at<kTileHeads>(a, un, u, u1, wave % a.side);
+    if (lane == 0 && wave < a.side) note_cut(a, un, sg, u, wave);
+    const int64_t u_here = u;
     u += sg.st1 - sg.st0;
     // q of head lo, dims 32 ks + 8 hi .. (FP8: the dims of the K bytes that the
     // lane loads, 64 j + 16 hi .., two k steps)
@@ -558,7 +579,7 @@ __global__ __launch_bounds__(kThreads, matrix_waves(D)) void paged_attn_matrix_k
     for (int64_t r0 = sg.st0; r0 < sg.st1; r0 += hold) {
       const int64_t r1 = min(r0 + hold, sg.st1), j0 = page_of(a, r0 << a.step_shift);
       load_pages(a, sg, r0, r1, run);
-      const int64_t t = wave * CH + (lane & (CH - 1));
+      const int64_t t = (wave / a.side) * CH + (lane & (CH - 1));
       int64_t off = token_offset(a, sg, run, j0, (r0 << a.step_shift) + t);
       uint64_t seen = __ballot(off >= 0);
       if (seen) {
@@ -701,30 +722,31 @@ __global__ __launch_bounds__(kThreads, matrix_waves(D)) void paged_attn_matrix_k
       }
     }
     __syncthreads();
-    for (int i = tid; i < sg.heads * (D / 4); i += kThreads) {
-      const int g = i / (D / 4), d = 4 * (i - g * (D / 4));
-      float top = m_lds[0][g], sum = 0.0f;
-      f32x4 x{0, 0, 0, 0};
-#pragma unroll
-      for (int w = 1; w < kWaves; ++w) top = max_nan(top, m_lds[w][g]);
-#pragma unroll
-      for (int w = 0; w < kWaves; ++w) {
-        const float f = weight_to(m_lds[w][g], top);
-        sum += l_lds[w][g] * f;
-        x += *reinterpret_cast<const f32x4*>(&acc_lds[w][g][d]) * f;
-      }
-      if (sg.whole) {
-        if (sum == 0.0f)
-          x = f32x4{0, 0, 0, 0};
-        else
-          x *= a.v_scale / sum;
-        store4(a.out, a.out_dtype, (sg.head0 + g) * D + d, x);
-      } else {
-        float* part = sg.part + g * (D + kPartPad);
-        *reinterpret_cast<f32x4*>(part + d) = x;
-        if (d == 0) {
-          part[D] = top;
-          part[D + 1] = sum;
+    for (int n = 0; n < a.side; ++n) {
+      const Segment sn = segment_at<kTileHeads>(a, un, u_here, u1, n);
+      for (int i = tid; i < sn.heads * (D / 4); i += kThreads) {
+        const int g = i / (D / 4), d = 4 * (i - g * (D / 4));
+        float top = m_lds[n][g], sum = 0.0f;
+        f32x4 x{0, 0, 0, 0};
+        for (int w = n + a.side; w < kWaves; w += a.side) top = max_nan(top, m_lds[w][g]);
+        for (int w = n; w < kWaves; w += a.side) {
+          const float f = weight_to(m_lds[w][g], top);
+          sum += l_lds[w][g] * f;
+          x += *reinterpret_cast<const f32x4*>(&acc_lds[w][g][d]) * f;
+        }
+        if (sn.whole) {
+          if (sum == 0.0f)
+            x = f32x4{0, 0, 0, 0};
+          else
+            x *= a.v_scale / sum;
+          store4(a.out, a.out_dtype, (sn.head0 + g) * D + d, x);
+        } else {
+          float* part = sn.part + g * (D + kPartPad);
+          *reinterpret_cast<f32x4*>(part + d) = x;
+          if (d == 0) {
+            part[D] = top;
+            part[D + 1] = sum;
+          }
         }
       }
     }
@@ -733,23 +755,23 @@ __global__ __launch_bounds__(kThreads, matrix_waves(D)) void paged_attn_matrix_k
 
 // ---- merge ---------------------------------------------------------------------
 //
-// A workgroup per (cut pair, head): threads take W dims of every n-th partial,
-// several partials loaded ahead of their use, and are joined in LDS.
+// A workgroup per pair that may be cut and `heads` of its heads: threads take W
+// dims of every n-th partial, several partials loaded ahead of their use, and are
+// joined in LDS.
 template <int W>
-__global__ __launch_bounds__(kThreads) void paged_attn_merge_kernel(PagedArgs a) {
+__global__ __launch_bounds__(kThreads) void paged_attn_merge_kernel(PagedArgs a, int heads) {
   constexpr int kAhead = 4;
   __shared__ float x_lds[kThreads][W], m_lds[kThreads], l_lds[kThreads];
-  const int64_t b = blockIdx.x;
-  const Cut cut = a.cuts[b];
-  const int g = blockIdx.y, tid = threadIdx.x;
-  if (g >= cut.heads) return;
-  const int D = a.head_dim, row = g * (D + kPartPad);
-  const int cols = (D + W - 1) / W, rows = kThreads / cols;
-  const int col = tid % cols, r = tid / cols;
+  const Cut cut = a.cuts[blockIdx.x];
+  const int tid = threadIdx.x, D = a.head_dim;
+  if ((int)blockIdx.y * heads >= cut.heads) return;
+  const int cols = (D + W - 1) / W, rows = kThreads / (cols * heads);
+  const int r = tid / (cols * heads), g = (int)blockIdx.y * heads + tid % (cols * heads) / cols;
+  const int col = tid % cols, row = g * (D + kPartPad);
   float m = -INFINITY, l = 0.0f, x[W];
 #pragma unroll
   for (int e = 0; e < W; ++e) x[e] = 0.0f;
-  if (r < rows) {
+  if (r < rows && g < cut.heads) {
     const int n = cut.more + 1, pairs = pairs_of(a);
     for (int i0 = r; i0 < n; i0 += kAhead * rows) {
       float pm[kAhead], pl[kAhead], px[kAhead][W];
@@ -761,9 +783,8 @@ __global__ __launch_bounds__(kThreads) void paged_attn_merge_kernel(PagedArgs a)
 #pragma unroll
         for (int e = 0; e < W; ++e) px[k][e] = 0.0f;
         if (i < n) {
-          const float* p = a.part +
-                           (2 * (b + (int64_t)i * pairs) + (i == 0 ? cut.slot : 0)) * a.part_stride +
-                           row;
+          const int64_t place = i == 0 ? cut.place : (cut.place & ~1) + 2 * (int64_t)i * pairs;
+          const float* p = a.part + place * a.part_stride + row;
           pm[k] = p[D];
           pl[k] = p[D + 1];
           if constexpr (W == 4) {
@@ -791,9 +812,9 @@ __global__ __launch_bounds__(kThreads) void paged_attn_merge_kernel(PagedArgs a)
 #pragma unroll
   for (int e = 0; e < W; ++e) x_lds[tid][e] = x[e];
   __syncthreads();
-  if (r > 0) return;
+  if (r > 0 || g >= cut.heads) return;
   for (int k = 1; k < rows; ++k) {
-    const int o = tid + k * cols;
+    const int o = tid + k * cols * heads;
     const float pm = m_lds[o], top = max_nan(m, pm);
     const float f = weight_to(m, top), pf = weight_to(pm, top);
     l = l * f + l_lds[o] * pf;
@@ -827,10 +848,10 @@ int64_t part_floats(int32_t group, int32_t head_dim) {
   return (int64_t)std::min<int32_t>(group, kTileHeads) * (head_dim + kPartPad);
 }
 
-// Workgroups that may leave partials: at least one share of every (KV head, head
-// tile).
-int64_t part_groups(int32_t num_kv_heads, int32_t group) {
-  return std::max<int64_t>(kGroups,
+// Places for partials: every pair of a launch's shares, of which there is one at
+// least.
+int64_t part_places(int32_t num_kv_heads, int32_t group) {
+  return std::max<int64_t>(kGroups * kWaves,
                            (int64_t)num_kv_heads * ((group + kGenHeads - 1) / kGenHeads));
 }
 
@@ -859,7 +880,7 @@ extern "C" int64_t amf_paged_decode_workspace_bytes(int32_t num_q_heads, int32_t
       head_dim > kMaxDim)
     return 0;
   const int32_t group = num_q_heads / num_kv_heads;
-  return part_groups(num_kv_heads, group) *
+  return part_places(num_kv_heads, group) *
          ((int64_t)sizeof(Cut) + 2 * part_floats(group, head_dim) * (int64_t)sizeof(float));
 }
 
@@ -949,11 +970,18 @@ extern "C" int amf_paged_decode_attn(
   if (pairs > 0x7FFFFFFF || (int64_t)num_seqs * num_q_heads > 0x7FFFFFFF)
     return fail(AMF_ERR_UNSUPPORTED, "%s: %d sequences of %d heads", who, num_seqs, num_q_heads);
   a.whole = steps <= kWholeSteps;
+  // pairs side by side in a workgroup: their rows lie side by side in memory
   const int64_t heads = (int64_t)num_kv_heads * a.tiles;
-  const int64_t shares = std::min(std::max<int64_t>(kGroups / heads, 1), num_seqs * steps);
-  const int64_t groups = a.whole ? pairs : shares * heads;
+  a.side = 1;
+  if (matrix && !a.whole && !pages) a.side = heads % 4 == 0 ? 4 : heads % 2 == 0 ? 2 : 1;
+  if (a.side > 1) a.step_shift -= a.side / 2;
+  const int64_t teams = heads / a.side;
+  const int64_t most_steps = num_seqs * ((tokens + (1 << a.step_shift) - 1) >> a.step_shift);
+  const int64_t shares = std::min(std::max<int64_t>(kGroups / teams, 1), most_steps);
+  const int64_t groups = (a.whole ? num_seqs : shares) * teams;
+  a.by_seq = num_seqs < shares;
   a.cuts = static_cast<Cut*>(workspace);
-  a.part = reinterpret_cast<float*>(a.cuts + part_groups(num_kv_heads, a.group));
+  a.part = reinterpret_cast<float*>(a.cuts + part_places(num_kv_heads, a.group));
   a.part_stride = part_floats(a.group, head_dim);
   a.err_flag = err_flag;
   hipStream_t st = as_stream(stream);
@@ -969,10 +997,16 @@ extern "C" int amf_paged_decode_attn(
     launch<AMF_DTYPE_F16, AMF_DTYPE_E4M3>(a, groups, matrix, st);
   if (int rc = check_launch(who)) return rc;
   if (a.whole) return ok();
-  const dim3 grid((unsigned)groups, (unsigned)std::min<int32_t>(a.group, tile));
+  // a head to a merge's workgroup where a pair has many partials, else more
+  const int32_t tile_heads = std::min<int32_t>(a.group, tile);
+  const int cols = matrix ? head_dim / 4 : head_dim;
+  int per = std::max(1, kThreads / cols / (shares >= 4 * (int64_t)num_seqs ? 8 : 2));
+  per = std::min<int>(per, tile_heads);
+  const dim3 grid((unsigned)(std::min<int64_t>(num_seqs, shares) * heads),
+                  (unsigned)((tile_heads + per - 1) / per));
   if (matrix)
-    paged_attn_merge_kernel<4><<<grid, kThreads, 0, st>>>(a);
+    paged_attn_merge_kernel<4><<<grid, kThreads, 0, st>>>(a, per);
   else
-    paged_attn_merge_kernel<1><<<grid, kThreads, 0, st>>>(a);
+    paged_attn_merge_kernel<1><<<grid, kThreads, 0, st>>>(a, per);
   return check_launch(who);
 }
