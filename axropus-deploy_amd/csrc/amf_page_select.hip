@@ -128,130 +128,110 @@ __device__ __forceinline__ uint64_t order_key(double x) {
 constexpr uint64_t kForced = ~0ull;  // first and last pages
 constexpr uint64_t kInfinite = 0xFFF0000000000000ull;  // order_key(inf)
 
-// A wave scores kTiles times 16 pages against SETS times 4 query heads with 4x4x4
-// products in 64 bits, four blocks side by side: lane (lo, hi) = (lane % 16,
+// A wave scores 16 pages against SETS times 4 query heads with 4x4x4 products in
+// 64 bits, four blocks side by side: lane (lo, hi) = (lane % 16,
 // lane / 16) holds page lo's bounds in dims 32 c + 8 hi + e as the A operand of
 // step (c, e), and as B head lo % 4's q in that dim, split as max(q, 0) against
 // hi and min(q, 0) against lo; D gives it page 4 (lo / 4) + hi of head lo % 4.
 // q waits in LDS as doubles.  (fp64 on the vector units took 95 us for 8
 // sequences x 65000 tokens, 64 / 8 heads of 128: a conversion, a choice and a
 // product per element and head, and a reduction over lanes.)
-constexpr int kTiles = 1;  // 1: 48.2 us, 2: 47.5 (13.9 / 14.3 for one sequence x 131072)
-constexpr int kScorePages = kThreads / 64 * 16 * kTiles;  // pages of a workgroup
+constexpr int kScorePages = kThreads / 64 * 16;  // pages that a workgroup takes at once
 constexpr int kHeadSet = 4;
 
 __device__ __forceinline__ double max64(double x, double y) { return x > y ? x : y; }
 
-// NC chunks of 32 dims; SETS of heads share a bound's conversion to a double.
-// The heads' workgroups of a page run side by side: their bounds lie together.
+// NC chunks of 32 dims; SETS of heads share a bound's conversion to a double.  The
+// heads' workgroups of a page run side by side: their bounds lie together.  A wave
+// takes one tile of 16 pages; walking several with the next one's bounds in flight
+// needs twice the registers and was slower (2 tiles 82 -> 87 us a selection with its
+// attention, 4 93).
 template <bool BF16, int NC, int SETS>
 __global__ __launch_bounds__(kThreads) void page_score_kernel(SelectArgs a) {
   // [dim in step order][set][hi][head] -> (max(q, 0), min(q, 0))
   __shared__ __attribute__((aligned(16))) double q_lds[NC * 8][SETS][4][kHeadSet][2];
   const int s = blockIdx.z, h = blockIdx.x;
-  const int64_t p0 = (int64_t)blockIdx.y * kScorePages;
   const int64_t n = seq_pages(a, s);
+  const int64_t p0 = (int64_t)blockIdx.y * kScorePages;
   if (p0 >= n || n <= a.num_pages) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int lo = lane & 15, hi = lane >> 4;
-  const int64_t base = p0 + wave * 16 * kTiles;
-  u32x4 b[kTiles][2][NC];
-  bool ok[kTiles];
-  int64_t id[kTiles];
-#pragma unroll
-  for (int t = 0; t < kTiles; ++t) {
-    const int64_t p = base + 16 * t + lo;
-    id[t] = p < n ? a.block_tables[s * a.bt_stride + p] : -1;
-    ok[t] = id[t] >= 0 && id[t] < a.pool_pages;
-  }
-#pragma unroll
-  for (int t = 0; t < kTiles; ++t) {
-    const uint16_t* src =
-        a.bounds + ((ok[t] ? id[t] : 0) * a.num_kv_heads + h) * 2 * a.head_dim + 8 * hi;
+  const int64_t base = p0 + wave * 16;
+  const int64_t id = base + lo < n ? a.block_tables[s * a.bt_stride + base + lo] : -1;
+  const bool ok = id >= 0 && id < a.pool_pages;
+  u32x4 b[2][NC];
+  {
+    const uint16_t* src = a.bounds + ((ok ? id : 0) * a.num_kv_heads + h) * 2 * a.head_dim + 8 * hi;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      b[t][0][c] = b[t][1][c] = u32x4{0, 0, 0, 0};
-      if (ok[t] && 32 * c + 8 * hi < a.head_dim) {
-        b[t][0][c] = ld_stream(reinterpret_cast<const u32x4*>(src + 32 * c));
-        b[t][1][c] = ld_stream(reinterpret_cast<const u32x4*>(src + a.head_dim + 32 * c));
+      b[0][c] = b[1][c] = u32x4{0, 0, 0, 0};
+      if (ok && 32 * c + 8 * hi < a.head_dim) {
+        b[0][c] = ld_stream(reinterpret_cast<const u32x4*>(src + 32 * c));
+        b[1][c] = ld_stream(reinterpret_cast<const u32x4*>(src + a.head_dim + 32 * c));
       }
     }
   }
-  double best[kTiles];
-  int fin[kTiles];
-#pragma unroll
-  for (int t = 0; t < kTiles; ++t) {
-    best[t] = -INFINITY;
-    fin[t] = 1;
-  }
+  double best = -INFINITY;
+  int fin = 1;
   for (int g0 = 0; g0 < a.group; g0 += SETS * kHeadSet) {
     __syncthreads();
-    for (int i = tid; i < NC * 32 * SETS * kHeadSet; i += kThreads) {
-      const int d = i % (NC * 32), g = i / (NC * 32);
-      float x = 0.0f;
-      if (d < a.head_dim && g0 + g < a.group)
-        x = half_lo<BF16>(a.q[s * a.q_seq + ((int64_t)h * a.group + g0 + g) * a.q_head + d]);
-      double* o = q_lds[8 * (d / 32) + d % 8][g / kHeadSet][d / 8 % 4][g % kHeadSet];
-      o[0] = x < 0.0f ? 0.0 : (double)x;  // a NaN stays one
-      o[1] = x < 0.0f ? (double)x : 0.0;
+    // 8 dims of a head to a thread (a dim to a thread: 82 -> 89 us as above)
+    for (int i = tid; i < NC * 4 * SETS * kHeadSet; i += kThreads) {
+      const int g = i % (SETS * kHeadSet), d = i / (SETS * kHeadSet);
+      float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+      if (8 * d < a.head_dim && g0 + g < a.group)
+        unpack8<BF16>(*reinterpret_cast<const u32x4*>(
+                          a.q + s * a.q_seq + ((int64_t)h * a.group + g0 + g) * a.q_head + 8 * d),
+                      x);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        double* o = q_lds[8 * (d / 4) + e][g / kHeadSet][d % 4][g % kHeadSet];
+        o[0] = x[e] < 0.0f ? 0.0f : x[e];  // a NaN stays one
+        o[1] = x[e] < 0.0f ? x[e] : 0.0f;
+      }
     }
     __syncthreads();
-    double u[kTiles][SETS];
+    double u[SETS];
 #pragma unroll
-    for (int t = 0; t < kTiles; ++t)
-#pragma unroll
-      for (int k = 0; k < SETS; ++k) u[t][k] = 0.0;
+    for (int k = 0; k < SETS; ++k) u[k] = 0.0;
 #pragma unroll
     for (int c = 0; c < NC; ++c)
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        double l[kTiles], m[kTiles];
-#pragma unroll
-        for (int t = 0; t < kTiles; ++t) {
-          uint32_t wl = b[t][0][c][e / 2], wh = b[t][1][c][e / 2];
-          asm volatile("" : "+v"(wl), "+v"(wh));  // converted here, not before the loop
-          l[t] = e % 2 ? half_hi<BF16>(wl) : half_lo<BF16>(wl);
-          m[t] = e % 2 ? half_hi<BF16>(wh) : half_lo<BF16>(wh);
-        }
+        uint32_t wl = b[0][c][e / 2], wh = b[1][c][e / 2];
+        asm volatile("" : "+v"(wl), "+v"(wh));  // converted here, not before the loop
+        const double l = e % 2 ? half_hi<BF16>(wl) : half_lo<BF16>(wl);
+        const double m = e % 2 ? half_hi<BF16>(wh) : half_lo<BF16>(wh);
 #pragma unroll
         for (int k = 0; k < SETS; ++k) {
           const double* q = q_lds[8 * c + e][k][hi][lo % 4];
-          const double qp = q[0], qm = q[1];
-#pragma unroll
-          for (int t = 0; t < kTiles; ++t) {
-            u[t][k] = __builtin_amdgcn_mfma_f64_4x4x4f64(m[t], qp, u[t][k], 0, 0, 0);
-            u[t][k] = __builtin_amdgcn_mfma_f64_4x4x4f64(l[t], qm, u[t][k], 0, 0, 0);
-          }
+          u[k] = __builtin_amdgcn_mfma_f64_4x4x4f64(m, q[0], u[k], 0, 0, 0);
+          u[k] = __builtin_amdgcn_mfma_f64_4x4x4f64(l, q[1], u[k], 0, 0, 0);
         }
       }
 #pragma unroll
-    for (int t = 0; t < kTiles; ++t)
+    for (int k = 0; k < SETS; ++k) {
+      fin &= u[k] - u[k] == 0.0;
+      if (g0 + k * kHeadSet + lo % 4 < a.group) best = max64(best, u[k]);
+    }
+  }
+  // the best of the heads, in the four lanes of a page
 #pragma unroll
-      for (int k = 0; k < SETS; ++k) {
-        fin[t] &= u[t][k] - u[t][k] == 0.0;
-        if (g0 + k * kHeadSet + lo % 4 < a.group) best[t] = max64(best[t], u[t][k]);
-      }
+  for (int o = 1; o < 4; o <<= 1) {
+    best = max64(best, __shfl_xor(best, o));
+    fin &= __shfl_xor(fin, o);
   }
   const int place = 4 * (lo / 4) + hi;
-#pragma unroll
-  for (int t = 0; t < kTiles; ++t) {
-    // the best of the heads, in the four lanes of a page
-#pragma unroll
-    for (int o = 1; o < 4; o <<= 1) {
-      best[t] = max64(best[t], __shfl_xor(best[t], o));
-      fin[t] &= __shfl_xor(fin[t], o);
+  const int good = __shfl((int)ok, place);
+  const int64_t p = base + place;
+  if (lo % 4 == 0 && p < n) {
+    uint64_t key = fin ? order_key(best) : kInfinite;
+    if (!good) {
+      key = 0;  // never scored: behind every page that can be read
+      if (a.err_flag) atomicOr(a.err_flag, AMF_ERRFLAG_BLOCK_RANGE);
     }
-    const int good = __shfl((int)ok[t], place);
-    const int64_t p = base + 16 * t + place;
-    if (lo % 4 == 0 && p < n) {
-      uint64_t key = fin[t] ? order_key(best[t]) : kInfinite;
-      if (!good) {
-        key = 0;  // never scored: behind every page that can be read
-        if (a.err_flag) atomicOr(a.err_flag, AMF_ERRFLAG_BLOCK_RANGE);
-      }
-      if (p < a.first_pages || p >= n - a.last_pages) key = kForced;
-      a.keys[((int64_t)s * a.num_kv_heads + h) * a.max_pages + p] = key;
-    }
+    if (p < a.first_pages || p >= n - a.last_pages) key = kForced;
+    a.keys[((int64_t)s * a.num_kv_heads + h) * a.max_pages + p] = key;
   }
 }
 
@@ -584,8 +564,10 @@ extern "C" int amf_select_pages(const void* q, int32_t dtype, int64_t q_seq_stri
                      max_pages, static_cast<uint64_t*>(workspace), pages, page_counts, err_flag};
   hipStream_t st = as_stream(stream);
   if (scored) {
-    const unsigned chunks = (unsigned)((max_pages + kScorePages - 1) / kScorePages);
-    const dim3 grid((unsigned)num_kv_heads, chunks, (unsigned)num_seqs);
+    const int64_t chunks = (max_pages + kScorePages - 1) / kScorePages;
+    if (chunks > 65535)
+      return fail(AMF_ERR_UNSUPPORTED, "%s: %lld pages of a sequence", who, (long long)max_pages);
+    const dim3 grid((unsigned)num_kv_heads, (unsigned)chunks, (unsigned)num_seqs);
     if (dtype == AMF_DTYPE_BF16)
       launch_score<true>(a, grid, st);
     else
