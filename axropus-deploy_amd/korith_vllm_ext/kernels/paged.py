@@ -35,7 +35,8 @@ _KV_TAGS = {**_TAGS, torch.float8_e4m3fn: amf_hip.DTYPE_E4M3}
 _HALVES = (torch.bfloat16, torch.float16)
 _I32 = torch.int32
 _I32_MAX = 0x7FFFFFFF
-_WS: dict = {}  # (entry point, sizes) -> workspace bytes
+_ATTN_WS, _SELECT_WS = "amf_paged_decode_workspace_bytes", "amf_select_pages_workspace_bytes"
+_WS: dict = {_ATTN_WS: {}, _SELECT_WS: {}}  # entry point -> {sizes: workspace bytes}
 
 # The checks below run on every call of a decode step, where the host's time is
 # what a small batch waits for: they compare in place and leave the words of an
@@ -60,22 +61,22 @@ def _launch(idx: int, func: str, *args) -> None:
 
 
 def _workspace(name: str, sizes: tuple, given: Optional[torch.Tensor], dev: torch.device,
-               stream: int) -> Tuple[Optional[int], int]:
-    """(address of the workspace, its bytes): the caller's, checked, or the
-    scratch buffer of this device and stream (a new one under graph capture)."""
-    key = (name, sizes)
-    need = _WS.get(key)
+               stream: int) -> Tuple[Optional[torch.Tensor], int]:
+    """(workspace, its bytes): the caller's, checked, or the scratch buffer of
+    this device and stream (a new one under graph capture)."""
+    known = _WS[name]
+    need = known.get(sizes)
     if need is None:
-        if len(_WS) > 4096:
-            _WS.clear()
-        need = _WS[key] = int(getattr(amf_hip.load(), name)(*sizes))
+        if len(known) > 4096:
+            known.clear()
+        need = known[sizes] = int(getattr(amf_hip.load(), name)(*sizes))
     if given is not None:
         _dispatch._check_buffer(given, "workspace", dev)
         have = given.numel() * given.element_size()
         if have < need:
             raise ValueError(f"workspace of {have} bytes, {need} needed")
-        return given.data_ptr(), have
-    return (_dispatch._scratch(dev, stream, need).data_ptr(), need) if need else (None, 0)
+        return given, have
+    return (_dispatch._scratch(dev, stream, need), need) if need else (None, 0)
 
 
 def _cache(k: torch.Tensor, v: Optional[torch.Tensor]) -> tuple:
@@ -238,13 +239,13 @@ def paged_decode_attention(q: torch.Tensor, k_cache: torch.Tensor,
     if out.dtype not in _TAGS:
         raise ValueError(f"paged decode: output dtype {out.dtype} is not bf16/fp16/fp32")
     stream = _raw_stream(idx)
-    ws, wsb = _workspace("amf_paged_decode_workspace_bytes", (Hq, H, D), workspace, dev, stream)
+    ws, wsb = _workspace(_ATTN_WS, (Hq, H, D), workspace, dev, stream)
     qs, qh, _ = q3.stride()
     _launch(
         idx, "amf_paged_decode_attn", q3.data_ptr(), _TAGS[qdt], qs, qh, out.data_ptr(),
         _TAGS[out.dtype], kp, vp, _KV_TAGS[kdt], ps, ts, hs, nb, bt, row, width, cl, pg, pc,
         max_pages, S, Hq, H, D, bs, most if most < _I32_MAX else _I32_MAX, scale, k_scale, v_scale,
-        ws, wsb, _flag(err_flag, idx), stream)
+        None if ws is None else ws.data_ptr(), wsb, _flag(err_flag, idx), stream)
     return out
 
 
@@ -350,13 +351,12 @@ def select_pages(q: torch.Tensor, bounds: torch.Tensor, block_tables: torch.Tens
         pg = _int32(pages, "pages", idx, (S, H, num_pages))
         pc = _int32(counts, "page counts", idx, (S, H))
     stream = _raw_stream(idx)
-    ws, wsb = _workspace("amf_select_pages_workspace_bytes", (S, H, width, block_size, most),
-                         workspace, dev, stream)
+    ws, wsb = _workspace(_SELECT_WS, (S, H, width, block_size, most), workspace, dev, stream)
     qs, qh, _ = q3.stride()
     _launch(
         idx, "amf_select_pages", q3.data_ptr(), _TAGS[dt], qs, qh, bounds.data_ptr(), nb, bt, row,
-        width, cl, most, S, Hq, H, D, block_size, num_pages, first_pages, last_pages, pg, pc, ws,
-        wsb, _flag(err_flag, idx), stream)
+        width, cl, most, S, Hq, H, D, block_size, num_pages, first_pages, last_pages, pg, pc,
+        None if ws is None else ws.data_ptr(), wsb, _flag(err_flag, idx), stream)
     return pages, counts
 
 
