@@ -487,7 +487,7 @@ extern "C" int amf_page_key_bounds(const void* k, int32_t kv_dtype, int64_t page
     pages = std::min<int64_t>(pages, ((int64_t)max_new_tokens + block_size - 2) / block_size + 1);
   const int64_t chunks = (int64_t)num_kv_heads * head_dim / 8;
   const int64_t groups = (pages * chunks + kThreads - 1) / kThreads;
-  if (chunks > 0x7FFFFFFF || groups > 0x7FFFFFFF)
+  if (chunks > 0x7FFFFFFF || groups > 0xFFFFFF)
     return fail(AMF_ERR_UNSUPPORTED, "%s: %lld pages of %lld channels", who, (long long)pages,
                 (long long)chunks * 8);
   const BoundsArgs a{static_cast<const uint8_t*>(k), page_stride * es, token_stride * es,

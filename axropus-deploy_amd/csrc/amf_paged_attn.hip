@@ -958,8 +958,8 @@ extern "C" int amf_paged_decode_attn(
   const int tile = matrix ? kTileHeads : kGenHeads;
   a.tiles = (a.group + tile - 1) / tile;
   a.out_dtype = out_dtype;
-  a.score_scale = (softmax_scale > 0.0f ? softmax_scale : 1.0f / sqrtf((float)head_dim)) *
-                  k_scale * kLog2e;
+  a.score_scale = (float)((softmax_scale > 0.0f ? (double)softmax_scale : 1.0 / sqrt((double)head_dim)) *
+                          (double)k_scale * 1.4426950408889634);
   a.v_scale = v_scale;
   // the most steps that a pair can have, as far as the host knows
   const int64_t tokens = pages ? (int64_t)max_pages * block_size
@@ -968,7 +968,7 @@ extern "C" int amf_paged_decode_attn(
   a.step_shift = __builtin_ctz(chunk * kWaves);
   const int64_t steps = std::max<int64_t>(1, (tokens + chunk * kWaves - 1) / (chunk * kWaves));
   const int64_t pairs = (int64_t)num_seqs * num_kv_heads * a.tiles;
-  if (pairs > 0x7FFFFFFF || (int64_t)num_seqs * num_q_heads > 0x7FFFFFFF)
+  if (pairs > 0xFFFFFF || (int64_t)num_seqs * num_q_heads > 0x7FFFFFFF)
     return fail(AMF_ERR_UNSUPPORTED, "%s: %d sequences of %d heads", who, num_seqs, num_q_heads);
   a.whole = steps <= kWholeSteps;
   // pairs side by side in a workgroup: their rows lie side by side in memory

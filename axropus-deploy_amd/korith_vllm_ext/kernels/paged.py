@@ -23,6 +23,9 @@ amf_hip.AmfHipUnavailable / RuntimeError.
 
 from __future__ import annotations
 
+import math
+import threading
+from collections import OrderedDict
 from typing import Any, NamedTuple, Optional, Tuple
 
 import torch
@@ -60,6 +63,30 @@ def _launch(idx: int, func: str, *args) -> None:
         amf_hip.check(func, rc)
 
 
+# Scratch kept between calls, one buffer per (device, stream, host thread): a call
+# is two launches, and another thread's may come between them on the same stream.
+# A stream under graph capture gets a buffer of its own per call instead.
+_SCRATCH: "OrderedDict[Tuple[int, int, int], torch.Tensor]" = OrderedDict()
+_SCRATCH_MAX = 16
+_SCRATCH_LOCK = threading.Lock()
+
+
+def _scratch(dev: torch.device, stream: int, nbytes: int) -> torch.Tensor:
+    if torch.cuda.is_current_stream_capturing():
+        return torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    key = (dev.index, stream, threading.get_ident())
+    buf = _SCRATCH.get(key)
+    if buf is not None and buf.numel() >= nbytes:
+        return buf
+    buf = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    with _SCRATCH_LOCK:
+        _SCRATCH[key] = buf
+        _SCRATCH.move_to_end(key)
+        while len(_SCRATCH) > _SCRATCH_MAX:  # a call under way keeps its buffer itself
+            _SCRATCH.popitem(last=False)
+    return buf
+
+
 def _workspace(name: str, sizes: tuple, given: Optional[torch.Tensor], dev: torch.device,
                stream: int) -> Tuple[Optional[torch.Tensor], int]:
     """(workspace, its bytes): the caller's, checked, or the scratch buffer of
@@ -76,7 +103,7 @@ def _workspace(name: str, sizes: tuple, given: Optional[torch.Tensor], dev: torc
         if have < need:
             raise ValueError(f"workspace of {have} bytes, {need} needed")
         return given, have
-    return (_dispatch._scratch(dev, stream, need), need) if need else (None, 0)
+    return (_scratch(dev, stream, need), need) if need else (None, 0)
 
 
 def _cache(k: torch.Tensor, v: Optional[torch.Tensor]) -> tuple:
@@ -212,8 +239,8 @@ def paged_decode_attention(q: torch.Tensor, k_cache: torch.Tensor,
     cl = _int32(context_lens, "context_lens", idx, (S,))
     if scale is None:
         scale = 0.0
-    elif not scale > 0.0:
-        raise ValueError(f"scale must be positive, got {scale}")
+    elif not 1.2e-38 < scale < math.inf:
+        raise ValueError(f"scale must be positive, finite and normal in fp32, got {scale}")
     pg = pc = None
     max_pages = 0
     if pages is not None:
@@ -224,6 +251,7 @@ def paged_decode_attention(q: torch.Tensor, k_cache: torch.Tensor,
         max_pages = pages.shape[2]
         pg = _int32(pages, "pages", idx, (S, H, max_pages))
         pc = _int32(page_counts, "page_counts", idx, (S, H))
+        pg = pg or pc  # lists without room hold nothing (an empty tensor has no address)
     elif page_counts is not None:
         raise ValueError("pages and page_counts come together")
     most = width * bs if max_context_len is None else int(max_context_len)
@@ -236,6 +264,8 @@ def paged_decode_attention(q: torch.Tensor, k_cache: torch.Tensor,
             raise ValueError(f"paged decode: out has shape {tuple(out.shape)}, q {tuple(q.shape)}")
         if out_dtype is not None and out.dtype != out_dtype:
             raise ValueError(f"paged decode: out is {out.dtype}, out_dtype asks for {out_dtype}")
+        if out.data_ptr() == q3.data_ptr() and S > 0:
+            raise ValueError("paged decode: out must not be q (it is read until the end)")
     if out.dtype not in _TAGS:
         raise ValueError(f"paged decode: output dtype {out.dtype} is not bf16/fp16/fp32")
     stream = _raw_stream(idx)

@@ -220,6 +220,59 @@ def test_page_lists(dtype, Hkv, D, block):
     assert not out[1, :4].any() and not out[4].any()
 
 
+def test_lists_without_room_hold_nothing():
+    lens = [40, 100]
+    q, kv, table = _case(BF, 8, 2, 128, 16, lens)
+    out = torch.full_like(q, 5.0)
+    _run(q, kv, table, lens, out=out, pages=torch.zeros(2, 2, 0, dtype=torch.int32, device=DEV),
+         page_counts=torch.full((2, 2), 3, dtype=torch.int32, device=DEV))
+    assert not out.any()
+
+
+@pytest.mark.parametrize("dtype,Hq,Hkv,D,seqs,hi", [
+    (BF, 8, 4, 64, 300, 3000),     # more sequences than shares, four KV heads a workgroup
+    (FP, 4, 2, 128, 40, 5000),     # two KV heads a workgroup
+    (F8, 6, 3, 128, 30, 4000),     # one
+    (BF, 40, 1, 64, 20, 3000),     # three head tiles
+    (F8, 68, 2, 64, 9, 5000),      # four tiles: two of each KV head
+    (BF, 4, 4, 256, 12, 2500),
+    (F32, 8, 2, 64, 25, 2000),     # the general kernel, two tiles of a group
+    (BF, 6, 1, 80, 270, 1500),
+])
+def test_shares_cut_sequences_anywhere(dtype, Hq, Hkv, D, seqs, hi):
+    """Many sequences of any length, most of them cut between workgroups, some
+    empty; a hint that is too small changes nothing but the cut."""
+    g = torch.Generator().manual_seed(seqs + D)
+    lens = torch.randint(1, hi + 1, (seqs,), generator=g)
+    lens[torch.rand(seqs, generator=g) < 0.2] = 0
+    lens[-1] = hi
+    lens = lens.tolist()
+    q, kv, table = _case(dtype, Hq, Hkv, D, 16, lens, seed=2)
+    ref = attend64(q, kv, table, lens, D ** -0.5)
+    out = _run(q, kv, table, lens, out_dtype=F32)
+    _check(out, ref, attend_tolerance(q, kv, lens, D ** -0.5))
+    out = _run(q, kv, table, lens, out_dtype=F32, max_context_len=1)
+    _check(out, ref, attend_tolerance(q, kv, lens, D ** -0.5))
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_every_fp8_code(dtype):
+    """All finite codes as keys and as values: exact in either query type."""
+    codes = torch.tensor([c for c in range(256) if c & 0x7F != 0x7F], dtype=torch.uint8)
+    D, T = 64, 256
+    kv = torch.zeros(2, 16, 16, 1, D, dtype=torch.uint8)
+    kv[0].view(T, D)[:254, 0] = codes
+    kv[1].view(T, D)[:254] = codes[:, None]
+    kv = kv.view(F8).to(DEV)
+    table = torch.arange(16, dtype=torch.int32)[None]
+    q = torch.zeros(1, 2, D, dtype=dtype, device=DEV)
+    q[0, 0, 0], q[0, 1, 0] = 0.0, 2.0 ** -7  # all weights equal; weights of e^-3.5 to e^3.5
+    ref = attend64(q, kv, table, [254], 1.0)
+    out = _run(q, kv, table, [254], scale=1.0, out_dtype=F32)
+    # 254 terms of at most 448 in fp32, weights off by 2^-22
+    assert float((out.cpu().double() - ref).abs().max()) <= 448 * 256 * 2.0 ** -24
+
+
 def test_every_page_listed_equals_no_list():
     lens = [300, 47]
     q, kv, table = _case(BF, 8, 2, 128, 16, lens)
@@ -327,6 +380,32 @@ def test_other_stream_and_shared_scratch():
     assert all(torch.equal(o, want) for o in outs)
 
 
+def test_threads_on_one_stream():
+    """Calls of several host threads on the same stream, whose launches may
+    fall between each other."""
+    import threading
+
+    cases = [_case(BF, 8, 2, 128, 16, [5000 - 900 * i, 2000], seed=i) + ([5000 - 900 * i, 2000],)
+             for i in range(4)]
+    want = [_run(*c) for c in cases]
+    bad, gate = [], threading.Barrier(4)
+    stream = torch.cuda.current_stream()
+
+    def work(i):
+        with torch.cuda.stream(stream):
+            gate.wait()
+            outs = [_run(*cases[i]) for _ in range(40)]
+            torch.cuda.synchronize()
+            bad.extend(i for o in outs if not torch.equal(o, want[i]))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
+
+
 @pytest.mark.parametrize("dtype,D", [(BF, 128), (F32, 80)])
 def test_captured_graph_replays(dtype, D):
     """A captured step replayed with other lengths and pages, eager work
@@ -385,7 +464,8 @@ def test_refusals():
         dict(out=torch.empty(2, 8, 64, dtype=BF, device=DEV)),
         dict(out=torch.empty(2, 8, 128, dtype=BF)),
         dict(out=torch.empty(2, 8, 256, dtype=BF, device=DEV)[..., ::2]),
-        dict(out=torch.empty_like(q), out_dtype=F32),
+        dict(out=torch.empty_like(q), out_dtype=F32), dict(out=q), dict(scale=1e-60),
+        dict(scale=float("inf")), dict(out_dtype=F8),
         dict(workspace=torch.empty(16, device=DEV)),
         dict(err_flag=torch.zeros(1, device=DEV)),
     ]
