@@ -150,11 +150,22 @@ template <bool BF16, int NC, int SETS>
 __global__ __launch_bounds__(kThreads) void page_score_kernel(SelectArgs a) {
   // [dim in step order][set][hi][head] -> (max(q, 0), min(q, 0))
   __shared__ __attribute__((aligned(16))) double q_lds[NC * 8][SETS][4][kHeadSet][2];
+  constexpr int kItems = NC * 4 * SETS * kHeadSet;  // 8 dims of a head to a thread
+  static_assert(kItems <= kThreads, "a thread takes at most one");
   const int s = blockIdx.z, h = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int q_g = tid % (SETS * kHeadSet), q_d = tid / (SETS * kHeadSet);
+  auto load_q = [&](int g0) {
+    u32x4 x{0, 0, 0, 0};
+    if (tid < kItems && 8 * q_d < a.head_dim && g0 + q_g < a.group)
+      x = *reinterpret_cast<const u32x4*>(
+          a.q + s * a.q_seq + ((int64_t)h * a.group + g0 + q_g) * a.q_head + 8 * q_d);
+    return x;
+  };
+  u32x4 q_raw = load_q(0);  // on its way before the lengths are known
   const int64_t n = seq_pages(a, s);
   const int64_t p0 = (int64_t)blockIdx.y * kScorePages;
   if (p0 >= n || n <= a.num_pages) return;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int lo = lane & 15, hi = lane >> 4;
   const int64_t base = p0 + wave * 16;
   const int64_t id = base + lo < n ? a.block_tables[s * a.bt_stride + base + lo] : -1;
@@ -174,18 +185,16 @@ __global__ __launch_bounds__(kThreads) void page_score_kernel(SelectArgs a) {
   double best = -INFINITY;
   int fin = 1;
   for (int g0 = 0; g0 < a.group; g0 += SETS * kHeadSet) {
-    __syncthreads();
-    // 8 dims of a head to a thread (a dim to a thread: 82 -> 89 us as above)
-    for (int i = tid; i < NC * 4 * SETS * kHeadSet; i += kThreads) {
-      const int g = i % (SETS * kHeadSet), d = i / (SETS * kHeadSet);
-      float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-      if (8 * d < a.head_dim && g0 + g < a.group)
-        unpack8<BF16>(*reinterpret_cast<const u32x4*>(
-                          a.q + s * a.q_seq + ((int64_t)h * a.group + g0 + g) * a.q_head + 8 * d),
-                      x);
+    if (g0 > 0) {
+      q_raw = load_q(g0);
+      __syncthreads();
+    }
+    if (tid < kItems) {
+      float x[8];
+      unpack8<BF16>(q_raw, x);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        double* o = q_lds[8 * (d / 4) + e][g / kHeadSet][d % 4][g % kHeadSet];
+        double* o = q_lds[8 * (q_d / 4) + e][q_g / kHeadSet][q_d % 4][q_g % kHeadSet];
         o[0] = x[e] < 0.0f ? 0.0f : x[e];  // a NaN stays one
         o[1] = x[e] < 0.0f ? x[e] : 0.0f;
       }
