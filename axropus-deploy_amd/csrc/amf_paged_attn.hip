@@ -759,14 +759,14 @@ __global__ __launch_bounds__(kThreads, matrix_waves(D)) void paged_attn_matrix_k
 // A workgroup per pair that may be cut and `heads` of its heads: threads take W
 // dims of every n-th partial, several partials loaded ahead of their use, and are
 // joined in LDS.
-template <int W>
-__global__ __launch_bounds__(kThreads) void paged_attn_merge_kernel(PagedArgs a, int heads) {
-  constexpr int kAhead = 4;
-  __shared__ float x_lds[kThreads][W], m_lds[kThreads], l_lds[kThreads];
+template <int W, int NT>
+__global__ __launch_bounds__(NT) void paged_attn_merge_kernel(PagedArgs a, int heads) {
+  constexpr int kAhead = 8;
+  __shared__ float x_lds[NT][W], m_lds[NT], l_lds[NT];
   const Cut cut = a.cuts[blockIdx.x];
   const int tid = threadIdx.x, D = a.head_dim;
   if ((int)blockIdx.y * heads >= cut.heads) return;
-  const int cols = (D + W - 1) / W, rows = kThreads / (cols * heads);
+  const int cols = (D + W - 1) / W, rows = NT / (cols * heads);
   const int r = tid / (cols * heads), g = (int)blockIdx.y * heads + tid % (cols * heads) / cols;
   const int col = tid % cols, row = g * (D + kPartPad);
   float m = -INFINITY, l = 0.0f, x[W];
@@ -998,16 +998,19 @@ extern "C" int amf_paged_decode_attn(
     launch<AMF_DTYPE_F16, AMF_DTYPE_E4M3>(a, groups, matrix, st);
   if (int rc = check_launch(who)) return rc;
   if (a.whole) return ok();
-  // a head to a merge's workgroup where a pair has many partials, else more
+  // partials of a pair, about: many take a workgroup a head, hundreds (one long
+  // context) a larger one (131072 tokens of one KV head 44 -> 26 us a call)
+  const int64_t parts = shares / num_seqs;
   const int32_t tile_heads = std::min<int32_t>(a.group, tile);
   const int cols = matrix ? head_dim / 4 : head_dim;
-  int per = std::max(1, kThreads / cols / (shares >= 4 * (int64_t)num_seqs ? 8 : 2));
-  per = std::min<int>(per, tile_heads);
+  const int per = std::min<int>(tile_heads, std::max(1, kThreads / cols / (parts >= 4 ? 8 : 2)));
   const dim3 grid((unsigned)(std::min<int64_t>(num_seqs, shares) * heads),
                   (unsigned)((tile_heads + per - 1) / per));
-  if (matrix)
-    paged_attn_merge_kernel<4><<<grid, kThreads, 0, st>>>(a, per);
+  if (!matrix)
+    paged_attn_merge_kernel<1, kThreads><<<grid, kThreads, 0, st>>>(a, per);
+  else if (parts >= 64)
+    paged_attn_merge_kernel<4, 1024><<<grid, 1024, 0, st>>>(a, per);
   else
-    paged_attn_merge_kernel<1><<<grid, kThreads, 0, st>>>(a, per);
+    paged_attn_merge_kernel<4, kThreads><<<grid, kThreads, 0, st>>>(a, per);
   return check_launch(who);
 }
