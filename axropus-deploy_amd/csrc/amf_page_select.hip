@@ -246,7 +246,6 @@ __global__ __launch_bounds__(kThreads) void page_score_kernel(SelectArgs a) {
 
 // ---- choice --------------------------------------------------------------------
 
-constexpr int kPickKeys = 8;  // consecutive keys of a thread
 constexpr int kDigit = 11;    // bits
 constexpr int kBins = 1 << kDigit;
 
@@ -280,13 +279,16 @@ __device__ __forceinline__ uint32_t pick_exclusive(uint32_t v, uint32_t* tmp, ui
 // digit (a histogram in LDS each), from the first bit in which the keys differ,
 // so that one or two digits separate scores that share sign and exponent; then
 // the pages above it and the first of its equals are written at their ranks.
-// Forced pages are left out of the search.  Up to NT * kPickKeys keys stay in
-// registers (MANY: they are read again for each pass).
+// Forced pages are left out of the search.  A thread takes KEYS consecutive keys;
+// up to NT * KEYS of a row stay in registers (MANY: they are read again for each
+// pass).
 //
-// Bound by its barriers: three a digit, on 16 waves or, for up to 2048 pages, 4.
-template <int NT, bool MANY>
+// Bound by its barriers, three a digit, and by the 64-bit shifts of a thread's keys:
+// 4063 pages, 8 / 16 / 32 keys a thread on 1024 / 512 / 256 threads, 9.7 / 12.0 /
+// 16.7 us.
+template <int NT, int KEYS, bool MANY>
 __global__ __launch_bounds__(NT) void page_pick_kernel(SelectArgs a) {
-  constexpr int kTile = NT * kPickKeys;
+  constexpr int kTile = NT * KEYS;
   constexpr int kMine = kBins / NT;  // bins of a thread
   __shared__ uint32_t hist[2][kBins];
   __shared__ uint32_t tmp[2][NT / 64];
@@ -309,11 +311,11 @@ __global__ __launch_bounds__(NT) void page_pick_kernel(SelectArgs a) {
     return;
   }
   const uint64_t* keys = a.keys + row * a.max_pages;
-  uint64_t kept[kPickKeys];
+  uint64_t kept[KEYS];
   auto load = [&](int64_t t0) {  // this thread's keys of a tile; 0 behind the last
 #pragma unroll
-    for (int e = 0; e < kPickKeys; ++e) {
-      const int64_t i = t0 + (int64_t)tid * kPickKeys + e;
+    for (int e = 0; e < KEYS; ++e) {
+      const int64_t i = t0 + (int64_t)tid * KEYS + e;
       kept[e] = i < n ? keys[i] : 0;
     }
   };
@@ -329,7 +331,7 @@ __global__ __launch_bounds__(NT) void page_pick_kernel(SelectArgs a) {
   };
   if constexpr (!MANY) load(0);
   auto searched = [&](int64_t t0, int e) {
-    return t0 + (int64_t)tid * kPickKeys + e < n && kept[e] != kForced;
+    return t0 + (int64_t)tid * KEYS + e < n && kept[e] != kForced;
   };
 #pragma unroll
   for (int k = 0; k < kMine; ++k) hist[0][tid + k * NT] = 0;
@@ -337,7 +339,7 @@ __global__ __launch_bounds__(NT) void page_pick_kernel(SelectArgs a) {
   uint64_t lo = ~0ull, hi = 0;
   each_tile([&](int64_t t0) {
 #pragma unroll
-    for (int e = 0; e < kPickKeys; ++e)
+    for (int e = 0; e < KEYS; ++e)
       if (searched(t0, e)) {
         lo = min(lo, kept[e]);
         hi = max(hi, kept[e]);
@@ -372,7 +374,7 @@ __global__ __launch_bounds__(NT) void page_pick_kernel(SelectArgs a) {
     const uint64_t above = shift == 64 ? 0 : cut >> shift;
     each_tile([&](int64_t t0) {
 #pragma unroll
-      for (int e = 0; e < kPickKeys; ++e)
+      for (int e = 0; e < KEYS; ++e)
         if (searched(t0, e) && (shift == 64 || kept[e] >> shift == above))
           atomicAdd(&hist[now][(kept[e] >> next) & (bins - 1)], 1u);
     });
@@ -408,8 +410,8 @@ __global__ __launch_bounds__(NT) void page_pick_kernel(SelectArgs a) {
   each_tile([&](int64_t t0) {
     uint32_t gt = 0, eq = 0;
 #pragma unroll
-    for (int e = 0; e < kPickKeys; ++e) {
-      const bool in = t0 + (int64_t)tid * kPickKeys + e < n;
+    for (int e = 0; e < KEYS; ++e) {
+      const bool in = t0 + (int64_t)tid * KEYS + e < n;
       gt += in && (kept[e] == kForced || kept[e] >> shift > cut);
       eq += in && kept[e] != kForced && kept[e] >> shift == cut;
     }
@@ -418,8 +420,8 @@ __global__ __launch_bounds__(NT) void page_pick_kernel(SelectArgs a) {
     now ^= 1;
     uint32_t g = gt0 + (both >> 16), q = eq0 + (both & 0xFFFFu);
 #pragma unroll
-    for (int e = 0; e < kPickKeys; ++e) {
-      const int64_t i = t0 + (int64_t)tid * kPickKeys + e;
+    for (int e = 0; e < KEYS; ++e) {
+      const int64_t i = t0 + (int64_t)tid * KEYS + e;
       if (i >= n) continue;
       const bool above = kept[e] == kForced || kept[e] >> shift > cut;
       const bool equal = kept[e] != kForced && kept[e] >> shift == cut;
@@ -584,11 +586,13 @@ extern "C" int amf_select_pages(const void* q, int32_t dtype, int64_t q_seq_stri
     if (int rc = check_launch(who)) return rc;
   }
   const dim3 rows((unsigned)num_kv_heads, (unsigned)num_seqs);
-  if (max_pages <= 256 * kPickKeys)
-    page_pick_kernel<256, false><<<rows, 256, 0, st>>>(a);
-  else if (max_pages <= 1024 * kPickKeys)
-    page_pick_kernel<1024, false><<<rows, 1024, 0, st>>>(a);
+  if (max_pages <= 1024)
+    page_pick_kernel<256, 4, false><<<rows, 256, 0, st>>>(a);
+  else if (max_pages <= 4096)
+    page_pick_kernel<1024, 4, false><<<rows, 1024, 0, st>>>(a);
+  else if (max_pages <= 8192)
+    page_pick_kernel<1024, 8, false><<<rows, 1024, 0, st>>>(a);
   else
-    page_pick_kernel<1024, true><<<rows, 1024, 0, st>>>(a);
+    page_pick_kernel<1024, 8, true><<<rows, 1024, 0, st>>>(a);
   return check_launch(who);
 }
