@@ -9,16 +9,22 @@
 // for its KV head.  Each K and V element is read once, for all query heads that
 // share it, and meets the running maximum m and sum l of each head's softmax.
 //
-// Work.  Steps of 4 waves x 32 or 64 tokens; the steps of all sequences, one
-// after the other, are cut into equal shares, and each share is taken by as many
-// workgroups as there are (KV head, head tile) pairs, side by side: they read the
-// same pages at the same time, and the grid is resident as a whole, so every
-// workgroup reads about the same number of tokens whatever the mix of context
-// lengths.  A workgroup finds its share by summing the lengths itself (they are
-// on the device), its waves take a quarter of a step each and are joined in LDS.
-// What of a sequence lies inside one share is finished there; where several share
-// it, each workgroup leaves a partial (acc, m, l), and a second launch joins
-// those.
+// Work.  The contexts of all sequences, one after the other, are steps, cut into
+// equal shares; a share is taken by a few workgroups side by side, each for one, two
+// or four (KV head, head tile) pairs.  They read the same pages at the same time,
+// and the grid is resident as a whole, so every workgroup reads about the same
+// number of tokens whatever the mix of context lengths.  A workgroup finds its share
+// by summing the lengths itself (they are on the device); waves of the same pair
+// split a step's tokens and are joined in LDS.  What of a sequence lies inside one
+// share is finished there; where several share it, each leaves a partial (acc, m,
+// l), and a second launch joins those.  Short contexts take a workgroup per
+// sequence and pair and no second launch.
+//
+// Measured (MI355X, bytes of K and V over the call's time): 32 sequences of 1K-32K
+// tokens, bf16, 32 / 8 heads of 128, 338 us, 6.6 TB/s; 8 x 126K tokens, FP8, 64 / 8
+// heads, 336 us, 6.1 TB/s; 200 chats of 1-1200 tokens, fp16, 101 us, 4.9 TB/s (a share
+// is two sequences there, and the beginning of each is latency); two short contexts
+// 11 us, nothing but latency.  The large ones are bound by HBM.
 #include <algorithm>
 
 #include "amf_attn.h"
@@ -835,14 +841,16 @@ __global__ __launch_bounds__(NT) void paged_attn_merge_kernel(PagedArgs a, int h
 
 // ---- launch --------------------------------------------------------------------
 
-#ifndef PG_WHOLE
-#define PG_WHOLE 8
-#endif
-#ifndef PG_GROUPS
-#define PG_GROUPS 512
-#endif
-constexpr int64_t kGroups = PG_GROUPS;  // workgroups that share a launch's steps
-constexpr int64_t kWholeSteps = PG_WHOLE;
+// Workgroups that share a launch's steps: two a CU, all resident (32 sequences of
+// 1K-32K tokens 364 us; 256: 385, 1024: 372; 2048 tokens of listed pages 28, 32, 33).
+constexpr int64_t kGroups = 512;
+// Short contexts take a workgroup a (sequence, pair) and no merge: at most so many
+// steps and pairs.  8 KV heads of 128, split / whole, us: 1 x 128 tokens 12.4 / 7.0,
+// 1 x 500 12.8 / 11.4, 64 x 500 33 / 26, 160 x 500 61 / 60; but 1 x 1000 13.3 / 17.1, 256
+// x 500 86 / 91, 256 x 128 30 / 37.  (Equal lengths; of mixed ones the longest would
+// decide.)
+constexpr int64_t kWholeSteps = 4;
+constexpr int64_t kWholePairs = 3 * kGroups;
 
 // Floats of a partial, for either kernel.
 int64_t part_floats(int32_t group, int32_t head_dim) {
@@ -970,8 +978,11 @@ extern "C" int amf_paged_decode_attn(
   const int64_t pairs = (int64_t)num_seqs * num_kv_heads * a.tiles;
   if (pairs > 0xFFFFFF || (int64_t)num_seqs * num_q_heads > 0x7FFFFFFF)
     return fail(AMF_ERR_UNSUPPORTED, "%s: %d sequences of %d heads", who, num_seqs, num_q_heads);
-  a.whole = steps <= kWholeSteps;
-  // pairs side by side in a workgroup: their rows lie side by side in memory
+  a.whole = steps <= kWholeSteps && pairs <= kWholePairs;
+  // pairs side by side on the waves of a workgroup: their rows lie side by side in
+  // memory and are asked for at the same time.  32 sequences of 1K-32K tokens 364 us
+  // with one pair a workgroup, 336 with four; page lists differ from head to head,
+  // and a whole sequence has too few workgroups.
   const int64_t heads = (int64_t)num_kv_heads * a.tiles;
   a.side = 1;
   if (matrix && !a.whole && !pages) a.side = heads % 4 == 0 ? 4 : heads % 2 == 0 ? 2 : 1;
