@@ -321,25 +321,48 @@ __device__ __forceinline__ void empty_seqs(const PagedArgs& a) {
 
 // ---- general kernel ------------------------------------------------------------
 //
-// Any element type, head_dim up to 256, strides and alignment: element loads.
-// A lane scores one token of the chunk (two lanes share its dims) and, for PV,
-// owns dims lane, lane + 64, ...
+// Any element type, head_dim up to 256, strides and alignment.  LPR lanes share a
+// token's row, 8 dims each (one or two 16-byte loads, or element by element where
+// rows are not aligned), so a wave reads 64 / LPR rows at once, kGenAhead of them
+// after each other in flight; every such group of lanes keeps its own m, l and
+// output for 4 query heads, and all groups of the workgroup are joined in LDS.
+// fp32, 12 / 4 heads of 96, 2 x 9500 tokens, 58 MB: 37 us, 1.6 TB/s; 32 / 8 of 128, 4 x
+// 9500, 311 MB: 79 us, 3.9 TB/s (a step's rows are not asked for before the last one's
+// are used).  A lane per token for the scores and a lane per dim for the output, with
+// element loads, took 88 us for the first.
 constexpr int kGenHeads = 4;  // query heads of a tile
-constexpr int kChunk = 32;     // tokens of a wave's step
+constexpr int kGenAhead = 4;  // rows of a group of lanes in a step
 
-template <int QDT, int KDT>
-__global__ __launch_bounds__(kThreads) void paged_attn_general_kernel(PagedArgs a) {
+// Eight consecutive elements, `n` of which are there.
+template <int DT>
+__device__ __forceinline__ void load_row8(const uint8_t* p, int n, bool aligned, float* x) {
+  constexpr int ES = DT == AMF_DTYPE_F32 ? 4 : DT == AMF_DTYPE_E4M3 ? 1 : 2;
+  if (n >= 8 && aligned) {
+    if constexpr (DT == AMF_DTYPE_E4M3) {
+      const u32x2 w = *reinterpret_cast<const u32x2*>(p);
+      e4m3x4_to_f32(w[0], x);
+      e4m3x4_to_f32(w[1], x + 4);
+    } else {
+      load8<DT>(p, x);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = e < n ? kv_elem<DT>(p + e * ES) : 0.0f;
+  }
+}
+
+template <int QDT, int KDT, int LPR>
+__global__ __launch_bounds__(kThreads) void paged_attn_general_kernel(PagedArgs a, bool aligned) {
   constexpr int ES = KDT == AMF_DTYPE_F32 ? 4 : KDT == AMF_DTYPE_E4M3 ? 1 : 2;
   constexpr int QS = QDT == AMF_DTYPE_F32 ? 4 : 2;
-  constexpr int DI = kMaxDim / 64;
+  constexpr int RG = 64 / LPR;          // groups of a wave
+  constexpr int PARTS = kWaves * RG;    // of the workgroup
   __shared__ PageRun run;
-  __shared__ float q_lds[kGenHeads][kMaxDim];
-  __shared__ float p_lds[kWaves][kGenHeads][kChunk];
-  __shared__ float acc_lds[kWaves][kGenHeads][kMaxDim];
-  __shared__ float m_lds[kWaves][kGenHeads], l_lds[kWaves][kGenHeads];
+  __shared__ __attribute__((aligned(16))) float acc_lds[PARTS][kGenHeads][8 * LPR];
+  __shared__ float m_lds[PARTS][kGenHeads], l_lds[PARTS][kGenHeads];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int D = a.head_dim, half = lane >> 5;
-  const int d0 = half ? (D + 1) / 2 : 0, d1 = half ? D : (D + 1) / 2;
+  const int D = a.head_dim, c = lane % LPR, grp = lane / LPR, part_id = wave * RG + grp;
+  const int dims = min(8, D - 8 * c);  // of this lane; none below 1
   empty_seqs(a);
   Unit un = find_unit(a);
   if (un.seq < 0) return;
@@ -349,92 +372,86 @@ __global__ __launch_bounds__(kThreads) void paged_attn_general_kernel(PagedArgs 
     const Segment sg = segment_at<kGenHeads>(a, un, u, u1, 0);
     if (tid == 0) note_cut(a, un, sg, u, 0);
     u += sg.st1 - sg.st0;
-    for (int i = tid; i < kGenHeads * D; i += kThreads) {
-      const int g = i / D, d = i - g * D;
+    float q[kGenHeads][8];
+#pragma unroll
+    for (int g = 0; g < kGenHeads; ++g) {
       const int64_t head = sg.head0 - (int64_t)sg.seq * a.num_q_heads + g;
-      q_lds[g][d] = g < sg.heads ? kv_elem<QDT>(static_cast<const uint8_t*>(a.q) +
-                                                (sg.seq * a.q_seq + head * a.q_head + d) * QS)
-                                 : 0.0f;
+      const uint8_t* p = static_cast<const uint8_t*>(a.q) +
+                         (sg.seq * a.q_seq + head * a.q_head + 8 * c) * QS;
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        q[g][e] = g < sg.heads && e < dims ? kv_elem<QDT>(p + e * QS) : 0.0f;
     }
-    float m[kGenHeads], l[kGenHeads], acc[kGenHeads][DI];
+    float m[kGenHeads], l[kGenHeads], acc[kGenHeads][8];
 #pragma unroll
     for (int g = 0; g < kGenHeads; ++g) {
       m[g] = -INFINITY;
       l[g] = 0.0f;
 #pragma unroll
-      for (int i = 0; i < DI; ++i) acc[g][i] = 0.0f;
+      for (int e = 0; e < 8; ++e) acc[g][e] = 0.0f;
     }
     const int64_t hold = run_steps(a);
     for (int64_t r0 = sg.st0; r0 < sg.st1; r0 += hold) {
       const int64_t r1 = min(r0 + hold, sg.st1), j0 = page_of(a, r0 << a.step_shift);
       load_pages(a, sg, r0, r1, run);
       for (int64_t st = r0; st < r1; ++st) {
-        const int64_t off =
-            token_offset(a, sg, run, j0, (st << a.step_shift) + wave * kChunk + (lane & 31));
-        const bool ok = off >= 0;
-        if (!__any(ok)) continue;
-        float x[kGenHeads];
+        float k[kGenAhead][8], v[kGenAhead][8];
+        bool ok[kGenAhead];
 #pragma unroll
-        for (int g = 0; g < kGenHeads; ++g) x[g] = 0.0f;
-        if (ok) {
-          for (int d = d0; d < d1; ++d) {
-            const float kd = kv_elem<KDT>(a.k + off + d * ES);
-#pragma unroll
-            for (int g = 0; g < kGenHeads; ++g) x[g] = __builtin_fmaf(q_lds[g][d], kd, x[g]);
-          }
+        for (int i = 0; i < kGenAhead; ++i) {
+          const int64_t t = (st << a.step_shift) + (wave * kGenAhead + i) * RG + grp;
+          const int64_t off = token_offset(a, sg, run, j0, t);
+          ok[i] = off >= 0;
+          const int n = ok[i] ? dims : 0;
+          load_row8<KDT>(a.k + off + 8 * c * ES, n, aligned, k[i]);
+          load_row8<KDT>(a.v + off + 8 * c * ES, n, aligned, v[i]);
         }
 #pragma unroll
         for (int g = 0; g < kGenHeads; ++g) {
-          x[g] += __shfl_xor(x[g], 32);
-          float top = ok ? x[g] * a.score_scale : -INFINITY;
-          for (int o = 16; o > 0; o >>= 1) top = max_nan(top, __shfl_xor(top, o));
-          const float mn = max_nan(m[g], top);
-          const float p =
-              ok ? __builtin_amdgcn_exp2f(__builtin_fmaf(x[g], a.score_scale, -mn)) : 0.0f;
-          const float w = weight_to(m[g], mn);
+          float x[kGenAhead], top = -INFINITY;
+#pragma unroll
+          for (int i = 0; i < kGenAhead; ++i) {
+            x[i] = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[i] = __builtin_fmaf(q[g][e], k[i][e], x[i]);
+#pragma unroll
+            for (int o = LPR / 2; o > 0; o >>= 1) x[i] += __shfl_xor(x[i], o, LPR);
+            top = max_nan(top, ok[i] ? x[i] * a.score_scale : -INFINITY);
+          }
+          const float mn = max_nan(m[g], top), w = weight_to(m[g], mn);
           m[g] = mn;
-          l[g] = l[g] * w + (half ? 0.0f : p);
+          l[g] *= w;
 #pragma unroll
-          for (int i = 0; i < DI; ++i) acc[g][i] *= w;
-          if (!half) p_lds[wave][g][lane] = p;
-        }
-        __builtin_amdgcn_wave_barrier();
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        for (int j = 0; j < kChunk; ++j) {
-          const int64_t row = __shfl(off, j);
-          if (row < 0) continue;
-          float w[kGenHeads];
+          for (int e = 0; e < 8; ++e) acc[g][e] *= w;
 #pragma unroll
-          for (int g = 0; g < kGenHeads; ++g) w[g] = p_lds[wave][g][j];
+          for (int i = 0; i < kGenAhead; ++i) {
+            const float p =
+                ok[i] ? __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], a.score_scale, -mn)) : 0.0f;
+            l[g] += p;
 #pragma unroll
-          for (int i = 0; i < DI; ++i) {
-            const int d = lane + 64 * i;
-            if (d >= D) continue;
-            const float vd = kv_elem<KDT>(a.v + row + d * ES);
-#pragma unroll
-            for (int g = 0; g < kGenHeads; ++g) acc[g][i] = __builtin_fmaf(w[g], vd, acc[g][i]);
+            for (int e = 0; e < 8; ++e) acc[g][e] = __builtin_fmaf(p, v[i][e], acc[g][e]);
           }
         }
-        __builtin_amdgcn_wave_barrier();
       }
     }
+    __syncthreads();  // the last pair's parts have been read
 #pragma unroll
     for (int g = 0; g < kGenHeads; ++g) {
-      float sum = l[g];
-      for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
-      if (lane == 0) {
-        m_lds[wave][g] = m[g];
-        l_lds[wave][g] = sum;
+      if (c == 0) {
+        m_lds[part_id][g] = m[g];
+        l_lds[part_id][g] = l[g];
       }
 #pragma unroll
-      for (int i = 0; i < DI; ++i) acc_lds[wave][g][lane + 64 * i] = acc[g][i];
+      for (int e = 0; e < 8; e += 4)
+        *reinterpret_cast<f32x4*>(&acc_lds[part_id][g][8 * c + e]) =
+            f32x4{acc[g][e], acc[g][e + 1], acc[g][e + 2], acc[g][e + 3]};
     }
     __syncthreads();
     for (int i = tid; i < sg.heads * D; i += kThreads) {
       const int g = i / D, d = i - g * D;
       float top = m_lds[0][g], sum = 0.0f, x = 0.0f;
-      for (int w = 1; w < kWaves; ++w) top = max_nan(top, m_lds[w][g]);
-      for (int w = 0; w < kWaves; ++w) {
+      for (int w = 1; w < PARTS; ++w) top = max_nan(top, m_lds[w][g]);
+      for (int w = 0; w < PARTS; ++w) {
         const float f = weight_to(m_lds[w][g], top);
         sum = __builtin_fmaf(l_lds[w][g], f, sum);
         x = __builtin_fmaf(acc_lds[w][g][d], f, x);
@@ -455,7 +472,7 @@ __global__ __launch_bounds__(kThreads) void paged_attn_general_kernel(PagedArgs 
 
 // ---- matrix kernel -------------------------------------------------------------
 //
-// bf16 and fp16 queries, head_dim 64, 128 or 256, rows of whole 16-byte vectors.
+// bf16 and fp16 queries, head_dim a multiple of 16, rows of whole 16-byte vectors.
 // A wave takes blocks of 32 tokens and up to 16 query heads on 16x16x32 tiles; lane
 // (lo, hi) = (lane % 16, lane / 16).
 //
@@ -504,7 +521,9 @@ constexpr int matrix_waves(int D) { return D == 256 ? 1 : 2; }  // per SIMD, at 
 // (8 x 128K 342 / 335 us).
 constexpr int matrix_chunk(int D) { return D <= 64 ? 64 : 32; }
 
-template <int QDT, int KDT, int D>
+// D: the head_dim, or (FULL false) the next of 64, 128 and 256 above a multiple of
+// 16, with zeros in the dims that are not there.
+template <int QDT, int KDT, int D, bool FULL>
 __global__ __launch_bounds__(kThreads, matrix_waves(D)) void paged_attn_matrix_kernel(PagedArgs a) {
   constexpr bool FP8 = KDT == AMF_DTYPE_E4M3;
   constexpr bool V16 = KDT == AMF_DTYPE_F16;  // V in two terms
@@ -521,6 +540,7 @@ __global__ __launch_bounds__(kThreads, matrix_waves(D)) void paged_attn_matrix_k
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lo = lane & 15, hi = lane >> 4;
+  const int dim = FULL ? D : a.head_dim;
   empty_seqs(a);
   Unit un = find_unit(a);
   if (un.seq < 0) return;
@@ -538,7 +558,7 @@ __global__ __launch_bounds__(kThreads, matrix_waves(D)) void paged_attn_matrix_k
     for (int ks = 0; ks < KS; ++ks) {
       const int d = FP8 ? 64 * (ks / 2) + 16 * hi + 8 * (ks % 2) : 32 * ks + 8 * hi;
       qf[ks] = u32x4{0, 0, 0, 0};
-      if (lo < sg.heads) {
+      if (lo < sg.heads && (FULL || d < dim)) {
         const int64_t head = sg.head0 - (int64_t)sg.seq * a.num_q_heads + lo;
         qf[ks] = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.q) +
                                                  sg.seq * a.q_seq + head * a.q_head + d);
@@ -558,7 +578,11 @@ __global__ __launch_bounds__(kThreads, matrix_waves(D)) void paged_attn_matrix_k
         const int64_t o = __shfl(off, 16 * i + lo);
         const uint8_t* p = a.k + (o < 0 ? head_off : o) + 16 * hi;
 #pragma unroll
-        for (int n = 0; n < KL; ++n) kr[i][n] = *reinterpret_cast<const u32x4*>(p + 64 * n);
+        for (int n = 0; n < KL; ++n) {
+          if (!FULL) kr[i][n] = u32x4{0, 0, 0, 0};
+          if (FULL || 16 * hi + 64 * n < dim * ES)
+            kr[i][n] = *reinterpret_cast<const u32x4*>(p + 64 * n);
+        }
       }
     };
     auto load_v = [&](int64_t off) {
@@ -566,6 +590,11 @@ __global__ __launch_bounds__(kThreads, matrix_waves(D)) void paged_attn_matrix_k
       for (int r = 0; r < 8 * NB; ++r) {
         const int64_t o = __shfl(off, 16 * (r / 4) + 4 * hi + r % 4);
         const uint8_t* p = a.v + (o < 0 ? head_off : o) + DP * ES * lo;
+        if (!FULL) {
+#pragma unroll
+          for (int w = 0; w < VW; ++w) vr[r][w] = 0;
+          if (DP * lo >= dim) continue;
+        }
         if constexpr (VW >= 4) {
 #pragma unroll
           for (int n = 0; n < VW / 4; ++n) {
@@ -731,8 +760,8 @@ __global__ __launch_bounds__(kThreads, matrix_waves(D)) void paged_attn_matrix_k
     __syncthreads();
     for (int n = 0; n < a.side; ++n) {
       const Segment sn = segment_at<kTileHeads>(a, un, u_here, u1, n);
-      for (int i = tid; i < sn.heads * (D / 4); i += kThreads) {
-        const int g = i / (D / 4), d = 4 * (i - g * (D / 4));
+      for (int i = tid; i < sn.heads * (dim / 4); i += kThreads) {
+        const int g = i / (dim / 4), d = 4 * (i - g * (dim / 4));
         float top = m_lds[n][g], sum = 0.0f;
         f32x4 x{0, 0, 0, 0};
         for (int w = n + a.side; w < kWaves; w += a.side) top = max_nan(top, m_lds[w][g]);
@@ -746,13 +775,13 @@ __global__ __launch_bounds__(kThreads, matrix_waves(D)) void paged_attn_matrix_k
             x = f32x4{0, 0, 0, 0};
           else
             x *= a.v_scale / sum;
-          store4(a.out, a.out_dtype, (sn.head0 + g) * D + d, x);
+          store4(a.out, a.out_dtype, (sn.head0 + g) * dim + d, x);
         } else {
-          float* part = sn.part + g * (D + kPartPad);
+          float* part = sn.part + g * (dim + kPartPad);
           *reinterpret_cast<f32x4*>(part + d) = x;
           if (d == 0) {
-            part[D] = top;
-            part[D + 1] = sum;
+            part[dim] = top;
+            part[dim + 1] = sum;
           }
         }
       }
@@ -864,21 +893,39 @@ int64_t part_places(int32_t num_kv_heads, int32_t group) {
                            (int64_t)num_kv_heads * ((group + kGenHeads - 1) / kGenHeads));
 }
 
+// The tile of head_dim in the matrix kernel.
+int matrix_dim(int32_t head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256; }
+
+// Lanes that share a row in the general kernel, and tokens of its steps.
+int general_lanes(int32_t head_dim) {
+  return head_dim <= 64 ? 8 : head_dim <= 128 ? 16 : 32;
+}
+
+template <int QDT, int KDT, int D>
+void launch_matrix(const PagedArgs& a, dim3 grid, hipStream_t st) {
+  if (a.head_dim == D)
+    paged_attn_matrix_kernel<QDT, KDT, D, true><<<grid, kThreads, 0, st>>>(a);
+  else
+    paged_attn_matrix_kernel<QDT, KDT, D, false><<<grid, kThreads, 0, st>>>(a);
+}
+
 template <int QDT, int KDT>
-void launch(const PagedArgs& a, int64_t groups, bool matrix, hipStream_t st) {
+void launch(const PagedArgs& a, int64_t groups, bool matrix, bool aligned, hipStream_t st) {
   const dim3 grid((unsigned)groups);
   if constexpr (QDT != AMF_DTYPE_F32) {
     if (matrix) {
-      if (a.head_dim == 64)
-        paged_attn_matrix_kernel<QDT, KDT, 64><<<grid, kThreads, 0, st>>>(a);
-      else if (a.head_dim == 128)
-        paged_attn_matrix_kernel<QDT, KDT, 128><<<grid, kThreads, 0, st>>>(a);
-      else
-        paged_attn_matrix_kernel<QDT, KDT, 256><<<grid, kThreads, 0, st>>>(a);
-      return;
+      switch (matrix_dim(a.head_dim)) {
+        case 64: return launch_matrix<QDT, KDT, 64>(a, grid, st);
+        case 128: return launch_matrix<QDT, KDT, 128>(a, grid, st);
+        default: return launch_matrix<QDT, KDT, 256>(a, grid, st);
+      }
     }
   }
-  paged_attn_general_kernel<QDT, KDT><<<grid, kThreads, 0, st>>>(a);
+  switch (general_lanes(a.head_dim)) {
+    case 8: paged_attn_general_kernel<QDT, KDT, 8><<<grid, kThreads, 0, st>>>(a, aligned); break;
+    case 16: paged_attn_general_kernel<QDT, KDT, 16><<<grid, kThreads, 0, st>>>(a, aligned); break;
+    default: paged_attn_general_kernel<QDT, KDT, 32><<<grid, kThreads, 0, st>>>(a, aligned);
+  }
 }
 
 }  // namespace
@@ -958,11 +1005,14 @@ extern "C" int amf_paged_decode_attn(
   a.block_size = block_size;
   a.block_shift = (block_size & (block_size - 1)) == 0 ? __builtin_ctz(block_size) : -1;
   a.group = num_q_heads / num_kv_heads;
-  // rows that 16-byte loads and stores reach
+  // rows that 16-byte loads and stores reach; 8 elements at a time in the general
+  // kernel
   const int64_t bits = (int64_t)((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) |
                        a.page_stride | a.token_stride | a.head_stride |
                        (q_seq_stride * qs) | (q_head_stride * qs);
-  const bool matrix = qs == 2 && split_head_dim(head_dim) && aligned16(bits);
+  const bool matrix = qs == 2 && head_dim % 16 == 0 && aligned16(bits);
+  const bool aligned = ((((uintptr_t)k | (uintptr_t)v) | a.page_stride | a.token_stride |
+                         a.head_stride) & (8 * es > 16 ? 15 : 8 * es - 1)) == 0;
   const int tile = matrix ? kTileHeads : kGenHeads;
   a.tiles = (a.group + tile - 1) / tile;
   a.out_dtype = out_dtype;
@@ -972,7 +1022,8 @@ extern "C" int amf_paged_decode_attn(
   // the most steps that a pair can have, as far as the host knows
   const int64_t tokens = pages ? (int64_t)max_pages * block_size
                                : std::min<int64_t>(max_context_len, (int64_t)table_pages * block_size);
-  const int chunk = matrix ? matrix_chunk(head_dim) : kChunk;
+  const int chunk = matrix ? matrix_chunk(matrix_dim(head_dim))
+                           : 64 / general_lanes(head_dim) * kGenAhead;
   a.step_shift = __builtin_ctz(chunk * kWaves);
   const int64_t steps = std::max<int64_t>(1, (tokens + chunk * kWaves - 1) / (chunk * kWaves));
   const int64_t pairs = (int64_t)num_seqs * num_kv_heads * a.tiles;
@@ -998,15 +1049,15 @@ extern "C" int amf_paged_decode_attn(
   a.err_flag = err_flag;
   hipStream_t st = as_stream(stream);
   if (kv_dtype == AMF_DTYPE_BF16)
-    launch<AMF_DTYPE_BF16, AMF_DTYPE_BF16>(a, groups, matrix, st);
+    launch<AMF_DTYPE_BF16, AMF_DTYPE_BF16>(a, groups, matrix, aligned, st);
   else if (kv_dtype == AMF_DTYPE_F16)
-    launch<AMF_DTYPE_F16, AMF_DTYPE_F16>(a, groups, matrix, st);
+    launch<AMF_DTYPE_F16, AMF_DTYPE_F16>(a, groups, matrix, aligned, st);
   else if (kv_dtype == AMF_DTYPE_F32)
-    launch<AMF_DTYPE_F32, AMF_DTYPE_F32>(a, groups, matrix, st);
+    launch<AMF_DTYPE_F32, AMF_DTYPE_F32>(a, groups, matrix, aligned, st);
   else if (q_dtype == AMF_DTYPE_BF16)
-    launch<AMF_DTYPE_BF16, AMF_DTYPE_E4M3>(a, groups, matrix, st);
+    launch<AMF_DTYPE_BF16, AMF_DTYPE_E4M3>(a, groups, matrix, aligned, st);
   else
-    launch<AMF_DTYPE_F16, AMF_DTYPE_E4M3>(a, groups, matrix, st);
+    launch<AMF_DTYPE_F16, AMF_DTYPE_E4M3>(a, groups, matrix, aligned, st);
   if (int rc = check_launch(who)) return rc;
   if (a.whole) return ok();
   // partials of a pair, about: many take a workgroup a head, hundreds (one long

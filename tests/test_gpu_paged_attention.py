@@ -65,6 +65,14 @@ SHAPES = [
     (FP, 5, 1, 33, 16, [50, 7], "thd"),        # odd head_dim
     (F8, 6, 3, 24, 8, [44], "thd"),
     (BF, 3, 3, 1, 4, [9], "thd"),
+    (FP, 8, 4, 112, 16, [200, 31], "thd"),     # multiples of 16 below a tile's dims
+    (BF, 8, 8, 16, 16, [300], "htd"),
+    (F8, 8, 8, 96, 16, [500, 3], "thd"),
+    (F8, 6, 2, 48, 32, [130], "htd"),
+    (BF, 16, 1, 144, 16, [90, 700], "thd"),
+    (F8, 4, 2, 240, 16, [65], "thd"),
+    (F32, 4, 4, 250, 16, [40, 600], "thd"),
+    (F32, 9, 1, 64, 16, [1000], "thd"),        # three tiles of a group
 ]
 
 
@@ -238,6 +246,7 @@ def test_lists_without_room_hold_nothing():
     (BF, 4, 4, 256, 12, 2500),
     (F32, 8, 2, 64, 25, 2000),     # the general kernel, two tiles of a group
     (BF, 6, 1, 80, 270, 1500),
+    (F32, 4, 4, 100, 300, 1200),
 ])
 def test_shares_cut_sequences_anywhere(dtype, Hq, Hkv, D, seqs, hi):
     """Many sequences of any length, most of them cut between workgroups, some
