@@ -896,7 +896,7 @@ int64_t part_places(int32_t num_kv_heads, int32_t group) {
 // The tile of head_dim in the matrix kernel.
 int matrix_dim(int32_t head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256; }
 
-// Lanes that share a row in the general kernel, and tokens of its steps.
+// Lanes that share a row in the general kernel.
 int general_lanes(int32_t head_dim) {
   return head_dim <= 64 ? 8 : head_dim <= 128 ? 16 : 32;
 }
@@ -1040,7 +1040,8 @@ extern "C" int amf_paged_decode_attn(
   if (a.side > 1) a.step_shift -= a.side / 2;
   const int64_t teams = heads / a.side;
   const int64_t most_steps = num_seqs * ((tokens + (1 << a.step_shift) - 1) >> a.step_shift);
-  const int64_t shares = std::min(std::max<int64_t>(kGroups / teams, 1), most_steps);
+  const int64_t shares =
+      std::max<int64_t>(1, std::min(std::max<int64_t>(kGroups / teams, 1), most_steps));
   const int64_t groups = (a.whole ? num_seqs : shares) * teams;
   a.by_seq = num_seqs < shares;
   a.cuts = static_cast<Cut*>(workspace);

@@ -67,12 +67,14 @@ __global__ __launch_bounds__(kThreads) void slot_maps_kernel(SlotArgs a) {
     if (s < a.num_seqs) {
       c = max(a.context_lens[s], 0);
       n = max(a.new_tokens[s], 0);
-      const int64_t need = (c + n + a.block_size - 1) / a.block_size;
-      fits = need <= a.table_pages && c + n <= 0x7FFFFFFF;
-      if (fits) grow = need - (c + a.block_size - 1) / a.block_size;
     }
     int64_t rows_all, grown_all;
     const int64_t row = rows + block_exclusive<kThreads>(n, tmp, &rows_all);
+    if (s < a.num_seqs) {
+      const int64_t need = (c + n + a.block_size - 1) / a.block_size;
+      fits = need <= a.table_pages && c + n <= 0x7FFFFFFF && (n == 0 || row + n <= a.num_tokens);
+      if (fits) grow = need - (c + a.block_size - 1) / a.block_size;
+    }
     const int64_t place = grown + block_exclusive<kThreads>(grow, tmp, &grown_all);
     if (!fits) flags |= AMF_ERRFLAG_CONTEXT;
     if (fits && grow > 0 && place + grow > avail) {
@@ -134,7 +136,6 @@ __global__ __launch_bounds__(kThreads) void slot_maps_kernel(SlotArgs a) {
       a.query_start[a.num_seqs] = (int32_t)min(rows, (int64_t)0x7FFFFFFF);
       if (a.free_used_out) *a.free_used_out = (int32_t)(used + ends[0]);
     }
-    if (rows > a.num_tokens) flags |= AMF_ERRFLAG_CONTEXT;
   }
   if (flags && a.err_flag) atomicOr(a.err_flag, flags);
 }

@@ -264,8 +264,11 @@ def paged_decode_attention(q: torch.Tensor, k_cache: torch.Tensor,
             raise ValueError(f"paged decode: out has shape {tuple(out.shape)}, q {tuple(q.shape)}")
         if out_dtype is not None and out.dtype != out_dtype:
             raise ValueError(f"paged decode: out is {out.dtype}, out_dtype asks for {out_dtype}")
-        if out.data_ptr() == q3.data_ptr() and S > 0:
-            raise ValueError("paged decode: out must not be q (it is read until the end)")
+        if S > 0:  # q is read until the end
+            st, at = q3.stride(), q3.data_ptr()
+            end = at + ((S - 1) * st[0] + (Hq - 1) * st[1] + D) * q3.element_size()
+            if at < out.data_ptr() + out.numel() * out.element_size() and out.data_ptr() < end:
+                raise ValueError("paged decode: out must not lie in q")
     if out.dtype not in _TAGS:
         raise ValueError(f"paged decode: output dtype {out.dtype} is not bf16/fp16/fp32")
     stream = _raw_stream(idx)
@@ -293,6 +296,8 @@ def page_key_bounds(k_cache: torch.Tensor, block_tables: torch.Tensor,
     most tokens that a sequence got (it sizes the grid: no sequence may have
     got more).  bounds [pages, Hkv, 2, D] of the cache's type (FP8: dtype, bf16
     by default) is updated in place, or made (zeros where nothing is written).
+    Sequences that share a page have to use as many tokens of it, as those do
+    that share a prefix in whole pages; else the bounds are either's.
     Returns bounds."""
     idx, kp, _, ps, ts, hs, nb, bs, H, D = _cache(k_cache, None)
     kdt = k_cache.dtype
@@ -365,8 +370,8 @@ def select_pages(q: torch.Tensor, bounds: torch.Tensor, block_tables: torch.Tens
     if num_pages <= 0 or first_pages < 0 or last_pages < 0 or first_pages + last_pages > num_pages:
         raise ValueError(f"num_pages {num_pages} has to hold first_pages {first_pages} and "
                          f"last_pages {last_pages}")
-    if block_size <= 0:
-        raise ValueError(f"block_size must be positive, got {block_size}")
+    if not 0 < block_size <= _I32_MAX:
+        raise ValueError(f"block_size must be positive and an int32, got {block_size}")
     most = width * block_size if max_context_len is None else int(max_context_len)
     if most < 0:
         raise ValueError(f"max_context_len must not be negative, got {max_context_len}")
@@ -417,9 +422,10 @@ def build_slot_maps(context_lens: torch.Tensor, new_tokens: torch.Tensor,
     already.  The slots go to amf_kv_scatter_slots (or an engine's own cache
     write) as they are.
 
-    A sequence whose pages the free list or its table row does not hold keeps
-    its length and gets slots of -1 (AMF_ERRFLAG_FREE_LIST / _CONTEXT in
-    err_flag), as do page ids outside [0, pool_pages)."""
+    A sequence whose pages the free list or its table row does not hold, or
+    whose tokens the rows do not, keeps its length and gets slots of -1
+    (AMF_ERRFLAG_FREE_LIST / _CONTEXT in err_flag); so do tokens of page ids
+    outside [0, pool_pages) (_BLOCK_RANGE), whose sequence grows."""
     if not isinstance(block_tables, torch.Tensor):
         raise TypeError("block_tables must be an int32 tensor")
     idx = block_tables.get_device()
@@ -428,7 +434,7 @@ def build_slot_maps(context_lens: torch.Tensor, new_tokens: torch.Tensor,
     bt, row, S, width = _table(block_tables, idx, None)
     cl = _int32(context_lens, "context_lens", idx, (S,))
     nt = _int32(new_tokens, "new_tokens", idx, (S,))
-    if block_size <= 0 or num_tokens < 0:
+    if not 0 < block_size <= _I32_MAX or num_tokens < 0:
         raise ValueError(f"bad block_size {block_size} or num_tokens {num_tokens}")
     if pool_pages is None:
         pool_pages = _I32_MAX

@@ -5,7 +5,8 @@
  * Scope: paged gather/scatter between a vLLM-style paged KV cache and the AMF
  * VRAM tier, the FP8 (e4m3fn) and INT4 codecs of the compressed VRAM pool
  * (quantize-on-save, dequantize+scatter-on-restore), and paged GQA decode
- * attention that reads INT4 KV with fused dequantization.
+ * attention that reads INT4 KV with fused dequantization, or vLLM's own cache
+ * in place, whole or in part, with the slot maps of a step.
  *
  * Conventions shared by every entry point
  * ---------------------------------------
@@ -413,8 +414,9 @@ int amf_paged_decode_attn(const void* q, int32_t q_dtype, int64_t q_seq_stride,
  * smallest, then the largest key of a page per channel, over the page's tokens
  * inside the context, for the pages of each sequence from the one of token
  * first_tokens[s] on (NULL: all).  max_new_tokens > 0 promises
- * context_lens[s] - first_tokens[s] <= max_new_tokens and sizes the grid.  Of
- * a page that sequences share, one sequence's bounds stay.  bounds_dtype is
+ * context_lens[s] - first_tokens[s] <= max_new_tokens and sizes the grid.
+ * Sequences that share a page have to use as many tokens of it (a prefix in
+ * whole pages does); else one's bounds stay, of either.  bounds_dtype is
  * kv_dtype, or for _E4M3 keys (taken without k_scale) bf16 or fp16; fp32
  * caches are AMF_ERR_UNSUPPORTED.  head_dim a multiple of 8 up to 256; keys and
  * strides aligned to 8 elements.  NaN keys make NaN bounds. */
@@ -433,10 +435,11 @@ int amf_page_key_bounds(const void* k, int32_t kv_dtype, int64_t page_stride,
  * and last last_pages always among them.  pages int32
  * [num_seqs][num_kv_heads][num_pages]: places in the block table in ascending
  * order, -1 behind the page_counts[s][h] = min(num_pages, pages of s) of them.
- * A page whose score is not finite ranks above all that are.  q, its strides
+ * A page with a bound or a score that is not finite ranks above the others.  q, its strides
  * and bounds 16-byte aligned, of one dtype (bf16 or fp16).
  * max_context_len: at least every context length (longer ones are cut, flagged
- * AMF_ERRFLAG_CONTEXT).  workspace: amf_select_pages_workspace_bytes() bytes, 8-byte
+ * AMF_ERRFLAG_CONTEXT); more than 65535 * 64 pages of a sequence are
+ * AMF_ERR_UNSUPPORTED.  workspace: amf_select_pages_workspace_bytes() bytes, 8-byte
  * aligned; calls sharing one must be ordered on one stream. */
 int64_t amf_select_pages_workspace_bytes(int32_t num_seqs, int32_t num_kv_heads,
                                          int32_t table_pages, int32_t block_size,
@@ -462,12 +465,11 @@ int amf_select_pages(const void* q, int32_t dtype, int64_t q_seq_stride, int64_t
  * *free_used + pages taken (free_used NULL = 0).  Outputs must not overlap
  * inputs.  num_tokens: rows of slot_mapping and positions; rows behind the last
  * token get slot -1 and position 0.
- * A sequence whose pages its table row cannot hold (AMF_ERRFLAG_CONTEXT), or
- * that the free list no longer holds (AMF_ERRFLAG_FREE_LIST; so do later ones
- * that need pages), gets none: its context_out is context_lens, its slots are
- * -1.  A page id outside [0, pool_pages) gives slots of -1
- * (AMF_ERRFLAG_BLOCK_RANGE); more tokens than num_tokens are left out
- * (AMF_ERRFLAG_CONTEXT).
+ * A sequence whose pages its table row cannot hold, or whose tokens reach
+ * behind num_tokens (AMF_ERRFLAG_CONTEXT), or whose pages the free list no
+ * longer holds (AMF_ERRFLAG_FREE_LIST; so do later ones that need pages), gets
+ * none: its context_out is context_lens, its slots are -1.  A page id outside
+ * [0, pool_pages) gives slots of -1 (AMF_ERRFLAG_BLOCK_RANGE).
  * Replaces the slots of AMFReqMeta.make (amf_kv_connector.py:90-115), built on
  * the host per request. */
 int amf_build_slot_maps(const int32_t* context_lens, const int32_t* new_tokens,

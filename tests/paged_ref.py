@@ -133,7 +133,7 @@ def slot_maps_ref(lens, new, table, block, rows, free=(), used=0, pool=1 << 31):
     for s, (c, n) in enumerate(zip(lens, new)):
         c, n = max(c, 0), max(n, 0)
         have, need = -(-c // block), -(-(c + n) // block)
-        ok = need <= width
+        ok = need <= width and (n == 0 or len(slots) + n <= rows)
         if not ok:
             flags |= 2
         elif need > have:
@@ -158,8 +158,6 @@ def slot_maps_ref(lens, new, table, block, rows, free=(), used=0, pool=1 << 31):
             slots.append(slot)
         starts.append(len(slots))
         out.append(c + n if ok else c)
-    if len(slots) > rows:
-        flags |= 2
     pad = max(0, rows - len(slots))
     return (slots[:rows] + [-1] * pad, pos[:rows] + [0] * pad, starts, out, used + end, table,
             flags)

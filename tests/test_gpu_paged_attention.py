@@ -228,6 +228,28 @@ def test_page_lists(dtype, Hkv, D, block):
     assert not out[1, :4].any() and not out[4].any()
 
 
+@pytest.mark.parametrize("what", ["lists", "tables", "hint"])
+def test_many_sequences_and_no_tokens_that_the_host_knows_of(what):
+    """More pairs than a workgroup each is for, and nothing to cut: zeros, or with a
+    max_context_len that is too small for the lengths still their attention."""
+    lens, kw = [3 + s % 60 for s in range(420)], {}
+    q, kv, table = _case(BF, 8, 4, 64, 16, lens)
+    ref = torch.zeros(len(lens), 8, 64, dtype=torch.float64)
+    if what == "lists":
+        kw = dict(pages=torch.empty((len(lens), 4, 0), dtype=torch.int32, device=DEV),
+                  page_counts=torch.zeros((len(lens), 4), dtype=torch.int32, device=DEV))
+    elif what == "tables":
+        table = table[:, :0].contiguous()
+    else:
+        kw = dict(max_context_len=0)
+        ref = attend64(q, kv, table, lens, 64 ** -0.5)
+    out = _run(q, kv, table, lens, out_dtype=F32, **kw)
+    if what == "hint":
+        _check(out, ref, attend_tolerance(q, kv, lens, 64 ** -0.5))
+    else:
+        assert torch.equal(out.cpu().double(), ref)
+
+
 def test_lists_without_room_hold_nothing():
     lens = [40, 100]
     q, kv, table = _case(BF, 8, 2, 128, 16, lens)
@@ -459,6 +481,7 @@ def test_refusals():
 
     pages = torch.zeros(2, 2, 3, dtype=torch.int32, device=DEV)
     counts = torch.zeros(2, 2, dtype=torch.int32, device=DEV)
+    three = torch.zeros(3, 8, 128, dtype=BF, device=DEV)
     bad = [
         dict(q=q.half()), dict(q=q.float()), dict(q=q[:, :7]), dict(q=q[..., :64]),
         dict(q=q[0]), dict(q=torch.stack([q, q], 2)), dict(q=q.cpu()), dict(k=kv[0, 0]),
@@ -474,6 +497,7 @@ def test_refusals():
         dict(out=torch.empty(2, 8, 128, dtype=BF)),
         dict(out=torch.empty(2, 8, 256, dtype=BF, device=DEV)[..., ::2]),
         dict(out=torch.empty_like(q), out_dtype=F32), dict(out=q), dict(scale=1e-60),
+        dict(max_context_len=-1), dict(q=three[:2], out=three[1:]),
         dict(scale=float("inf")), dict(out_dtype=F8),
         dict(workspace=torch.empty(16, device=DEV)),
         dict(err_flag=torch.zeros(1, device=DEV)),

@@ -106,6 +106,19 @@ def test_bad_pages_and_too_few_rows():
     _compare(lens, new, 16, 10, table, free)
 
 
+def test_sequences_behind_the_rows_do_not_grow():
+    """Their new pages have no rows that would write them into the table."""
+    table, free = _start([16, 16, 16], 16, torch.Generator().manual_seed(6), 2)
+    m = _compare([16, 16, 16], [2, 2, 2], 16, 5, table, free)
+    assert m.context_lens.tolist() == [18, 18, 16] and m.slot_mapping[4] == -1
+    g = torch.Generator().manual_seed(7)
+    lens = torch.randint(0, 40, (700,), generator=g).tolist()
+    new = torch.randint(0, 9, (700,), generator=g).tolist()
+    for rows in (0, 1, sum(new) // 2, sum(new) - 1):
+        table, free = _start(lens, 16, g, 2)
+        _compare(lens, new, 16, rows, table, free, used=2)
+
+
 def test_outputs_given_and_refusals():
     from korith_vllm_ext.kernels import SlotMaps, build_slot_maps
 
