@@ -323,21 +323,23 @@ __device__ __forceinline__ void empty_seqs(const PagedArgs& a) {
 //
 // Any element type, head_dim up to 256, strides and alignment.  LPR lanes share a
 // token's row, 8 dims each (one or two 16-byte loads, or element by element where
-// rows are not aligned), so a wave reads 64 / LPR rows at once, kGenAhead of them
+// rows are not aligned or end inside one), so a wave reads 64 / LPR rows at once, kGenAhead of them
 // after each other in flight; every such group of lanes keeps its own m, l and
 // output for 4 query heads, and all groups of the workgroup are joined in LDS.
-// fp32, 12 / 4 heads of 96, 2 x 9500 tokens, 58 MB: 37 us, 1.6 TB/s; 32 / 8 of 128, 4 x
-// 9500, 311 MB: 79 us, 3.9 TB/s (a step's rows are not asked for before the last one's
-// are used).  A lane per token for the scores and a lane per dim for the output, with
-// element loads, took 88 us for the first.
+// fp32, 12 / 4 heads of 96, 2 x 9500 tokens, 58 MB: 34 us, 1.7 TB/s; 32 / 8 of 128, 4 x
+// 9500, 311 MB: 79 us, 4.0 TB/s, where the beginning and the merge are some 20 us.  A
+// branch around the loads, in place of page 0's rows, 37 and 79 us; the next step's rows
+// asked for before this one's are used 34 and 79; a lane per token for the scores and a
+// lane per dim for the output, with element loads, 88 us for the first.
 constexpr int kGenHeads = 4;  // query heads of a tile
 constexpr int kGenAhead = 4;  // rows of a group of lanes in a step
 
-// Eight consecutive elements, `n` of which are there.
-template <int DT>
-__device__ __forceinline__ void load_row8(const uint8_t* p, int n, bool aligned, float* x) {
+// Eight consecutive elements, `n` of which are there.  ROWS: all or none are, and the
+// first 8 at p can be read all the same: no branch, whose end would wait for the load.
+template <int DT, bool ROWS>
+__device__ __forceinline__ void load_row8(const uint8_t* p, int n, float* x) {
   constexpr int ES = DT == AMF_DTYPE_F32 ? 4 : DT == AMF_DTYPE_E4M3 ? 1 : 2;
-  if (n >= 8 && aligned) {
+  if constexpr (ROWS) {
     if constexpr (DT == AMF_DTYPE_E4M3) {
       const u32x2 w = *reinterpret_cast<const u32x2*>(p);
       e4m3x4_to_f32(w[0], x);
@@ -345,14 +347,16 @@ __device__ __forceinline__ void load_row8(const uint8_t* p, int n, bool aligned,
     } else {
       load8<DT>(p, x);
     }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = n > 0 ? x[e] : 0.0f;
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] = e < n ? kv_elem<DT>(p + e * ES) : 0.0f;
   }
 }
 
-template <int QDT, int KDT, int LPR>
-__global__ __launch_bounds__(kThreads) void paged_attn_general_kernel(PagedArgs a, bool aligned) {
+template <int QDT, int KDT, int LPR, bool ROWS>
+__global__ __launch_bounds__(kThreads) void paged_attn_general_kernel(PagedArgs a) {
   constexpr int ES = KDT == AMF_DTYPE_F32 ? 4 : KDT == AMF_DTYPE_E4M3 ? 1 : 2;
   constexpr int QS = QDT == AMF_DTYPE_F32 ? 4 : 2;
   constexpr int RG = 64 / LPR;          // groups of a wave
@@ -372,6 +376,8 @@ __global__ __launch_bounds__(kThreads) void paged_attn_general_kernel(PagedArgs 
     const Segment sg = segment_at<kGenHeads>(a, un, u, u1, 0);
     if (tid == 0) note_cut(a, un, sg, u, 0);
     u += sg.st1 - sg.st0;
+    // where there is no row, page 0's is read, and its first dims where there are none
+    const int64_t head_off = sg.hkv * a.head_stride, at = ROWS && dims <= 0 ? 0 : 8 * c * ES;
     float q[kGenHeads][8];
 #pragma unroll
     for (int g = 0; g < kGenHeads; ++g) {
@@ -403,8 +409,9 @@ __global__ __launch_bounds__(kThreads) void paged_attn_general_kernel(PagedArgs 
           const int64_t off = token_offset(a, sg, run, j0, t);
           ok[i] = off >= 0;
           const int n = ok[i] ? dims : 0;
-          load_row8<KDT>(a.k + off + 8 * c * ES, n, aligned, k[i]);
-          load_row8<KDT>(a.v + off + 8 * c * ES, n, aligned, v[i]);
+          const int64_t o = (ROWS && off < 0 ? head_off : off) + at;
+          load_row8<KDT, ROWS>(a.k + o, n, k[i]);
+          load_row8<KDT, ROWS>(a.v + o, n, v[i]);
         }
 #pragma unroll
         for (int g = 0; g < kGenHeads; ++g) {
@@ -909,8 +916,16 @@ void launch_matrix(const PagedArgs& a, dim3 grid, hipStream_t st) {
     paged_attn_matrix_kernel<QDT, KDT, D, false><<<grid, kThreads, 0, st>>>(a);
 }
 
+template <int QDT, int KDT, int LPR>
+void launch_general(const PagedArgs& a, dim3 grid, bool rows, hipStream_t st) {
+  if (rows)
+    paged_attn_general_kernel<QDT, KDT, LPR, true><<<grid, kThreads, 0, st>>>(a);
+  else
+    paged_attn_general_kernel<QDT, KDT, LPR, false><<<grid, kThreads, 0, st>>>(a);
+}
+
 template <int QDT, int KDT>
-void launch(const PagedArgs& a, int64_t groups, bool matrix, bool aligned, hipStream_t st) {
+void launch(const PagedArgs& a, int64_t groups, bool matrix, bool rows, hipStream_t st) {
   const dim3 grid((unsigned)groups);
   if constexpr (QDT != AMF_DTYPE_F32) {
     if (matrix) {
@@ -922,9 +937,9 @@ void launch(const PagedArgs& a, int64_t groups, bool matrix, bool aligned, hipSt
     }
   }
   switch (general_lanes(a.head_dim)) {
-    case 8: paged_attn_general_kernel<QDT, KDT, 8><<<grid, kThreads, 0, st>>>(a, aligned); break;
-    case 16: paged_attn_general_kernel<QDT, KDT, 16><<<grid, kThreads, 0, st>>>(a, aligned); break;
-    default: paged_attn_general_kernel<QDT, KDT, 32><<<grid, kThreads, 0, st>>>(a, aligned);
+    case 8: return launch_general<QDT, KDT, 8>(a, grid, rows, st);
+    case 16: return launch_general<QDT, KDT, 16>(a, grid, rows, st);
+    default: return launch_general<QDT, KDT, 32>(a, grid, rows, st);
   }
 }
 
@@ -1011,8 +1026,9 @@ extern "C" int amf_paged_decode_attn(
                        a.page_stride | a.token_stride | a.head_stride |
                        (q_seq_stride * qs) | (q_head_stride * qs);
   const bool matrix = qs == 2 && head_dim % 16 == 0 && aligned16(bits);
-  const bool aligned = ((((uintptr_t)k | (uintptr_t)v) | a.page_stride | a.token_stride |
-                         a.head_stride) & (8 * es > 16 ? 15 : 8 * es - 1)) == 0;
+  const bool rows = head_dim % 8 == 0 && ((((uintptr_t)k | (uintptr_t)v) | a.page_stride |
+                                           a.token_stride | a.head_stride) &
+                                          (8 * es > 16 ? 15 : 8 * es - 1)) == 0;
   const int tile = matrix ? kTileHeads : kGenHeads;
   a.tiles = (a.group + tile - 1) / tile;
   a.out_dtype = out_dtype;
@@ -1050,15 +1066,15 @@ extern "C" int amf_paged_decode_attn(
   a.err_flag = err_flag;
   hipStream_t st = as_stream(stream);
   if (kv_dtype == AMF_DTYPE_BF16)
-    launch<AMF_DTYPE_BF16, AMF_DTYPE_BF16>(a, groups, matrix, aligned, st);
+    launch<AMF_DTYPE_BF16, AMF_DTYPE_BF16>(a, groups, matrix, rows, st);
   else if (kv_dtype == AMF_DTYPE_F16)
-    launch<AMF_DTYPE_F16, AMF_DTYPE_F16>(a, groups, matrix, aligned, st);
+    launch<AMF_DTYPE_F16, AMF_DTYPE_F16>(a, groups, matrix, rows, st);
   else if (kv_dtype == AMF_DTYPE_F32)
-    launch<AMF_DTYPE_F32, AMF_DTYPE_F32>(a, groups, matrix, aligned, st);
+    launch<AMF_DTYPE_F32, AMF_DTYPE_F32>(a, groups, matrix, rows, st);
   else if (q_dtype == AMF_DTYPE_BF16)
-    launch<AMF_DTYPE_BF16, AMF_DTYPE_E4M3>(a, groups, matrix, aligned, st);
+    launch<AMF_DTYPE_BF16, AMF_DTYPE_E4M3>(a, groups, matrix, rows, st);
   else
-    launch<AMF_DTYPE_F16, AMF_DTYPE_E4M3>(a, groups, matrix, aligned, st);
+    launch<AMF_DTYPE_F16, AMF_DTYPE_E4M3>(a, groups, matrix, rows, st);
   if (int rc = check_launch(who)) return rc;
   if (a.whole) return ok();
   // partials of a pair, about: many take a workgroup a head, hundreds (one long
