@@ -522,7 +522,10 @@ __device__ __forceinline__ uint32_t e4m3_pair(uint32_t w) {
 }
 
 constexpr int kTileHeads = 16;
-constexpr int matrix_waves(int D) { return D == 256 ? 1 : 2; }  // per SIMD, at least
+// Waves per SIMD, at least.  256 dims of 16 bits spill at two (164 sequences of 4700
+// fp16 tokens 272 -> 434 us); of FP8 they are faster with a few words spilled (174 ->
+// 154, 200 chats 53 -> 47).
+constexpr int matrix_waves(int D, int es) { return D == 256 && es == 2 ? 1 : 2; }
 // Tokens of a wave's step.  64 of 64 dims (two sequences of 700 tokens 12.3 -> 11.6
 // us; fewer, larger steps); 64 of 128 FP8 dims are as many bytes but slower than 32
 // (8 x 128K 342 / 335 us).
@@ -531,7 +534,8 @@ constexpr int matrix_chunk(int D) { return D <= 64 ? 64 : 32; }
 // D: the head_dim, or (FULL false) the next of 64, 128 and 256 above a multiple of
 // 16, with zeros in the dims that are not there.
 template <int QDT, int KDT, int D, bool FULL>
-__global__ __launch_bounds__(kThreads, matrix_waves(D)) void paged_attn_matrix_kernel(PagedArgs a) {
+__global__ __launch_bounds__(kThreads, matrix_waves(D, KDT == AMF_DTYPE_E4M3 ? 1 : 2)) void
+paged_attn_matrix_kernel(PagedArgs a) {
   constexpr bool FP8 = KDT == AMF_DTYPE_E4M3;
   constexpr bool V16 = KDT == AMF_DTYPE_F16;  // V in two terms
   constexpr int ES = FP8 ? 1 : 2;
@@ -1056,8 +1060,12 @@ extern "C" int amf_paged_decode_attn(
   if (a.side > 1) a.step_shift -= a.side / 2;
   const int64_t teams = heads / a.side;
   const int64_t most_steps = num_seqs * ((tokens + (1 << a.step_shift) - 1) >> a.step_shift);
+  // one workgroup a CU where two do not fit: 512 shares of 256 dims are taken in two
+  // rounds (164 sequences of 4700 fp16 tokens 288 us, 272 with 256)
+  const bool half = matrix && matrix_waves(matrix_dim(head_dim), es) == 1;
+  const int64_t resident = half ? kGroups / 2 : kGroups;
   const int64_t shares =
-      std::max<int64_t>(1, std::min(std::max<int64_t>(kGroups / teams, 1), most_steps));
+      std::max<int64_t>(1, std::min(std::max<int64_t>(resident / teams, 1), most_steps));
   const int64_t groups = (a.whole ? num_seqs : shares) * teams;
   a.by_seq = num_seqs < shares;
   a.cuts = static_cast<Cut*>(workspace);
