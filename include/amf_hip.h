@@ -430,7 +430,7 @@ int amf_page_key_bounds(const void* k, int32_t kv_dtype, int64_t page_stride,
 
 /* The num_pages pages of each (sequence, KV head) with the largest
  *   max over the KV head's query heads of sum_d max(q_d lo_d, q_d hi_d)
- * over the bounds above, which no key of the page can exceed; summed in 64
+ * over the bounds above (lo <= hi), which no key of the page can exceed; summed in 64
  * bits, the lower place first among equals, the sequence's first first_pages
  * and last last_pages always among them.  pages int32
  * [num_seqs][num_kv_heads][num_pages]: places in the block table in ascending
