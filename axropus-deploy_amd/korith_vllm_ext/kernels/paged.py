@@ -257,7 +257,10 @@ def paged_decode_attention(q: torch.Tensor, k_cache: torch.Tensor,
     most = width * bs if max_context_len is None else int(max_context_len)
     dev = q.device
     if out is None:
-        out = torch.empty(q.shape, dtype=out_dtype or qdt, device=dev)
+        if out_dtype is None and q.is_contiguous():
+            out = torch.empty_like(q)
+        else:
+            out = torch.empty(q.shape, dtype=out_dtype or qdt, device=dev)
     else:
         _dispatch._check_buffer(out, "out", dev)
         if out.shape != q.shape and tuple(out.shape) != (S, Hq, D):
@@ -378,8 +381,8 @@ def select_pages(q: torch.Tensor, bounds: torch.Tensor, block_tables: torch.Tens
     most = min(most, _I32_MAX)
     dev = bounds.device
     if out is None:
-        pages = torch.empty((S, H, num_pages), dtype=_I32, device=dev)
-        counts = torch.empty((S, H), dtype=_I32, device=dev)
+        pages = context_lens.new_empty((S, H, num_pages))
+        counts = pages.new_empty((S, H))
         pg, pc = pages.data_ptr(), counts.data_ptr()
     else:
         pages, counts = out
@@ -449,9 +452,9 @@ def build_slot_maps(context_lens: torch.Tensor, new_tokens: torch.Tensor,
     fu = None if free_used is None else _int32(free_used, "free_used", idx, (1,))
     if out is None:
         dev = block_tables.device
-        slots, pos = torch.empty((2, num_tokens), dtype=torch.int64, device=dev).unbind(0)
-        start, lens, used = torch.empty(2 * S + 2, dtype=_I32, device=dev).split_with_sizes(
-            (S + 1, S, 1))
+        slots = torch.empty(num_tokens, dtype=torch.int64, device=dev)
+        pos = torch.empty_like(slots)
+        start, lens, used = new_tokens.new_empty(2 * S + 2).split_with_sizes((S + 1, S, 1))
         out = SlotMaps(slots, pos, start, lens, used)
         ptrs = (slots.data_ptr(), pos.data_ptr(), start.data_ptr(), lens.data_ptr(),
                 used.data_ptr())
