@@ -267,6 +267,8 @@ def test_lists_without_room_hold_nothing():
     (F8, 68, 2, 64, 9, 5000),      # four tiles: two of each KV head
     (BF, 4, 4, 256, 12, 2500),
     (F32, 8, 2, 64, 25, 2000),     # the general kernel, two tiles of a group
+    (FP, 16, 2, 256, 30, 2500),    # one workgroup a CU
+    (F8, 8, 4, 256, 30, 2500),
     (BF, 6, 1, 80, 270, 1500),
     (F32, 4, 4, 100, 300, 1200),
 ])
