@@ -280,10 +280,21 @@ __device__ __forceinline__ int64_t token_offset(const PagedArgs& a, const Segmen
 
 // ---- joining -------------------------------------------------------------------
 
-// 2^(m - top), 1 where they are equal (-inf: nothing seen yet, or only scores
-// of -inf, whose sum is NaN already).
+// A part with m = -inf has seen no token (l = 0) or only scores of -inf (l > 0, which
+// no longer sums weights).  Next to a finite score both weigh nothing.
+
+// 2^(m - top), 1 where they are equal.
 __device__ __forceinline__ float weight_to(float m, float top) {
   return m == top ? 1.0f : __builtin_amdgcn_exp2f(m - top);
+}
+
+// What is taken from a score before 2^x: the maximum, or 0 where that is -inf (the
+// difference would be NaN, and stay, where another part has finite scores).
+__device__ __forceinline__ float exp_base(float m) { return m == -INFINITY ? 0.0f : m; }
+
+// The factor of a head's weighted rows, for l > 0: NaN where all scores are -inf.
+__device__ __forceinline__ float row_factor(float v_scale, float m, float l) {
+  return m == -INFINITY ? __builtin_nanf("") : v_scale / l;
 }
 
 // The larger, NaN if either is.
@@ -402,12 +413,13 @@ __global__ __launch_bounds__(kThreads) void paged_attn_general_kernel(PagedArgs 
       load_pages(a, sg, r0, r1, run);
       for (int64_t st = r0; st < r1; ++st) {
         float k[kGenAhead][8], v[kGenAhead][8];
-        bool ok[kGenAhead];
+        bool ok[kGenAhead], any = false;
 #pragma unroll
         for (int i = 0; i < kGenAhead; ++i) {
           const int64_t t = (st << a.step_shift) + (wave * kGenAhead + i) * RG + grp;
           const int64_t off = token_offset(a, sg, run, j0, t);
           ok[i] = off >= 0;
+          any |= ok[i];
           const int n = ok[i] ? dims : 0;
           const int64_t o = (ROWS && off < 0 ? head_off : off) + at;
           load_row8<KDT, ROWS>(a.k + o, n, k[i]);
@@ -425,15 +437,16 @@ __global__ __launch_bounds__(kThreads) void paged_attn_general_kernel(PagedArgs 
             for (int o = LPR / 2; o > 0; o >>= 1) x[i] += __shfl_xor(x[i], o, LPR);
             top = max_nan(top, ok[i] ? x[i] * a.score_scale : -INFINITY);
           }
-          const float mn = max_nan(m[g], top), w = weight_to(m[g], mn);
+          const float mn = max_nan(m[g], top), w = weight_to(m[g], mn), base = exp_base(mn);
           m[g] = mn;
           l[g] *= w;
+          if (mn == -INFINITY && any) l[g] = 1.0f;
 #pragma unroll
           for (int e = 0; e < 8; ++e) acc[g][e] *= w;
 #pragma unroll
           for (int i = 0; i < kGenAhead; ++i) {
             const float p =
-                ok[i] ? __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], a.score_scale, -mn)) : 0.0f;
+                ok[i] ? __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], a.score_scale, -base)) : 0.0f;
             l[g] += p;
 #pragma unroll
             for (int e = 0; e < 8; ++e) acc[g][e] = __builtin_fmaf(p, v[i][e], acc[g][e]);
@@ -464,7 +477,7 @@ __global__ __launch_bounds__(kThreads) void paged_attn_general_kernel(PagedArgs 
         x = __builtin_fmaf(acc_lds[w][g][d], f, x);
       }
       if (sg.whole) {
-        store_out(a, (sg.head0 + g) * D + d, sum == 0.0f ? 0.0f : x * (a.v_scale / sum));
+        store_out(a, (sg.head0 + g) * D + d, sum == 0.0f ? 0.0f : x * row_factor(a.v_scale, top, sum));
       } else {
         float* part = sg.part + g * (D + kPartPad);
         part[d] = x;
@@ -675,7 +688,7 @@ paged_attn_matrix_kernel(PagedArgs a) {
           top = max_nan(top, __shfl_xor(top, 16));
           top = max_nan(top, __shfl_xor(top, 32));
           const float mn = max_nan(m, top);
-          const float w = weight_to(m, mn);
+          const float w = weight_to(m, mn), base = exp_base(mn);
           m = mn;
           float sum = 0.0f;
 #pragma unroll
@@ -683,11 +696,11 @@ paged_attn_matrix_kernel(PagedArgs a) {
 #pragma unroll
             for (int r = 0; r < 8; ++r) {
               p[b][r] = counts(b, r) ? __builtin_amdgcn_exp2f(
-                                           __builtin_fmaf(x[b][r], a.score_scale, -mn))
+                                           __builtin_fmaf(x[b][r], a.score_scale, -base))
                                      : 0.0f;
               sum += p[b][r];
             }
-          l = l * w + sum;
+          l = mn == -INFINITY ? 1.0f : l * w + sum;
           if (__any(w != 1.0f)) {
 #pragma unroll
             for (int j = 0; j < DP; ++j) acc[j] *= w;
@@ -785,7 +798,7 @@ paged_attn_matrix_kernel(PagedArgs a) {
           if (sum == 0.0f)
             x = f32x4{0, 0, 0, 0};
           else
-            x *= a.v_scale / sum;
+            x *= row_factor(a.v_scale, top, sum);
           store4(a.out, a.out_dtype, (sn.head0 + g) * dim + d, x);
         } else {
           float* part = sn.part + g * (dim + kPartPad);
@@ -869,7 +882,7 @@ __global__ __launch_bounds__(NT) void paged_attn_merge_kernel(PagedArgs a, int h
     for (int e = 0; e < W; ++e) x[e] = x[e] * f + x_lds[o][e] * pf;
     m = top;
   }
-  const float scale = l == 0.0f ? 0.0f : a.v_scale / l;
+  const float scale = l == 0.0f ? 0.0f : row_factor(a.v_scale, m, l);
   const int64_t at = (int64_t)(cut.head0 + g) * D + W * col;
   if constexpr (W == 4)
     store4(a.out, a.out_dtype, at,

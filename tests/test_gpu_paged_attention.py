@@ -180,6 +180,42 @@ def test_non_finite_tokens_show(dtype, D):
     assert float((out - ref)[ok].abs().max()) <= attend_tolerance(q, kv, lens, 0.1)
 
 
+@pytest.mark.parametrize("dtype,Hq,D", [(BF, 8, 128), (FP, 8, 64), (BF, 8, 256), (FP, 8, 80),
+                                        (F32, 8, 96), (BF, 6, 33)])
+@pytest.mark.parametrize("lists", [False, True])
+def test_runs_of_minus_infinity_weigh_nothing(dtype, Hq, D, lists):
+    """Scores of -inf for whole steps and shares of a context, beside finite
+    ones; NaN only where a head has no other."""
+    lens = [40, 300, 5000, 70]
+    q, kv, table = _case(dtype, Hq, 2, D, 16, lens, seed=6)
+    q[:, :, 0] = 1.0
+
+    def gone(s, h, tokens):
+        t = torch.tensor(tokens)
+        kv[0, table[s, t // 16].long().to(DEV), (t % 16).to(DEV), h, 0] = float("-inf")
+
+    gone(0, 0, range(32))           # the first step of a wave
+    gone(0, 1, range(39))           # all but the last token
+    gone(1, 0, range(64, 300))      # all behind the first tokens
+    gone(1, 1, [t for t in range(300) if t % 16 != 5])
+    gone(2, 0, range(4000))         # whole shares
+    gone(2, 1, range(1, 5000))
+    gone(3, 0, range(70))           # all of them: NaN, as softmax gives
+    kw, ref_kw = {}, {}
+    if lists:
+        n = table.shape[1]
+        pages = torch.arange(n, dtype=torch.int32).expand(4, 2, n).contiguous()
+        counts = torch.tensor([[-(-c // 16)] * 2 for c in lens], dtype=torch.int32)
+        kw = dict(pages=pages.to(DEV), page_counts=counts.to(DEV))
+        ref_kw = dict(pages=pages, counts=counts)
+    ref = attend64(q, kv, table, lens, D ** -0.5, **ref_kw)
+    out = _run(q, kv, table, lens, out_dtype=F32, **kw).cpu().double()
+    nan = torch.isnan(ref)
+    assert nan[3, :Hq // 2].all() and int(nan.sum()) == Hq // 2 * D
+    assert torch.equal(torch.isnan(out), nan)
+    assert float((out - ref)[~nan].abs().max()) <= attend_tolerance(q, kv, lens, D ** -0.5)
+
+
 @pytest.mark.parametrize("dtype", [BF, FP])
 def test_small_weights_keep_their_bits(dtype):
     """One token with V = 0 holds nearly all of the softmax; the output is what
