@@ -107,9 +107,10 @@ __global__ __launch_bounds__(kThreads) void slot_maps_kernel(SlotArgs a) {
         if (id < 0 || id >= a.pool_pages) {
           id = -1;
           flags |= AMF_ERRFLAG_BLOCK_RANGE;
-        } else if (page >= have && at == 0) {
-          *entry = (int32_t)id;
         }
+        // -1 for an id outside the pool: the next step must not take what the row held
+        // before for this sequence's page
+        if (page >= have && at == 0) *entry = (int32_t)id;
       }
       a.slot_mapping[r] = id < 0 ? -1 : id * a.block_size + at;
       a.positions[r] = pos;

@@ -428,7 +428,8 @@ def build_slot_maps(context_lens: torch.Tensor, new_tokens: torch.Tensor,
     A sequence whose pages the free list or its table row does not hold, or
     whose tokens the rows do not, keeps its length and gets slots of -1
     (AMF_ERRFLAG_FREE_LIST / _CONTEXT in err_flag); so do tokens of page ids
-    outside [0, pool_pages) (_BLOCK_RANGE), whose sequence grows."""
+    outside [0, pool_pages) (_BLOCK_RANGE), whose sequence grows, with an entry
+    of -1 where the free list held such an id."""
     if not isinstance(block_tables, torch.Tensor):
         raise TypeError("block_tables must be an int32 tensor")
     idx = block_tables.get_device()

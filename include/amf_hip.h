@@ -469,7 +469,8 @@ int amf_select_pages(const void* q, int32_t dtype, int64_t q_seq_stride, int64_t
  * behind num_tokens (AMF_ERRFLAG_CONTEXT), or whose pages the free list no
  * longer holds (AMF_ERRFLAG_FREE_LIST; so do later ones that need pages), gets
  * none: its context_out is context_lens, its slots are -1.  A page id outside
- * [0, pool_pages) gives slots of -1 (AMF_ERRFLAG_BLOCK_RANGE).
+ * [0, pool_pages) gives slots of -1 (AMF_ERRFLAG_BLOCK_RANGE), and one from the
+ * free list a block_tables entry of -1, so that later steps flag it again.
  * Replaces the slots of AMFReqMeta.make (amf_kv_connector.py:90-115), built on
  * the host per request. */
 int amf_build_slot_maps(const int32_t* context_lens, const int32_t* new_tokens,

@@ -106,6 +106,25 @@ def test_bad_pages_and_too_few_rows():
     _compare(lens, new, 16, 10, table, free)
 
 
+@pytest.mark.parametrize("bad_id", [1000, -5, (1 << 31) - 1])
+def test_bad_page_of_the_free_list_stays_bad(bad_id):
+    """A reused row still holds old page ids behind its last page; a page id
+    outside the pool must not leave them in place for the next step."""
+    from korith_vllm_ext.kernels import build_slot_maps
+
+    bt = torch.tensor([[4, 7, 9], [5, 6, 8]], dtype=torch.int32, device=DEV)
+    free, used, flag = _i32([bad_id, 3, 11]), _i32([0]), _i32([0])
+    m = build_slot_maps(_i32([16, 15]), _i32([2, 3]), bt, block_size=16, num_tokens=5,
+                        free_pages=free, free_used=used, pool_pages=20, err_flag=flag)
+    assert m.slot_mapping.tolist() == [-1, -1, 95, 48, 49] and int(flag) == 1
+    assert m.context_lens.tolist() == [18, 18] and m.free_used.tolist() == [2]
+    assert bt.tolist() == [[4, -1, 9], [5, 3, 8]]
+    flag.zero_()
+    m = build_slot_maps(m.context_lens, _i32([1, 1]), bt, block_size=16, num_tokens=2,
+                        free_pages=free, free_used=m.free_used, pool_pages=20, err_flag=flag)
+    assert m.slot_mapping.tolist() == [-1, 50] and int(flag) == 1
+
+
 def test_sequences_behind_the_rows_do_not_grow():
     """Their new pages have no rows that would write them into the table."""
     table, free = _start([16, 16, 16], 16, torch.Generator().manual_seed(6), 2)
