@@ -110,8 +110,8 @@ def _cache(k: torch.Tensor, v: Optional[torch.Tensor]) -> tuple:
     """(device index, K address, V address, strides of page, token and head,
     pages, block, heads, dim) of a layer [2, pages, block, heads, dim] (v
     None), or of K and V planes [pages, block, heads, dim] with the same
-    strides; a plane alone holds both.  The last dim is contiguous, the others
-    may be strided."""
+    strides; of a plane alone it is K's address twice.  The last dim is
+    contiguous, the others may be strided."""
     if not isinstance(k, torch.Tensor):
         raise TypeError(f"a K/V cache is a tensor, got {type(k).__name__}")
     idx = k.get_device()
@@ -219,7 +219,8 @@ def paged_decode_attention(q: torch.Tensor, k_cache: torch.Tensor,
 
     q [seqs, Hq, D] or [seqs, Hq, 1, D]; k_cache a layer [2, pages, block, Hkv,
     D], or the K plane [pages, block, Hkv, D] with v_cache the V plane of the
-    same strides (any order of block and heads); D at most 256, Hq a multiple
+    same strides (any order of block and heads; k_cache itself, if one plane
+    holds both); D at most 256, Hq a multiple
     of Hkv.  q has the cache's type, with an FP8 cache bf16 or fp16.
     block_tables int32 [seqs, max_pages], context_lens int32 [seqs] (tokens in
     the cache, the new one among them); a sequence without tokens gives zeros.
@@ -228,6 +229,8 @@ def paged_decode_attention(q: torch.Tensor, k_cache: torch.Tensor,
     to the listed places of the block table (select_pages makes them).  out:
     contiguous, q's shape; otherwise one of out_dtype (q's type)."""
     idx, kp, vp, ps, ts, hs, nb, bs, H, D = _cache(k_cache, v_cache)
+    if v_cache is None and k_cache.dim() == 4:
+        raise ValueError("a K plane comes with the V plane (v_cache=k_cache where it holds both)")
     q3 = _query(q, idx, D)
     S, Hq, _ = q3.shape
     kdt, qdt = k_cache.dtype, q3.dtype

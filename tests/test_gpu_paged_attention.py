@@ -399,6 +399,23 @@ def test_strided_inputs_and_separate_planes():
     _check(out, ref, attend_tolerance(q, kv, lens, 0.1))
 
 
+def test_plane_alone_is_refused():
+    """A K plane without its V plane; one plane that is both has to be said."""
+    from korith_vllm_ext.int4_decode_attention import int4_decode_attention
+
+    lens = [77, 300]
+    q, kv, table = _case(BF, 8, 2, 128, 16, lens)
+    with pytest.raises(ValueError, match="V plane"):
+        _run(q, kv[0], table, lens)
+    with pytest.raises(ValueError, match="V plane"):
+        int4_decode_attention(q, kv[0], block_tables=table.to(DEV),
+                              context_lens=torch.tensor(lens, dtype=torch.int32, device=DEV))
+    both = torch.stack((kv[0], kv[0]))
+    out = _run(q, kv[0], table, lens, v_cache=kv[0], out_dtype=F32)
+    _check(out, attend64(q, both, table, lens, 128 ** -0.5),
+           attend_tolerance(q, both, lens, 128 ** -0.5))
+
+
 def test_far_pages():
     """Byte offsets past 32 bits: pages at the end of a 5 GB plane."""
     pool, lens = 160000, [90, 40]
