@@ -57,14 +57,13 @@ __global__ __launch_bounds__(kThreads) void page_key_bounds_kernel(BoundsArgs a)
   const int s = blockIdx.y;
   const int64_t item = (int64_t)blockIdx.x * kThreads + threadIdx.x;
   const int64_t c = a.context_lens[s];
+  // here, not where a page is missed: the grid may end with the table's pages
+  if (item == 0 && a.err_flag && c > (int64_t)a.table_pages * a.block_size)
+    atomicOr(a.err_flag, AMF_ERRFLAG_CONTEXT);
   int64_t page = item / a.chunks;
   const int chunk = (int)(item - page * a.chunks);
   if (a.first_tokens) page += max(a.first_tokens[s], 0) / a.block_size;
-  if (page * a.block_size >= c) return;
-  if (page >= a.table_pages) {
-    if (a.err_flag) atomicOr(a.err_flag, AMF_ERRFLAG_CONTEXT);
-    return;
-  }
+  if (page * a.block_size >= c || page >= a.table_pages) return;
   const int64_t id = a.block_tables[s * a.bt_stride + page];
   if (id < 0 || id >= a.pool_pages) {
     if (a.err_flag) atomicOr(a.err_flag, AMF_ERRFLAG_BLOCK_RANGE);
@@ -490,8 +489,8 @@ extern "C" int amf_page_key_bounds(const void* k, int32_t kv_dtype, int64_t page
       (es == 2 && bounds_dtype != kv_dtype))
     return fail(AMF_ERR_INVALID_ARG, "%s: bounds of type %d for a cache of type %d", who,
                 bounds_dtype, kv_dtype);
-  if (num_seqs == 0 || table_pages == 0) return ok();
-  if (!k || !block_tables || !context_lens || !bounds)
+  if (num_seqs == 0 || (table_pages == 0 && !err_flag)) return ok();
+  if (!k || (table_pages > 0 && !block_tables) || !context_lens || !bounds)
     return fail(AMF_ERR_INVALID_ARG, "%s: null pointer", who);
   const int align = 8 * es;  // bytes of a thread's load
   if ((page_stride * es) % align || (token_stride * es) % align || (head_stride * es) % align ||
@@ -503,7 +502,8 @@ extern "C" int amf_page_key_bounds(const void* k, int32_t kv_dtype, int64_t page
   if (first_tokens && max_new_tokens > 0)
     pages = std::min<int64_t>(pages, ((int64_t)max_new_tokens + block_size - 2) / block_size + 1);
   const int64_t chunks = (int64_t)num_kv_heads * head_dim / 8;
-  const int64_t groups = (pages * chunks + kThreads - 1) / kThreads;
+  // one at least, for the flag
+  const int64_t groups = std::max<int64_t>(1, (pages * chunks + kThreads - 1) / kThreads);
   if (chunks > 0x7FFFFFFF || groups > 0xFFFFFF)
     return fail(AMF_ERR_UNSUPPORTED, "%s: %lld pages of %lld channels", who, (long long)pages,
                 (long long)chunks * 8);

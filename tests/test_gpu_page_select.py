@@ -74,6 +74,30 @@ def test_bounds_leave_stale_tokens_out_and_show_nan():
     assert int(flag) == 1 | 2
 
 
+@pytest.mark.parametrize("lens,width,first,new,want", [
+    ([33], 2, None, None, 2), ([32], 2, None, None, 0),
+    ([33], 2, [0], None, 2), ([33], 2, [0], 33, 2), ([33], 2, [15], 18, 2),
+    ([33], 2, [33], 1, 2), ([20, 40, 7], 2, None, None, 2), ([20, 32, 7], 2, [3, 3, 3], 29, 0),
+    ([5], 0, None, None, 2), ([0, -2], 0, None, None, 0), ([5], 0, [2], 3, 2),
+])
+def test_bounds_flag_a_context_that_the_table_does_not_hold(lens, width, first, new, want):
+    """Whatever part of the pages the call writes; 8 heads of 128 fill the
+    grid's workgroups, so that no thread lies behind the table's pages."""
+    from korith_vllm_ext.kernels import page_key_bounds
+
+    g = torch.Generator().manual_seed(3)
+    kv = make_cache(8, 16, 8, 128, BF, g)
+    table = torch.arange(len(lens) * width, dtype=torch.int32).view(len(lens), width)
+    flag = torch.zeros(1, dtype=torch.int32, device=DEV)
+    got = page_key_bounds(kv, table.to(DEV), _i32(lens), max_new_tokens=new, err_flag=flag,
+                          first_tokens=None if first is None else _i32(first))
+    assert int(flag) == want
+    ref = torch.zeros_like(got)
+    for i, b in bounds64(kv[0].float(), table, lens, 16, first).items():
+        ref[i] = b.to(BF)
+    assert torch.equal(got, ref)
+
+
 def _selection(dtype, Hq, H, D, block, lens, seed=0):
     g = torch.Generator().manual_seed(seed + D + Hq)
     table, pool = make_tables(lens, block, g)
