@@ -401,12 +401,13 @@ def hip_decode_attention(q: torch.Tensor, k: Any, v: Any = None, scale: Optional
                          workspace: Optional[torch.Tensor] = None,
                          pages: Optional[torch.Tensor] = None,
                          page_counts: Optional[torch.Tensor] = None, k_scale: float = 1.0,
-                         v_scale: float = 1.0) -> torch.Tensor:
+                         v_scale: float = 1.0,
+                         err_flag: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The gfx950 decode kernel: positional arguments as the reference's
     (q, k, v, scale=None, mask=None); with block_tables/context_lens keywords,
     a paged GQA kernel runs over k, an INT4 page pool (v unused) or a tensor:
     a layer's cache, or its K plane with v the V plane (paged_decode_attention,
-    which takes pages, page_counts, k_scale and v_scale)."""
+    which takes pages, page_counts, k_scale, v_scale and err_flag)."""
     if block_tables is not None or context_lens is not None:
         if block_tables is None or context_lens is None:
             raise ValueError("paged decode needs both block_tables and context_lens")
@@ -419,16 +420,18 @@ def hip_decode_attention(q: torch.Tensor, k: Any, v: Any = None, scale: Optional
                 q, k, v, block_tables=block_tables, context_lens=context_lens, scale=scale,
                 max_context_len=max_context_len, pages=pages, page_counts=page_counts,
                 k_scale=k_scale, v_scale=v_scale, out=out, out_dtype=out_dtype,
-                workspace=workspace)
-        if pages is not None or page_counts is not None or k_scale != 1.0 or v_scale != 1.0:
-            raise ValueError("pages and scales are for a cache given as a tensor")
+                workspace=workspace, err_flag=err_flag)
+        if (pages is not None or page_counts is not None or k_scale != 1.0 or v_scale != 1.0
+                or err_flag is not None):
+            raise ValueError("pages, scales and err_flag are for a cache given as a tensor")
         if v is not None and v is not k:
             raise ValueError("paged decode reads K and V from the one page pool passed as k")
         return paged_int4_decode(q, k, block_tables, context_lens, scale=scale,
                                  max_context_len=max_context_len, out=out, out_dtype=out_dtype,
                                  algo=algo, workspace=workspace)
-    if pages is not None or page_counts is not None or k_scale != 1.0 or v_scale != 1.0:
-        raise ValueError("pages and scales need block_tables and context_lens")
+    if (pages is not None or page_counts is not None or k_scale != 1.0 or v_scale != 1.0
+            or err_flag is not None):
+        raise ValueError("pages, scales and err_flag need block_tables and context_lens")
     res = int4_sym_attention(q, k, v, scale, mask, out_dtype)
     if res is None:
         res = dense_attention(q, _to_tensor(k, q), _to_tensor(v, q), scale, mask, out_dtype)

@@ -450,6 +450,18 @@ def test_reached_through_the_dispatch():
         int4_decode_attention(q, kv, algo="valu", **kw)
 
 
+def test_dispatch_reports_bad_pages():
+    from korith_vllm_ext.int4_decode_attention import int4_decode_attention
+
+    q, kv, table = _case(BF, 8, 2, 128, 16, [100, 18])
+    table[0, 2] = kv.shape[1]
+    flag = torch.zeros(1, dtype=torch.int32, device=DEV)
+    cl = torch.tensor([100, 500], dtype=torch.int32, device=DEV)
+    out = int4_decode_attention(q, kv, block_tables=table.to(DEV), context_lens=cl, err_flag=flag)
+    assert int(flag) == 1 | 2
+    assert torch.equal(out, _run(q, kv, table, [100, 500]))
+
+
 def test_other_stream_and_shared_scratch():
     """Two streams at once, each with its own scratch; the same bits."""
     lens = [5000, 300]

@@ -101,6 +101,18 @@ def test_workspace_sizes():
     assert g(0, 2, 100, 16, 17) == g(4, 2, 0, 16, 17) == g(4, 2, 100, 16, 0) == 0
 
 
+def test_dispatch_takes_an_error_flag_with_a_cache_only():
+    """Over an INT4 pool or dense K/V nothing would be written to it."""
+    from korith_vllm_ext.kernels import hip_decode_attention
+
+    q = torch.zeros(1, 4, 1, 64, dtype=torch.bfloat16)
+    i = torch.zeros(1, dtype=torch.int32)
+    with pytest.raises(ValueError, match="err_flag"):
+        hip_decode_attention(q, object(), block_tables=i[None], context_lens=i, err_flag=i)
+    with pytest.raises(ValueError, match="err_flag"):
+        hip_decode_attention(q, q, q, err_flag=i)
+
+
 def test_python_calls_need_the_gpu():
     """CPU tensors are turned away before anything is launched."""
     from korith_vllm_ext import kernels
