@@ -407,7 +407,10 @@ def hip_decode_attention(q: torch.Tensor, k: Any, v: Any = None, scale: Optional
     (q, k, v, scale=None, mask=None); with block_tables/context_lens keywords,
     a paged GQA kernel runs over k, an INT4 page pool (v unused) or a tensor:
     a layer's cache, or its K plane with v the V plane (paged_decode_attention,
-    which takes pages, page_counts, k_scale, v_scale and err_flag)."""
+    which takes pages, page_counts, k_scale, v_scale and err_flag).
+    block_tables and context_lens may be lists, of other integer types or on
+    the host with either, at the cost of a copy; int32 tensors on the device
+    are taken as they are, tables with rows apart too."""
     if block_tables is not None or context_lens is not None:
         if block_tables is None or context_lens is None:
             raise ValueError("paged decode needs both block_tables and context_lens")
@@ -416,8 +419,14 @@ def hip_decode_attention(q: torch.Tensor, k: Any, v: Any = None, scale: Optional
         if isinstance(k, torch.Tensor):
             if algo != "auto":
                 raise ValueError(f"algo {algo!r} is for INT4 pools")
+            bt = block_tables
+            if not (isinstance(bt, torch.Tensor) and bt.dtype == torch.int32
+                    and bt.device == k.device and bt.dim() == 2 and bt.stride(1) == 1
+                    and bt.stride(0) >= bt.shape[1]):
+                bt = _index_tensor(bt, k.device)
+            context_lens = _index_tensor(context_lens, k.device)
             return paged_decode_attention(
-                q, k, v, block_tables=block_tables, context_lens=context_lens, scale=scale,
+                q, k, v, block_tables=bt, context_lens=context_lens, scale=scale,
                 max_context_len=max_context_len, pages=pages, page_counts=page_counts,
                 k_scale=k_scale, v_scale=v_scale, out=out, out_dtype=out_dtype,
                 workspace=workspace, err_flag=err_flag)

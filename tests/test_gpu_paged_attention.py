@@ -450,6 +450,29 @@ def test_reached_through_the_dispatch():
         int4_decode_attention(q, kv, algo="valu", **kw)
 
 
+@pytest.mark.parametrize("how", ["lists", "int64", "host", "slices", "strided"])
+def test_dispatch_takes_tables_as_over_an_int4_pool(how):
+    from korith_vllm_ext.kernels import hip_decode_attention
+
+    lens = [200, 18]
+    q, kv, table = _case(BF, 8, 2, 128, 16, lens)
+    want = _run(q, kv, table, lens)
+    cl = torch.tensor(lens, dtype=torch.int32)
+    if how == "lists":
+        bt, cl = table.tolist(), lens
+    elif how == "int64":
+        bt, cl = table.long().to(DEV), cl.long().to(DEV)
+    elif how == "host":
+        bt = table
+    elif how == "strided":
+        bt = table.t().contiguous().to(DEV).t()
+        cl = torch.stack((cl, cl), 1).to(DEV)[:, 0]
+    else:
+        bt = torch.cat((table, table), 1).to(DEV)[:, :table.shape[1]]
+        cl = cl.to(DEV)
+    assert torch.equal(hip_decode_attention(q, kv, block_tables=bt, context_lens=cl), want)
+
+
 def test_dispatch_reports_bad_pages():
     from korith_vllm_ext.int4_decode_attention import int4_decode_attention
 
