@@ -132,7 +132,9 @@ def _cache(k: torch.Tensor, v: Optional[torch.Tensor]) -> tuple:
         nb, bs, H, D = shape
         ps, ts, hs, ds = st
         if v is not None and v is not k:
-            if not isinstance(v, torch.Tensor) or v.shape != shape or v.stride() != st:
+            if (not isinstance(v, torch.Tensor) or v.shape != shape
+                    or (v.stride() != st and any(a != b and n > 1 for a, b, n in
+                                                 zip(v.stride(), st, shape)))):
                 raise ValueError("K and V planes differ in shape or strides")
             if v.dtype != k.dtype or v.device != k.device:
                 raise ValueError("K and V planes differ in type or device")
@@ -143,6 +145,8 @@ def _cache(k: torch.Tensor, v: Optional[torch.Tensor]) -> tuple:
         raise ValueError("the cache's last dim must be contiguous")
     if not (nb and bs and H and D):
         raise ValueError(f"empty K/V cache {tuple(shape)}")
+    if H == 1 or bs == 1 or nb == 1:  # strides that are never used, whatever their alignment
+        ps, ts, hs = ps * (nb > 1), ts * (bs > 1), hs * (H > 1)
     return idx, kp, vp, ps, ts, hs, nb, bs, H, D
 
 

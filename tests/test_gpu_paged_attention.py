@@ -416,6 +416,24 @@ def test_plane_alone_is_refused():
            attend_tolerance(q, both, lens, 128 ** -0.5))
 
 
+@pytest.mark.parametrize("lens,block,H", [([77, 300], 16, 1), ([9, 4], 1, 2), ([5], 16, 2)])
+def test_planes_with_other_strides_where_a_dim_has_one_element(lens, block, H):
+    """One KV head (or token, or page): its stride is never used."""
+    g = torch.Generator().manual_seed(2)
+    table, pool = make_tables(lens, block, g, spare=0)
+    kv = make_cache(pool, block, H, 64, BF, g)
+    k, v = kv[0], kv[1].clone()
+    v = v.as_strided(v.shape, [7 if n == 1 else st for n, st in zip(v.shape, v.stride())])
+    assert k.stride() != v.stride() and torch.equal(v, kv[1])
+    from korith_vllm_ext.kernels import page_key_bounds
+
+    bt, cl = table.to(DEV), torch.tensor(lens, dtype=torch.int32, device=DEV)
+    assert torch.equal(page_key_bounds(v, bt, cl), page_key_bounds(kv[1], bt, cl))
+    q = torch.randn(len(lens), 4, 64, generator=g).to(BF).to(DEV)
+    out = _run(q, k, table, lens, v_cache=v, out_dtype=F32)
+    _check(out, attend64(q, kv, table, lens, 0.125), attend_tolerance(q, kv, lens, 0.125))
+
+
 def test_far_pages():
     """Byte offsets past 32 bits: pages at the end of a 5 GB plane."""
     pool, lens = 160000, [90, 40]
