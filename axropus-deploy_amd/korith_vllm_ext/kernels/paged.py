@@ -65,6 +65,7 @@ def _launch(idx: int, func: str, *args) -> None:
 
 # Scratch kept between calls, one buffer per (device, stream, host thread): a call
 # is two launches, and another thread's may come between them on the same stream.
+# The least recently used is dropped, those of threads that ended among them.
 # A stream under graph capture gets a buffer of its own per call instead.
 _SCRATCH: "OrderedDict[Tuple[int, int, int], torch.Tensor]" = OrderedDict()
 _SCRATCH_MAX = 16
@@ -77,6 +78,10 @@ def _scratch(dev: torch.device, stream: int, nbytes: int) -> torch.Tensor:
     key = (dev.index, stream, threading.get_ident())
     buf = _SCRATCH.get(key)
     if buf is not None and buf.numel() >= nbytes:
+        try:
+            _SCRATCH.move_to_end(key)  # one step under the interpreter's lock
+        except KeyError:
+            pass  # another thread's call has just dropped it
         return buf
     buf = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     with _SCRATCH_LOCK:

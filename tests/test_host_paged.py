@@ -113,6 +113,30 @@ def test_dispatch_takes_an_error_flag_with_a_cache_only():
         hip_decode_attention(q, q, q, err_flag=i)
 
 
+@pytest.fixture
+def scratch(monkeypatch):
+    """kernels.paged with an empty store of CPU scratch buffers, nothing captured."""
+    from collections import OrderedDict
+
+    from korith_vllm_ext.kernels import paged
+
+    monkeypatch.setattr(paged, "_SCRATCH", OrderedDict())
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(paged, "_current_device", lambda: None)  # a CPU tensor's index
+    return paged
+
+
+def test_scratch_keeps_the_buffers_in_use(scratch):
+    """More streams than buffers are kept for: the busy one's stays."""
+    dev = torch.device("cpu")
+    busy = scratch._scratch(dev, 0, 64)
+    for stream in range(1, 3 * scratch._SCRATCH_MAX):
+        scratch._scratch(dev, stream, 64)
+        assert scratch._scratch(dev, 0, 64) is busy
+        assert len(scratch._SCRATCH) <= scratch._SCRATCH_MAX
+    assert scratch._scratch(dev, 0, 65) is not busy
+
+
 def test_python_calls_need_the_gpu():
     """CPU tensors are turned away before anything is launched."""
     from korith_vllm_ext import kernels
