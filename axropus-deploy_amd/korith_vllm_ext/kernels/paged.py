@@ -72,8 +72,17 @@ _SCRATCH_MAX = 16
 _SCRATCH_LOCK = threading.Lock()
 
 
+def _capturing(idx: int) -> bool:
+    """Whether the current stream of device idx, which the call launches on, is
+    under graph capture; torch answers for the current device's."""
+    if _current_device() == idx:
+        return torch.cuda.is_current_stream_capturing()
+    with torch.cuda.device(idx):
+        return torch.cuda.is_current_stream_capturing()
+
+
 def _scratch(dev: torch.device, stream: int, nbytes: int) -> torch.Tensor:
-    if torch.cuda.is_current_stream_capturing():
+    if _capturing(dev.index):
         return torch.empty(nbytes, dtype=torch.uint8, device=dev)
     key = (dev.index, stream, threading.get_ident())
     buf = _SCRATCH.get(key)

@@ -137,6 +137,36 @@ def test_scratch_keeps_the_buffers_in_use(scratch):
     assert scratch._scratch(dev, 0, 65) is not busy
 
 
+@pytest.mark.parametrize("current,captured,kept", [(0, None, True), (0, 0, True), (0, 1, False),
+                                                   (1, 0, True), (1, 1, False)])
+def test_scratch_under_capture_is_of_the_tensors_device(scratch, monkeypatch, current, captured,
+                                                        kept):
+    """A buffer is kept between calls unless the stream of device 1, which
+    holds the tensors, is captured, whichever device is current."""
+    now = [current]
+
+    class Guard:
+        def __init__(self, idx):
+            self.idx = idx
+
+        def __enter__(self):
+            self.before, now[0] = now[0], self.idx
+
+        def __exit__(self, *_):
+            now[0] = self.before
+
+    class Device:
+        index = 1
+
+    empty = torch.empty
+    monkeypatch.setattr(scratch, "_current_device", lambda: now[0])
+    monkeypatch.setattr(torch.cuda, "device", Guard)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: now[0] == captured)
+    monkeypatch.setattr(torch, "empty", lambda n, dtype, device: empty(n, dtype=dtype))
+    bufs = [scratch._scratch(Device(), 5, 64) for _ in range(2)]
+    assert (bufs[0] is bufs[1]) == kept and now[0] == current
+
+
 def test_python_calls_need_the_gpu():
     """CPU tensors are turned away before anything is launched."""
     from korith_vllm_ext import kernels
