@@ -440,7 +440,8 @@ def build_slot_maps(context_lens: torch.Tensor, new_tokens: torch.Tensor,
 
     context_lens, new_tokens int32 [seqs]; block_tables int32 [seqs,
     max_pages], extended in place with pages free_pages[free_used:] (int32
-    [n], int32 [1]) in sequence order; num_tokens: rows of the step's buffers,
+    [n], int32 [1]) in sequence order; out: buffers to write into, apart from
+    each other and from what is read; num_tokens: rows of the step's buffers,
     at least the new tokens (rows behind the last one get slot -1, position
     0).  Without free_pages the tables must hold the new tokens' pages
     already.  The slots go to amf_kv_scatter_slots (or an engine's own cache
@@ -472,6 +473,7 @@ def build_slot_maps(context_lens: torch.Tensor, new_tokens: torch.Tensor,
         n_free = free_pages.shape[0]
         fp = _int32(free_pages, "free_pages", idx, (n_free,))
     fu = None if free_used is None else _int32(free_used, "free_used", idx, (1,))
+    ef = _flag(err_flag, idx)
     if out is None:
         dev = block_tables.device
         slots = torch.empty(num_tokens, dtype=torch.int64, device=dev)
@@ -490,13 +492,21 @@ def build_slot_maps(context_lens: torch.Tensor, new_tokens: torch.Tensor,
                 _int32(out.query_start, "out.query_start", idx, (S + 1,)),
                 _int32(out.context_lens, "out.context_lens", idx, (S,)),
                 _int32(out.free_used, "out.free_used", idx, (1,)))
-        for p, name in ((cl, "context_lens"), (nt, "new_tokens"), (fu, "free_used")):
-            if p and p in ptrs:
-                raise ValueError(f"{name} must not be one of the outputs")
+        given = [(p, p + 8 * num_tokens) for p in ptrs[:2]]
+        given += [(p, p + 4 * n) for p, n in zip(ptrs[2:], (S + 1, S, 1))]
+        taken = {"context_lens": (cl, 4 * S), "new_tokens": (nt, 4 * S),
+                 "free_used": (fu or 0, 4), "free_pages": (fp or 0, 4 * n_free),
+                 "block_tables": (bt, 4 * ((S - 1) * row + width)),
+                 "err_flag": (ef or 0, 4)}
+        for i, (lo, hi) in enumerate(given):  # the launch's workgroups have no order
+            for name, (at, n) in taken.items():
+                if at < hi and lo < at + n and n > 0:
+                    raise ValueError(f"{name} must not overlap out.{SlotMaps._fields[i]}")
+            if any(a < hi and lo < b for a, b in given[:i]):
+                raise ValueError(f"out.{SlotMaps._fields[i]} must not overlap another output")
     _launch(
         idx, "amf_build_slot_maps", cl, nt, S, bt, row, width, block_size, pool_pages,
-        fp if n_free else None, n_free, fu, num_tokens, *ptrs, _flag(err_flag, idx),
-        _raw_stream(idx))
+        fp if n_free else None, n_free, fu, num_tokens, *ptrs, ef, _raw_stream(idx))
     return out
 
 

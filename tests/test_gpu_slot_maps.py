@@ -138,6 +138,37 @@ def test_sequences_behind_the_rows_do_not_grow():
         _compare(lens, new, 16, rows, table, free, used=2)
 
 
+def test_outputs_that_overlap_are_refused():
+    from korith_vllm_ext.kernels import SlotMaps, build_slot_maps
+
+    buf = torch.zeros(64, dtype=torch.int32, device=DEV)
+    wide = torch.zeros(8, dtype=torch.int64, device=DEV)
+    table = torch.tensor([[4, -1], [7, 1]], dtype=torch.int32, device=DEV)
+    good = dict(context_lens=buf[0:2], new_tokens=buf[2:4], block_tables=table, block_size=16,
+                num_tokens=3, free_pages=buf[4:7], free_used=buf[7:8], err_flag=buf[8:9])
+    out = SlotMaps(wide[:3], wide[3:6], buf[9:12], buf[12:14], buf[14:15])
+    buf[:8] = _i32([16, 20, 1, 1, 6, 5, 3, 0])
+    want = build_slot_maps(**{k: v.clone() if isinstance(v, torch.Tensor) else v
+                              for k, v in good.items()})
+    for o in (
+        out._replace(context_lens=buf[1:3]),   # half of context_lens, half of new_tokens
+        out._replace(query_start=buf[1:4]), out._replace(free_used=buf[3:4]),
+        out._replace(query_start=buf[6:9]), out._replace(context_lens=buf[5:7]),
+        out._replace(free_used=buf[7:8]), out._replace(free_used=buf[8:9]),
+        out._replace(context_lens=table[1]), out._replace(slot_mapping=buf[:6].view(torch.int64)),
+        out._replace(positions=wide[2:5]), out._replace(context_lens=buf[11:13]),
+        out._replace(free_used=buf[13:14]), out._replace(free_used=buf[9:10]),
+    ):
+        with pytest.raises(ValueError, match="overlap"):
+            build_slot_maps(out=o, **good)
+    got = build_slot_maps(out=out, **good)  # side by side
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and int(buf[8]) == 0
+    # no rows, no sequences: nothing that could overlap
+    none = SlotMaps(wide[:0], wide[:0], buf[9:10], buf[9:9], buf[14:15])
+    build_slot_maps(buf[0:0], buf[0:0], table[:0], block_size=16, num_tokens=0, out=none)
+    assert none.query_start.tolist() == [0] and none.free_used.tolist() == [0]
+
+
 def test_outputs_given_and_refusals():
     from korith_vllm_ext.kernels import SlotMaps, build_slot_maps
 
