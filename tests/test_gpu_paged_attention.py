@@ -264,6 +264,49 @@ def test_page_lists(dtype, Hkv, D, block):
     assert not out[1, :4].any() and not out[4].any()
 
 
+@pytest.mark.parametrize("dtype,Hq,Hkv,D,block,seqs,n", [
+    (BF, 8, 2, 128, 16, 1, 300),      # one sequence over many workgroups
+    (BF, 32, 8, 128, 16, 9, 110),
+    (FP, 16, 8, 64, 32, 90, 70),      # more sequences than shares
+    (F8, 8, 4, 128, 16, 150, 70),
+    (F8, 6, 2, 48, 5, 40, 260),       # pages that end inside a step
+    (BF, 40, 2, 256, 16, 6, 100),     # two head tiles of a group, one workgroup a CU
+    (F32, 12, 4, 96, 16, 3, 150),
+    (F32, 8, 1, 64, 16, 60, 80),      # the general kernel, two tiles
+    (BF, 3, 3, 33, 1, 5, 1500),       # pages of one token, odd head_dim
+])
+def test_page_lists_cut_between_workgroups(dtype, Hq, Hkv, D, block, seqs, n):
+    """Lists long enough to be cut: KV heads with full, short and empty lists
+    in one sequence (partials that saw no token), gaps, repeats, places behind
+    the context and outside the table, empty sequences."""
+    g = torch.Generator().manual_seed(n + seqs)
+    top = (n + n // 4) * block
+    lens = torch.randint(1, top + 1, (seqs,), generator=g).tolist()
+    lens[0] = top
+    for s in range(2, seqs, 7):
+        lens[s] = 0
+    q, kv, table = _case(dtype, Hq, Hkv, D, block, lens, seed=4)
+    pages = torch.full((seqs, Hkv, n), -1, dtype=torch.int32)
+    counts = torch.zeros(seqs, Hkv, dtype=torch.int32)
+    for s, c in enumerate(lens):
+        m = -(-c // block)
+        for h in range(Hkv):
+            k = min(n, m)
+            pages[s, h, :k] = torch.randperm(max(m, 1), generator=g)[:k].sort()[0].int()
+            counts[s, h] = (k, 0, min(k, 1), n, k // 2)[(s + h) % 5]
+            if k > 8:
+                pages[s, h, 3], pages[s, h, 5] = -1, pages[s, h, 4]
+                pages[s, h, 6], pages[s, h, 7] = 1 << 20, table.shape[1] - 1
+    if seqs > 3:
+        counts[3] = 0  # tokens, but no list
+    ref = attend64(q, kv, table, lens, 0.15, pages=pages, counts=counts)
+    out = _run(q, kv, table, lens, scale=0.15, out_dtype=F32, pages=pages.to(DEV),
+               page_counts=counts.to(DEV))
+    _check(out, ref, attend_tolerance(q, kv, lens, 0.15))
+    none = (ref == 0).all(-1)
+    assert torch.equal((out == 0).all(-1).cpu(), none) and (seqs < 4 or none[3].all())
+
+
 @pytest.mark.parametrize("what", ["lists", "tables", "hint"])
 def test_many_sequences_and_no_tokens_that_the_host_knows_of(what):
     """More pairs than a workgroup each is for, and nothing to cut: zeros, or with a
