@@ -133,6 +133,21 @@ def test_select(dtype, Hq, H, D, block, lens, keep, first, last):
     assert torch.equal(counts.cpu(), want[1]) and torch.equal(pages.cpu(), want[0])
 
 
+@pytest.mark.parametrize("n", [1023, 1024, 1025, 4095, 4096, 4097, 8191, 8192, 8193, 16385])
+def test_select_around_the_choices_row_sizes(n):
+    """Rows that the choice keeps in registers of 256 and 1024 threads, and
+    reads again for each pass; half of the pages have equal scores."""
+    lens = [n * 4, n * 4 - 3, (n - 1) * 4, n]
+    q, b, table = _selection(BF, 4, 1, 8, 4, lens, seed=n)
+    even = torch.randperm(b.shape[0], generator=torch.Generator().manual_seed(n))[::2].to(DEV)
+    b[even] = b[int(table[0, 1])].clone()  # in the middle of the scores: ties at the cut
+    for keep in (1, n // 4, n // 2, n - 1):
+        first, last = (0, 0) if keep == 1 else (1, 2)
+        pages, counts = _select(q, b, table, lens, 4, keep, first, last)
+        want = select64(q, b, table, lens, 4, keep, first, last)
+        assert torch.equal(counts.cpu(), want[1]) and torch.equal(pages.cpu(), want[0]), keep
+
+
 @pytest.mark.parametrize("kind", ["equal", "few", "near", "zero"])
 def test_select_ties(kind):
     """Equal scores go to the lowest places; scores one step apart in the last
@@ -288,6 +303,43 @@ def test_decode_loop(dtype, Hq, H, D):
         assert float((out.cpu().double() - ref).abs().max()) <= tol
         ref = attend64(q, kv, tab, lens, D ** -0.5)
         assert float((full.cpu().double() - ref).abs().max()) <= tol
+
+
+def test_captured_bounds_are_the_graphs_own():
+    """A captured bounds launch writes what the eager one does, over whatever
+    the buffer held before the replay."""
+    from korith_vllm_ext.kernels import page_key_bounds
+
+    g = torch.Generator().manual_seed(14)
+    table, pool = make_tables([300, 90, 16], 16, g)
+    kv = make_cache(pool, 16, 2, 64, BF, g)
+    bt, cl, ft = table.to(DEV), _i32([300, 90, 16]), _i32([0, 0, 0])
+    held = torch.zeros(pool, 2, 2, 64, dtype=BF, device=DEV)
+
+    def call(bounds):
+        return page_key_bounds(kv, bt, cl, first_tokens=ft, bounds=bounds)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call(held)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(held)
+    for lens, first in (([300, 90, 16], [0, 0, 0]), ([299, 33, 0], [250, 32, 0]),
+                        ([17, 90, 5], [0, 89, 0])):
+        cl.copy_(_i32(lens))
+        ft.copy_(_i32(first))
+        held.fill_(9.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        want = call(torch.full_like(held, 9.0))
+        assert torch.equal(held, want)
+        for i, b in bounds64(kv[0].float(), table, lens, 16, first).items():
+            assert torch.equal(held[i], b.to(BF).to(DEV))
+            want[i] = 9.0
+        assert bool((want == 9.0).all())
 
 
 def test_captured_step():
