@@ -315,6 +315,13 @@ def _index_tensor(t: Any, dev: torch.device) -> torch.Tensor:
     return torch.as_tensor(t, dtype=torch.int32).to(dev).contiguous()
 
 
+def _rows_apart(t: Any, idx: int) -> bool:
+    """Whether t is an int32 table on device idx whose rows are contiguous and
+    apart, such as a slice of a wider one."""
+    return (isinstance(t, torch.Tensor) and t.dtype == torch.int32 and t.get_device() == idx
+            and t.dim() == 2 and t.stride(1) == 1 and t.stride(0) >= t.shape[1])
+
+
 _ALGOS = {"auto": amf_hip.DECODE_AUTO, "valu": amf_hip.DECODE_VALU, "mfma": amf_hip.DECODE_MFMA,
           "mfma_precise": amf_hip.DECODE_MFMA_PRECISE}
 
@@ -419,14 +426,16 @@ def hip_decode_attention(q: torch.Tensor, k: Any, v: Any = None, scale: Optional
         if isinstance(k, torch.Tensor):
             if algo != "auto":
                 raise ValueError(f"algo {algo!r} is for INT4 pools")
-            bt = block_tables
-            if not (isinstance(bt, torch.Tensor) and bt.dtype == torch.int32
-                    and bt.device == k.device and bt.dim() == 2 and bt.stride(1) == 1
-                    and bt.stride(0) >= bt.shape[1]):
-                bt = _index_tensor(bt, k.device)
-            context_lens = _index_tensor(context_lens, k.device)
+            idx = k.get_device()
+            for t in (block_tables, context_lens):
+                if not (isinstance(t, torch.Tensor) and t.dtype is torch.int32
+                        and t.get_device() == idx and t.is_contiguous()):
+                    if not _rows_apart(block_tables, idx):
+                        block_tables = _index_tensor(block_tables, k.device)
+                    context_lens = _index_tensor(context_lens, k.device)
+                    break
             return paged_decode_attention(
-                q, k, v, block_tables=bt, context_lens=context_lens, scale=scale,
+                q, k, v, block_tables=block_tables, context_lens=context_lens, scale=scale,
                 max_context_len=max_context_len, pages=pages, page_counts=page_counts,
                 k_scale=k_scale, v_scale=v_scale, out=out, out_dtype=out_dtype,
                 workspace=workspace, err_flag=err_flag)

@@ -72,19 +72,16 @@ _SCRATCH_MAX = 16
 _SCRATCH_LOCK = threading.Lock()
 
 
-def _capturing(idx: int) -> bool:
-    """Whether the current stream of device idx, which the call launches on, is
-    under graph capture; torch answers for the current device's."""
-    if _current_device() == idx:
-        return torch.cuda.is_current_stream_capturing()
-    with torch.cuda.device(idx):
-        return torch.cuda.is_current_stream_capturing()
-
-
 def _scratch(dev: torch.device, stream: int, nbytes: int) -> torch.Tensor:
-    if _capturing(dev.index):
+    idx = dev.index
+    if _current_device() == idx:
+        capturing = torch.cuda.is_current_stream_capturing()
+    else:  # torch answers for the current device's stream, not that of the launch
+        with torch.cuda.device(idx):
+            capturing = torch.cuda.is_current_stream_capturing()
+    if capturing:
         return torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    key = (dev.index, stream, threading.get_ident())
+    key = (idx, stream, threading.get_ident())
     buf = _SCRATCH.get(key)
     if buf is not None and buf.numel() >= nbytes:
         try:
@@ -120,12 +117,12 @@ def _workspace(name: str, sizes: tuple, given: Optional[torch.Tensor], dev: torc
     return (_scratch(dev, stream, need), need) if need else (None, 0)
 
 
-def _cache(k: torch.Tensor, v: Optional[torch.Tensor]) -> tuple:
+def _cache(k: torch.Tensor, v: Optional[torch.Tensor], keys: bool = False) -> tuple:
     """(device index, K address, V address, strides of page, token and head,
     pages, block, heads, dim) of a layer [2, pages, block, heads, dim] (v
     None), or of K and V planes [pages, block, heads, dim] with the same
-    strides; of a plane alone it is K's address twice.  The last dim is
-    contiguous, the others may be strided."""
+    strides; `keys`: a K plane alone will do.  The last dim is contiguous, the
+    others may be strided."""
     if not isinstance(k, torch.Tensor):
         raise TypeError(f"a K/V cache is a tensor, got {type(k).__name__}")
     idx = k.get_device()
@@ -153,6 +150,9 @@ def _cache(k: torch.Tensor, v: Optional[torch.Tensor]) -> tuple:
             if v.dtype != k.dtype or v.device != k.device:
                 raise ValueError("K and V planes differ in type or device")
             vp = v.data_ptr()
+        elif v is None and not keys:
+            raise ValueError("a K plane comes with the V plane (v_cache=k_cache where it holds "
+                             "both)")
     if k.dtype not in _KV_TAGS:
         raise TypeError(f"paged cache of {k.dtype}: bf16, fp16, fp32 or float8_e4m3fn")
     if ds != 1 and D != 1:
@@ -247,8 +247,6 @@ def paged_decode_attention(q: torch.Tensor, k_cache: torch.Tensor,
     to the listed places of the block table (select_pages makes them).  out:
     contiguous, q's shape; otherwise one of out_dtype (q's type)."""
     idx, kp, vp, ps, ts, hs, nb, bs, H, D = _cache(k_cache, v_cache)
-    if v_cache is None and k_cache.dim() == 4:
-        raise ValueError("a K plane comes with the V plane (v_cache=k_cache where it holds both)")
     q3 = _query(q, idx, D)
     S, Hq, _ = q3.shape
     kdt, qdt = k_cache.dtype, q3.dtype
@@ -323,7 +321,7 @@ def page_key_bounds(k_cache: torch.Tensor, block_tables: torch.Tensor,
     Sequences that share a page have to use as many tokens of it, as those do
     that share a prefix in whole pages; else the bounds are either's.
     Returns bounds."""
-    idx, kp, _, ps, ts, hs, nb, bs, H, D = _cache(k_cache, None)
+    idx, kp, _, ps, ts, hs, nb, bs, H, D = _cache(k_cache, None, True)
     kdt = k_cache.dtype
     if kdt is torch.float32 or D % 8 or D > 256:
         raise ValueError(f"page bounds need a bf16, fp16 or FP8 cache with head_dim a multiple of "
