@@ -6,8 +6,10 @@
 //   out[s, h] = v_scale * sum_t softmax_t(k_scale * scale * q[s, h] . k[t]) v[t]
 //
 // over the context_lens[s] tokens of the sequence, or those of the pages listed
-// for its KV head.  Each K and V element is read once, for all query heads that
-// share it, and meets the running maximum m and sum l of each head's softmax.
+// for its KV head.  Each K and V element is read once for a tile of the query heads
+// that share it (up to 16 in the matrix kernel, 4 in the general one; larger groups
+// read it again for each tile), and meets the running maximum m and sum l of each
+// head's softmax.
 //
 // Work.  The contexts of all sequences, one after the other, are steps, cut into
 // equal shares; a share is taken by a few workgroups side by side, each for one, two
@@ -21,8 +23,8 @@
 // sequence and pair and no second launch.
 //
 // Measured (MI355X, bytes of K and V over the call's time): 32 sequences of 1K-32K
-// tokens, bf16, 32 / 8 heads of 128, 338 us, 6.6 TB/s; 8 x 126K tokens, FP8, 64 / 8
-// heads, 336 us, 6.1 TB/s; 200 chats of 1-1200 tokens, fp16, 101 us, 4.9 TB/s (a share
+// tokens, bf16, 32 / 8 heads of 128, 340 us, 6.5 TB/s; 8 x 126K tokens, FP8, 64 / 8
+// heads, 336 us, 6.1 TB/s; 200 chats of 1-1200 tokens, fp16, 105 us, 4.7 TB/s (a share
 // is two sequences there, and the beginning of each is latency); two short contexts
 // 11 us, nothing but latency.  The large ones are bound by HBM.
 #include <algorithm>
@@ -334,14 +336,16 @@ __device__ __forceinline__ void empty_seqs(const PagedArgs& a) {
 //
 // Any element type, head_dim up to 256, strides and alignment.  LPR lanes share a
 // token's row, 8 dims each (one or two 16-byte loads, or element by element where
-// rows are not aligned or end inside one), so a wave reads 64 / LPR rows at once, kGenAhead of them
-// after each other in flight; every such group of lanes keeps its own m, l and
+// rows are not aligned or end inside one), so a wave reads 64 / LPR rows at once,
+// kGenAhead of them after each other in flight; every such group of lanes keeps its own m, l and
 // output for 4 query heads, and all groups of the workgroup are joined in LDS.
-// fp32, 12 / 4 heads of 96, 2 x 9500 tokens, 58 MB: 34 us, 1.7 TB/s; 32 / 8 of 128, 4 x
-// 9500, 311 MB: 79 us, 4.0 TB/s, where the beginning and the merge are some 20 us.  A
-// branch around the loads, in place of page 0's rows, 37 and 79 us; the next step's rows
-// asked for before this one's are used 34 and 79; a lane per token for the scores and a
-// lane per dim for the output, with element loads, 88 us for the first.
+// fp32, 12 / 4 heads of 96, 2 x 9500 tokens, 58 MB: 33 us, 1.75 TB/s; 32 / 8 of 128, 4 x
+// 9500, 311 MB: 78 us, 4.0 TB/s, where the beginning and the merge are some 20 us; 64 / 8
+// of 128, whose K and V are read twice, 111 us; 36 dims of fp16, element by element, 37
+// MB in 58 us.  Tried, against 34 and 79 us of the first two: a branch around the loads,
+// in place of page 0's rows, 37 and 79; the next step's rows asked for before this one's
+// are used, 34 and 79; a lane per token for the scores and a lane per dim for the
+// output, with element loads, 88 for the first.
 constexpr int kGenHeads = 4;  // query heads of a tile
 constexpr int kGenAhead = 4;  // rows of a group of lanes in a step
 
@@ -536,8 +540,8 @@ __device__ __forceinline__ uint32_t e4m3_pair(uint32_t w) {
 
 constexpr int kTileHeads = 16;
 // Waves per SIMD, at least.  256 dims of 16 bits spill at two (164 sequences of 4700
-// fp16 tokens 272 -> 434 us); of FP8 they are faster with a few words spilled (174 ->
-// 154, 200 chats 53 -> 47).
+// fp16 tokens 272 -> 434 us); of FP8 they are faster with 12 to 15 words spilled (the same
+// 170 -> 163, 200 chats 53 -> 48).
 constexpr int matrix_waves(int D, int es) { return D == 256 && es == 2 ? 1 : 2; }
 // Tokens of a wave's step.  64 of 64 dims (two sequences of 700 tokens 12.3 -> 11.6
 // us; fewer, larger steps); 64 of 128 FP8 dims are as many bytes but slower than 32
@@ -895,13 +899,18 @@ __global__ __launch_bounds__(NT) void paged_attn_merge_kernel(PagedArgs a, int h
 // ---- launch --------------------------------------------------------------------
 
 // Workgroups that share a launch's steps: two a CU, all resident (32 sequences of
-// 1K-32K tokens 364 us; 256: 385, 1024: 372; 2048 tokens of listed pages 28, 32, 33).
+// 1K-32K tokens 337 us; 256: 343, 1024: 348; 8 x 126K FP8 tokens 339, 483, 360; a
+// selection and 4096 listed tokens each of 8 sequences 80, 80, 86).
 constexpr int64_t kGroups = 512;
 // Short contexts take a workgroup a (sequence, pair) and no merge: at most so many
-// steps and pairs.  8 KV heads of 128, split / whole, us: 1 x 128 tokens 12.4 / 7.0,
-// 1 x 500 12.8 / 11.4, 64 x 500 33 / 26, 160 x 500 61 / 60; but 1 x 1000 13.3 / 17.1, 256
-// x 500 86 / 91, 256 x 128 30 / 37.  (Equal lengths; of mixed ones the longest would
-// decide.)
+// steps and pairs.  8 KV heads of 128, bf16, split / whole, us: 1 x 128 tokens 12.5 / 7.0,
+// 1 x 500 12.9 / 11.4, 64 x 500 33 / 26, 160 x 500 68 / 66; but 1 x 1000 13.4 / 17.2, 256
+// x 128 30 / 37.  (Equal lengths; of mixed ones the longest would decide.)  FP8 and 64
+// dims are alike (1 x 500 12.7 / 11.1, 12.3 / 9.2; 160 x 500 47 / 43, 20 / 15), fp32 by
+// rows too (12 / 4 heads of 96, 1 x 128 12.8 / 11.8).  256 dims of 16 bits, whose step is
+// twice the bytes at one workgroup a CU, are slower whole but for one short sequence (2
+// KV heads, 1 x 128 15.7 / 11.7; 1 x 500 16 / 25, 160 x 128 23 / 25, 160 x 500 48 / 54):
+// the rule does not look at that yet.
 constexpr int64_t kWholeSteps = 4;
 constexpr int64_t kWholePairs = 3 * kGroups;
 
@@ -1064,8 +1073,8 @@ extern "C" int amf_paged_decode_attn(
     return fail(AMF_ERR_UNSUPPORTED, "%s: %d sequences of %d heads", who, num_seqs, num_q_heads);
   a.whole = steps <= kWholeSteps && pairs <= kWholePairs;
   // pairs side by side on the waves of a workgroup: their rows lie side by side in
-  // memory and are asked for at the same time.  32 sequences of 1K-32K tokens 364 us
-  // with one pair a workgroup, 336 with four; page lists differ from head to head,
+  // memory and are asked for at the same time.  32 sequences of 1K-32K tokens 365 us
+  // with one pair a workgroup, 337 with four (8 x 126K FP8 389, 339); page lists differ from head to head,
   // and a whole sequence has too few workgroups.
   const int64_t heads = (int64_t)num_kv_heads * a.tiles;
   a.side = 1;
@@ -1074,7 +1083,7 @@ extern "C" int amf_paged_decode_attn(
   const int64_t teams = heads / a.side;
   const int64_t most_steps = num_seqs * ((tokens + (1 << a.step_shift) - 1) >> a.step_shift);
   // one workgroup a CU where two do not fit: 512 shares of 256 dims are taken in two
-  // rounds (164 sequences of 4700 fp16 tokens 288 us, 272 with 256)
+  // rounds (164 sequences of 4700 fp16 tokens 289 us, 272 with 256)
   const bool half = matrix && matrix_waves(matrix_dim(head_dim), es) == 1;
   const int64_t resident = half ? kGroups / 2 : kGroups;
   const int64_t shares =
@@ -1099,7 +1108,7 @@ extern "C" int amf_paged_decode_attn(
   if (int rc = check_launch(who)) return rc;
   if (a.whole) return ok();
   // partials of a pair, about: many take a workgroup a head, hundreds (one long
-  // context) a larger one (131072 tokens of one KV head 44 -> 26 us a call)
+  // context) a larger one (131072 tokens of one KV head 44 -> 27 us a call)
   const int64_t parts = shares / num_seqs;
   const int32_t tile_heads = std::min<int32_t>(a.group, tile);
   const int cols = matrix ? head_dim / 4 : head_dim;

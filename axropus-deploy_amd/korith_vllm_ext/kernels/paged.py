@@ -238,8 +238,10 @@ def paged_decode_attention(q: torch.Tensor, k_cache: torch.Tensor,
     q [seqs, Hq, D] or [seqs, Hq, 1, D]; k_cache a layer [2, pages, block, Hkv,
     D], or the K plane [pages, block, Hkv, D] with v_cache the V plane of the
     same strides (any order of block and heads; k_cache itself, if one plane
-    holds both); D at most 256, Hq a multiple
-    of Hkv.  q has the cache's type, with an FP8 cache bf16 or fp16.
+    holds both); D at most 256, Hq a multiple of Hkv.  q has the cache's type,
+    with an FP8 cache bf16 or fp16 (one kept as uint8 is given as
+    k_cache.view(torch.float8_e4m3fn)).  16-byte aligned rows and out, and D a
+    multiple of 16, take matrix tiles; other calls and fp32 a slower kernel.
     block_tables int32 [seqs, max_pages], context_lens int32 [seqs] (tokens in
     the cache, the new one among them); a sequence without tokens gives zeros.
     max_context_len, where the caller knows one, helps to cut the work.  pages
@@ -441,8 +443,8 @@ def build_slot_maps(context_lens: torch.Tensor, new_tokens: torch.Tensor,
     [n], int32 [1]) in sequence order; out: buffers to write into, apart from
     each other and from what is read; num_tokens: rows of the step's buffers,
     at least the new tokens (rows behind the last one get slot -1, position
-    0).  Without free_pages the tables must hold the new tokens' pages
-    already.  The slots go to amf_kv_scatter_slots (or an engine's own cache
+    0).  Without free_pages no sequence gets a page: new tokens have room only
+    in the pages that context_lens reaches already.  The slots go to amf_kv_scatter_slots (or an engine's own cache
     write) as they are.
 
     A sequence whose pages the free list or its table row does not hold, or

@@ -389,7 +389,9 @@ int amf_int4_paged_decode_attn_noalloc(const void* q, int32_t q_dtype, void* out
  * sequence's block table that the KV head attends to, of which the first
  * page_counts[s][h] count; negative entries are skipped, a place listed twice
  * counts twice.  A sequence without tokens gives zeros; scores that are all
- * -inf, or hold a NaN or +inf, give NaN, as softmax does.
+ * -inf, or hold a NaN or +inf, give NaN, as softmax does.  Matrix tiles take
+ * 16-bit q with head_dim a multiple of 16 where q, k, v, out and every stride
+ * are 16-byte aligned; all other calls, fp32 among them, take a slower kernel.
  * softmax_scale <= 0 selects 1/sqrt(head_dim).  max_context_len: at least every
  * context length (only a hint of how to cut the work).
  * workspace: amf_paged_decode_workspace_bytes() bytes, 16-byte aligned; calls
@@ -416,7 +418,9 @@ int amf_paged_decode_attn(const void* q, int32_t q_dtype, int64_t q_seq_stride,
  * first_tokens[s] on (NULL: all).  max_new_tokens > 0 promises
  * context_lens[s] - first_tokens[s] <= max_new_tokens and sizes the grid.
  * Sequences that share a page have to use as many tokens of it (a prefix in
- * whole pages does); else one's bounds stay, of either.  bounds_dtype is
+ * whole pages does); else one's bounds stay, of either.  Nothing else keeps
+ * bounds up: after a restore into the pages they are the caller's to make.
+ * bounds_dtype is
  * kv_dtype, or for _E4M3 keys (taken without k_scale) bf16 or fp16; fp32
  * caches are AMF_ERR_UNSUPPORTED.  head_dim a multiple of 8 up to 256; keys and
  * strides aligned to 8 elements.  NaN keys make NaN bounds. */
@@ -435,7 +439,9 @@ int amf_page_key_bounds(const void* k, int32_t kv_dtype, int64_t page_stride,
  * and last last_pages always among them.  pages int32
  * [num_seqs][num_kv_heads][num_pages]: places in the block table in ascending
  * order, -1 behind the page_counts[s][h] = min(num_pages, pages of s) of them.
- * A page with a bound or a score that is not finite ranks above the others.  q, its strides
+ * A page with a bound or a score that is not finite ranks above the others, one
+ * whose id is outside [0, pool_pages) behind them; a sequence of no more than
+ * num_pages pages gets all of them, and no id is looked at.  q, its strides
  * and bounds 16-byte aligned, of one dtype (bf16 or fp16).
  * max_context_len: at least every context length (longer ones are cut, flagged
  * AMF_ERRFLAG_CONTEXT); more than 65535 * 64 pages of a sequence are
@@ -471,8 +477,10 @@ int amf_select_pages(const void* q, int32_t dtype, int64_t q_seq_stride, int64_t
  * none: its context_out is context_lens, its slots are -1.  A page id outside
  * [0, pool_pages) gives slots of -1 (AMF_ERRFLAG_BLOCK_RANGE), and one from the
  * free list a block_tables entry of -1, so that later steps flag it again.
- * Replaces the slots of AMFReqMeta.make (amf_kv_connector.py:90-115), built on
- * the host per request. */
+ * n_free = 0: no sequence gets a page, so that new tokens have room only in the
+ * pages that context_lens reaches already.
+ * The device form of the slots that AMFReqMeta.make (amf_kv_connector.py:90-115)
+ * makes on the host, per request; the connector uses the host form. */
 int amf_build_slot_maps(const int32_t* context_lens, const int32_t* new_tokens,
                         int32_t num_seqs, int32_t* block_tables, int64_t bt_stride,
                         int32_t table_pages, int32_t block_size, int64_t pool_pages,
