@@ -337,8 +337,9 @@ __device__ __forceinline__ void empty_seqs(const PagedArgs& a) {
 // Any element type, head_dim up to 256, strides and alignment.  LPR lanes share a
 // token's row, 8 dims each (one or two 16-byte loads, or element by element where
 // rows are not aligned or end inside one), so a wave reads 64 / LPR rows at once,
-// kGenAhead of them after each other in flight; every such group of lanes keeps its own m, l and
-// output for 4 query heads, and all groups of the workgroup are joined in LDS.
+// kGenAhead of them after each other in flight; every such group of lanes keeps its
+// own m, l and output for 4 query heads, and all groups of the workgroup are joined in
+// LDS.
 // fp32, 12 / 4 heads of 96, 2 x 9500 tokens, 58 MB: 33 us, 1.75 TB/s; 32 / 8 of 128, 4 x
 // 9500, 311 MB: 78 us, 4.0 TB/s, where the beginning and the merge are some 20 us; 64 / 8
 // of 128, whose K and V are read twice, 111 us; 36 dims of fp16, element by element, 37
@@ -481,7 +482,8 @@ __global__ __launch_bounds__(kThreads) void paged_attn_general_kernel(PagedArgs 
         x = __builtin_fmaf(acc_lds[w][g][d], f, x);
       }
       if (sg.whole) {
-        store_out(a, (sg.head0 + g) * D + d, sum == 0.0f ? 0.0f : x * row_factor(a.v_scale, top, sum));
+        store_out(a, (sg.head0 + g) * D + d,
+                  sum == 0.0f ? 0.0f : x * row_factor(a.v_scale, top, sum));
       } else {
         float* part = sg.part + g * (D + kPartPad);
         part[d] = x;
@@ -1074,8 +1076,8 @@ extern "C" int amf_paged_decode_attn(
   a.whole = steps <= kWholeSteps && pairs <= kWholePairs;
   // pairs side by side on the waves of a workgroup: their rows lie side by side in
   // memory and are asked for at the same time.  32 sequences of 1K-32K tokens 365 us
-  // with one pair a workgroup, 337 with four (8 x 126K FP8 389, 339); page lists differ from head to head,
-  // and a whole sequence has too few workgroups.
+  // with one pair a workgroup, 337 with four (8 x 126K FP8 389, 339); page lists differ
+  // from head to head, and a whole sequence has too few workgroups.
   const int64_t heads = (int64_t)num_kv_heads * a.tiles;
   a.side = 1;
   if (matrix && !a.whole && !pages) a.side = heads % 4 == 0 ? 4 : heads % 2 == 0 ? 2 : 1;

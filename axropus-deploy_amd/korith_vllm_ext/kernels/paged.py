@@ -444,8 +444,8 @@ def build_slot_maps(context_lens: torch.Tensor, new_tokens: torch.Tensor,
     each other and from what is read; num_tokens: rows of the step's buffers,
     at least the new tokens (rows behind the last one get slot -1, position
     0).  Without free_pages no sequence gets a page: new tokens have room only
-    in the pages that context_lens reaches already.  The slots go to amf_kv_scatter_slots (or an engine's own cache
-    write) as they are.
+    in the pages that context_lens reaches already.  The slots go to
+    amf_kv_scatter_slots (or an engine's own cache write) as they are.
 
     A sequence whose pages the free list or its table row does not hold, or
     whose tokens the rows do not, keeps its length and gets slots of -1
