@@ -59,6 +59,7 @@ LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libamf_hip.
 _c_i32 = ctypes.c_int32
 _c_i64 = ctypes.c_int64
 _c_f32 = ctypes.c_float
+_c_f64 = ctypes.c_double
 _c_ptr = ctypes.c_void_p
 _c_u32 = ctypes.c_uint32
 _c_u64 = ctypes.c_uint64
@@ -155,6 +156,36 @@ SIGNATURES = {
         [_c_ptr, _c_i32, _c_i64, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_i64, _c_i32, _c_ptr, _c_i32,
          _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_ptr, _c_ptr, _c_ptr,
          _c_i64, _c_ptr, _c_ptr],
+    ),
+    "amf_rotary_embedding": (
+        _c_i32,
+        [_c_ptr, _c_i64, _c_i64, _c_ptr, _c_i64, _c_i64, _c_i32, _c_ptr, _c_i64, _c_i64, _c_ptr,
+         _c_i64, _c_i64, _c_i32, _c_i32, _c_i64, _c_i32, _c_ptr, _c_ptr, _c_i32, _c_i32, _c_f64,
+         _c_ptr],
+    ),
+    "amf_kv_write": (
+        _c_i32,
+        [_c_ptr, _c_i64, _c_i64, _c_ptr, _c_i64, _c_i64, _c_i32, _c_i64, _c_i32, _c_i32, _c_ptr,
+         _c_ptr, _c_ptr, _c_i32, _c_i64, _c_i64, _c_i64, _c_i64, _c_i32, _c_f32, _c_f32, _c_ptr,
+         _c_ptr, _c_i32, _c_i32, _c_f64, _c_ptr, _c_i64, _c_i64, _c_ptr, _c_i64, _c_i64, _c_i32,
+         _c_ptr, _c_ptr],
+    ),
+    "amf_int4_kv_write": (
+        _c_i32,
+        [_c_ptr, _c_i64, _c_i64, _c_ptr, _c_i64, _c_i64, _c_i32, _c_i64, _c_i32, _c_i32, _c_ptr,
+         _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_ptr, _c_ptr, _c_i32, _c_i32, _c_f64, _c_ptr,
+         _c_i64, _c_i64, _c_ptr, _c_i64, _c_i64, _c_i32, _c_ptr, _c_ptr],
+    ),
+    "amf_kv_read": (
+        _c_i32,
+        [_c_ptr, _c_ptr, _c_i32, _c_i64, _c_i64, _c_i64, _c_i64, _c_i32, _c_f32, _c_f32, _c_ptr,
+         _c_ptr, _c_i64, _c_i64, _c_ptr, _c_i64, _c_i64, _c_i32, _c_i64, _c_i32, _c_i32, _c_ptr,
+         _c_ptr],
+    ),
+    "amf_int4_kv_read": (
+        _c_i32,
+        [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_ptr, _c_ptr, _c_i64, _c_i64, _c_ptr, _c_i64,
+         _c_i64, _c_i32, _c_i64, _c_i32, _c_i32, _c_ptr, _c_ptr],
     ),
     "amf_build_slot_maps": (
         _c_i32,

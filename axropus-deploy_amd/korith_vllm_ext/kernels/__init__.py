@@ -21,12 +21,22 @@ from .paged import (
     paged_decode_attention,
     select_pages,
 )
+from .step import (
+    Rotary,
+    int4_page_pool,
+    read_kv_cache,
+    rotary_embedding,
+    rotary_frequencies,
+    write_kv_cache,
+)
 
 __all__ = [
     "KERNEL_DISPATCH",
+    "Rotary",
     "SlotMaps",
     "build_slot_maps",
     "dense_attention",
+    "int4_page_pool",
     "int4_sym_attention",
     "dispatch_kernel",
     "fallback_fp16_kernel",
@@ -35,7 +45,11 @@ __all__ = [
     "page_key_bounds",
     "paged_decode_attention",
     "paged_int4_decode",
+    "read_kv_cache",
     "register_kernel",
+    "rotary_embedding",
+    "rotary_frequencies",
     "select_pages",
     "try_load_cuda_extension",
+    "write_kv_cache",
 ]

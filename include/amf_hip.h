@@ -489,6 +489,83 @@ int amf_build_slot_maps(const int32_t* context_lens, const int32_t* new_tokens,
                         int32_t* query_start, int32_t* context_out, int32_t* free_used_out,
                         int32_t* err_flag, void* stream);
 
+/* ---- the rows of a step -------------------------------------------------------
+ * Rows are [n_rows][heads][head_dim] with strides in elements, dims contiguous,
+ * of `dtype` (bf16, fp16, fp32).  slot_mapping: device int64 [n_rows], page id *
+ * block_size + place in the page, as amf_build_slot_maps writes it; negative =
+ * no slot, and a slot outside the pool is none either (AMF_ERRFLAG_BLOCK_RANGE).
+ * head_dim at most 512, n_rows at most 2^25.  n_rows = 0 does nothing.  Chunks of
+ * 8 elements are moved where n_pairs and head_dim are multiples of 8 and every
+ * pointer and stride is 16-byte aligned (FP8 caches: 8), single ones elsewhere.
+ * No counterpart in the reference.
+ *
+ * Rotary positions: pair i of a head, dims (i, i + n_pairs) or, interleaved,
+ * (2i, 2i + 1), turns by the angle positions[row] * freqs[i] (device int64 of
+ * either sign, device double [n_pairs], radians):
+ *   (a, b) -> factor * (a cos - b sin, b cos + a sin)
+ * in 64 bits, rounded to fp32 and then to dtype.  Dims from 2 * n_pairs on stay.
+ * n_pairs = 0 rotates nothing (positions and freqs may be NULL).
+ *
+ * amf_rotary_embedding: q into q_out, k into k_out, each in place (the same
+ * address and strides) or apart; either may have 0 heads. */
+int amf_rotary_embedding(const void* q, int64_t q_row_stride, int64_t q_head_stride, void* q_out,
+                         int64_t qo_row_stride, int64_t qo_head_stride, int32_t num_q_heads,
+                         const void* k, int64_t k_row_stride, int64_t k_head_stride, void* k_out,
+                         int64_t ko_row_stride, int64_t ko_head_stride, int32_t num_kv_heads,
+                         int32_t dtype, int64_t n_rows, int32_t head_dim,
+                         const int64_t* positions, const double* freqs, int32_t n_pairs,
+                         int32_t interleaved, double factor, void* stream);
+
+/* Row r of k (rotated, rounded to dtype) and of v at slot_mapping[r] of a cache
+ * with the strides of amf_paged_decode_attn: of dtype, as they are; of
+ * AMF_DTYPE_E4M3, e4m3fn_rne(clamp(x / scale, -448, 448)), NaN for a NaN.  q
+ * (num_q_heads > 0) is rotated into q_out in the same launch.  Rows without a
+ * slot are left out; where several have the same slot, it holds values of any
+ * of them. */
+int amf_kv_write(const void* k, int64_t k_row_stride, int64_t k_head_stride, const void* v,
+                 int64_t v_row_stride, int64_t v_head_stride, int32_t dtype, int64_t n_rows,
+                 int32_t num_kv_heads, int32_t head_dim, const int64_t* slot_mapping,
+                 void* k_cache, void* v_cache, int32_t kv_dtype, int64_t page_stride,
+                 int64_t token_stride, int64_t head_stride, int64_t pool_pages,
+                 int32_t block_size, float k_scale, float v_scale, const int64_t* positions,
+                 const double* freqs, int32_t n_pairs, int32_t interleaved, double factor,
+                 const void* q, int64_t q_row_stride, int64_t q_head_stride, void* q_out,
+                 int64_t qo_row_stride, int64_t qo_head_stride, int32_t num_q_heads,
+                 int32_t* err_flag, void* stream);
+
+/* The same into an AMF_FMT_INT4_ASYM_G32 pool (planes 16-byte aligned, head_dim a
+ * multiple of 32): the codes and params that amf_int4_quant_gather makes of a
+ * cache holding these rows; the page's other tokens stay.  Rows that follow each
+ * other at consecutive slots of an 8-token half page are written together; the
+ * order of rows does not matter otherwise.  Several rows of one slot leave that
+ * token's V codes a mixture of theirs. */
+int amf_int4_kv_write(const void* k, int64_t k_row_stride, int64_t k_head_stride, const void* v,
+                      int64_t v_row_stride, int64_t v_head_stride, int32_t dtype, int64_t n_rows,
+                      int32_t num_kv_heads, int32_t head_dim, const int64_t* slot_mapping,
+                      void* k_codes, void* k_params, void* v_codes, void* v_params,
+                      int64_t pool_pages, const int64_t* positions, const double* freqs,
+                      int32_t n_pairs, int32_t interleaved, double factor, const void* q,
+                      int64_t q_row_stride, int64_t q_head_stride, void* q_out,
+                      int64_t qo_row_stride, int64_t qo_head_stride, int32_t num_q_heads,
+                      int32_t* err_flag, void* stream);
+
+/* Rows k, v of slots of a cache: as they are (kv_dtype = dtype), or
+ * dtype(fp32(code) * scale) of AMF_DTYPE_E4M3.  Rows without a slot become zeros. */
+int amf_kv_read(const void* k_cache, const void* v_cache, int32_t kv_dtype, int64_t page_stride,
+                int64_t token_stride, int64_t head_stride, int64_t pool_pages,
+                int32_t block_size, float k_scale, float v_scale, const int64_t* slot_mapping,
+                void* k, int64_t k_row_stride, int64_t k_head_stride, void* v,
+                int64_t v_row_stride, int64_t v_head_stride, int32_t dtype, int64_t n_rows,
+                int32_t num_kv_heads, int32_t head_dim, int32_t* err_flag, void* stream);
+
+/* The same of an AMF_FMT_INT4_ASYM_G32 pool: dtype(u * s + z), as
+ * amf_int4_dequant_scatter restores it. */
+int amf_int4_kv_read(const void* k_codes, const void* k_params, const void* v_codes,
+                     const void* v_params, int64_t pool_pages, const int64_t* slot_mapping,
+                     void* k, int64_t k_row_stride, int64_t k_head_stride, void* v,
+                     int64_t v_row_stride, int64_t v_head_stride, int32_t dtype, int64_t n_rows,
+                     int32_t num_kv_heads, int32_t head_dim, int32_t* err_flag, void* stream);
+
 /* ---- prefix keys (host functions, no device work) ---------------------------
  * FNV-1a over bytes, continuing from hash h (pass AMF_FNV_OFFSET to start).
  * Replaces _fnv1a_bytes (amf_kv_manager.py:69-72; C++ hash_bytes of

@@ -1,0 +1,130 @@
+"""Argument checks of the step operators' C entry points, and the rotary
+frequencies, on the CPU: every call fails validation (or has nothing to do)
+before any HIP call."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+import amf_hip
+
+FAKE = 1 << 20  # never dereferenced
+
+pytestmark = pytest.mark.skipif(torch.cuda.is_available(),
+                                reason="argument-validation calls run on the CPU only")
+
+Q = dict(q=FAKE, q_row=512, q_head=64, qo=FAKE, qo_row=512, qo_head=64, hq=8)
+ROT = dict(pos=FAKE, freqs=FAKE, pairs=32, inter=0, factor=1.0)
+KV = dict(k=FAKE, k_row=128, k_head=64, v=FAKE, v_row=128, v_head=64, dtype=2, rows=4, hkv=2,
+          dim=64, slots=FAKE)
+CACHE = dict(kc=FAKE, vc=FAKE, kv_dtype=2, page=2048, token=128, head=64, pool=8, block=16,
+             ks=1.0, vs=1.0)
+POOL = dict(kc=FAKE, kp=FAKE, vc=FAKE, vp=FAKE, pool=8)
+END = dict(err=None, stream=None)
+OUT = dict(slots=FAKE, k=FAKE, k_row=128, k_head=64, v=FAKE, v_row=128, v_head=64, dtype=2,
+           rows=4, hkv=2, dim=64)
+CALLS = {
+    "amf_rotary_embedding": Q | dict(k=FAKE, k_row=128, k_head=64, ko=FAKE, ko_row=128, ko_head=64,
+                                     hkv=2, dtype=2, rows=4, dim=64) | ROT | dict(stream=None),
+    "amf_kv_write": KV | CACHE | ROT | Q | END,
+    "amf_int4_kv_write": KV | POOL | ROT | Q | END,
+    "amf_kv_read": CACHE | OUT | END,
+    "amf_int4_kv_read": POOL | OUT | END,
+}
+INV, UNS = amf_hip.ERR_INVALID_ARG, amf_hip.ERR_UNSUPPORTED
+ALL = [(n, c, w, d) for n in CALLS for c, w, d in (
+    (INV, "dtype", dict(dtype=3)), (INV, "n_rows", dict(rows=-1)), (UNS, "n_rows",
+                                                                   dict(rows=(1 << 25) + 1)),
+    (UNS, "head_dim", dict(dim=544)), (INV, "heads", dict(hkv=-1)), (INV, "null", dict(k=None)))]
+
+
+@pytest.mark.parametrize("name,code,word,change", ALL + [
+    ("amf_rotary_embedding", INV, "pairs", dict(pairs=33)),
+    ("amf_rotary_embedding", INV, "pairs", dict(pos=None)),
+    ("amf_rotary_embedding", INV, "null", dict(qo=None)),
+    ("amf_rotary_embedding", INV, "heads", dict(hq=0, hkv=0)),
+    ("amf_kv_write", INV, "pairs", dict(freqs=None)),
+    ("amf_kv_write", UNS, "type", dict(kv_dtype=0)),
+    ("amf_kv_write", INV, "block_size", dict(block=0)),
+    ("amf_kv_write", INV, "pool_pages", dict(pool=0)),
+    ("amf_kv_write", INV, "scales", dict(ks=0.0)),
+    ("amf_kv_write", INV, "scales", dict(vs=float("nan"))),
+    ("amf_kv_write", INV, "null", dict(slots=None)),
+    ("amf_kv_write", INV, "null", dict(q=None)),
+    ("amf_int4_kv_write", UNS, "multiple", dict(dim=80)),
+    ("amf_int4_kv_write", INV, "aligned", dict(vp=FAKE + 4)),
+    ("amf_int4_kv_write", INV, "pool_pages", dict(pool=0)),
+    ("amf_kv_read", UNS, "type", dict(kv_dtype=1)),
+    ("amf_kv_read", INV, "block_size", dict(block=-1)),
+    ("amf_int4_kv_read", UNS, "multiple", dict(dim=40)),
+    ("amf_int4_kv_read", INV, "aligned", dict(kc=FAKE + 8)),
+    ("amf_int4_kv_read", INV, "null", dict(kp=None)),
+])
+def test_refused(name, code, word, change):
+    with pytest.raises(amf_hip.AmfHipError) as e:
+        amf_hip.call(name, *(CALLS[name] | change).values())
+    assert e.value.code == code and word in e.value.message
+
+
+@pytest.mark.parametrize("name", list(CALLS))
+def test_nothing_to_do(name):
+    amf_hip.call(name, *(CALLS[name] | dict(rows=0, k=None)).values())
+
+
+def _turns(f, context):
+    return context * f / (2 * math.pi)
+
+
+def test_frequencies():
+    """Each scaling against its definition, pair by pair."""
+    from korith_vllm_ext.kernels import rotary_frequencies as make
+
+    def freqs(**kw):
+        r = make(64, base=10000.0, device="cpu", **kw)
+        return r.frequencies.tolist(), r.factor
+
+    plain = [10000.0 ** (-2 * i / 64) for i in range(32)]
+    f, factor = freqs()
+    assert factor == 1.0 and all(math.isclose(a, b, rel_tol=1e-14) for a, b in zip(f, plain))
+    f, _ = freqs(scaling="linear", factor=4.0)
+    assert all(math.isclose(4 * a, b, rel_tol=1e-14) for a, b in zip(f, plain))
+    f, _ = freqs(scaling="ntk", factor=4.0)  # the slowest pair is interpolated, the first stays
+    assert f[0] == 1.0 and math.isclose(4 * f[-1], plain[-1], rel_tol=1e-12)
+    f, _ = freqs(scaling="bands", factor=8.0, original_context=512)
+    for a, b in zip(f, plain):
+        t = _turns(b, 512)
+        keep = 1.0 if t > 4 else 0.0 if t < 1 else (t - 1) / 3
+        assert math.isclose(a, b * keep + b / 8 * (1 - keep), rel_tol=1e-12)
+    f, factor = freqs(scaling="yarn", factor=4.0, original_context=4096)
+    assert math.isclose(factor, 0.1 * math.log(4) + 1)
+    for i, (a, b) in enumerate(zip(f, plain)):
+        assert b / 4 * (1 - 1e-12) <= a <= b
+        if _turns(plain[max(i - 1, 0)], 4096) < 1:
+            assert math.isclose(4 * a, b, rel_tol=1e-12)
+        if _turns(plain[min(i + 1, 31)], 4096) > 32:
+            assert math.isclose(a, b, rel_tol=1e-12)
+    f, factor = freqs(scaling="pairs", pair_factors=[1.0 + i for i in range(32)],
+                      attention_factor=1.25)
+    assert factor == 1.25
+    assert all(math.isclose(a * (1 + i), b, rel_tol=1e-14)
+               for i, (a, b) in enumerate(zip(f, plain)))
+
+
+def test_tensors_on_the_host_are_refused():
+    from korith_vllm_ext.kernels import (Rotary, int4_page_pool, read_kv_cache, rotary_embedding,
+                                         write_kv_cache)
+
+    x = torch.zeros(1, 2, 64)
+    i = torch.zeros(1, dtype=torch.int64)
+    cache = torch.zeros(2, 1, 16, 2, 64)
+    with pytest.raises(RuntimeError, match="GPU"):
+        rotary_embedding(x, x, i, Rotary(torch.ones(32, dtype=torch.float64)))
+    with pytest.raises(RuntimeError, match="GPU"):
+        write_kv_cache(x, x, cache, slot_mapping=i)
+    with pytest.raises(RuntimeError, match="GPU"):
+        read_kv_cache(cache, slot_mapping=i)
+    with pytest.raises(RuntimeError, match="GPU"):
+        read_kv_cache(int4_page_pool(1, 2, 64, device="cpu"), slot_mapping=i)
