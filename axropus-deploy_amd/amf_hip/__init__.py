@@ -157,6 +157,19 @@ SIGNATURES = {
          _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_ptr, _c_ptr, _c_ptr,
          _c_i64, _c_ptr, _c_ptr],
     ),
+    "amf_paged_attn_rows_workspace_bytes": (_c_i64, [_c_i32, _c_i32, _c_i32]),
+    "amf_paged_attn_rows": (
+        _c_i32,
+        [_c_ptr, _c_i32, _c_i64, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_ptr, _c_ptr, _c_i32, _c_i64,
+         _c_i64, _c_i64, _c_i64, _c_ptr, _c_i64, _c_i32, _c_ptr, _c_i32, _c_i32, _c_i32, _c_i32,
+         _c_i32, _c_f32, _c_f32, _c_f32, _c_ptr, _c_i64, _c_ptr, _c_ptr],
+    ),
+    "amf_int4_paged_attn_rows": (
+        _c_i32,
+        [_c_ptr, _c_i32, _c_i64, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr,
+         _c_i64, _c_ptr, _c_i64, _c_i32, _c_ptr, _c_i32, _c_i32, _c_i32, _c_i32, _c_f32, _c_ptr,
+         _c_i64, _c_ptr, _c_ptr],
+    ),
     "amf_rotary_embedding": (
         _c_i32,
         [_c_ptr, _c_i64, _c_i64, _c_ptr, _c_i64, _c_i64, _c_i32, _c_ptr, _c_i64, _c_i64, _c_ptr,

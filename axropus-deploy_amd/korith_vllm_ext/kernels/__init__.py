@@ -21,6 +21,7 @@ from .paged import (
     paged_decode_attention,
     select_pages,
 )
+from .rows import paged_attention
 from .step import (
     Rotary,
     int4_page_pool,
@@ -43,6 +44,7 @@ __all__ = [
     "get_current_sm_version",
     "hip_decode_attention",
     "page_key_bounds",
+    "paged_attention",
     "paged_decode_attention",
     "paged_int4_decode",
     "read_kv_cache",

@@ -409,7 +409,8 @@ def hip_decode_attention(q: torch.Tensor, k: Any, v: Any = None, scale: Optional
                          pages: Optional[torch.Tensor] = None,
                          page_counts: Optional[torch.Tensor] = None, k_scale: float = 1.0,
                          v_scale: float = 1.0,
-                         err_flag: Optional[torch.Tensor] = None) -> torch.Tensor:
+                         err_flag: Optional[torch.Tensor] = None,
+                         query_start: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The gfx950 decode kernel: positional arguments as the reference's
     (q, k, v, scale=None, mask=None); with block_tables/context_lens keywords,
     a paged GQA kernel runs over k, an INT4 page pool (v unused) or a tensor:
@@ -417,7 +418,21 @@ def hip_decode_attention(q: torch.Tensor, k: Any, v: Any = None, scale: Optional
     which takes pages, page_counts, k_scale, v_scale and err_flag).
     block_tables and context_lens may be lists, of other integer types or on
     the host with either, at the cost of a copy; int32 tensors on the device
-    are taken as they are, tables with rows apart too."""
+    are taken as they are, tables with rows apart too.  query_start (int32
+    [seqs + 1] on the device) makes it the attention of several rows per sequence
+    (paged_attention) over either, q then [rows, heads, head_dim]."""
+    if query_start is not None:
+        if block_tables is None or context_lens is None:
+            raise ValueError("query_start needs block_tables and context_lens")
+        if mask is not None or pages is not None or page_counts is not None or algo != "auto":
+            raise ValueError("query_start takes no mask, page lists or algo")
+        if out_dtype is not None and out_dtype != q.dtype:
+            raise ValueError(f"attention of several rows gives q's type, not {out_dtype}")
+        from .rows import paged_attention  # it imports what imports this module
+
+        return paged_attention(q, k, v, query_start=query_start, block_tables=block_tables,
+                               context_lens=context_lens, scale=scale, k_scale=k_scale,
+                               v_scale=v_scale, out=out, workspace=workspace, err_flag=err_flag)
     if block_tables is not None or context_lens is not None:
         if block_tables is None or context_lens is None:
             raise ValueError("paged decode needs both block_tables and context_lens")

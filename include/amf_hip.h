@@ -566,6 +566,54 @@ int amf_int4_kv_read(const void* k_codes, const void* k_params, const void* v_co
                      int64_t v_row_stride, int64_t v_head_stride, int32_t dtype, int64_t n_rows,
                      int32_t num_kv_heads, int32_t head_dim, int32_t* err_flag, void* stream);
 
+/* ---- attention of several new rows per sequence ------------------------------
+ * Rows query_start[s] .. query_start[s + 1] - 1 of q are the last tokens of
+ * sequence s, in order (device int32 [num_seqs + 1], as amf_build_slot_maps
+ * writes it; context_lens counts them): row j of n, at position
+ * p = context_lens[s] - n + j, gets
+ *   out[row][h] = v_scale * softmax_{t <= p}(q[row][h] . K[t] * softmax_scale * k_scale) V
+ * in fp32 but for the weights (bf16 beside a bf16 V, else fp16 scaled by the row's
+ * largest), rounded to out, of q's type, contiguous [n_rows][num_q_heads][head_dim].
+ * Rows that belong to no sequence are left as they are.  q's rows, heads, the
+ * cache's strides, block tables, page ids and the end of a table as in
+ * amf_paged_decode_attn; a row without tokens gives zeros, scores that are all
+ * -inf, or hold a NaN or +inf, give NaN.  A sequence whose rows lie outside
+ * [0, n_rows) or end before they begin has none (AMF_ERRFLAG_CONTEXT).
+ * kv_dtype: q_dtype, or AMF_DTYPE_E4M3 with q bf16 or fp16.  head_dim at most 256;
+ * n_rows * num_q_heads at most 2^26, table_pages * block_size at most 2^30.  Matrix
+ * tiles take 16-bit q with head_dim 64, 128 or 256 and at most 128 query heads a KV
+ * head, where q, k, v, out and every stride are 16-byte aligned; all other calls a
+ * slower kernel.  Rows of one sequence must not be listed under another (their
+ * results are either's then).  softmax_scale <= 0 selects 1/sqrt(head_dim).
+ * workspace: amf_paged_attn_rows_workspace_bytes() bytes, 16-byte aligned; calls
+ * sharing one must be ordered on one stream.  No counterpart in the reference. */
+int64_t amf_paged_attn_rows_workspace_bytes(int32_t num_q_heads, int32_t num_kv_heads,
+                                            int32_t head_dim);
+
+int amf_paged_attn_rows(const void* q, int32_t q_dtype, int64_t q_row_stride,
+                        int64_t q_head_stride, void* out, int64_t n_rows,
+                        const int32_t* query_start, const void* k, const void* v,
+                        int32_t kv_dtype, int64_t page_stride, int64_t token_stride,
+                        int64_t head_stride, int64_t pool_pages, const int32_t* block_tables,
+                        int64_t bt_stride, int32_t table_pages, const int32_t* context_lens,
+                        int32_t num_seqs, int32_t num_q_heads, int32_t num_kv_heads,
+                        int32_t head_dim, int32_t block_size, float softmax_scale, float k_scale,
+                        float v_scale, void* workspace, int64_t workspace_bytes,
+                        int32_t* err_flag, void* stream);
+
+/* The same over an AMF_FMT_INT4_ASYM_G32 pool (planes 16-byte aligned; q bf16 or
+ * fp16, head_dim a multiple of 32), over the values that amf_int4_kv_read gives in
+ * q's type. */
+int amf_int4_paged_attn_rows(const void* q, int32_t q_dtype, int64_t q_row_stride,
+                             int64_t q_head_stride, void* out, int64_t n_rows,
+                             const int32_t* query_start, const void* k_codes,
+                             const void* k_params, const void* v_codes, const void* v_params,
+                             int64_t pool_pages, const int32_t* block_tables, int64_t bt_stride,
+                             int32_t table_pages, const int32_t* context_lens, int32_t num_seqs,
+                             int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                             float softmax_scale, void* workspace, int64_t workspace_bytes,
+                             int32_t* err_flag, void* stream);
+
 /* ---- prefix keys (host functions, no device work) ---------------------------
  * FNV-1a over bytes, continuing from hash h (pass AMF_FNV_OFFSET to start).
  * Replaces _fnv1a_bytes (amf_kv_manager.py:69-72; C++ hash_bytes of

@@ -34,6 +34,15 @@ CALLS = {
     "amf_kv_read": CACHE | OUT | END,
     "amf_int4_kv_read": POOL | OUT | END,
 }
+ROWS = dict(q=FAKE, q_dtype=2, q_row=512, q_head=64, out=FAKE, rows=4, start=FAKE)
+TABLES = dict(bt=FAKE, bt_stride=4, table=4, cl=FAKE, seqs=2, hq=8, hkv=2, dim=64)
+WORK = dict(ws=FAKE, wsb=1 << 30, err=None, stream=None)
+ATTEND = {
+    "amf_paged_attn_rows": ROWS | dict(k=FAKE, v=FAKE, kv_dtype=2, page=2048, token=128, head=64,
+                                       pool=8) | TABLES | dict(block=16, scale=0.0, ks=1.0, vs=1.0)
+    | WORK,
+    "amf_int4_paged_attn_rows": ROWS | POOL | TABLES | dict(scale=0.0) | WORK,
+}
 INV, UNS = amf_hip.ERR_INVALID_ARG, amf_hip.ERR_UNSUPPORTED
 ALL = [(n, c, w, d) for n in CALLS for c, w, d in (
     (INV, "dtype", dict(dtype=3)), (INV, "n_rows", dict(rows=-1)), (UNS, "n_rows",
@@ -128,3 +137,44 @@ def test_tensors_on_the_host_are_refused():
         read_kv_cache(cache, slot_mapping=i)
     with pytest.raises(RuntimeError, match="GPU"):
         read_kv_cache(int4_page_pool(1, 2, 64, device="cpu"), slot_mapping=i)
+
+
+BOTH = [(n, c, w, d) for n in ATTEND for c, w, d in (
+    (INV, "heads", dict(hq=7)), (INV, "num_seqs", dict(seqs=-1)), (INV, "n_rows", dict(rows=-1)),
+    (INV, "bt_stride", dict(bt_stride=3)), (INV, "pool_pages", dict(pool=0)),
+    (UNS, "head_dim", dict(dim=288)), (UNS, "rows", dict(rows=1 << 24)),
+    (UNS, "block tables", dict(table=1 << 27, bt_stride=1 << 27)),
+    (UNS, "dtype", dict(q_dtype=3)), (INV, "null", dict(q=None)), (INV, "null", dict(start=None)),
+    (INV, "null", dict(bt=None)), (INV, "aligned", dict(out=FAKE + 1)),
+    (amf_hip.ERR_WORKSPACE, "workspace", dict(ws=None)),
+    (amf_hip.ERR_WORKSPACE, "workspace", dict(wsb=1000)),
+    (amf_hip.ERR_WORKSPACE, "workspace", dict(ws=FAKE + 8)))]
+
+
+@pytest.mark.parametrize("name,code,word,change", BOTH + [
+    ("amf_paged_attn_rows", UNS, "type", dict(kv_dtype=0)),
+    ("amf_paged_attn_rows", UNS, "type", dict(q_dtype=1, kv_dtype=3)),
+    ("amf_paged_attn_rows", INV, "scales", dict(ks=0.0)),
+    ("amf_paged_attn_rows", INV, "block_size", dict(block=0)),
+    ("amf_paged_attn_rows", INV, "aligned", dict(v=FAKE + 1)),
+    ("amf_int4_paged_attn_rows", UNS, "multiple", dict(dim=80)),
+    ("amf_int4_paged_attn_rows", UNS, "dtype", dict(q_dtype=1)),
+    ("amf_int4_paged_attn_rows", INV, "null", dict(vp=None)),
+    ("amf_int4_paged_attn_rows", INV, "aligned", dict(kp=FAKE + 4)),
+])
+def test_attention_refused(name, code, word, change):
+    with pytest.raises(amf_hip.AmfHipError) as e:
+        amf_hip.call(name, *(ATTEND[name] | change).values())
+    assert e.value.code == code and word in e.value.message
+
+
+@pytest.mark.parametrize("name", list(ATTEND))
+def test_no_rows_to_attend(name):
+    amf_hip.call(name, *(ATTEND[name] | dict(rows=0)).values())
+    amf_hip.call(name, *(ATTEND[name] | dict(seqs=0)).values())
+
+
+def test_workspace_of_the_attention():
+    f = amf_hip.load().amf_paged_attn_rows_workspace_bytes
+    assert f(32, 8, 128) % 16 == 0 and f(64, 8, 256) > f(32, 8, 128) > f(32, 8, 64) > 0
+    assert f(32, 8, 80) == 16 and f(7, 2, 64) == f(8, 0, 64) == f(8, 8, 300) == 0
