@@ -89,6 +89,7 @@ struct RowsArgs {
   int32_t block_shift;  // log2(block_size), or -1
   int32_t group;        // query heads of a KV head
   int32_t tile_rows;    // query rows of a tile
+  bool by16;            // 16 tokens at a multiple of 16 lie in one page
   int32_t shares;       // of the grid
   float score_scale;    // softmax scale * k_scale * log2(e)
   float v_scale;
@@ -203,9 +204,19 @@ constexpr int tile_tokens(int D) { return D == 256 ? 32 : 64; }
 constexpr int k_stride(int D) { return 2 * D + 16; }
 constexpr int v_stride(int D) { return 2 * D + 64; }
 
+// Two fp32 values as a pair of type T in one conversion, round to nearest even.
 template <int T>
 __device__ __forceinline__ uint32_t pair16(float a, float b) {
-  return pack2<T == AMF_DTYPE_BF16>(a, b);
+  if constexpr (T == AMF_DTYPE_BF16)
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), bf16x2_t));
+  else
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), f16x2_t));
+}
+
+// Read by the scalar unit: nothing that a launch writes.
+typedef const __attribute__((address_space(4))) int32_t scalar_i32;
+__device__ __forceinline__ int32_t scalar_load(const int32_t* p, int i) {
+  return ((scalar_i32*)(uintptr_t)p)[i];
 }
 
 // Whether a pair of 16-bit values holds one that is not finite.
@@ -230,47 +241,79 @@ struct Mover {
 
   const RowsArgs& a;
   const int32_t* table;
-  const uint8_t* kb;
-  const uint8_t* vb;
+  int head;
   int end;  // tokens behind it are not read
   int32_t ids[CH];
   u32x4 kr[CH], vr[CH];
 
   __device__ __forceinline__ Mover(const RowsArgs& args) : a(args) {}
   __device__ __forceinline__ int row(int i) const { return threadIdx.x / CPR + i * STEP; }
-  __device__ __forceinline__ void start(int seq, int head, int e) {
+  // the wave's first row: its rows lie in one aligned group of 16
+  static_assert(64 / CPR <= 16, "a wave's rows lie in a page of 16 tokens or more");
+  __device__ __forceinline__ int wave_row(int i) const {
+    return __builtin_amdgcn_readfirstlane(row(i));
+  }
+  __device__ __forceinline__ bool good(int32_t id) const { return id >= 0 && id < a.pool_pages; }
+  __device__ __forceinline__ int page_of(int t) const {
+    return a.block_shift >= 0 ? t >> a.block_shift : (int)((uint32_t)t / (uint32_t)a.block_size);
+  }
+  __device__ __forceinline__ void start(int seq, int h, int e) {
     table = a.block_tables + seq * a.bt_stride;
-    kb = a.k + head * a.head_stride + (threadIdx.x % CPR) * 16;
-    vb = a.v + head * a.head_stride + (threadIdx.x % CPR) * 16;
+    head = h;
     end = e;
   }
-  __device__ __forceinline__ void pages(int64_t t0) {
+  // Page ids of a tile: of the wave's rows, or of each lane's.
+  __device__ __forceinline__ void pages(int t0) {
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
-      const uint32_t t = (uint32_t)(t0 + row(i));
       ids[i] = -1;
-      if (t < end) ids[i] = table[a.block_shift >= 0 ? t >> a.block_shift : t / a.block_size];
-    }
-  }
-  // bad: bits of the tile's tokens whose page is none
-  __device__ __forceinline__ void fetch(int t0) {
-#pragma unroll
-    for (int i = 0; i < CH; ++i) {
-      const uint32_t t = (uint32_t)(t0 + row(i));
-      kr[i] = vr[i] = u32x4{0, 0, 0, 0};
-      if (ids[i] >= 0 && ids[i] < a.pool_pages) {
-        const uint32_t at = a.block_shift >= 0 ? t & (a.block_size - 1) : t % a.block_size;
-        const int64_t off = ids[i] * a.page_stride + at * a.token_stride;
-        kr[i] = *reinterpret_cast<const u32x4*>(kb + off);
-        vr[i] = *reinterpret_cast<const u32x4*>(vb + off);
+      if (a.by16) {
+        const int t = t0 + wave_row(i);
+        if (t < end) ids[i] = scalar_load(table, page_of(t));
+      } else if (t0 + row(i) < end) {
+        ids[i] = table[page_of(t0 + row(i))];
       }
     }
   }
+  __device__ __forceinline__ void fetch(int t0) {
+    if (a.by16) {
+      bool all = t0 + BT <= end;
+#pragma unroll
+      for (int i = 0; i < CH; ++i) all = all && good(__builtin_amdgcn_readfirstlane(ids[i]));
+      if (all) {
+        // a uniform base and one offset a lane
+        const uint32_t lane = (threadIdx.x % 64) / CPR * (uint32_t)a.token_stride +
+                              threadIdx.x % CPR * 16;
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {
+          const int t = t0 + wave_row(i);
+          const int64_t off = __builtin_amdgcn_readfirstlane(ids[i]) * a.page_stride +
+                              (t - page_of(t) * a.block_size) * a.token_stride +
+                              head * a.head_stride;
+          kr[i] = *reinterpret_cast<const u32x4*>(a.k + off + lane);
+          vr[i] = *reinterpret_cast<const u32x4*>(a.v + off + lane);
+        }
+        return;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      const int t = t0 + row(i);
+      kr[i] = vr[i] = u32x4{0, 0, 0, 0};
+      if (t < end && good(ids[i])) {
+        const int64_t off = ids[i] * a.page_stride +
+                            (t - page_of(t) * a.block_size) * a.token_stride +
+                            head * a.head_stride + threadIdx.x % CPR * 16;
+        kr[i] = *reinterpret_cast<const u32x4*>(a.k + off);
+        vr[i] = *reinterpret_cast<const u32x4*>(a.v + off);
+      }
+    }
+  }
+  // bad: bits of the tile's tokens whose page is none
   __device__ __forceinline__ void note_pages(int t0, uint32_t* bad) const {
 #pragma unroll
     for (int i = 0; i < CH; ++i)
-      if (t0 + row(i) < end && (ids[i] < 0 || ids[i] >= a.pool_pages))
-        atomicOr(bad + row(i) / 32, 1u << (row(i) % 32));
+      if (!good(ids[i]) && t0 + row(i) < end) atomicOr(bad + row(i) / 32, 1u << (row(i) % 32));
   }
   // wild: bits of the tokens with a V element that is not finite, which is stored as 0
   template <bool CHECK>
@@ -319,7 +362,7 @@ struct Mover {
     if (found) atomicOr(wild + r / 32, 1u << (r % 32));
   }
   // Element d of token t's V row, from memory (pages are good where this is asked).
-  __device__ __forceinline__ float v_elem(int t, int head, int d) const {
+  __device__ __forceinline__ float v_elem(int t, int d) const {
     const int64_t off = table[t / a.block_size] * a.page_stride +
                         t % a.block_size * a.token_stride + head * a.head_stride;
     return kv_elem<KV>(a.v + off + d * EB);
@@ -365,22 +408,24 @@ struct Mover<QT, kInt4, D> {
     ks = 0;
     const int i = item();
     if (has_k() && good(k_id)) {
-      const int64_t line = ((int64_t)k_id * a.num_kv_heads + head) * 16 + k_row() % 16;
-      kr = *reinterpret_cast<const u32x4*>(a.k + line * (D / 2) + 16 * (i % G));
-      ks = a.kp[line * G + i % G];
+      // K items of a (page, head) block follow each other
+      const int64_t block = (int64_t)k_id * a.num_kv_heads + head;
+      const uint32_t at = i % (16 * G);
+      kr = *reinterpret_cast<const u32x4*>(a.k + block * 8 * D + 16 * at);
+      ks = a.kp[block * 16 * G + at];
     }
     if (has_v() && good(v_id)) {
       const int64_t block = (int64_t)v_id * a.num_kv_heads + head;
-      const int x = i % (D / 2);
+      const uint32_t x = i % (D / 2);
       vr = *reinterpret_cast<const u32x4*>(a.v + block * 8 * D + 16 * x);
-      const u32x4* p =
-          reinterpret_cast<const u32x4*>(a.vp + (block * G + x / 16) * 16 + x / 2 % 2 * 8);
-      vs[0] = p[0];
-      vs[1] = p[1];
+      const u32x4* p = reinterpret_cast<const u32x4*>(a.vp + block * 16 * G);
+      const uint32_t q = x / 16 * 4 + x / 2 % 2 * 2;
+      vs[0] = p[q];
+      vs[1] = p[q + 1];
     }
   }
   __device__ __forceinline__ void note_pages(int t0, uint32_t* bad) const {
-    if (has_k() && t0 + k_row() < end && !good(k_id))
+    if (!good(k_id) && has_k() && t0 + k_row() < end)
       atomicOr(bad + k_row() / 32, 1u << (k_row() % 32));
   }
   // The 8 nibbles of w as bytes' fp32 values, in order.
@@ -439,8 +484,8 @@ struct Mover<QT, kInt4, D> {
       }
     }
   }
-  __device__ __forceinline__ float v_elem(int t, int h, int d) const {
-    const int64_t block = (int64_t)table[t / 16] * a.num_kv_heads + h;
+  __device__ __forceinline__ float v_elem(int t, int d) const {
+    const int64_t block = (int64_t)table[t / 16] * a.num_kv_heads + head;
     const int at = t % 16;
     const uint8_t c = a.v[block * 8 * D + 64 * (d / 8) + 32 * (at / 8) + 4 * (d % 8) + at % 8 / 2];
     const uint32_t p = a.vp[(block * G + d / 32) * 16 + at];
@@ -461,11 +506,14 @@ __device__ __forceinline__ f32x16 mfma32(const u32x4& x, const u32x4& y, const f
                                                   __builtin_bit_cast(f16x8_t, y), c, 0, 0, 0);
 }
 
-// Weights in fp16 run to 2^14 instead of 1, so that those down to 2^-28 of the
+// The running maximum is raised, and sum and accumulators scaled, only when a score
+// exceeds it by 2^kSlack; weights run to 2^kSlack then, which fp32 sums hold as well.
+// Weights in fp16 run to 2^(7 + kSlack) instead, so that those down to 2^-21 of the
 // largest keep their 11 bits.
+constexpr float kSlack = 8.0f;
 template <int T>
 constexpr float weight_shift() {
-  return T == AMF_DTYPE_F16 ? 14.0f : 0.0f;
+  return T == AMF_DTYPE_F16 ? 7.0f : 0.0f;
 }
 
 template <int QT, int KV, int D>
@@ -475,7 +523,8 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void rows_kernel(RowsAr
   __shared__ __attribute__((aligned(16))) uint8_t k_lds[BT * KS];
   __shared__ __attribute__((aligned(16))) uint8_t v_lds[BT * VS];
   __shared__ uint32_t marks[2][4];  // of even and odd tiles: bad pages (2 words), wild V (2)
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lc = lane & 31, h = lane >> 5;
 
   Cut cut{};
@@ -572,8 +621,10 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void rows_kernel(RowsAr
           mv.fetch(t0 + BT);
         }
         __syncthreads();
-        const uint64_t bad = (uint64_t)marks[par][1] << 32 | marks[par][0];
-        const uint64_t wild = (uint64_t)marks[par][3] << 32 | marks[par][2];
+        auto mark = [&](int i) {
+          return (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane(marks[par][i]);
+        };
+        const uint64_t bad = mark(1) << 32 | mark(0), wild = mark(3) << 32 | mark(2);
         if (tid < 4) marks[par ^ 1][tid] = 0;
         bad_seen |= bad != 0;
         if (!wave_on || t0 > pos0 + wave_last) continue;  // nothing for this wave
@@ -592,14 +643,17 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void rows_kernel(RowsAr
         if (t0 + BT > t_hi || t0 + BT - 1 > pos0 + wave_first || bad) {
           const int left = last - t0 - 4 * h;
 #pragma unroll
-          for (int tb = 0; tb < BT / 32; ++tb)
+          for (int tb = 0; tb < BT / 32; ++tb) {
+            uint32_t gone = (uint32_t)(bad >> (32 * tb)) >> (4 * h);
+            asm volatile("" : "+v"(gone));  // no masks kept over the loop
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
               const int t = 32 * tb + 8 * (i >> 2) + (i & 3);
-              const bool hide = t > left || (bad >> (t + 4 * h) & 1);
+              const bool hide = t > left || (gone >> (t % 32) & 1);
               if (hide) s[tb][i] = -INFINITY;
               seen |= !hide;
             }
+          }
         } else {
           seen = true;
         }
@@ -609,18 +663,18 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void rows_kernel(RowsAr
 #pragma unroll
           for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[tb][i]);
         mx = fmaxf(mx, __shfl_xor(mx, 32)) * c2 - weight_shift<VT>();
-        const float m_new = fmaxf(m_run, mx);
         // a row with every score so far -inf keeps l = 0 and acc = 0
-        const float m_use = m_new == -INFINITY ? 0.0f : m_new;
-        if (__any(m_new > m_run)) {
-          const float alpha = __builtin_amdgcn_exp2f(m_run - m_use);
+        if (__any(mx > m_run + kSlack)) {
+          const float m_new = fmaxf(m_run, mx);
+          const float alpha = __builtin_amdgcn_exp2f(m_run - (m_new == -INFINITY ? 0.0f : m_new));
           l_run *= alpha;
 #pragma unroll
           for (int d = 0; d < D / 32; ++d)
 #pragma unroll
             for (int i = 0; i < 16; ++i) acc[d][i] *= alpha;
+          m_run = m_new;
         }
-        m_run = m_new;
+        const float m_use = m_run == -INFINITY ? 0.0f : m_run;
         if (wild) {
           // elements that are not finite, for the rows that see their token
           for (uint64_t w = wild; w; w &= w - 1) {
@@ -635,7 +689,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void rows_kernel(RowsAr
             for (int d = 0; d < D / 32; ++d)
 #pragma unroll
               for (int n = 0; n < 16; ++n) {
-                const float v = mv.v_elem(t0 + t, head, 32 * d + 8 * (n >> 2) + 4 * h + (n & 3));
+                const float v = mv.v_elem(t0 + t, 32 * d + 8 * (n >> 2) + 4 * h + (n & 3));
                 if (!(fabsf(v) < INFINITY)) acc[d][n] += p * v;
               }
           }
@@ -959,6 +1013,7 @@ void finish_args(RowsArgs* a, void* workspace, float softmax_scale, float k_scal
   a->tile_rows = std::max(1, kRows / a->group);
   const int b = a->block_size;
   a->block_shift = (b & (b - 1)) == 0 ? __builtin_ctz((unsigned)b) : -1;
+  a->by16 = b % 16 == 0 && a->token_stride >= 0 && a->token_stride < (1 << 27);
   const float scale =
       softmax_scale > 0.0f ? softmax_scale : 1.0f / __builtin_sqrtf((float)a->head_dim);
   a->score_scale = scale * k_scale * kLog2e;

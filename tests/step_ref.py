@@ -63,8 +63,9 @@ def rows_tolerance(q, k, want, mass, tokens, scale, weight, k_scale=1.0):
     (D + 4) 2^-24 of |q| |k|, and its weight by twice that (its own and the
     sum's), by half a step of the type that it is multiplied in, and by the 2^x and
     the sum over tokens (2^-21, 2 (tokens / 32 + 64) 2^-24); what a weight is off by
-    reaches the output by weight * |v|, which `mass` sums.  fp16 weights below
-    2^-28 of the largest lose bits: 2^-39 each.  Then the output's own rounding."""
+    reaches the output by weight * |v|, which `mass` sums.  fp16 weights are held
+    2^7 times as large or more, of the row's largest, so their smallest step, 2^-24,
+    rounds a weight off by at most 2^-25 / 2^7 of that: 2^-32 each.  Then the output's own rounding."""
     if not k.numel():
         return mass + torch.finfo(q.dtype).tiny  # no token: zeros
     # |q| |k|, by their largest elements where norms overflow
@@ -75,5 +76,5 @@ def rows_tolerance(q, k, want, mass, tokens, scale, weight, k_scale=1.0):
            + HALF_STEP[weight] + 2.0 ** -21 + 2 * (tokens / 32 + 64) * 2.0 ** -24)
     fi = torch.finfo(q.dtype)
     big = torch.nan_to_num(mass, 0, 0, 0).max() if mass.numel() else 0.0
-    return (mass * rel * (1 + HALF_STEP[q.dtype]) + tokens * 2.0 ** -39 * big
+    return (mass * rel * (1 + HALF_STEP[q.dtype]) + tokens * 2.0 ** -32 * big
             + want.abs() * HALF_STEP[q.dtype] * 1.01 + fi.tiny * fi.eps)
