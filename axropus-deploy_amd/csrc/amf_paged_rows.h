@@ -1,0 +1,545 @@
+// amf_paged_rows.h - what a workgroup of the attention of several rows reads of K and
+// V: its arguments, and tiles of a paged cache or an INT4 pool brought into LDS.
+#pragma once
+
+#include "amf_attn.h"
+#include "amf_int4_asym.h"
+#include "amf_paged.h"
+
+namespace amf {
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef s16x4 __attribute__((address_space(3))) lds_s16x4;
+typedef uint8_t __attribute__((address_space(3))) lds_u8;
+
+constexpr int kRowsWaves = 4;
+constexpr int kRowsThreads = 64 * kRowsWaves;
+constexpr int kInt4 = 16;  // beside the AMF_DTYPE_* of a cache
+
+// A tile that does not end in the share where it begins.
+struct Cut {
+  int32_t more;   // shares after it that hold pieces, 0: there is none
+  int32_t share;
+  int32_t row0;   // the tile's first row
+  int32_t cols;   // its columns
+  int32_t head;   // KV head
+  int32_t pad[3];
+};
+
+struct RowsArgs {
+  const uint8_t* q;
+  int64_t q_row, q_head;  // bytes
+  uint16_t* out;
+  int64_t n_rows;
+  const int32_t* query_start;
+  const uint8_t* k;  // or codes
+  const uint8_t* v;
+  const uint32_t* kp;  // INT4 params
+  const uint32_t* vp;
+  int64_t page_stride, token_stride, head_stride;  // bytes
+  int64_t pool_pages;
+  const int32_t* block_tables;
+  int64_t bt_stride;
+  int32_t table_pages;
+  const int32_t* context_lens;
+  int32_t num_seqs, num_q_heads, num_kv_heads, head_dim, block_size;
+  int32_t block_shift;  // by16: log2(block_size)
+  int32_t group;        // query heads of a KV head
+  int32_t tile_rows;    // query rows of a tile
+  bool by16;            // block_size is 16, 32, 64, .., and page and token strides are
+  uint32_t page_units, token_units;  // these many times 16 bytes, a plane below 2^32 of them
+  int32_t shares;       // of the grid
+  float score_scale;    // softmax scale * k_scale * log2(e)
+  float v_scale;
+  Cut* cuts;            // [workgroup]
+  float* part;          // [share][2][kRows][head_dim + kPartPad]
+  int32_t* err_flag;
+};
+
+// Tokens of a tile in LDS.
+constexpr int tile_tokens(int D) { return D == 256 ? 32 : 64; }
+
+// A row of D 16-bit values in LDS, its 16-byte chunks permuted so that reads meet each
+// bank once: chunk c of row r lies at place c ^ swizzle(r).  K is read as the same chunk
+// of 16 consecutive rows, V (by the transposing read) as 64 bytes of 4 consecutive rows.
+template <int D>
+__device__ __forceinline__ int k_swizzle(int r) {
+  return D == 64 ? r >> 1 & 7 : r & 15;
+}
+template <int D>
+__device__ __forceinline__ int v_swizzle(int r) {
+  return D == 64 ? (r >> 1 & 1) << 2 : (r & 3) << 2;
+}
+template <int D>
+__device__ __forceinline__ int k_place(int r, int c) {
+  return r * 2 * D + ((c ^ k_swizzle<D>(r)) << 4);
+}
+template <int D>
+__device__ __forceinline__ int v_place(int r, int c) {
+  return r * 2 * D + ((c ^ v_swizzle<D>(r)) << 4);
+}
+
+// Two fp32 values as a pair of type T in one conversion, round to nearest even.
+template <int T>
+__device__ __forceinline__ uint32_t pair16(float a, float b) {
+  if constexpr (T == AMF_DTYPE_BF16)
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), bf16x2_t));
+  else
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), f16x2_t));
+}
+
+// Read by the scalar unit: nothing that a launch writes.
+typedef const __attribute__((address_space(4))) int32_t scalar_i32;
+__device__ __forceinline__ int32_t scalar_load(const int32_t* p, int i) {
+  return ((scalar_i32*)(uintptr_t)p)[i];
+}
+
+// Sets values that are not finite to 0; whether there were any.
+template <int T, int N>
+__device__ __forceinline__ bool clean(uint32_t (&v)[N]) {
+  constexpr uint32_t m = T == AMF_DTYPE_BF16 ? 0x7F80u : 0x7C00u;
+  bool found = false;
+#pragma unroll
+  for (int w = 0; w < N; ++w) {
+    const bool lo = (v[w] & m) == m, hi = (v[w] >> 16 & m) == m;
+    v[w] &= (lo ? 0xFFFF0000u : ~0u) & (hi ? 0xFFFFu : ~0u);
+    found |= lo | hi;
+  }
+  return found;
+}
+
+// x, of which the compiler knows nothing: what seldom branches derive from it is not
+// computed ahead and kept in registers over the loop.
+__device__ __forceinline__ int opaque(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
+// Marks row r where `is`.
+__device__ __forceinline__ void mark_row(uint32_t* marks, int r, bool is) {
+  atomicOr(marks + r / 32, is ? 1u << (r % 32) : 0u);
+}
+
+// A mover brings tiles of one (block table, KV head) into LDS, K one tile ahead of V:
+// next(t) looks up, and of quantised caches loads, K of the tile at t and V of the one
+// before; store_k and store_v put what the last next() found into LDS, complete after
+// wait() and a barrier.  `end`: tokens that are read; behind them K rows hold anything
+// (they are hidden), V rows zeros.  Rows whose page is none are marked by store_k, and
+// are zeros in V.  CHECK: V values that are not finite become 0, *wild != 0 then.
+//
+// Branches in next() and the stores are the same for all lanes of a wave, or select.
+
+// What movers of caches (EB bytes an element) share.  Wave w of the workgroup takes rows
+// RPW w .. of a tile, which lie in one aligned group of 16: with pages of 16, 32, 64 ..
+// tokens (by16) it looks up one page a tile, on the scalar unit.  (With every wave's
+// rows spread over the tile's pages each looked up them all: 420 scalar instructions
+// a tile, which the CU's one scalar unit takes longer for than the matrix cores for the
+// products.)  A lane takes 16 bytes of a row, CH rows RPI apart.
+template <int EB, int D>
+struct CacheMover {
+  static constexpr int BT = tile_tokens(D);
+  static constexpr int CPR = D * EB / 16;          // 16-byte chunks of a row
+  static constexpr int RPI = 64 / CPR;             // rows of a load instruction
+  static constexpr int RPW = BT / kRowsWaves;      // rows of a wave
+  static constexpr int CH = RPW / RPI;
+  static_assert(CH >= 1 && RPW <= 16 && 64 % CPR == 0, "a wave's rows are whole loads");
+
+  const RowsArgs& a;
+  const int32_t* table;
+  int end;
+  const uint8_t *kb, *vb;  // the KV head's
+  int32_t k_id, v_id;      // by16: pages of the wave's rows; -1 behind `end`
+  uint32_t k_off, v_off;   // and their place, in units of 16 bytes
+
+  __device__ __forceinline__ CacheMover(const RowsArgs& args) : a(args) {}
+  static __device__ __forceinline__ int wave_row() {
+    return __builtin_amdgcn_readfirstlane(threadIdx.x / 64) * RPW;
+  }
+  static __device__ __forceinline__ int lane_row(int i, int tid = threadIdx.x) {
+    return tid % 64 / CPR + i * RPI;
+  }
+  static __device__ __forceinline__ int row(int i, int tid = threadIdx.x) {
+    return tid / 64 * RPW + lane_row(i, tid);
+  }
+  __device__ __forceinline__ bool good(int32_t id) const { return id >= 0 && id < a.pool_pages; }
+  // Byte offset of token t's row in page id, of any block size.
+  __device__ __forceinline__ int page_of(int t) const {
+    return (int)((uint32_t)t / (uint32_t)a.block_size);
+  }
+  __device__ __forceinline__ int64_t place(int32_t id, int t) const {
+    return id * a.page_stride + (t - page_of(t) * a.block_size) * a.token_stride;
+  }
+  __device__ __forceinline__ void start(int seq, int head, int e) {
+    table = a.block_tables + seq * a.bt_stride;
+    end = e;
+    kb = a.k + head * a.head_stride;
+    vb = a.v + head * a.head_stride;
+    k_id = -1;
+    k_off = 0;
+  }
+  __device__ __forceinline__ void look_up(int t0) {
+    v_id = k_id;
+    v_off = k_off;
+    const int t = t0 + wave_row();
+    k_id = __builtin_amdgcn_readfirstlane(t < end ? scalar_load(table, t >> a.block_shift) : -1);
+    k_off = (uint32_t)k_id * a.page_units + (uint32_t)(t & (a.block_size - 1)) * a.token_units;
+  }
+  // The wave's rows behind `off`, and a lane's bytes of row i behind that.
+  static __device__ __forceinline__ const uint8_t* base(const uint8_t* plane, uint32_t off) {
+    return plane + ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane(off) << 4);
+  }
+  __device__ __forceinline__ uint32_t lane_off(int i, int chunk) const {
+    return (lane_row(i) * a.token_units + chunk) << 4;
+  }
+  // 16 bytes of token t's row from byte c on, zeros where it is not there; *bad: its page
+  // is none.
+  __device__ __forceinline__ u32x4 lane_row_of(const uint8_t* plane, int t, int c,
+                                               bool* bad) const {
+    const int32_t id = table[page_of(min(t, end - 1))];
+    const bool ok = t < end && good(id);
+    *bad = t < end && !good(id);
+    u32x4 x = *reinterpret_cast<const u32x4*>(plane + place(ok ? id : 0, ok ? t : 0) + c);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) x[w] = ok ? x[w] : 0u;
+    return x;
+  }
+  __device__ __forceinline__ bool there(int t) const { return good(table[page_of(t)]); }
+  // Element d of token t's row of K or V, from memory.
+  template <int KV>
+  __device__ __forceinline__ float elem(const uint8_t* plane, int t, int d) const {
+    return kv_elem<KV>(plane + place(table[page_of(t)], t) + d * EB);
+  }
+};
+
+// 16-bit rows go to LDS directly (no registers; a lane's 16 bytes land at its place, so
+// it loads the chunk that belongs there); V rows that need a check, and pages of other
+// sizes, pass through registers.
+template <int QT, int KV, int D>
+struct Mover : CacheMover<2, D> {
+  using Base = CacheMover<2, D>;
+  using Base::a, Base::row, Base::end, Base::kb, Base::vb, Base::k_id, Base::v_id;
+  static constexpr int VT = QT, BT = Base::BT;
+
+  __device__ __forceinline__ Mover(const RowsArgs& args) : Base(args) {}
+  __device__ __forceinline__ void next(int t0) {
+    if (a.by16) this->look_up(t0);
+  }
+  // 16 bytes of each lane, at base + off, to 16 lane bytes behind `lds`.  In assembly, as
+  // the compiler waits for all loads in flight before LDS reads that it cannot tell from
+  // what they write; wait() does that.
+  static __device__ __forceinline__ void load_lds(const uint8_t* base, uint32_t off,
+                                                  uint8_t* lds) {
+    const uint32_t at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_u8*)lds);
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+                 : : "v"(off), "s"(base), "s"(at) : "memory", "m0");
+  }
+  static __device__ __forceinline__ void wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+  __device__ __forceinline__ void store_k(int t0, uint8_t* lds, uint32_t* bad) const {
+    if (a.by16) {
+      const int32_t id = __builtin_amdgcn_readfirstlane(k_id);
+      const int wr = Base::wave_row(), c = threadIdx.x % Base::CPR;
+      if (this->good(id)) {
+        const uint8_t* b = Base::base(kb, this->k_off);
+#pragma unroll
+        for (int i = 0; i < Base::CH; ++i)
+          load_lds(b, this->lane_off(i, c ^ k_swizzle<D>(row(i))),
+                   lds + (wr + i * Base::RPI) * 2 * D);
+      } else if (t0 + wr < end) {
+#pragma unroll
+        for (int i = 0; i < Base::CH; ++i) mark_row(bad, row(i, opaque(threadIdx.x)), true);
+      }
+      return;
+    }
+    const int tid = opaque(threadIdx.x), c = tid % Base::CPR;
+#pragma unroll 1
+    for (int i = 0; i < Base::CH; ++i) {
+      const int r = row(i, tid);
+      bool none;
+      const u32x4 k = this->lane_row_of(kb, t0 + r, 16 * c, &none);
+      mark_row(bad, r, none);
+      *reinterpret_cast<u32x4*>(lds + k_place<D>(r, c)) = k;
+    }
+  }
+  template <bool CHECK>
+  __device__ __forceinline__ void store_v(int t0, uint8_t* lds, uint32_t* wild) const {
+    const int32_t id = __builtin_amdgcn_readfirstlane(v_id);
+    if (!CHECK && a.by16 && this->good(id) && t0 + BT <= end) {
+      const int wr = Base::wave_row(), c = threadIdx.x % Base::CPR;
+      const uint8_t* b = Base::base(vb, this->v_off);
+#pragma unroll
+      for (int i = 0; i < Base::CH; ++i)
+        load_lds(b, this->lane_off(i, c ^ v_swizzle<D>(row(i))),
+                 lds + (wr + i * Base::RPI) * 2 * D);
+      return;
+    }
+    const int tid = opaque(threadIdx.x), c = tid % Base::CPR;
+#pragma unroll 1
+    for (int i = 0; i < Base::CH; ++i) {
+      const int r = row(i, tid);
+      bool none;
+      const u32x4 x = this->lane_row_of(vb, t0 + r, 16 * c, &none);
+      uint32_t w[4] = {x[0], x[1], x[2], x[3]};
+      if constexpr (CHECK) {
+        const bool found = clean<VT>(w);
+        mark_row(wild, 0, found);
+      }
+      *reinterpret_cast<u32x4*>(lds + v_place<D>(r, c)) = u32x4{w[0], w[1], w[2], w[3]};
+    }
+  }
+  __device__ __forceinline__ float k_elem(int t, int d) const {
+    return this->template elem<KV>(kb, t, d);
+  }
+  __device__ __forceinline__ float v_elem(int t, int d) const {
+    return this->template elem<KV>(vb, t, d);
+  }
+};
+
+// FP8 rows: 16 values a chunk, converted on their way from registers to LDS.  V becomes
+// fp16, which holds its values exactly as bf16 does.
+template <int QT, int D>
+struct Mover<QT, AMF_DTYPE_E4M3, D> : CacheMover<1, D> {
+  using Base = CacheMover<1, D>;
+  using Base::a, Base::row, Base::end, Base::kb, Base::vb, Base::k_id, Base::v_id;
+  static constexpr int VT = AMF_DTYPE_F16, BT = Base::BT;
+  u32x4 kr[Base::CH], vr[Base::CH];
+  int bad;  // bits of the lane's K rows whose pages are none
+
+  __device__ __forceinline__ Mover(const RowsArgs& args) : Base(args) {}
+  static __device__ __forceinline__ void wait() {}
+  __device__ __forceinline__ void next(int t0) {
+    bad = 0;
+    if (a.by16) {
+      this->look_up(t0);
+      const int32_t ki = __builtin_amdgcn_readfirstlane(k_id);
+      const int32_t vi = __builtin_amdgcn_readfirstlane(v_id);
+      const int c = threadIdx.x % Base::CPR;
+#pragma unroll
+      for (int i = 0; i < Base::CH; ++i) kr[i] = vr[i] = u32x4{0, 0, 0, 0};
+      if (this->good(ki)) {
+        const uint8_t* b = Base::base(kb, this->k_off);
+#pragma unroll
+        for (int i = 0; i < Base::CH; ++i)
+          kr[i] = *reinterpret_cast<const u32x4*>(b + this->lane_off(i, c));
+      } else {
+#pragma unroll
+        for (int i = 0; i < Base::CH; ++i) bad |= (t0 + row(i) < end) << i;
+      }
+      if (this->good(vi)) {
+        const uint8_t* b = Base::base(vb, this->v_off);
+#pragma unroll
+        for (int i = 0; i < Base::CH; ++i)
+          vr[i] = *reinterpret_cast<const u32x4*>(b + this->lane_off(i, c));
+      }
+      return;
+    }
+    const int tid = opaque(threadIdx.x), c = tid % Base::CPR * 16;
+#pragma unroll
+    for (int i = 0; i < Base::CH; ++i) {
+      const int t = t0 + row(i, tid);
+      bool none;
+      kr[i] = this->lane_row_of(kb, t, c, &none);
+      bad |= none ? 1 << i : 0;
+      vr[i] = this->lane_row_of(vb, max(t - BT, 0), c, &none);
+    }
+  }
+  template <int T, bool HIGH>
+  static __device__ __forceinline__ uint32_t pair(uint32_t w) {
+    if constexpr (T == AMF_DTYPE_BF16)
+      return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, HIGH));
+    else
+      return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, HIGH));
+  }
+  __device__ __forceinline__ void store_k(int, uint8_t* lds, uint32_t* marks) const {
+    const int c = threadIdx.x % Base::CPR * 2;
+    if (__any(bad)) {
+      const int tid = opaque(threadIdx.x);
+#pragma unroll
+      for (int i = 0; i < Base::CH; ++i) mark_row(marks, row(i, tid), bad >> i & 1);
+    }
+#pragma unroll
+    for (int i = 0; i < Base::CH; ++i)
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const uint32_t x = kr[i][2 * n], y = kr[i][2 * n + 1];
+        *reinterpret_cast<u32x4*>(lds + k_place<D>(row(i), c + n)) =
+            u32x4{pair<QT, false>(x), pair<QT, true>(x), pair<QT, false>(y), pair<QT, true>(y)};
+      }
+  }
+  template <bool CHECK>
+  __device__ __forceinline__ void store_v(int t0, uint8_t* lds, uint32_t* wild) const {
+    const int c = threadIdx.x % Base::CPR * 2;
+#pragma unroll
+    for (int i = 0; i < Base::CH; ++i)
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const uint32_t x = vr[i][2 * n], y = vr[i][2 * n + 1];
+        uint32_t w[4] = {pair<VT, false>(x), pair<VT, true>(x), pair<VT, false>(y),
+                         pair<VT, true>(y)};
+        if constexpr (CHECK) {
+          const bool in = t0 + row(i) < end;
+#pragma unroll
+          for (int m = 0; m < 4; ++m) w[m] = in ? w[m] : 0u;
+          const bool found = clean<VT>(w);
+          mark_row(wild, 0, found);
+        }
+        *reinterpret_cast<u32x4*>(lds + v_place<D>(row(i), c + n)) =
+            u32x4{w[0], w[1], w[2], w[3]};
+      }
+  }
+  __device__ __forceinline__ float k_elem(int t, int d) const {
+    return this->template elem<AMF_DTYPE_E4M3>(kb, t, d);
+  }
+  __device__ __forceinline__ float v_elem(int t, int d) const {
+    return this->template elem<AMF_DTYPE_E4M3>(vb, t, d);
+  }
+};
+
+// INT4 pages: K rows of 32 dims (16 bytes, one param) a thread, V in chunks of 4 dims
+// by 8 tokens (16 bytes, 8 params), dequantised on their way from registers to LDS.  At
+// head_dim 64 half the threads move K, half V.
+template <int QT, int D>
+struct Mover<QT, kInt4, D> {
+  static constexpr int BT = tile_tokens(D);
+  static constexpr int VT = QT, G = D / 32, N = BT * G;  // items of K, and of V
+  static constexpr bool HALF = N * 2 == kRowsThreads;
+  static_assert(HALF || N == kRowsThreads, "an item per thread");
+
+  const RowsArgs& a;
+  const int32_t* table;
+  int head;
+  int end;
+  u32x4 kr, vr, vs[2];
+  uint32_t ks;
+  int bad;  // the lane's K row has no page
+
+  __device__ __forceinline__ Mover(const RowsArgs& args) : a(args) {}
+  static __device__ __forceinline__ void wait() {}
+  // the same in a wave
+  static __device__ __forceinline__ bool has_k() {
+    return !HALF || __builtin_amdgcn_readfirstlane(threadIdx.x) < N;
+  }
+  static __device__ __forceinline__ bool has_v() {
+    return !HALF || __builtin_amdgcn_readfirstlane(threadIdx.x) >= N;
+  }
+  static __device__ __forceinline__ int item() { return threadIdx.x % N; }
+  static __device__ __forceinline__ int k_row() { return item() / G; }
+  static __device__ __forceinline__ int v_page() { return item() / (D / 2); }
+  __device__ __forceinline__ bool good(int32_t id) const { return id >= 0 && id < a.pool_pages; }
+  __device__ __forceinline__ void start(int seq, int h, int e) {
+    table = a.block_tables + seq * a.bt_stride;
+    head = h;
+    end = e;
+  }
+  // The page of the lane's items, those of the wave's first at t: one page a wave, or (HALF)
+  // one for each half of it.  -1 outside the context.
+  __device__ __forceinline__ int32_t page(int t) const {
+    auto at = [&](int x) { return x >= 0 && x < end ? scalar_load(table, x / 16) : -1; };
+    if constexpr (!HALF) return __builtin_amdgcn_readfirstlane(at(t));
+    return threadIdx.x & 32 ? at(t + 16) : at(t);
+  }
+  __device__ __forceinline__ void next(int t0) {
+    kr = vr = vs[0] = vs[1] = u32x4{0, 0, 0, 0};
+    ks = 0;
+    bad = 0;
+    const uint32_t i = item();
+    if (has_k()) {
+      const int32_t id = page(t0 + __builtin_amdgcn_readfirstlane(k_row()) / 16 * 16);
+      const bool ok = good(id);
+      bad = !ok && t0 + k_row() < end;
+      if (HALF || ok) {
+        // K items of a (page, head) block follow each other; where it is none, page 0
+        const int64_t block = (int64_t)(ok ? id : 0) * a.num_kv_heads + head;
+        const uint32_t at = i % (16 * G);
+        kr = *reinterpret_cast<const u32x4*>(a.k + block * 8 * D + 16 * at);
+        ks = a.kp[block * 16 * G + at];
+      }
+    }
+    if (has_v()) {
+      const int32_t id = page(t0 - BT + 16 * __builtin_amdgcn_readfirstlane(v_page()));
+      const bool ok = good(id);
+      if (HALF || ok) {
+        const int64_t block = (int64_t)(ok ? id : 0) * a.num_kv_heads + head;
+        const uint32_t x = i % (D / 2), q = x / 16 * 4 + x / 2 % 2 * 2;
+        vr = *reinterpret_cast<const u32x4*>(a.v + block * 8 * D + 16 * x);
+        const u32x4* p = reinterpret_cast<const u32x4*>(a.vp + block * 16 * G);
+        vs[0] = p[q];
+        vs[1] = p[q + 1];
+        if constexpr (HALF)
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {  // scale and zero of a page that is none: zeros
+            vs[0][w] = ok ? vs[0][w] : 0;
+            vs[1][w] = ok ? vs[1][w] : 0;
+          }
+      }
+    }
+  }
+  // The 8 nibbles of w as fp32 values, in order.
+  static __device__ __forceinline__ void nibbles(uint32_t w, float* x) {
+    uint32_t ev = w & 0x0F0F0F0Fu, od = (w >> 4) & 0x0F0F0F0Fu;
+    asm("" : "+v"(ev));
+    asm("" : "+v"(od));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[2 * i] = (float)((ev >> (8 * i)) & 0xFFu);
+      x[2 * i + 1] = (float)((od >> (8 * i)) & 0xFFu);
+    }
+  }
+  // u * s is exact (4 bits by 11), so the fma rounds as the codec's multiply and add.
+  __device__ __forceinline__ void store_k(int, uint8_t* lds, uint32_t* marks) const {
+    if (!has_k()) return;
+    if (__any(bad)) mark_row(marks, k_row(), bad);
+    const float s = param_scale(ks), z = param_zero(ks);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      float x[8];
+      nibbles(kr[w], x);
+      u32x4 y;
+#pragma unroll
+      for (int n = 0; n < 4; ++n)
+        y[n] = pair16<QT>(__builtin_fmaf(x[2 * n], s, z), __builtin_fmaf(x[2 * n + 1], s, z));
+      *reinterpret_cast<u32x4*>(lds + k_place<D>(k_row(), 4 * (item() % G) + w)) = y;
+    }
+  }
+  template <bool CHECK>
+  __device__ __forceinline__ void store_v(int t0, uint8_t* lds, uint32_t* wild) const {
+    if (!has_v()) return;
+    const int c = item() % (D / 2);
+    const int r0 = 16 * v_page() + c / 2 % 2 * 8;
+    float x[4][8];
+#pragma unroll
+    for (int d = 0; d < 4; ++d) nibbles(vr[d], x[d]);
+#pragma unroll
+    for (int t = 0; t < 8; ++t) {
+      const uint32_t p = vs[t / 4][t % 4];
+      const float s = param_scale(p), z = param_zero(p);
+      uint32_t y[2] = {pair16<QT>(__builtin_fmaf(x[0][t], s, z), __builtin_fmaf(x[1][t], s, z)),
+                       pair16<QT>(__builtin_fmaf(x[2][t], s, z), __builtin_fmaf(x[3][t], s, z))};
+      if constexpr (CHECK) {
+        const bool in = t0 + r0 + t < end;
+        y[0] = in ? y[0] : 0u;
+        y[1] = in ? y[1] : 0u;
+        const bool found = clean<VT>(y);
+        mark_row(wild, 0, found);
+      }
+      *reinterpret_cast<u32x2*>(lds + v_place<D>(r0 + t, c / 4) + c % 2 * 8) = u32x2{y[0], y[1]};
+    }
+  }
+  __device__ __forceinline__ bool there(int t) const { return good(table[t / 16]); }
+  __device__ __forceinline__ float k_elem(int t, int d) const {
+    const int64_t line = ((int64_t)table[t / 16] * a.num_kv_heads + head) * 16 + t % 16;
+    const uint8_t c = a.k[line * (D / 2) + d / 2];
+    const uint32_t p = a.kp[line * G + d / 32];
+    return round_to<QT>(
+        __builtin_fmaf((float)(d % 2 ? c >> 4 : c & 15), param_scale(p), param_zero(p)));
+  }
+  __device__ __forceinline__ float v_elem(int t, int d) const {
+    const int64_t block = (int64_t)table[t / 16] * a.num_kv_heads + head;
+    const int at = t % 16;
+    const uint8_t c = a.v[block * 8 * D + 64 * (d / 8) + 32 * (at / 8) + 4 * (d % 8) + at % 8 / 2];
+    const uint32_t p = a.vp[(block * G + d / 32) * 16 + at];
+    return round_to<QT>(
+        __builtin_fmaf((float)(at % 2 ? c >> 4 : c & 15), param_scale(p), param_zero(p)));
+  }
+};
+
+}  // namespace amf

@@ -31,9 +31,7 @@
 // matrix time of the whole for bits that the result's type drops.
 #include <algorithm>
 
-#include "amf_attn.h"
-#include "amf_int4_asym.h"
-#include "amf_paged.h"
+#include "amf_paged_rows.h"
 
 // Held to a tolerance, as the other attention kernels: multiplies and adds may
 // fuse.
@@ -46,57 +44,15 @@ using namespace amf;
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef s16x4 __attribute__((address_space(3))) lds_s16x4;
 
-constexpr int kWaves = 4;
-constexpr int kThreads = 64 * kWaves;
+constexpr int kWaves = kRowsWaves;
+constexpr int kThreads = kRowsThreads;
 constexpr int kRows = 32 * kWaves;  // columns of a workgroup
 constexpr int kMaxDim = 256;
 constexpr int kMaxShares = 512;     // two workgroups a CU
 constexpr int kMinShare = 256;      // tokens
 constexpr int kTileCost = 64;       // tokens' worth of a tile's beginning and end, >= BT
 constexpr int kMaxContext = 1 << 30;
-constexpr int kInt4 = 16;           // beside the AMF_DTYPE_* of a cache
-
-// A tile that does not end in the share where it begins.
-struct Cut {
-  int32_t more;   // shares after it that hold pieces, 0: there is none
-  int32_t share;
-  int32_t row0;   // the tile's first row
-  int32_t cols;   // its columns
-  int32_t head;   // KV head
-  int32_t pad[3];
-};
-
-struct RowsArgs {
-  const uint8_t* q;
-  int64_t q_row, q_head;  // bytes
-  uint16_t* out;
-  int64_t n_rows;
-  const int32_t* query_start;
-  const uint8_t* k;  // or codes
-  const uint8_t* v;
-  const uint32_t* kp;  // INT4 params
-  const uint32_t* vp;
-  int64_t page_stride, token_stride, head_stride;  // bytes
-  int64_t pool_pages;
-  const int32_t* block_tables;
-  int64_t bt_stride;
-  int32_t table_pages;
-  const int32_t* context_lens;
-  int32_t num_seqs, num_q_heads, num_kv_heads, head_dim, block_size;
-  int32_t block_shift;  // log2(block_size), or -1
-  int32_t group;        // query heads of a KV head
-  int32_t tile_rows;    // query rows of a tile
-  bool by16;            // 16 tokens at a multiple of 16 lie in one page
-  int32_t shares;       // of the grid
-  float score_scale;    // softmax scale * k_scale * log2(e)
-  float v_scale;
-  Cut* cuts;            // [workgroup]
-  float* part;          // [share][2][kRows][head_dim + kPartPad]
-  int32_t* err_flag;
-};
 
 // ---- sequences and shares ------------------------------------------------------
 
@@ -194,306 +150,6 @@ __device__ __forceinline__ Share find_share(const RowsArgs& a) {
   return r;
 }
 
-// ---- K and V of a tile into LDS --------------------------------------------------
-
-constexpr int tile_tokens(int D) { return D == 256 ? 32 : 64; }
-// LDS row strides in bytes.  K rows are read as 16-byte vectors of 32 consecutive
-// rows: 16 more than the row moves each by 4 banks.  V rows are read by the
-// transposing read, 4 rows of 64 bytes per half wave: 64 more than the row puts them
-// 16 banks apart.
-constexpr int k_stride(int D) { return 2 * D + 16; }
-constexpr int v_stride(int D) { return 2 * D + 64; }
-
-// Two fp32 values as a pair of type T in one conversion, round to nearest even.
-template <int T>
-__device__ __forceinline__ uint32_t pair16(float a, float b) {
-  if constexpr (T == AMF_DTYPE_BF16)
-    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), bf16x2_t));
-  else
-    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), f16x2_t));
-}
-
-// Read by the scalar unit: nothing that a launch writes.
-typedef const __attribute__((address_space(4))) int32_t scalar_i32;
-__device__ __forceinline__ int32_t scalar_load(const int32_t* p, int i) {
-  return ((scalar_i32*)(uintptr_t)p)[i];
-}
-
-// Whether a pair of 16-bit values holds one that is not finite.
-template <int T>
-__device__ __forceinline__ bool not_finite(uint32_t w) {
-  constexpr uint32_t m = T == AMF_DTYPE_BF16 ? 0x7F80u : 0x7C00u;
-  return (w & m) == m || (w >> 16 & m) == m;
-}
-
-// What a thread moves of a tile of BT tokens of one (page table, KV head): raw values
-// in registers between fetch() and stage().
-template <int QT, int KV, int D>
-struct Mover {
-  static constexpr int BT = tile_tokens(D), KS = k_stride(D), VS = v_stride(D);
-  // types of K and V in LDS; FP8 values are exact in both
-  static constexpr int VT = KV == AMF_DTYPE_E4M3 ? AMF_DTYPE_F16 : QT;
-  static constexpr int EB = KV == AMF_DTYPE_E4M3 ? 1 : 2;    // bytes of a cache element
-  static constexpr int CPR = D * EB / 16;                    // 16-byte chunks of a row
-  static constexpr int CH = BT * CPR / kThreads;             // chunks of a thread
-  static constexpr int STEP = kThreads / CPR;                // rows between them
-  static_assert(CH >= 1 && kThreads % CPR == 0, "a tile is whole chunks per thread");
-
-  const RowsArgs& a;
-  const int32_t* table;
-  int head;
-  int end;  // tokens behind it are not read
-  int32_t ids[CH];
-  u32x4 kr[CH], vr[CH];
-
-  __device__ __forceinline__ Mover(const RowsArgs& args) : a(args) {}
-  __device__ __forceinline__ int row(int i) const { return threadIdx.x / CPR + i * STEP; }
-  // the wave's first row: its rows lie in one aligned group of 16
-  static_assert(64 / CPR <= 16, "a wave's rows lie in a page of 16 tokens or more");
-  __device__ __forceinline__ int wave_row(int i) const {
-    return __builtin_amdgcn_readfirstlane(row(i));
-  }
-  __device__ __forceinline__ bool good(int32_t id) const { return id >= 0 && id < a.pool_pages; }
-  __device__ __forceinline__ int page_of(int t) const {
-    return a.block_shift >= 0 ? t >> a.block_shift : (int)((uint32_t)t / (uint32_t)a.block_size);
-  }
-  __device__ __forceinline__ void start(int seq, int h, int e) {
-    table = a.block_tables + seq * a.bt_stride;
-    head = h;
-    end = e;
-  }
-  // Page ids of a tile: of the wave's rows, or of each lane's.
-  __device__ __forceinline__ void pages(int t0) {
-#pragma unroll
-    for (int i = 0; i < CH; ++i) {
-      ids[i] = -1;
-      if (a.by16) {
-        const int t = t0 + wave_row(i);
-        if (t < end) ids[i] = scalar_load(table, page_of(t));
-      } else if (t0 + row(i) < end) {
-        ids[i] = table[page_of(t0 + row(i))];
-      }
-    }
-  }
-  __device__ __forceinline__ void fetch(int t0) {
-    if (a.by16) {
-      bool all = t0 + BT <= end;
-#pragma unroll
-      for (int i = 0; i < CH; ++i) all = all && good(__builtin_amdgcn_readfirstlane(ids[i]));
-      if (all) {
-        // a uniform base and one offset a lane
-        const uint32_t lane = (threadIdx.x % 64) / CPR * (uint32_t)a.token_stride +
-                              threadIdx.x % CPR * 16;
-#pragma unroll
-        for (int i = 0; i < CH; ++i) {
-          const int t = t0 + wave_row(i);
-          const int64_t off = __builtin_amdgcn_readfirstlane(ids[i]) * a.page_stride +
-                              (t - page_of(t) * a.block_size) * a.token_stride +
-                              head * a.head_stride;
-          kr[i] = *reinterpret_cast<const u32x4*>(a.k + off + lane);
-          vr[i] = *reinterpret_cast<const u32x4*>(a.v + off + lane);
-        }
-        return;
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < CH; ++i) {
-      const int t = t0 + row(i);
-      kr[i] = vr[i] = u32x4{0, 0, 0, 0};
-      if (t < end && good(ids[i])) {
-        const int64_t off = ids[i] * a.page_stride +
-                            (t - page_of(t) * a.block_size) * a.token_stride +
-                            head * a.head_stride + threadIdx.x % CPR * 16;
-        kr[i] = *reinterpret_cast<const u32x4*>(a.k + off);
-        vr[i] = *reinterpret_cast<const u32x4*>(a.v + off);
-      }
-    }
-  }
-  // bad: bits of the tile's tokens whose page is none
-  __device__ __forceinline__ void note_pages(int t0, uint32_t* bad) const {
-#pragma unroll
-    for (int i = 0; i < CH; ++i)
-      if (!good(ids[i]) && t0 + row(i) < end) atomicOr(bad + row(i) / 32, 1u << (row(i) % 32));
-  }
-  // wild: bits of the tokens with a V element that is not finite, which is stored as 0
-  template <bool CHECK>
-  __device__ __forceinline__ void stage(uint8_t* k_lds, uint8_t* v_lds, uint32_t* wild) const {
-    const int c = threadIdx.x % CPR;
-#pragma unroll
-    for (int i = 0; i < CH; ++i) {
-      u32x4 k[2 / EB], v[2 / EB];
-      if constexpr (EB == 2) {
-        k[0] = kr[i];
-        v[0] = vr[i];
-      } else {
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          k[w / 2][2 * (w % 2)] = fp8_pair<QT, false>(kr[i][w]);
-          k[w / 2][2 * (w % 2) + 1] = fp8_pair<QT, true>(kr[i][w]);
-          v[w / 2][2 * (w % 2)] = fp8_pair<VT, false>(vr[i][w]);
-          v[w / 2][2 * (w % 2) + 1] = fp8_pair<VT, true>(vr[i][w]);
-        }
-      }
-      if constexpr (CHECK) clean(v, 2 / EB, row(i), wild);
-#pragma unroll
-      for (int n = 0; n < 2 / EB; ++n) {
-        *reinterpret_cast<u32x4*>(k_lds + row(i) * KS + (2 / EB) * 16 * c + 16 * n) = k[n];
-        *reinterpret_cast<u32x4*>(v_lds + row(i) * VS + (2 / EB) * 16 * c + 16 * n) = v[n];
-      }
-    }
-  }
-  template <int T, bool HIGH>
-  static __device__ __forceinline__ uint32_t fp8_pair(uint32_t w) {
-    if constexpr (T == AMF_DTYPE_BF16)
-      return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, HIGH));
-    else
-      return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, HIGH));
-  }
-  static __device__ __forceinline__ void clean(u32x4* v, int n, int r, uint32_t* wild) {
-    bool found = false;
-    for (int m = 0; m < n; ++m)
-#pragma unroll
-      for (int w = 0; w < 4; ++w)
-        if (not_finite<VT>(v[m][w])) {
-          found = true;
-          if (not_finite<VT>(v[m][w] & 0xFFFFu)) v[m][w] &= 0xFFFF0000u;
-          if (not_finite<VT>(v[m][w] & 0xFFFF0000u)) v[m][w] &= 0xFFFFu;
-        }
-    if (found) atomicOr(wild + r / 32, 1u << (r % 32));
-  }
-  // Element d of token t's V row, from memory (pages are good where this is asked).
-  __device__ __forceinline__ float v_elem(int t, int d) const {
-    const int64_t off = table[t / a.block_size] * a.page_stride +
-                        t % a.block_size * a.token_stride + head * a.head_stride;
-    return kv_elem<KV>(a.v + off + d * EB);
-  }
-};
-
-// INT4 pages: K rows of 32 dims (16 bytes, one param) a thread, V in chunks of 4 dims
-// by 8 tokens (16 bytes, 8 params).  At head_dim 64 half the threads move K, half V.
-template <int QT, int D>
-struct Mover<QT, kInt4, D> {
-  static constexpr int BT = tile_tokens(D), KS = k_stride(D), VS = v_stride(D);
-  static constexpr int VT = QT, G = D / 32, N = BT * G;  // items of K, and of V
-  static constexpr bool HALF = N * 2 == kThreads;
-  static_assert(HALF || N == kThreads, "an item per thread");
-
-  const RowsArgs& a;
-  const int32_t* table;
-  int end;
-  int32_t head;
-  int32_t k_id, v_id;
-  u32x4 kr, vr, vs[2];
-  uint32_t ks;
-
-  __device__ __forceinline__ Mover(const RowsArgs& args) : a(args) {}
-  __device__ __forceinline__ bool has_k() const { return !HALF || threadIdx.x < N; }
-  __device__ __forceinline__ bool has_v() const { return !HALF || threadIdx.x >= N; }
-  __device__ __forceinline__ int item() const { return threadIdx.x % N; }
-  __device__ __forceinline__ int k_row() const { return item() / G; }
-  __device__ __forceinline__ int v_page() const { return item() / (D / 2); }
-  __device__ __forceinline__ void start(int seq, int h, int e) {
-    table = a.block_tables + seq * a.bt_stride;
-    head = h;
-    end = e;
-  }
-  __device__ __forceinline__ void pages(int64_t t0) {
-    k_id = v_id = -1;
-    if (t0 + k_row() < end) k_id = table[(t0 + k_row()) / 16];
-    if (t0 + 16 * v_page() < end) v_id = table[t0 / 16 + v_page()];
-  }
-  __device__ __forceinline__ bool good(int32_t id) const { return id >= 0 && id < a.pool_pages; }
-  __device__ __forceinline__ void fetch(int t0) {
-    kr = vr = vs[0] = vs[1] = u32x4{0, 0, 0, 0};
-    ks = 0;
-    const int i = item();
-    if (has_k() && good(k_id)) {
-      // K items of a (page, head) block follow each other
-      const int64_t block = (int64_t)k_id * a.num_kv_heads + head;
-      const uint32_t at = i % (16 * G);
-      kr = *reinterpret_cast<const u32x4*>(a.k + block * 8 * D + 16 * at);
-      ks = a.kp[block * 16 * G + at];
-    }
-    if (has_v() && good(v_id)) {
-      const int64_t block = (int64_t)v_id * a.num_kv_heads + head;
-      const uint32_t x = i % (D / 2);
-      vr = *reinterpret_cast<const u32x4*>(a.v + block * 8 * D + 16 * x);
-      const u32x4* p = reinterpret_cast<const u32x4*>(a.vp + block * 16 * G);
-      const uint32_t q = x / 16 * 4 + x / 2 % 2 * 2;
-      vs[0] = p[q];
-      vs[1] = p[q + 1];
-    }
-  }
-  __device__ __forceinline__ void note_pages(int t0, uint32_t* bad) const {
-    if (!good(k_id) && has_k() && t0 + k_row() < end)
-      atomicOr(bad + k_row() / 32, 1u << (k_row() % 32));
-  }
-  // The 8 nibbles of w as bytes' fp32 values, in order.
-  static __device__ __forceinline__ void nibbles(uint32_t w, float* x) {
-    uint32_t ev = w & 0x0F0F0F0Fu, od = (w >> 4) & 0x0F0F0F0Fu;
-    asm("" : "+v"(ev));
-    asm("" : "+v"(od));
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[2 * i] = (float)((ev >> (8 * i)) & 0xFFu);
-      x[2 * i + 1] = (float)((od >> (8 * i)) & 0xFFu);
-    }
-  }
-  template <bool CHECK>
-  __device__ __forceinline__ void stage(uint8_t* k_lds, uint8_t* v_lds, uint32_t* wild) const {
-    const int i = item();
-    // u * s is exact (4 bits by 11), so the fma rounds as the codec's multiply and add
-    if (has_k()) {
-      const float s = param_scale(ks), z = param_zero(ks);
-      uint8_t* o = k_lds + k_row() * KS + 64 * (i % G);
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        float x[8];
-        nibbles(kr[w], x);
-        u32x4 y;
-#pragma unroll
-        for (int n = 0; n < 4; ++n)
-          y[n] = pair16<QT>(__builtin_fmaf(x[2 * n], s, z), __builtin_fmaf(x[2 * n + 1], s, z));
-        *reinterpret_cast<u32x4*>(o + 16 * w) = y;
-      }
-    }
-    if (has_v()) {
-      const int x0 = i % (D / 2);
-      const int r0 = 16 * v_page() + x0 / 2 % 2 * 8;
-      uint8_t* o = v_lds + r0 * VS + (x0 / 4 * 8 + x0 % 2 * 4) * 2;
-      float x[4][8];
-#pragma unroll
-      for (int d = 0; d < 4; ++d) nibbles(vr[d], x[d]);
-#pragma unroll
-      for (int t = 0; t < 8; ++t) {
-        const uint32_t p = vs[t / 4][t % 4];
-        const float s = param_scale(p), z = param_zero(p);
-        u32x2 y = {pair16<QT>(__builtin_fmaf(x[0][t], s, z), __builtin_fmaf(x[1][t], s, z)),
-                   pair16<QT>(__builtin_fmaf(x[2][t], s, z), __builtin_fmaf(x[3][t], s, z))};
-        if constexpr (CHECK) {
-          if (not_finite<VT>(y[0]) || not_finite<VT>(y[1])) {
-            atomicOr(wild + (r0 + t) / 32, 1u << ((r0 + t) % 32));
-#pragma unroll
-            for (int n = 0; n < 2; ++n) {
-              if (not_finite<VT>(y[n] & 0xFFFFu)) y[n] &= 0xFFFF0000u;
-              if (not_finite<VT>(y[n] & 0xFFFF0000u)) y[n] &= 0xFFFFu;
-            }
-          }
-        }
-        *reinterpret_cast<u32x2*>(o + t * VS) = y;
-      }
-    }
-  }
-  __device__ __forceinline__ float v_elem(int t, int d) const {
-    const int64_t block = (int64_t)table[t / 16] * a.num_kv_heads + head;
-    const int at = t % 16;
-    const uint8_t c = a.v[block * 8 * D + 64 * (d / 8) + 32 * (at / 8) + 4 * (d % 8) + at % 8 / 2];
-    const uint32_t p = a.vp[(block * G + d / 32) * 16 + at];
-    return round_to<QT>(
-        __builtin_fmaf((float)(at % 2 ? c >> 4 : c & 15), param_scale(p), param_zero(p)));
-  }
-};
-
 // ---- the matrix kernel -------------------------------------------------------------
 
 template <int T>
@@ -507,22 +163,34 @@ __device__ __forceinline__ f32x16 mfma32(const u32x4& x, const u32x4& y, const f
 }
 
 // The running maximum is raised, and sum and accumulators scaled, only when a score
-// exceeds it by 2^kSlack; weights run to 2^kSlack then, which fp32 sums hold as well.
-// Weights in fp16 run to 2^(7 + kSlack) instead, so that those down to 2^-21 of the
-// largest keep their 11 bits.
-constexpr float kSlack = 8.0f;
+// exceeds it by 2^slack; weights run to 2^slack then.  Weights in bf16 and the fp32 sums
+// keep their bits at any size.  Weights in fp16 are held 2^shift times as large as the
+// maximum makes them, so that those down to 2^-21 of the largest keep their 11 bits.
+template <int T>
+constexpr float slack() {
+  return T == AMF_DTYPE_F16 ? 8.0f : 30.0f;
+}
 template <int T>
 constexpr float weight_shift() {
   return T == AMF_DTYPE_F16 ? 7.0f : 0.0f;
 }
 
+// The larger of x here and in lane ^ 32.
+__device__ __forceinline__ float max_of_halves(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(f2u(x), f2u(x), false, false);
+  return fmaxf(u2f(r[0]), u2f(r[1]));
+}
+
 template <int QT, int KV, int D>
 __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void rows_kernel(RowsArgs a) {
   using Move = Mover<QT, KV, D>;
-  constexpr int BT = Move::BT, KS = Move::KS, VS = Move::VS, VT = Move::VT;
-  __shared__ __attribute__((aligned(16))) uint8_t k_lds[BT * KS];
-  __shared__ __attribute__((aligned(16))) uint8_t v_lds[BT * VS];
-  __shared__ uint32_t marks[2][4];  // of even and odd tiles: bad pages (2 words), wild V (2)
+  constexpr int BT = Move::BT, VT = Move::VT, RB = 2 * D;
+  // Two buffers each: while the values of a tile and the keys of the next are multiplied,
+  // the next values and the keys after are on their way, with one barrier a tile.
+  constexpr int TB = BT * RB;
+  __shared__ __attribute__((aligned(16))) uint8_t k_lds[2 * TB];
+  __shared__ __attribute__((aligned(16))) uint8_t v_lds[2 * TB];
+  __shared__ uint32_t marks[4][2];  // of K tiles, by turns; [3]: the piece's wild V
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lc = lane & 31, h = lane >> 5;
@@ -533,7 +201,6 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void rows_kernel(RowsAr
     if (tid == 0) a.cuts[blockIdx.x] = cut;
     return;
   }
-  if (tid < 8) marks[tid >> 2][tid & 3] = 0;
   int flags = 0;
   Move mv(a);
   int head = sh.head, seq = sh.seq;
@@ -551,16 +218,18 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void rows_kernel(RowsAr
   const int G = a.group;
   const float c2 = a.score_scale;
   bool bad_seen = false;
-  int par = 0;  // of the tiles, over all pieces
 
-  // addresses of this lane's LDS reads
-  const uint8_t* k_rd = k_lds + lc * KS + 16 * h;
-  const int l16 = lane & 15;
-  const uint8_t* v_rd = v_lds + (4 * h + (l16 >> 2)) * VS + 32 * ((lane >> 4) & 1) + 8 * (l16 & 3);
+  // This lane's LDS reads.  K: chunk 2 ks + h of row lc, whose swizzle the rows 32
+  // further share.  V: 8 bytes of row 4 h + l16 / 4, whose swizzle depends on l16 alone,
+  // for dims 32 d of each d.
+  const int k_at = lc * RB, k_x = (h ^ k_swizzle<D>(lc)) << 4;
+  const int l16 = lane & 15, v_row = 4 * h + (l16 >> 2);
+  const int v_at = v_row * RB + 8 * (l16 & 1);
+  const int v_x = (((lane >> 4 & 1) * 2 + (l16 >> 1 & 1)) ^ v_swizzle<D>(v_row)) << 4;
   // A operand of V^T: dims 32 d .. + 31, 16 tokens in the order of the scores
   auto read_v = [](const uint8_t* vp) {
     const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(vp));
-    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(vp + 8 * VS));
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(vp + 8 * RB));
     const u32x2 l2 = __builtin_bit_cast(u32x2, lo), h2 = __builtin_bit_cast(u32x2, hi);
     return u32x4{l2[0], l2[1], h2[0], h2[1]};
   };
@@ -592,65 +261,75 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void rows_kernel(RowsAr
 #pragma unroll
         for (int ks = 0; ks < D / 16; ++ks)
           qb[ks] = *reinterpret_cast<const u32x4*>(qp + 32 * ks);
+        // here, and not before the first product of every tile, where the wait would be for
+        // the next tile's loads as well
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) asm volatile("" : "+v"(qb[ks]));
       }
       // the row's last token
       const int last = min(pos0 + qi, t_hi - 1);
       float m_run = -INFINITY, l_run = 0.0f;  // l_run: this lane's tokens
       bool seen = false;                      // a token that the row attends to
-      f32x16 acc[D / 32];
+      f32x16 acc[D / 32], s[BT / 32];
 #pragma unroll
       for (int d = 0; d < D / 32; ++d)
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[d][i] = 0.0f;
 
+      const int n = (t_hi - t_lo + BT - 1) / BT;  // tiles
       mv.start(seq, head, t_hi);
-      mv.pages(t_lo);
-      mv.fetch(t_lo);
-      for (int t0 = t_lo; t0 < t_hi; t0 += BT, par ^= 1) {
-        __syncthreads();  // the previous tile has been read
-        mv.note_pages(t0, &marks[par][0]);
-        // tokens that some rows see and others do not: V has to be finite there, as 0 * inf
-        // is not 0
-        const bool diagonal = t0 + BT > pos0 + 1;
-        if (diagonal)
-          mv.template stage<true>(k_lds, v_lds, &marks[par][2]);
-        else
-          mv.template stage<false>(k_lds, v_lds, nullptr);
-        if (t0 + BT < t_hi) {
-          mv.pages(t0 + BT);
-          mv.fetch(t0 + BT);
+      __syncthreads();  // the last piece's marks have been read
+      marks[tid & 3][tid >> 2 & 1] = 0;
+      __syncthreads();
+      // Turn i stores K of tile i + 2 and V of tile i + 1, and multiplies V of tile i and K
+      // of tile i + 1.
+      int m0 = 0, m1 = 1, m2 = 2;  // marks of K tiles i + 2, i + 3, i + 1
+      auto move = [&](int i) __attribute__((always_inline)) {
+        const int t2 = t_lo + (i + 2) * BT, t1 = t2 - BT;
+        marks[m1][tid & 1] = 0;
+        if (i + 2 < n) mv.store_k(t2, k_lds + (i & 1) * TB, marks[m0]);
+        if (i >= -1 && i + 1 < n) {
+          // tokens that some rows see and others do not: V has to be finite there, as
+          // 0 * inf is not 0
+          if (t1 + BT > pos0 + 1)
+            mv.template store_v<true>(t1, v_lds + (i + 1 & 1) * TB, marks[3]);
+          else
+            mv.template store_v<false>(t1, v_lds + (i + 1 & 1) * TB, marks[3]);
         }
-        __syncthreads();
-        auto mark = [&](int i) {
-          return (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane(marks[par][i]);
-        };
-        const uint64_t bad = mark(1) << 32 | mark(0), wild = mark(3) << 32 | mark(2);
-        if (tid < 4) marks[par ^ 1][tid] = 0;
-        bad_seen |= bad != 0;
-        if (!wave_on || t0 > pos0 + wave_last) continue;  // nothing for this wave
-
-        f32x16 s[BT / 32];
+        if (i + 2 < n) mv.next(t2 + BT);
+        const int m = m2;
+        m2 = m0;
+        m0 = m1;
+        m1 = m;
+      };
+      // Scores of tile i, and their maximum.
+      auto score = [&](int i) __attribute__((always_inline)) {
+        const uint8_t* k_rd = k_lds + (i & 1) * TB + k_at;
+        const int t0 = t_lo + i * BT;
 #pragma unroll
         for (int tb = 0; tb < BT / 32; ++tb) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) s[tb][i] = 0.0f;
+          for (int e = 0; e < 16; ++e) s[tb][e] = 0.0f;
 #pragma unroll
           for (int ks = 0; ks < D / 16; ++ks)
-            s[tb] = mfma32<QT>(*reinterpret_cast<const u32x4*>(k_rd + 32 * tb * KS + 32 * ks),
-                               qb[ks], s[tb]);
+            s[tb] = mfma32<QT>(
+                *reinterpret_cast<const u32x4*>(k_rd + 32 * tb * RB + (k_x ^ (32 * ks))), qb[ks],
+                s[tb]);
         }
-        // token of score element i of block tb: t0 + 32 tb + 8 (i / 4) + 4 h + i % 4
-        if (t0 + BT > t_hi || t0 + BT - 1 > pos0 + wave_first || bad) {
+        // token of score element e of block tb: t0 + 32 tb + 8 (e / 4) + 4 h + e % 4
+        const uint32_t bad[2] = {(uint32_t)__builtin_amdgcn_readfirstlane(marks[m1][0]),
+                                 (uint32_t)__builtin_amdgcn_readfirstlane(marks[m1][1])};
+        if (t0 + BT > t_hi || t0 + BT - 1 > pos0 + wave_first || (bad[0] | bad[1])) {
           const int left = last - t0 - 4 * h;
+          bad_seen |= (bad[0] | bad[1]) != 0;
 #pragma unroll
           for (int tb = 0; tb < BT / 32; ++tb) {
-            uint32_t gone = (uint32_t)(bad >> (32 * tb)) >> (4 * h);
-            asm volatile("" : "+v"(gone));  // no masks kept over the loop
+            const uint32_t gone = opaque(bad[tb] >> (4 * h));  // no masks kept over the loop
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const int t = 32 * tb + 8 * (i >> 2) + (i & 3);
+            for (int e = 0; e < 16; ++e) {
+              const int t = 32 * tb + 8 * (e >> 2) + (e & 3);
               const bool hide = t > left || (gone >> (t % 32) & 1);
-              if (hide) s[tb][i] = -INFINITY;
+              s[tb][e] = hide ? -INFINITY : s[tb][e];
               seen |= !hide;
             }
           }
@@ -661,57 +340,66 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void rows_kernel(RowsAr
 #pragma unroll
         for (int tb = 0; tb < BT / 32; ++tb)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[tb][i]);
-        mx = fmaxf(mx, __shfl_xor(mx, 32)) * c2 - weight_shift<VT>();
-        // a row with every score so far -inf keeps l = 0 and acc = 0
-        if (__any(mx > m_run + kSlack)) {
+          for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[tb][e]);
+        return max_of_halves(mx) * c2 - weight_shift<VT>();
+      };
+      float mx = -INFINITY;
+      if (n > 0) {
+        mv.next(t_lo);
+        for (int i = -2; i < (wave_on ? 0 : n); ++i) {
+          move(i);
+          if (wave_on && i == -1) mx = score(0);
+          mv.wait();
+          __syncthreads();
+        }
+        // The inner loop changes the accumulators by products alone: with a branch in it that
+        // scales them they were held, and moved, twice.  A wave that meets scores too
+        // large for its maximum leaves it.
+        for (int i = 0; wave_on && i < n;) {
           const float m_new = fmaxf(m_run, mx);
-          const float alpha = __builtin_amdgcn_exp2f(m_run - (m_new == -INFINITY ? 0.0f : m_new));
+          // a row with every score so far -inf keeps l = 0 and acc = 0
+          const float m_use = m_new == -INFINITY ? 0.0f : m_new;
+          const float alpha = __builtin_amdgcn_exp2f(m_run - m_use);
           l_run *= alpha;
 #pragma unroll
           for (int d = 0; d < D / 32; ++d)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) acc[d][i] *= alpha;
+            for (int e = 0; e < 16; ++e) acc[d][e] *= alpha;
           m_run = m_new;
-        }
-        const float m_use = m_run == -INFINITY ? 0.0f : m_run;
-        if (wild) {
-          // elements that are not finite, for the rows that see their token
-          for (uint64_t w = wild; w; w &= w - 1) {
-            const int t = __ffsll((unsigned long long)w) - 1;
-            const int e0 = t / 32 * 16 + t % 32 / 8 * 4 + t % 4;  // its element, in half t / 4 % 2
-            float x = 0.0f;
+          bool over;
+          do {
+            move(i);
+            const uint8_t* v_rd = v_lds + (i & 1) * TB + v_at;
+            u32x4 pb[BT / 16];  // weights of 16 tokens each, 8 per lane
 #pragma unroll
-            for (int i = 0; i < BT / 2; ++i) x = i == e0 ? s[i / 16][i % 16] : x;
-            const float p = __builtin_amdgcn_exp2f(__shfl(x, lc + t / 4 % 2 * 32) * c2 - m_use);
-            if (t0 + t > last) continue;
+            for (int st = 0; st < BT / 16; ++st)
 #pragma unroll
-            for (int d = 0; d < D / 32; ++d)
-#pragma unroll
-              for (int n = 0; n < 16; ++n) {
-                const float v = mv.v_elem(t0 + t, 32 * d + 8 * (n >> 2) + 4 * h + (n & 3));
-                if (!(fabsf(v) < INFINITY)) acc[d][n] += p * v;
+              for (int e = 0; e < 4; ++e) {
+                const float p0 =
+                    __builtin_amdgcn_exp2f(s[st >> 1][8 * (st & 1) + 2 * e] * c2 - m_use);
+                const float p1 =
+                    __builtin_amdgcn_exp2f(s[st >> 1][8 * (st & 1) + 2 * e + 1] * c2 - m_use);
+                l_run += p0;
+                l_run += p1;
+                pb[st][e] = pair16<VT>(p0, p1);
               }
-          }
-        }
 #pragma unroll
-        for (int st = 0; st < BT / 16; ++st) {
-          u32x4 pb;  // weights of 16 tokens, 8 per lane
+            for (int st = 0; st < BT / 16; ++st)
 #pragma unroll
-          for (int n = 0; n < 4; ++n) {
-            const float p0 =
-                __builtin_amdgcn_exp2f(s[st >> 1][8 * (st & 1) + 2 * n] * c2 - m_use);
-            const float p1 =
-                __builtin_amdgcn_exp2f(s[st >> 1][8 * (st & 1) + 2 * n + 1] * c2 - m_use);
-            l_run += p0;
-            l_run += p1;
-            pb[n] = pair16<VT>(p0, p1);
-          }
-#pragma unroll
-          for (int d = 0; d < D / 32; ++d)
-            acc[d] = mfma32<VT>(read_v(v_rd + 16 * st * VS + 64 * d), pb, acc[d]);
+              for (int d = 0; d < D / 32; ++d)
+                acc[d] = mfma32<VT>(read_v(v_rd + 16 * st * RB + (v_x ^ (64 * d))), pb[st], acc[d]);
+            ++i;
+            over = false;
+            if (i < n) {
+              mx = score(i);
+              over = __any(mx > m_run + slack<VT>());
+            }
+            mv.wait();
+            __syncthreads();
+          } while (i < n && !over);
         }
       }
+      const bool wild_seen = n > 0 && marks[3][0] != 0;
 
       float l = l_run + __shfl_xor(l_run, 32);
       seen |= __shfl_xor((int)seen, 32) != 0;
@@ -747,6 +435,35 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void rows_kernel(RowsAr
           if (h == 0) {
             p[D] = m_run;
             p[D + 1] = seen && l == 0.0f ? -1.0f : l;  // -1: tokens, all of them -inf
+          }
+        }
+        if (wild_seen) {
+          // V elements that are not finite were multiplied as 0: what they make of the rows
+          // that see their tokens.  (Of those in unchecked tiles nothing changes.)
+          const uint8_t* q = a.q + (int64_t)qrow * a.q_row + qh * a.q_head;
+          for (int t = max(t_lo, pos0 + 1 - BT); t <= last; ++t) {
+            if (!mv.there(t)) continue;
+            float p = 0.0f;
+            bool known = false;
+            for (int i = 0; i < D / 2; ++i) {  // the dims that this lane has stored
+              const int d = i / 4 * 8 + 4 * h + i % 4;
+              const float v = mv.v_elem(t, d);
+              if (fabsf(v) < INFINITY) continue;
+              if (!known) {
+                float x = 0.0f;
+                for (int n = 0; n < D; ++n) x += kv_elem<QT>(q + 2 * n) * mv.k_elem(t, n);
+                p = __builtin_amdgcn_exp2f(x * c2 - m_run);
+                known = true;
+              }
+              if (whole) {
+                uint16_t* o = a.out + ((int64_t)qrow * a.num_q_heads + qh) * D + d;
+                const float x = kv_elem<QT>(reinterpret_cast<const uint8_t*>(o));
+                *o = (uint16_t)pair16<QT>(x + p * v * a.v_scale, 0.0f);
+              } else {
+                float* o = a.part + ((sh.index * 2 + begins) * kRows + col) * (D + kPartPad) + d;
+                *o += p * v;
+              }
+            }
           }
         }
       }
@@ -1012,8 +729,14 @@ void finish_args(RowsArgs* a, void* workspace, float softmax_scale, float k_scal
   a->group = a->num_q_heads / a->num_kv_heads;
   a->tile_rows = std::max(1, kRows / a->group);
   const int b = a->block_size;
-  a->block_shift = (b & (b - 1)) == 0 ? __builtin_ctz((unsigned)b) : -1;
-  a->by16 = b % 16 == 0 && a->token_stride >= 0 && a->token_stride < (1 << 27);
+  a->block_shift = __builtin_ctz((unsigned)b);
+  a->by16 = b % 16 == 0 && (b & (b - 1)) == 0 && a->page_stride >= 0 && a->token_stride >= 0 &&
+            a->page_stride % 16 == 0 && a->token_stride % 16 == 0 &&
+            a->token_stride < ((int64_t)1 << 27) && a->page_stride < ((int64_t)1 << 35) &&
+            (a->pool_pages - 1) * (a->page_stride / 16) + b * (a->token_stride / 16) <
+                ((int64_t)1 << 32);
+  a->page_units = (uint32_t)(a->page_stride / 16);
+  a->token_units = (uint32_t)(a->token_stride / 16);
   const float scale =
       softmax_scale > 0.0f ? softmax_scale : 1.0f / __builtin_sqrtf((float)a->head_dim);
   a->score_scale = scale * k_scale * kLog2e;
