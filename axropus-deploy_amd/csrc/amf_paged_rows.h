@@ -11,6 +11,11 @@ namespace amf {
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef s16x4 __attribute__((address_space(3))) lds_s16x4;
 typedef uint8_t __attribute__((address_space(3))) lds_u8;
+typedef u32x4 __attribute__((address_space(3))) lds_u32x4;
+
+__device__ __forceinline__ uint32_t lds_address(const uint8_t* p) {
+  return (uint32_t)(uintptr_t)(lds_u8*)p;
+}
 
 constexpr int kRowsWaves = 4;
 constexpr int kRowsThreads = 64 * kRowsWaves;
@@ -123,9 +128,9 @@ __device__ __forceinline__ void mark_row(uint32_t* marks, int r, bool is) {
 // A mover brings tiles of one (block table, KV head) into LDS, K one tile ahead of V:
 // next(t) looks up, and of quantised caches loads, K of the tile at t and V of the one
 // before; store_k and store_v put what the last next() found into LDS, complete after
-// wait() and a barrier.  `end`: tokens that are read; behind them K rows hold anything
+// settle() and a barrier.  `end`: tokens that are read; behind them K rows hold anything
 // (they are hidden), V rows zeros.  Rows whose page is none are marked by store_k, and
-// are zeros in V.  CHECK: V values that are not finite become 0, *wild != 0 then.
+// are zeros in V.  check: V values that are not finite become 0, *wild != 0 then.
 //
 // Branches in next() and the stores are the same for all lanes of a wave, or select.
 
@@ -188,8 +193,8 @@ struct CacheMover {
   static __device__ __forceinline__ const uint8_t* base(const uint8_t* plane, uint32_t off) {
     return plane + ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane(off) << 4);
   }
-  __device__ __forceinline__ uint32_t lane_off(int i, int chunk) const {
-    return (lane_row(i) * a.token_units + chunk) << 4;
+  __device__ __forceinline__ uint32_t lane_off(int i, int chunk, int lane) const {
+    return (lane_row(i, lane) * a.token_units + chunk) << 4;
   }
   // 16 bytes of token t's row from byte c on, zeros where it is not there; *bad: its page
   // is none.
@@ -220,29 +225,53 @@ struct Mover : CacheMover<2, D> {
   using Base::a, Base::row, Base::end, Base::kb, Base::vb, Base::k_id, Base::v_id;
   static constexpr int VT = QT, BT = Base::BT;
 
-  __device__ __forceinline__ Mover(const RowsArgs& args) : Base(args) {}
+  __device__ __forceinline__ Mover(const RowsArgs& args) : Base(args), look(false) {}
   __device__ __forceinline__ void next(int t0) {
     if (a.by16) this->look_up(t0);
   }
   // 16 bytes of each lane, at base + off, to 16 lane bytes behind `lds`.  In assembly, as
   // the compiler waits for all loads in flight before LDS reads that it cannot tell from
-  // what they write; wait() does that.
+  // what they write; settle() does that.
   static __device__ __forceinline__ void load_lds(const uint8_t* base, uint32_t off,
                                                   uint8_t* lds) {
-    const uint32_t at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_u8*)lds);
+    const uint32_t at = __builtin_amdgcn_readfirstlane(lds_address(lds));
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
                  : : "v"(off), "s"(base), "s"(at) : "memory", "m0");
   }
-  static __device__ __forceinline__ void wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+  // What store_v() has left to be looked at, once it is there: rows of this wave.
+  bool look;
+  int look_t;
+  uint8_t* look_lds;
+  __device__ __forceinline__ void settle(uint32_t* wild) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if (!look) return;
+    look = false;
+    const int tid = opaque(threadIdx.x);
+    const bool ok = this->good(__builtin_amdgcn_readfirstlane(look_id));
+    uint8_t* p = look_lds + Base::wave_row() * 2 * D + tid % 64 * 16;
+    bool found = false;
+#pragma unroll
+    for (int i = 0; i < Base::CH; ++i) {
+      const bool in = ok && look_t + row(i, tid) < end;
+      const u32x4 x = *reinterpret_cast<const u32x4*>(p + i * 1024);
+      uint32_t w[4] = {in ? x[0] : 0u, in ? x[1] : 0u, in ? x[2] : 0u, in ? x[3] : 0u};
+      found |= clean<VT>(w);
+      *reinterpret_cast<u32x4*>(p + i * 1024) = u32x4{w[0], w[1], w[2], w[3]};
+    }
+    mark_row(wild, 0, found);
+  }
+  int32_t look_id;
   __device__ __forceinline__ void store_k(int t0, uint8_t* lds, uint32_t* bad) const {
     if (a.by16) {
       const int32_t id = __builtin_amdgcn_readfirstlane(k_id);
-      const int wr = Base::wave_row(), c = threadIdx.x % Base::CPR;
+      const int wr = Base::wave_row();
       if (this->good(id)) {
         const uint8_t* b = Base::base(kb, this->k_off);
+        // (offsets made here, not kept in registers over the loop)
+        const int tid = opaque(threadIdx.x), c = tid % Base::CPR;
 #pragma unroll
         for (int i = 0; i < Base::CH; ++i)
-          load_lds(b, this->lane_off(i, c ^ k_swizzle<D>(row(i))),
+          load_lds(b, this->lane_off(i, c ^ k_swizzle<D>(row(i, tid)), tid),
                    lds + (wr + i * Base::RPI) * 2 * D);
       } else if (t0 + wr < end) {
 #pragma unroll
@@ -260,15 +289,20 @@ struct Mover : CacheMover<2, D> {
       *reinterpret_cast<u32x4*>(lds + k_place<D>(r, c)) = k;
     }
   }
-  template <bool CHECK>
-  __device__ __forceinline__ void store_v(int t0, uint8_t* lds, uint32_t* wild) const {
-    const int32_t id = __builtin_amdgcn_readfirstlane(v_id);
-    if (!CHECK && a.by16 && this->good(id) && t0 + BT <= end) {
-      const int wr = Base::wave_row(), c = threadIdx.x % Base::CPR;
+  __device__ __forceinline__ void store_v(int t0, uint8_t* lds, bool check, uint32_t* wild) {
+    if (a.by16) {
+      const int32_t id = __builtin_amdgcn_readfirstlane(v_id);
+      const int wr = Base::wave_row();
+      look = check || !this->good(id) || t0 + BT > end;
+      look_t = t0;
+      look_lds = lds;
+      look_id = id;
+      if (!this->good(id)) return;
       const uint8_t* b = Base::base(vb, this->v_off);
+      const int tid = opaque(threadIdx.x), c = tid % Base::CPR;
 #pragma unroll
       for (int i = 0; i < Base::CH; ++i)
-        load_lds(b, this->lane_off(i, c ^ v_swizzle<D>(row(i))),
+        load_lds(b, this->lane_off(i, c ^ v_swizzle<D>(row(i, tid)), tid),
                  lds + (wr + i * Base::RPI) * 2 * D);
       return;
     }
@@ -279,7 +313,7 @@ struct Mover : CacheMover<2, D> {
       bool none;
       const u32x4 x = this->lane_row_of(vb, t0 + r, 16 * c, &none);
       uint32_t w[4] = {x[0], x[1], x[2], x[3]};
-      if constexpr (CHECK) {
+      if (check) {
         const bool found = clean<VT>(w);
         mark_row(wild, 0, found);
       }
@@ -305,7 +339,7 @@ struct Mover<QT, AMF_DTYPE_E4M3, D> : CacheMover<1, D> {
   int bad;  // bits of the lane's K rows whose pages are none
 
   __device__ __forceinline__ Mover(const RowsArgs& args) : Base(args) {}
-  static __device__ __forceinline__ void wait() {}
+  static __device__ __forceinline__ void settle(uint32_t*) {}
   __device__ __forceinline__ void next(int t0) {
     bad = 0;
     if (a.by16) {
@@ -319,7 +353,7 @@ struct Mover<QT, AMF_DTYPE_E4M3, D> : CacheMover<1, D> {
         const uint8_t* b = Base::base(kb, this->k_off);
 #pragma unroll
         for (int i = 0; i < Base::CH; ++i)
-          kr[i] = *reinterpret_cast<const u32x4*>(b + this->lane_off(i, c));
+          kr[i] = *reinterpret_cast<const u32x4*>(b + this->lane_off(i, c, threadIdx.x));
       } else {
 #pragma unroll
         for (int i = 0; i < Base::CH; ++i) bad |= (t0 + row(i) < end) << i;
@@ -328,7 +362,7 @@ struct Mover<QT, AMF_DTYPE_E4M3, D> : CacheMover<1, D> {
         const uint8_t* b = Base::base(vb, this->v_off);
 #pragma unroll
         for (int i = 0; i < Base::CH; ++i)
-          vr[i] = *reinterpret_cast<const u32x4*>(b + this->lane_off(i, c));
+          vr[i] = *reinterpret_cast<const u32x4*>(b + this->lane_off(i, c, threadIdx.x));
       }
       return;
     }
@@ -350,9 +384,8 @@ struct Mover<QT, AMF_DTYPE_E4M3, D> : CacheMover<1, D> {
       return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, HIGH));
   }
   __device__ __forceinline__ void store_k(int, uint8_t* lds, uint32_t* marks) const {
-    const int c = threadIdx.x % Base::CPR * 2;
+    const int tid = opaque(threadIdx.x), c = tid % Base::CPR * 2;
     if (__any(bad)) {
-      const int tid = opaque(threadIdx.x);
 #pragma unroll
       for (int i = 0; i < Base::CH; ++i) mark_row(marks, row(i, tid), bad >> i & 1);
     }
@@ -361,30 +394,33 @@ struct Mover<QT, AMF_DTYPE_E4M3, D> : CacheMover<1, D> {
 #pragma unroll
       for (int n = 0; n < 2; ++n) {
         const uint32_t x = kr[i][2 * n], y = kr[i][2 * n + 1];
-        *reinterpret_cast<u32x4*>(lds + k_place<D>(row(i), c + n)) =
+        *reinterpret_cast<u32x4*>(lds + k_place<D>(row(i, tid), c + n)) =
             u32x4{pair<QT, false>(x), pair<QT, true>(x), pair<QT, false>(y), pair<QT, true>(y)};
       }
   }
-  template <bool CHECK>
-  __device__ __forceinline__ void store_v(int t0, uint8_t* lds, uint32_t* wild) const {
-    const int c = threadIdx.x % Base::CPR * 2;
+  __device__ __forceinline__ void store_v(int t0, uint8_t* lds, bool check,
+                                          uint32_t* wild) const {
+    const int tid = opaque(threadIdx.x), c = tid % Base::CPR * 2;
 #pragma unroll
-    for (int i = 0; i < Base::CH; ++i)
+    for (int i = 0; i < Base::CH; ++i) {
+      uint32_t w[8];
 #pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        const uint32_t x = vr[i][2 * n], y = vr[i][2 * n + 1];
-        uint32_t w[4] = {pair<VT, false>(x), pair<VT, true>(x), pair<VT, false>(y),
-                         pair<VT, true>(y)};
-        if constexpr (CHECK) {
-          const bool in = t0 + row(i) < end;
-#pragma unroll
-          for (int m = 0; m < 4; ++m) w[m] = in ? w[m] : 0u;
-          const bool found = clean<VT>(w);
-          mark_row(wild, 0, found);
-        }
-        *reinterpret_cast<u32x4*>(lds + v_place<D>(row(i), c + n)) =
-            u32x4{w[0], w[1], w[2], w[3]};
+      for (int n = 0; n < 4; ++n) {
+        w[2 * n] = pair<VT, false>(vr[i][n]);
+        w[2 * n + 1] = pair<VT, true>(vr[i][n]);
       }
+      if (check) {
+        const bool in = t0 + row(i, tid) < end;
+#pragma unroll
+        for (int n = 0; n < 8; ++n) w[n] = in ? w[n] : 0u;
+        const bool found = clean<VT>(w);
+        mark_row(wild, 0, found);
+      }
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+        *reinterpret_cast<u32x4*>(lds + v_place<D>(row(i, tid), c + n)) =
+            u32x4{w[4 * n], w[4 * n + 1], w[4 * n + 2], w[4 * n + 3]};
+    }
   }
   __device__ __forceinline__ float k_elem(int t, int d) const {
     return this->template elem<AMF_DTYPE_E4M3>(kb, t, d);
@@ -413,7 +449,7 @@ struct Mover<QT, kInt4, D> {
   int bad;  // the lane's K row has no page
 
   __device__ __forceinline__ Mover(const RowsArgs& args) : a(args) {}
-  static __device__ __forceinline__ void wait() {}
+  static __device__ __forceinline__ void settle(uint32_t*) {}
   // the same in a wave
   static __device__ __forceinline__ bool has_k() {
     return !HALF || __builtin_amdgcn_readfirstlane(threadIdx.x) < N;
@@ -421,9 +457,11 @@ struct Mover<QT, kInt4, D> {
   static __device__ __forceinline__ bool has_v() {
     return !HALF || __builtin_amdgcn_readfirstlane(threadIdx.x) >= N;
   }
-  static __device__ __forceinline__ int item() { return threadIdx.x % N; }
-  static __device__ __forceinline__ int k_row() { return item() / G; }
-  static __device__ __forceinline__ int v_page() { return item() / (D / 2); }
+  static __device__ __forceinline__ int item(int tid = threadIdx.x) { return tid % N; }
+  static __device__ __forceinline__ int k_row(int tid = threadIdx.x) { return item(tid) / G; }
+  static __device__ __forceinline__ int v_page(int tid = threadIdx.x) {
+    return item(tid) / (D / 2);
+  }
   __device__ __forceinline__ bool good(int32_t id) const { return id >= 0 && id < a.pool_pages; }
   __device__ __forceinline__ void start(int seq, int h, int e) {
     table = a.block_tables + seq * a.bt_stride;
@@ -487,7 +525,8 @@ struct Mover<QT, kInt4, D> {
   // u * s is exact (4 bits by 11), so the fma rounds as the codec's multiply and add.
   __device__ __forceinline__ void store_k(int, uint8_t* lds, uint32_t* marks) const {
     if (!has_k()) return;
-    if (__any(bad)) mark_row(marks, k_row(), bad);
+    const int tid = opaque(threadIdx.x);
+    if (__any(bad)) mark_row(marks, k_row(tid), bad);
     const float s = param_scale(ks), z = param_zero(ks);
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
@@ -497,32 +536,35 @@ struct Mover<QT, kInt4, D> {
 #pragma unroll
       for (int n = 0; n < 4; ++n)
         y[n] = pair16<QT>(__builtin_fmaf(x[2 * n], s, z), __builtin_fmaf(x[2 * n + 1], s, z));
-      *reinterpret_cast<u32x4*>(lds + k_place<D>(k_row(), 4 * (item() % G) + w)) = y;
+      *reinterpret_cast<u32x4*>(lds + k_place<D>(k_row(tid), 4 * (item(tid) % G) + w)) = y;
     }
   }
-  template <bool CHECK>
-  __device__ __forceinline__ void store_v(int t0, uint8_t* lds, uint32_t* wild) const {
+  __device__ __forceinline__ void store_v(int t0, uint8_t* lds, bool check,
+                                          uint32_t* wild) const {
     if (!has_v()) return;
-    const int c = item() % (D / 2);
-    const int r0 = 16 * v_page() + c / 2 % 2 * 8;
+    const int tid = opaque(threadIdx.x), c = item(tid) % (D / 2);
+    const int r0 = 16 * v_page(tid) + c / 2 % 2 * 8;
     float x[4][8];
+    uint32_t y[16];
 #pragma unroll
     for (int d = 0; d < 4; ++d) nibbles(vr[d], x[d]);
 #pragma unroll
     for (int t = 0; t < 8; ++t) {
       const uint32_t p = vs[t / 4][t % 4];
       const float s = param_scale(p), z = param_zero(p);
-      uint32_t y[2] = {pair16<QT>(__builtin_fmaf(x[0][t], s, z), __builtin_fmaf(x[1][t], s, z)),
-                       pair16<QT>(__builtin_fmaf(x[2][t], s, z), __builtin_fmaf(x[3][t], s, z))};
-      if constexpr (CHECK) {
-        const bool in = t0 + r0 + t < end;
-        y[0] = in ? y[0] : 0u;
-        y[1] = in ? y[1] : 0u;
-        const bool found = clean<VT>(y);
-        mark_row(wild, 0, found);
-      }
-      *reinterpret_cast<u32x2*>(lds + v_place<D>(r0 + t, c / 4) + c % 2 * 8) = u32x2{y[0], y[1]};
+      y[2 * t] = pair16<QT>(__builtin_fmaf(x[0][t], s, z), __builtin_fmaf(x[1][t], s, z));
+      y[2 * t + 1] = pair16<QT>(__builtin_fmaf(x[2][t], s, z), __builtin_fmaf(x[3][t], s, z));
     }
+    if (check) {
+#pragma unroll
+      for (int t = 0; t < 16; ++t) y[t] = t0 + r0 + t / 2 < end ? y[t] : 0u;
+      const bool found = clean<VT>(y);
+      mark_row(wild, 0, found);
+    }
+#pragma unroll
+    for (int t = 0; t < 8; ++t)
+      *reinterpret_cast<u32x2*>(lds + v_place<D>(r0 + t, c / 4) + c % 2 * 8) =
+          u32x2{y[2 * t], y[2 * t + 1]};
   }
   __device__ __forceinline__ bool there(int t) const { return good(table[t / 16]); }
   __device__ __forceinline__ float k_elem(int t, int d) const {

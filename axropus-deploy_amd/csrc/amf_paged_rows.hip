@@ -185,11 +185,13 @@ template <int QT, int KV, int D>
 __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void rows_kernel(RowsArgs a) {
   using Move = Mover<QT, KV, D>;
   constexpr int BT = Move::BT, VT = Move::VT, RB = 2 * D;
+  // products of K and q with a tile's 32 tokens, of all of them; V fragments, and products
+  constexpr int KS = D / 16, QN = BT / 32 * KS, DN = D / 32, PN = BT / 16 * DN;
   // Two buffers each: while the values of a tile and the keys of the next are multiplied,
   // the next values and the keys after are on their way, with one barrier a tile.
   constexpr int TB = BT * RB;
-  __shared__ __attribute__((aligned(16))) uint8_t k_lds[2 * TB];
-  __shared__ __attribute__((aligned(16))) uint8_t v_lds[2 * TB];
+  __shared__ __attribute__((aligned(2 * D))) uint8_t k_lds[2 * TB];
+  __shared__ __attribute__((aligned(2 * D))) uint8_t v_lds[2 * TB];
   __shared__ uint32_t marks[4][2];  // of K tiles, by turns; [3]: the piece's wild V
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -221,15 +223,16 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void rows_kernel(RowsAr
 
   // This lane's LDS reads.  K: chunk 2 ks + h of row lc, whose swizzle the rows 32
   // further share.  V: 8 bytes of row 4 h + l16 / 4, whose swizzle depends on l16 alone,
-  // for dims 32 d of each d.
-  const int k_at = lc * RB, k_x = (h ^ k_swizzle<D>(lc)) << 4;
+  // for dims 32 d of each d.  Rows are aligned to their length, so ks and d flip bits
+  // of one address.
   const int l16 = lane & 15, v_row = 4 * h + (l16 >> 2);
-  const int v_at = v_row * RB + 8 * (l16 & 1);
-  const int v_x = (((lane >> 4 & 1) * 2 + (l16 >> 1 & 1)) ^ v_swizzle<D>(v_row)) << 4;
+  const uint32_t k_at = lds_address(k_lds) + k_place<D>(lc, h);
+  const uint32_t v_at = lds_address(v_lds) + 8 * (l16 & 1) +
+                        v_place<D>(v_row, (lane >> 4 & 1) * 2 + (l16 >> 1 & 1));
   // A operand of V^T: dims 32 d .. + 31, 16 tokens in the order of the scores
-  auto read_v = [](const uint8_t* vp) {
-    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(vp));
-    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(vp + 8 * RB));
+  auto read_v = [](uint32_t at) __attribute__((always_inline)) {
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)at);
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + 8 * RB));
     const u32x2 l2 = __builtin_bit_cast(u32x2, lo), h2 = __builtin_bit_cast(u32x2, hi);
     return u32x4{l2[0], l2[1], h2[0], h2[1]};
   };
@@ -261,10 +264,6 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void rows_kernel(RowsAr
 #pragma unroll
         for (int ks = 0; ks < D / 16; ++ks)
           qb[ks] = *reinterpret_cast<const u32x4*>(qp + 32 * ks);
-        // here, and not before the first product of every tile, where the wait would be for
-        // the next tile's loads as well
-#pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks) asm volatile("" : "+v"(qb[ks]));
       }
       // the row's last token
       const int last = min(pos0 + qi, t_hi - 1);
@@ -291,10 +290,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void rows_kernel(RowsAr
         if (i >= -1 && i + 1 < n) {
           // tokens that some rows see and others do not: V has to be finite there, as
           // 0 * inf is not 0
-          if (t1 + BT > pos0 + 1)
-            mv.template store_v<true>(t1, v_lds + (i + 1 & 1) * TB, marks[3]);
-          else
-            mv.template store_v<false>(t1, v_lds + (i + 1 & 1) * TB, marks[3]);
+          mv.store_v(t1, v_lds + (i + 1 & 1) * TB, t1 + BT > pos0 + 1, marks[3]);
         }
         if (i + 2 < n) mv.next(t2 + BT);
         const int m = m2;
@@ -302,54 +298,66 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void rows_kernel(RowsAr
         m0 = m1;
         m1 = m;
       };
-      // Scores of tile i, and their maximum.
-      auto score = [&](int i) __attribute__((always_inline)) {
-        const uint8_t* k_rd = k_lds + (i & 1) * TB + k_at;
+      // K fragment q of a tile: dims 16 (q % KS) .. of tokens 32 (q / KS) ..
+      auto read_k = [](uint32_t at, int q) __attribute__((always_inline)) {
+        return *(const lds_u32x4*)((at ^ (32 * (q % KS))) + 32 * (q / KS) * RB);
+      };
+      // Whether tile i holds tokens that some of the wave's rows do not see; then they
+      // are hidden.  Token of score element e of block tb: t0 + 32 tb + 8 (e / 4) + 4 h + e % 4.
+      auto hide = [&](int i) __attribute__((always_inline)) {
         const int t0 = t_lo + i * BT;
-#pragma unroll
-        for (int tb = 0; tb < BT / 32; ++tb) {
-#pragma unroll
-          for (int e = 0; e < 16; ++e) s[tb][e] = 0.0f;
-#pragma unroll
-          for (int ks = 0; ks < D / 16; ++ks)
-            s[tb] = mfma32<QT>(
-                *reinterpret_cast<const u32x4*>(k_rd + 32 * tb * RB + (k_x ^ (32 * ks))), qb[ks],
-                s[tb]);
-        }
-        // token of score element e of block tb: t0 + 32 tb + 8 (e / 4) + 4 h + e % 4
         const uint32_t bad[2] = {(uint32_t)__builtin_amdgcn_readfirstlane(marks[m1][0]),
                                  (uint32_t)__builtin_amdgcn_readfirstlane(marks[m1][1])};
-        if (t0 + BT > t_hi || t0 + BT - 1 > pos0 + wave_first || (bad[0] | bad[1])) {
-          const int left = last - t0 - 4 * h;
-          bad_seen |= (bad[0] | bad[1]) != 0;
-#pragma unroll
-          for (int tb = 0; tb < BT / 32; ++tb) {
-            const uint32_t gone = opaque(bad[tb] >> (4 * h));  // no masks kept over the loop
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const int t = 32 * tb + 8 * (e >> 2) + (e & 3);
-              const bool hide = t > left || (gone >> (t % 32) & 1);
-              s[tb][e] = hide ? -INFINITY : s[tb][e];
-              seen |= !hide;
-            }
-          }
-        } else {
+        if (t0 + BT <= t_hi && t0 + BT - 1 <= pos0 + wave_first && !(bad[0] | bad[1])) {
           seen = true;
+          return false;
         }
-        float mx = -INFINITY;
+        const int left = last - t0 - 4 * h;
+        bad_seen |= (bad[0] | bad[1]) != 0;
+#pragma unroll
+        for (int tb = 0; tb < BT / 32; ++tb) {
+          const uint32_t gone = opaque(bad[tb] >> (4 * h));  // no masks kept over the loop
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int t = 32 * tb + 8 * (e >> 2) + (e & 3);
+            const bool hidden = t > left || (gone >> (t % 32) & 1);
+            s[tb][e] = hidden ? -INFINITY : s[tb][e];
+            seen |= !hidden;
+          }
+        }
+        return true;
+      };
+      auto largest = [&]() __attribute__((always_inline)) {
+        float x = -INFINITY;
 #pragma unroll
         for (int tb = 0; tb < BT / 32; ++tb)
 #pragma unroll
-          for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[tb][e]);
-        return max_of_halves(mx) * c2 - weight_shift<VT>();
+          for (int e = 0; e < 16; ++e) x = fmaxf(x, s[tb][e]);
+        return x;
       };
+      auto scaled = [&](float x) { return max_of_halves(x) * c2 - weight_shift<VT>(); };
       float mx = -INFINITY;
       if (n > 0) {
         mv.next(t_lo);
         for (int i = -2; i < (wave_on ? 0 : n); ++i) {
           move(i);
-          if (wave_on && i == -1) mx = score(0);
-          mv.wait();
+          if (wave_on && i == -1) {
+            // q is waited for here, not before the first product of every tile, where that
+            // would be for the next tiles' loads as well
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(qb[ks]));
+#pragma unroll
+            for (int tb = 0; tb < BT / 32; ++tb) {
+#pragma unroll
+              for (int e = 0; e < 16; ++e) s[tb][e] = 0.0f;
+#pragma unroll
+              for (int ks = 0; ks < KS; ++ks)
+                s[tb] = mfma32<QT>(read_k(k_at, tb * KS + ks), qb[ks], s[tb]);
+            }
+            hide(0);
+            mx = scaled(largest());
+          }
+          mv.settle(marks[3]);
           __syncthreads();
         }
         // The inner loop changes the accumulators by products alone: with a branch in it that
@@ -369,32 +377,66 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void rows_kernel(RowsAr
           bool over;
           do {
             move(i);
-            const uint8_t* v_rd = v_lds + (i & 1) * TB + v_at;
+            const uint32_t k_rd = k_at + (~i & 1) * TB, v_rd = v_at + (i & 1) * TB;
             u32x4 pb[BT / 16];  // weights of 16 tokens each, 8 per lane
+            float l2 = 0.0f;
+            // weights of elements 2 e, 2 e + 1 of block tb
+            auto weigh = [&](int tb, int e) __attribute__((always_inline)) {
+              const float p0 = __builtin_amdgcn_exp2f(s[tb][2 * e] * c2 - m_use);
+              const float p1 = __builtin_amdgcn_exp2f(s[tb][2 * e + 1] * c2 - m_use);
+              l_run += p0;
+              l2 += p1;
+              pb[2 * tb + e / 4][e % 4] = pair16<VT>(p0, p1);
+            };
+            // The order of the products and of what is done in their shadow: weights of the
+            // first 32 tokens; scores of the next tile's first 32 over them, beside the
+            // other weights; the other scores, beside the first reads of V; then V's
+            // products, beside the maximum.  Reads are four products and more ahead.
+            constexpr int AHEAD = 4;
+            u32x4 kf[AHEAD], vf[2][DN];
 #pragma unroll
-            for (int st = 0; st < BT / 16; ++st)
+            for (int q = 0; q < AHEAD; ++q) kf[q] = read_k(k_rd, q);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const float p0 =
-                    __builtin_amdgcn_exp2f(s[st >> 1][8 * (st & 1) + 2 * e] * c2 - m_use);
-                const float p1 =
-                    __builtin_amdgcn_exp2f(s[st >> 1][8 * (st & 1) + 2 * e + 1] * c2 - m_use);
-                l_run += p0;
-                l_run += p1;
-                pb[st][e] = pair16<VT>(p0, p1);
-              }
+            for (int e = 0; e < 8; ++e) weigh(0, e);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int st = 0; st < BT / 16; ++st)
+            for (int q = 0; q < QN; ++q) {
+              const int tb = q / KS, ks = q % KS;
+              if (ks == 0)
 #pragma unroll
-              for (int d = 0; d < D / 32; ++d)
-                acc[d] = mfma32<VT>(read_v(v_rd + 16 * st * RB + (v_x ^ (64 * d))), pb[st], acc[d]);
+                for (int e = 0; e < 16; ++e) s[tb][e] = 0.0f;
+              s[tb] = mfma32<QT>(kf[q % AHEAD], qb[ks], s[tb]);
+              if (q + AHEAD < QN) kf[q % AHEAD] = read_k(k_rd, q + AHEAD);
+              if (tb + 1 < BT / 32)
+#pragma unroll
+                for (int e = ks * 8 / KS; e < (ks + 1) * 8 / KS; ++e) weigh(tb + 1, e);
+              else if (ks < DN)
+                vf[0][ks] = read_v(v_rd ^ (64 * ks));
+              __builtin_amdgcn_sched_barrier(0);
+            }
+            float big = -INFINITY;
+#pragma unroll
+            for (int p = 0; p < PN; ++p) {
+              const int st = p / DN, d = p % DN;
+              acc[d] = mfma32<VT>(vf[st & 1][d], pb[st], acc[d]);
+              if (st + 1 < BT / 16)
+                vf[(st + 1) & 1][d] = read_v((v_rd ^ (64 * d)) + 16 * (st + 1) * RB);
+#pragma unroll
+              for (int e = p * (BT / 2) / PN; e < (p + 1) * (BT / 2) / PN; ++e)
+                big = fmaxf(big, s[e / 16][e % 16]);
+              __builtin_amdgcn_sched_barrier(0);
+            }
+            l_run += l2;
+            // (behind the last tile the scores are of what lies in LDS, and not used)
             ++i;
             over = false;
             if (i < n) {
-              mx = score(i);
+              if (hide(i)) big = largest();
+              mx = scaled(big);
               over = __any(mx > m_run + slack<VT>());
             }
-            mv.wait();
+            mv.settle(marks[3]);
             __syncthreads();
           } while (i < n && !over);
         }
