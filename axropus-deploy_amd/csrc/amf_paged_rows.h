@@ -120,19 +120,27 @@ __device__ __forceinline__ int opaque(int x) {
   return x;
 }
 
+// The thread's index, for addresses that the turns of a piece keep in registers (KEEP; `id`
+// is the piece's own, so that they are not kept over all pieces) or compute again each.
+template <bool KEEP>
+__device__ __forceinline__ int thread(int id) {
+  return KEEP ? id : opaque(threadIdx.x);
+}
+
 // Marks row r where `is`.
 __device__ __forceinline__ void mark_row(uint32_t* marks, int r, bool is) {
   atomicOr(marks + r / 32, is ? 1u << (r % 32) : 0u);
 }
 
 // A mover brings tiles of one (block table, KV head) into LDS, K one tile ahead of V:
-// next(t) looks up, and of quantised caches loads, K of the tile at t and V of the one
-// before; store_k and store_v put what the last next() found into LDS, complete after
-// settle() and a barrier.  `end`: tokens that are read; behind them K rows hold anything
+// next(t) finds the pages, and of quantised caches loads, K of the tile at t and V of the
+// one before; store_k and store_v put what the last next() found into LDS, complete
+// after settle() and a barrier.  kInRegisters: what it found can be copied, and stored after
+// the following next().  `end`: tokens that are read; behind them K rows hold anything
 // (they are hidden), V rows zeros.  Rows whose page is none are marked by store_k, and
 // are zeros in V.  check: V values that are not finite become 0, *wild != 0 then.
 //
-// Branches in next() and the stores are the same for all lanes of a wave, or select.
+// KEEP: there are registers for addresses.  Branches in next() and the stores are the same for all lanes of a wave, or select.
 
 // What movers of caches (EB bytes an element) share.  Wave w of the workgroup takes rows
 // RPW w .. of a tile, which lie in one aligned group of 16: with pages of 16, 32, 64 ..
@@ -152,6 +160,7 @@ struct CacheMover {
   const RowsArgs& a;
   const int32_t* table;
   int end;
+  int id;                  // of the thread
   const uint8_t *kb, *vb;  // the KV head's
   int32_t k_id, v_id;      // by16: pages of the wave's rows; -1 behind `end`
   uint32_t k_off, v_off;   // and their place, in units of 16 bytes
@@ -174,19 +183,20 @@ struct CacheMover {
   __device__ __forceinline__ int64_t place(int32_t id, int t) const {
     return id * a.page_stride + (t - page_of(t) * a.block_size) * a.token_stride;
   }
-  __device__ __forceinline__ void start(int seq, int head, int e) {
+  __device__ __forceinline__ void start(int seq, int head, int, int e) {
     table = a.block_tables + seq * a.bt_stride;
     end = e;
+    id = opaque(threadIdx.x);
     kb = a.k + head * a.head_stride;
     vb = a.v + head * a.head_stride;
     k_id = -1;
     k_off = 0;
   }
-  __device__ __forceinline__ void look_up(int t0) {
+  __device__ __forceinline__ void found(int t0, int32_t id) {
     v_id = k_id;
     v_off = k_off;
     const int t = t0 + wave_row();
-    k_id = __builtin_amdgcn_readfirstlane(t < end ? scalar_load(table, t >> a.block_shift) : -1);
+    k_id = __builtin_amdgcn_readfirstlane(t < end ? id : -1);
     k_off = (uint32_t)k_id * a.page_units + (uint32_t)(t & (a.block_size - 1)) * a.token_units;
   }
   // The wave's rows behind `off`, and a lane's bytes of row i behind that.
@@ -222,12 +232,15 @@ struct CacheMover {
 template <int QT, int KV, int D>
 struct Mover : CacheMover<2, D> {
   using Base = CacheMover<2, D>;
-  using Base::a, Base::row, Base::end, Base::kb, Base::vb, Base::k_id, Base::v_id;
+  using Base::a, Base::id, Base::row, Base::end, Base::kb, Base::vb, Base::k_id, Base::v_id;
   static constexpr int VT = QT, BT = Base::BT;
+  static constexpr bool kInRegisters = false;
 
   __device__ __forceinline__ Mover(const RowsArgs& args) : Base(args), look(false) {}
+  template <bool KEEP>
   __device__ __forceinline__ void next(int t0) {
-    if (a.by16) this->look_up(t0);
+    const int t = t0 + Base::wave_row();
+    if (a.by16) this->found(t0, t < end ? scalar_load(this->table, t >> a.block_shift) : -1);
   }
   // 16 bytes of each lane, at base + off, to 16 lane bytes behind `lds`.  In assembly, as
   // the compiler waits for all loads in flight before LDS reads that it cannot tell from
@@ -247,7 +260,7 @@ struct Mover : CacheMover<2, D> {
     if (!look) return;
     look = false;
     const int tid = opaque(threadIdx.x);
-    const bool ok = this->good(__builtin_amdgcn_readfirstlane(look_id));
+    const bool ok = this->good(__builtin_amdgcn_readfirstlane(look_page));
     uint8_t* p = look_lds + Base::wave_row() * 2 * D + tid % 64 * 16;
     bool found = false;
 #pragma unroll
@@ -260,26 +273,27 @@ struct Mover : CacheMover<2, D> {
     }
     mark_row(wild, 0, found);
   }
-  int32_t look_id;
+  int32_t look_page;
+  template <bool KEEP>
   __device__ __forceinline__ void store_k(int t0, uint8_t* lds, uint32_t* bad) const {
     if (a.by16) {
-      const int32_t id = __builtin_amdgcn_readfirstlane(k_id);
+      const int32_t page = __builtin_amdgcn_readfirstlane(k_id);
       const int wr = Base::wave_row();
-      if (this->good(id)) {
+      if (this->good(page)) {
         const uint8_t* b = Base::base(kb, this->k_off);
         // (offsets made here, not kept in registers over the loop)
-        const int tid = opaque(threadIdx.x), c = tid % Base::CPR;
+        const int tid = thread<KEEP>(id), c = tid % Base::CPR;
 #pragma unroll
         for (int i = 0; i < Base::CH; ++i)
           load_lds(b, this->lane_off(i, c ^ k_swizzle<D>(row(i, tid)), tid),
                    lds + (wr + i * Base::RPI) * 2 * D);
       } else if (t0 + wr < end) {
 #pragma unroll
-        for (int i = 0; i < Base::CH; ++i) mark_row(bad, row(i, opaque(threadIdx.x)), true);
+        for (int i = 0; i < Base::CH; ++i) mark_row(bad, row(i, thread<KEEP>(id)), true);
       }
       return;
     }
-    const int tid = opaque(threadIdx.x), c = tid % Base::CPR;
+    const int tid = thread<KEEP>(id), c = tid % Base::CPR;
 #pragma unroll 1
     for (int i = 0; i < Base::CH; ++i) {
       const int r = row(i, tid);
@@ -289,24 +303,25 @@ struct Mover : CacheMover<2, D> {
       *reinterpret_cast<u32x4*>(lds + k_place<D>(r, c)) = k;
     }
   }
+  template <bool KEEP>
   __device__ __forceinline__ void store_v(int t0, uint8_t* lds, bool check, uint32_t* wild) {
     if (a.by16) {
-      const int32_t id = __builtin_amdgcn_readfirstlane(v_id);
+      const int32_t page = __builtin_amdgcn_readfirstlane(v_id);
       const int wr = Base::wave_row();
-      look = check || !this->good(id) || t0 + BT > end;
+      look = check || !this->good(page) || t0 + BT > end;
       look_t = t0;
       look_lds = lds;
-      look_id = id;
-      if (!this->good(id)) return;
+      look_page = page;
+      if (!this->good(page)) return;
       const uint8_t* b = Base::base(vb, this->v_off);
-      const int tid = opaque(threadIdx.x), c = tid % Base::CPR;
+      const int tid = thread<KEEP>(id), c = tid % Base::CPR;
 #pragma unroll
       for (int i = 0; i < Base::CH; ++i)
         load_lds(b, this->lane_off(i, c ^ v_swizzle<D>(row(i, tid)), tid),
                  lds + (wr + i * Base::RPI) * 2 * D);
       return;
     }
-    const int tid = opaque(threadIdx.x), c = tid % Base::CPR;
+    const int tid = thread<KEEP>(id), c = tid % Base::CPR;
 #pragma unroll 1
     for (int i = 0; i < Base::CH; ++i) {
       const int r = row(i, tid);
@@ -333,47 +348,56 @@ struct Mover : CacheMover<2, D> {
 template <int QT, int D>
 struct Mover<QT, AMF_DTYPE_E4M3, D> : CacheMover<1, D> {
   using Base = CacheMover<1, D>;
-  using Base::a, Base::row, Base::end, Base::kb, Base::vb, Base::k_id, Base::v_id;
+  using Base::a, Base::id, Base::row, Base::end, Base::kb, Base::vb, Base::k_id, Base::v_id;
   static constexpr int VT = AMF_DTYPE_F16, BT = Base::BT;
+  static constexpr bool kInRegisters = true;
   u32x4 kr[Base::CH], vr[Base::CH];
-  int bad;  // bits of the lane's K rows whose pages are none
+  int bad;    // bits of the lane's K rows whose pages are none
+  bool none;  // by16: no page for the wave's V rows
+  int32_t ahead;  // by16: the table's entry for the tile after K's
 
   __device__ __forceinline__ Mover(const RowsArgs& args) : Base(args) {}
   static __device__ __forceinline__ void settle(uint32_t*) {}
+  __device__ __forceinline__ void start(int seq, int head, int t0, int e) {
+    Base::start(seq, head, t0, e);
+    if (a.by16 && e > 0) look_up(t0);
+  }
+  // The entry is asked for a turn before it is used, as the tile's loads depend on it.  A
+  // vector load: reads of LDS behind a scalar one wait for it.
+  __device__ __forceinline__ void look_up(int t0) {
+    ahead = this->table[opaque(min(t0 + Base::wave_row(), end - 1) >> a.block_shift)];
+  }
+  // As many loads on every way, so that a wait for the tile before is not one for this.
+  // Where no page is, any is read.
+  template <bool KEEP>
   __device__ __forceinline__ void next(int t0) {
     bad = 0;
     if (a.by16) {
-      this->look_up(t0);
+      this->found(t0, ahead);
+      look_up(t0 + BT);
       const int32_t ki = __builtin_amdgcn_readfirstlane(k_id);
       const int32_t vi = __builtin_amdgcn_readfirstlane(v_id);
-      const int c = threadIdx.x % Base::CPR;
+      const int tid = thread<KEEP>(id), c = tid % Base::CPR;
+      const uint8_t* kp = Base::base(kb, this->good(ki) ? this->k_off : 0u);
+      const uint8_t* vp = Base::base(vb, this->good(vi) ? this->v_off : 0u);
 #pragma unroll
-      for (int i = 0; i < Base::CH; ++i) kr[i] = vr[i] = u32x4{0, 0, 0, 0};
-      if (this->good(ki)) {
-        const uint8_t* b = Base::base(kb, this->k_off);
-#pragma unroll
-        for (int i = 0; i < Base::CH; ++i)
-          kr[i] = *reinterpret_cast<const u32x4*>(b + this->lane_off(i, c, threadIdx.x));
-      } else {
-#pragma unroll
-        for (int i = 0; i < Base::CH; ++i) bad |= (t0 + row(i) < end) << i;
+      for (int i = 0; i < Base::CH; ++i) {
+        kr[i] = *reinterpret_cast<const u32x4*>(kp + this->lane_off(i, c, tid));
+        vr[i] = *reinterpret_cast<const u32x4*>(vp + this->lane_off(i, c, tid));
+        bad |= (!this->good(ki) && t0 + row(i, tid) < end) << i;
       }
-      if (this->good(vi)) {
-        const uint8_t* b = Base::base(vb, this->v_off);
-#pragma unroll
-        for (int i = 0; i < Base::CH; ++i)
-          vr[i] = *reinterpret_cast<const u32x4*>(b + this->lane_off(i, c, threadIdx.x));
-      }
+      none = !this->good(vi);
       return;
     }
-    const int tid = opaque(threadIdx.x), c = tid % Base::CPR * 16;
+    none = false;
+    const int tid = thread<KEEP>(id), c = tid % Base::CPR * 16;
 #pragma unroll
     for (int i = 0; i < Base::CH; ++i) {
       const int t = t0 + row(i, tid);
-      bool none;
-      kr[i] = this->lane_row_of(kb, t, c, &none);
-      bad |= none ? 1 << i : 0;
-      vr[i] = this->lane_row_of(vb, max(t - BT, 0), c, &none);
+      bool gone;
+      kr[i] = this->lane_row_of(kb, t, c, &gone);
+      bad |= gone ? 1 << i : 0;
+      vr[i] = this->lane_row_of(vb, max(t - BT, 0), c, &gone);
     }
   }
   template <int T, bool HIGH>
@@ -383,8 +407,9 @@ struct Mover<QT, AMF_DTYPE_E4M3, D> : CacheMover<1, D> {
     else
       return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, HIGH));
   }
+  template <bool KEEP>
   __device__ __forceinline__ void store_k(int, uint8_t* lds, uint32_t* marks) const {
-    const int tid = opaque(threadIdx.x), c = tid % Base::CPR * 2;
+    const int tid = thread<KEEP>(id), c = tid % Base::CPR * 2;
     if (__any(bad)) {
 #pragma unroll
       for (int i = 0; i < Base::CH; ++i) mark_row(marks, row(i, tid), bad >> i & 1);
@@ -398,9 +423,10 @@ struct Mover<QT, AMF_DTYPE_E4M3, D> : CacheMover<1, D> {
             u32x4{pair<QT, false>(x), pair<QT, true>(x), pair<QT, false>(y), pair<QT, true>(y)};
       }
   }
+  template <bool KEEP>
   __device__ __forceinline__ void store_v(int t0, uint8_t* lds, bool check,
                                           uint32_t* wild) const {
-    const int tid = opaque(threadIdx.x), c = tid % Base::CPR * 2;
+    const int tid = thread<KEEP>(id), c = tid % Base::CPR * 2;
 #pragma unroll
     for (int i = 0; i < Base::CH; ++i) {
       uint32_t w[8];
@@ -409,8 +435,8 @@ struct Mover<QT, AMF_DTYPE_E4M3, D> : CacheMover<1, D> {
         w[2 * n] = pair<VT, false>(vr[i][n]);
         w[2 * n + 1] = pair<VT, true>(vr[i][n]);
       }
-      if (check) {
-        const bool in = t0 + row(i, tid) < end;
+      if (check || none) {
+        const bool in = !none && t0 + row(i, tid) < end;
 #pragma unroll
         for (int n = 0; n < 8; ++n) w[n] = in ? w[n] : 0u;
         const bool found = clean<VT>(w);
@@ -439,14 +465,18 @@ struct Mover<QT, kInt4, D> {
   static constexpr int VT = QT, G = D / 32, N = BT * G;  // items of K, and of V
   static constexpr bool HALF = N * 2 == kRowsThreads;
   static_assert(HALF || N == kRowsThreads, "an item per thread");
+  static constexpr bool kInRegisters = true;
 
   const RowsArgs& a;
   const int32_t* table;
   int head;
   int end;
+  int id;  // of the thread
   u32x4 kr, vr, vs[2];
   uint32_t ks;
-  int bad;  // the lane's K row has no page
+  int bad;             // the lane's K row has no page
+  bool none;           // its V items have none
+  int32_t k_id, ahead; // the items' page, of K, and in the tile after
 
   __device__ __forceinline__ Mover(const RowsArgs& args) : a(args) {}
   static __device__ __forceinline__ void settle(uint32_t*) {}
@@ -459,105 +489,110 @@ struct Mover<QT, kInt4, D> {
   }
   static __device__ __forceinline__ int item(int tid = threadIdx.x) { return tid % N; }
   static __device__ __forceinline__ int k_row(int tid = threadIdx.x) { return item(tid) / G; }
-  static __device__ __forceinline__ int v_page(int tid = threadIdx.x) {
-    return item(tid) / (D / 2);
+  // First token of the page that the lane's items lie in, of K and of V: one page a wave,
+  // or (HALF) one for each half of it.
+  static __device__ __forceinline__ int page_row(int tid = threadIdx.x) {
+    const int x = item(tid) / (D / 2) * 16;
+    return HALF ? x : __builtin_amdgcn_readfirstlane(x);
   }
   __device__ __forceinline__ bool good(int32_t id) const { return id >= 0 && id < a.pool_pages; }
-  __device__ __forceinline__ void start(int seq, int h, int e) {
+  __device__ __forceinline__ void start(int seq, int h, int t0, int e) {
     table = a.block_tables + seq * a.bt_stride;
     head = h;
     end = e;
+    id = opaque(threadIdx.x);
+    k_id = -1;
+    if (e > 0) look_up(t0);
   }
-  // The page of the lane's items, those of the wave's first at t: one page a wave, or (HALF)
-  // one for each half of it.  -1 outside the context.
-  __device__ __forceinline__ int32_t page(int t) const {
-    auto at = [&](int x) { return x >= 0 && x < end ? scalar_load(table, x / 16) : -1; };
-    if constexpr (!HALF) return __builtin_amdgcn_readfirstlane(at(t));
-    return threadIdx.x & 32 ? at(t + 16) : at(t);
+  // As for a cache.
+  __device__ __forceinline__ void look_up(int t0) {
+    ahead = table[opaque(min(t0 + page_row(), end - 1) / 16)];
   }
+  __device__ __forceinline__ int64_t block(int32_t id) const {
+    int32_t x = good(id) ? id : 0;
+    if constexpr (!HALF) x = __builtin_amdgcn_readfirstlane(x);
+    return (int64_t)x * a.num_kv_heads + head;
+  }
+  template <bool KEEP>
   __device__ __forceinline__ void next(int t0) {
-    kr = vr = vs[0] = vs[1] = u32x4{0, 0, 0, 0};
-    ks = 0;
-    bad = 0;
-    const uint32_t i = item();
-    if (has_k()) {
-      const int32_t id = page(t0 + __builtin_amdgcn_readfirstlane(k_row()) / 16 * 16);
-      const bool ok = good(id);
-      bad = !ok && t0 + k_row() < end;
-      if (HALF || ok) {
-        // K items of a (page, head) block follow each other; where it is none, page 0
-        const int64_t block = (int64_t)(ok ? id : 0) * a.num_kv_heads + head;
-        const uint32_t at = i % (16 * G);
-        kr = *reinterpret_cast<const u32x4*>(a.k + block * 8 * D + 16 * at);
-        ks = a.kp[block * 16 * G + at];
-      }
+    const int tid = thread<KEEP>(id);
+    const uint32_t i = item(tid);
+    const int32_t v_id = k_id;
+    k_id = t0 + page_row(tid) < end ? ahead : -1;
+    look_up(t0 + BT);
+    bad = !good(k_id) && t0 + k_row(tid) < end;
+    none = !good(v_id);
+    if (has_k()) {  // items of a (page, head) block follow each other
+      const int64_t b = block(k_id);
+      const uint32_t at = i % (16 * G);
+      kr = *reinterpret_cast<const u32x4*>(a.k + b * 8 * D + 16 * at);
+      ks = (a.kp + b * 16 * G)[at];
     }
     if (has_v()) {
-      const int32_t id = page(t0 - BT + 16 * __builtin_amdgcn_readfirstlane(v_page()));
-      const bool ok = good(id);
-      if (HALF || ok) {
-        const int64_t block = (int64_t)(ok ? id : 0) * a.num_kv_heads + head;
-        const uint32_t x = i % (D / 2), q = x / 16 * 4 + x / 2 % 2 * 2;
-        vr = *reinterpret_cast<const u32x4*>(a.v + block * 8 * D + 16 * x);
-        const u32x4* p = reinterpret_cast<const u32x4*>(a.vp + block * 16 * G);
-        vs[0] = p[q];
-        vs[1] = p[q + 1];
-        if constexpr (HALF)
-#pragma unroll
-          for (int w = 0; w < 4; ++w) {  // scale and zero of a page that is none: zeros
-            vs[0][w] = ok ? vs[0][w] : 0;
-            vs[1][w] = ok ? vs[1][w] : 0;
-          }
-      }
+      const int64_t b = block(v_id);
+      const uint32_t x = i % (D / 2), q = x / 16 * 4 + x / 2 % 2 * 2;
+      vr = *reinterpret_cast<const u32x4*>(a.v + b * 8 * D + 16 * x);
+      const u32x4* p = reinterpret_cast<const u32x4*>(a.vp + b * 16 * G);
+      vs[0] = p[q];
+      vs[1] = p[q + 1];
     }
   }
-  // The 8 nibbles of w as fp32 values, in order.
-  static __device__ __forceinline__ void nibbles(uint32_t w, float* x) {
-    uint32_t ev = w & 0x0F0F0F0Fu, od = (w >> 4) & 0x0F0F0F0Fu;
-    asm("" : "+v"(ev));
-    asm("" : "+v"(od));
+  // Codes as fp16 numbers, two an instruction: a code u in the low bits of an fp16 is
+  // u 2^-24, four bits further u 2^-20, and its scale comes 2^24 or 2^20 times as large.
+  // c[i]: codes i and 4 + i of w, at i odd four bits further.
+  static __device__ __forceinline__ void codes(uint32_t w, uint32_t (&c)[4]) {
+    const uint32_t x = w >> 8;
+    c[0] = w & 0x000F000Fu;
+    c[1] = w & 0x00F000F0u;
+    c[2] = x & 0x000F000Fu;
+    c[3] = x & 0x00F000F0u;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[2 * i] = (float)((ev >> (8 * i)) & 0xFFu);
-      x[2 * i + 1] = (float)((od >> (8 * i)) & 0xFFu);
-    }
+    for (int i = 0; i < 4; ++i) asm("" : "+v"(c[i]));
   }
-  // u * s is exact (4 bits by 11), so the fma rounds as the codec's multiply and add.
+  static constexpr float unit(int i) { return i % 2 ? 0x1p20f : 0x1p24f; }
+  // Code i of c.  The product with its scale is exact (4 bits by 11), so the fma rounds as the
+  // codec's multiply and add.
+  static __device__ __forceinline__ float value(const uint32_t (&c)[4], int i, float s,
+                                                float z) {
+    const f16x2_t u = __builtin_bit_cast(f16x2_t, c[i % 4]);
+    return __builtin_fmaf((float)u[i / 4], s, z);
+  }
+  template <bool KEEP>
   __device__ __forceinline__ void store_k(int, uint8_t* lds, uint32_t* marks) const {
     if (!has_k()) return;
-    const int tid = opaque(threadIdx.x);
+    const int tid = thread<KEEP>(id);
     if (__any(bad)) mark_row(marks, k_row(tid), bad);
-    const float s = param_scale(ks), z = param_zero(ks);
+    const float z = param_zero(ks), s[2] = {param_scale(ks) * unit(0), param_scale(ks) * unit(1)};
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      float x[8];
-      nibbles(kr[w], x);
+      uint32_t c[4];
+      codes(kr[w], c);
       u32x4 y;
 #pragma unroll
       for (int n = 0; n < 4; ++n)
-        y[n] = pair16<QT>(__builtin_fmaf(x[2 * n], s, z), __builtin_fmaf(x[2 * n + 1], s, z));
+        y[n] = pair16<QT>(value(c, 2 * n, s[0], z), value(c, 2 * n + 1, s[1], z));
       *reinterpret_cast<u32x4*>(lds + k_place<D>(k_row(tid), 4 * (item(tid) % G) + w)) = y;
     }
   }
+  template <bool KEEP>
   __device__ __forceinline__ void store_v(int t0, uint8_t* lds, bool check,
                                           uint32_t* wild) const {
     if (!has_v()) return;
-    const int tid = opaque(threadIdx.x), c = item(tid) % (D / 2);
-    const int r0 = 16 * v_page(tid) + c / 2 % 2 * 8;
-    float x[4][8];
-    uint32_t y[16];
+    const int tid = thread<KEEP>(id), c = item(tid) % (D / 2);
+    const int r0 = item(tid) / (D / 2) * 16 + c / 2 % 2 * 8;
+    uint32_t x[4][4], y[16];
 #pragma unroll
-    for (int d = 0; d < 4; ++d) nibbles(vr[d], x[d]);
+    for (int d = 0; d < 4; ++d) codes(vr[d], x[d]);
 #pragma unroll
     for (int t = 0; t < 8; ++t) {
       const uint32_t p = vs[t / 4][t % 4];
-      const float s = param_scale(p), z = param_zero(p);
-      y[2 * t] = pair16<QT>(__builtin_fmaf(x[0][t], s, z), __builtin_fmaf(x[1][t], s, z));
-      y[2 * t + 1] = pair16<QT>(__builtin_fmaf(x[2][t], s, z), __builtin_fmaf(x[3][t], s, z));
+      const float s = param_scale(p) * unit(t), z = param_zero(p);
+      y[2 * t] = pair16<QT>(value(x[0], t, s, z), value(x[1], t, s, z));
+      y[2 * t + 1] = pair16<QT>(value(x[2], t, s, z), value(x[3], t, s, z));
     }
-    if (check) {
+    if (check || __any(none)) {
 #pragma unroll
-      for (int t = 0; t < 16; ++t) y[t] = t0 + r0 + t / 2 < end ? y[t] : 0u;
+      for (int t = 0; t < 16; ++t) y[t] = !none && t0 + r0 + t / 2 < end ? y[t] : 0u;
       const bool found = clean<VT>(y);
       mark_row(wild, 0, found);
     }

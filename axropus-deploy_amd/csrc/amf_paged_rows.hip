@@ -30,6 +30,7 @@
 // FP8 one, whose values fp16 holds exactly; three bf16 terms would cost twice the
 // matrix time of the whole for bits that the result's type drops.
 #include <algorithm>
+#include <type_traits>
 
 #include "amf_paged_rows.h"
 
@@ -51,7 +52,7 @@ constexpr int kRows = 32 * kWaves;  // columns of a workgroup
 constexpr int kMaxDim = 256;
 constexpr int kMaxShares = 512;     // two workgroups a CU
 constexpr int kMinShare = 256;      // tokens
-constexpr int kTileCost = 64;       // tokens' worth of a tile's beginning and end, >= BT
+constexpr int kTileCost = 256;      // tokens' worth of a tile's beginning and end, >= BT
 constexpr int kMaxContext = 1 << 30;
 
 // ---- sequences and shares ------------------------------------------------------
@@ -185,8 +186,6 @@ template <int QT, int KV, int D>
 __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void rows_kernel(RowsArgs a) {
   using Move = Mover<QT, KV, D>;
   constexpr int BT = Move::BT, VT = Move::VT, RB = 2 * D;
-  // products of K and q with a tile's 32 tokens, of all of them; V fragments, and products
-  constexpr int KS = D / 16, QN = BT / 32 * KS, DN = D / 32, PN = BT / 16 * DN;
   // Two buffers each: while the values of a tile and the keys of the next are multiplied,
   // the next values and the keys after are on their way, with one barrier a tile.
   constexpr int TB = BT * RB;
@@ -249,34 +248,43 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void rows_kernel(RowsAr
     const int hi = (int)min(sh.end - start, (int64_t)length);
     const int t_lo = min(e, lo / BT * BT);
     const int t_hi = hi == length ? e : min(e, hi / BT * BT);
-    if (begins || t_lo < e) {
-      const int cols = rows * G;
-      const int col = wave * 32 + lc;
+    const int cols = rows * G;
+    // CG groups of 32 columns.  With fewer groups than waves, several waves work on one:
+    // TS of them on 32 tokens of a tile each, DS on parts of V's dims.
+    auto piece = [&](auto groups) __attribute__((always_inline)) {
+      constexpr int CG = decltype(groups)::value, NW = kWaves / CG;
+      constexpr bool KEEP = CG < kWaves;
+      constexpr int TS = NW < BT / 32 ? NW : BT / 32, DS = NW / TS;
+      constexpr int NB = BT / 32 / TS, DN = D / 32 / DS;  // a wave's blocks of 32: tokens, dims
+      // its products of K and q of 32 tokens, and of all; of V
+      constexpr int KS = D / 16, QN = NB * KS, PN = 2 * NB * DN;
+      const int cg = wave % CG, tok = wave / CG % TS * 32, dim = wave / CG / TS * DN * 32;
+      const uint32_t k_wave = k_at + tok * RB, v_wave = (v_at ^ (2 * dim)) + tok * RB;
+      const int col = cg * 32 + lc;
       const int qi = min(col, cols - 1) / G;
       const int qh = head * G + min(col, cols - 1) - qi * G;
       const int qrow = sq.row0 + row_lo + qi;
-      const bool wave_on = wave * 32 < cols;
-      const int wave_first = wave * 32 / G;                         // rows of the wave
-      const int wave_last = (min(wave * 32 + 32, cols) - 1) / G;
-      u32x4 qb[D / 16];  // B operand: dims 16 ks + 8 h .. + 7
+      const bool wave_on = cg * 32 < cols;
+      const int wave_first = cg * 32 / G;  // the wave's first row
+      u32x4 qb[KS];  // B operand: dims 16 ks + 8 h .. + 7
       {
         const uint8_t* qp = a.q + qrow * a.q_row + qh * a.q_head + 16 * h;
 #pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks)
+        for (int ks = 0; ks < KS; ++ks)
           qb[ks] = *reinterpret_cast<const u32x4*>(qp + 32 * ks);
       }
       // the row's last token
       const int last = min(pos0 + qi, t_hi - 1);
       float m_run = -INFINITY, l_run = 0.0f;  // l_run: this lane's tokens
       bool seen = false;                      // a token that the row attends to
-      f32x16 acc[D / 32], s[BT / 32];
+      f32x16 acc[DN], s[NB];
 #pragma unroll
-      for (int d = 0; d < D / 32; ++d)
+      for (int d = 0; d < DN; ++d)
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[d][i] = 0.0f;
 
       const int n = (t_hi - t_lo + BT - 1) / BT;  // tiles
-      mv.start(seq, head, t_hi);
+      mv.start(seq, head, t_lo, t_hi);
       __syncthreads();  // the last piece's marks have been read
       marks[tid & 3][tid >> 2 & 1] = 0;
       __syncthreads();
@@ -286,36 +294,47 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void rows_kernel(RowsAr
       auto move = [&](int i) __attribute__((always_inline)) {
         const int t2 = t_lo + (i + 2) * BT, t1 = t2 - BT;
         marks[m1][tid & 1] = 0;
-        if (i + 2 < n) mv.store_k(t2, k_lds + (i & 1) * TB, marks[m0]);
-        if (i >= -1 && i + 1 < n) {
-          // tokens that some rows see and others do not: V has to be finite there, as
-          // 0 * inf is not 0
-          mv.store_v(t1, v_lds + (i + 1 & 1) * TB, t1 + BT > pos0 + 1, marks[3]);
+        // tokens that some rows see and others do not: V has to be finite there, as
+        // 0 * inf is not 0
+        const bool check = t1 + BT > pos0 + 1;
+        uint8_t *k_to = k_lds + (i & 1) * TB, *v_to = v_lds + (i + 1 & 1) * TB;
+        const bool more_k = i + 2 < n, more_v = i >= -1 && i + 1 < n;
+        if constexpr (Move::kInRegisters) {
+          const Move now = mv;
+          mv.template next<KEEP>(t2 + BT);
+          if (more_k) now.template store_k<KEEP>(t2, k_to, marks[m0]);
+          if (more_v) now.template store_v<KEEP>(t1, v_to, check, marks[3]);
+        } else {
+          if (more_k) mv.template store_k<KEEP>(t2, k_to, marks[m0]);
+          if (more_v) mv.template store_v<KEEP>(t1, v_to, check, marks[3]);
+          if (more_k) mv.template next<KEEP>(t2 + BT);
         }
-        if (i + 2 < n) mv.next(t2 + BT);
         const int m = m2;
         m2 = m0;
         m0 = m1;
         m1 = m;
       };
       // K fragment q of a tile: dims 16 (q % KS) .. of tokens 32 (q / KS) ..
-      auto read_k = [](uint32_t at, int q) __attribute__((always_inline)) {
+      auto read_k = [&](uint32_t at, int q) __attribute__((always_inline)) {
         return *(const lds_u32x4*)((at ^ (32 * (q % KS))) + 32 * (q / KS) * RB);
       };
       // Whether tile i holds tokens that some of the wave's rows do not see; then they
-      // are hidden.  Token of score element e of block tb: t0 + 32 tb + 8 (e / 4) + 4 h + e % 4.
+      // are hidden.  Token of score element e of block tb: t0 + tok + 32 tb + 8 (e / 4) + 4 h
+      // + e % 4.
       auto hide = [&](int i) __attribute__((always_inline)) {
         const int t0 = t_lo + i * BT;
-        const uint32_t bad[2] = {(uint32_t)__builtin_amdgcn_readfirstlane(marks[m1][0]),
-                                 (uint32_t)__builtin_amdgcn_readfirstlane(marks[m1][1])};
-        if (t0 + BT <= t_hi && t0 + BT - 1 <= pos0 + wave_first && !(bad[0] | bad[1])) {
+        uint32_t bad[NB], any = 0;
+#pragma unroll
+        for (int tb = 0; tb < NB; ++tb)
+          any |= bad[tb] = __builtin_amdgcn_readfirstlane(marks[m1][tok / 32 + tb]);
+        if (t0 + BT <= t_hi && t0 + BT - 1 <= pos0 + wave_first && !any) {
           seen = true;
           return false;
         }
-        const int left = last - t0 - 4 * h;
-        bad_seen |= (bad[0] | bad[1]) != 0;
+        const int left = last - t0 - tok - 4 * h;
+        bad_seen |= any != 0;
 #pragma unroll
-        for (int tb = 0; tb < BT / 32; ++tb) {
+        for (int tb = 0; tb < NB; ++tb) {
           const uint32_t gone = opaque(bad[tb] >> (4 * h));  // no masks kept over the loop
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
@@ -330,7 +349,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void rows_kernel(RowsAr
       auto largest = [&]() __attribute__((always_inline)) {
         float x = -INFINITY;
 #pragma unroll
-        for (int tb = 0; tb < BT / 32; ++tb)
+        for (int tb = 0; tb < NB; ++tb)
 #pragma unroll
           for (int e = 0; e < 16; ++e) x = fmaxf(x, s[tb][e]);
         return x;
@@ -338,7 +357,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void rows_kernel(RowsAr
       auto scaled = [&](float x) { return max_of_halves(x) * c2 - weight_shift<VT>(); };
       float mx = -INFINITY;
       if (n > 0) {
-        mv.next(t_lo);
+        mv.template next<KEEP>(t_lo);
         for (int i = -2; i < (wave_on ? 0 : n); ++i) {
           move(i);
           if (wave_on && i == -1) {
@@ -347,12 +366,12 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void rows_kernel(RowsAr
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(qb[ks]));
 #pragma unroll
-            for (int tb = 0; tb < BT / 32; ++tb) {
+            for (int tb = 0; tb < NB; ++tb) {
 #pragma unroll
               for (int e = 0; e < 16; ++e) s[tb][e] = 0.0f;
 #pragma unroll
               for (int ks = 0; ks < KS; ++ks)
-                s[tb] = mfma32<QT>(read_k(k_at, tb * KS + ks), qb[ks], s[tb]);
+                s[tb] = mfma32<QT>(read_k(k_wave, tb * KS + ks), qb[ks], s[tb]);
             }
             hide(0);
             mx = scaled(largest());
@@ -370,15 +389,15 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void rows_kernel(RowsAr
           const float alpha = __builtin_amdgcn_exp2f(m_run - m_use);
           l_run *= alpha;
 #pragma unroll
-          for (int d = 0; d < D / 32; ++d)
+          for (int d = 0; d < DN; ++d)
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[d][e] *= alpha;
           m_run = m_new;
           bool over;
           do {
             move(i);
-            const uint32_t k_rd = k_at + (~i & 1) * TB, v_rd = v_at + (i & 1) * TB;
-            u32x4 pb[BT / 16];  // weights of 16 tokens each, 8 per lane
+            const uint32_t k_rd = k_wave + (~i & 1) * TB, v_rd = v_wave + (i & 1) * TB;
+            u32x4 pb[2 * NB];  // weights of 16 tokens each, 8 per lane
             float l2 = 0.0f;
             // weights of elements 2 e, 2 e + 1 of block tb
             auto weigh = [&](int tb, int e) __attribute__((always_inline)) {
@@ -408,7 +427,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void rows_kernel(RowsAr
                 for (int e = 0; e < 16; ++e) s[tb][e] = 0.0f;
               s[tb] = mfma32<QT>(kf[q % AHEAD], qb[ks], s[tb]);
               if (q + AHEAD < QN) kf[q % AHEAD] = read_k(k_rd, q + AHEAD);
-              if (tb + 1 < BT / 32)
+              if (tb + 1 < NB)
 #pragma unroll
                 for (int e = ks * 8 / KS; e < (ks + 1) * 8 / KS; ++e) weigh(tb + 1, e);
               else if (ks < DN)
@@ -420,10 +439,10 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void rows_kernel(RowsAr
             for (int p = 0; p < PN; ++p) {
               const int st = p / DN, d = p % DN;
               acc[d] = mfma32<VT>(vf[st & 1][d], pb[st], acc[d]);
-              if (st + 1 < BT / 16)
+              if (st + 1 < 2 * NB)
                 vf[(st + 1) & 1][d] = read_v((v_rd ^ (64 * d)) + 16 * (st + 1) * RB);
 #pragma unroll
-              for (int e = p * (BT / 2) / PN; e < (p + 1) * (BT / 2) / PN; ++e)
+              for (int e = p * (16 * NB) / PN; e < (p + 1) * (16 * NB) / PN; ++e)
                 big = fmaxf(big, s[e / 16][e % 16]);
               __builtin_amdgcn_sched_barrier(0);
             }
@@ -445,6 +464,36 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void rows_kernel(RowsAr
 
       float l = l_run + __shfl_xor(l_run, 32);
       seen |= __shfl_xor((int)seen, 32) != 0;
+      if constexpr (TS > 1) {  // the tokens' parts become one in the first of their waves
+        static_assert(TS == 2, "two parts");
+        f32x4* x = reinterpret_cast<f32x4*>(k_lds) + (cg + dim / 32 / DN * CG) * (DN * 256) + lane;
+        float* y = reinterpret_cast<float*>(v_lds) + (cg + dim / 32 / DN * CG) * 192 + lane;
+        if (tok) {
+#pragma unroll
+          for (int i = 0; i < 4 * DN; ++i)
+            x[64 * i] = f32x4{acc[i / 4][4 * (i % 4)], acc[i / 4][4 * (i % 4) + 1],
+                              acc[i / 4][4 * (i % 4) + 2], acc[i / 4][4 * (i % 4) + 3]};
+          y[0] = m_run;
+          y[64] = l;
+          y[128] = seen;
+        }
+        __syncthreads();
+        if (!tok) {
+          const float m = fmaxf(m_run, y[0]), m_use = m == -INFINITY ? 0.0f : m;
+          const float f0 = __builtin_amdgcn_exp2f(m_run - m_use);
+          const float f1 = __builtin_amdgcn_exp2f(y[0] - m_use);
+          l = l * f0 + y[64] * f1;
+          seen |= y[128] != 0.0f;
+          m_run = m;
+#pragma unroll
+          for (int i = 0; i < 4 * DN; ++i) {
+            const f32x4 o = x[64 * i];
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+              acc[i / 4][4 * (i % 4) + n] = acc[i / 4][4 * (i % 4) + n] * f0 + o[n] * f1;
+          }
+        }
+      }
       const bool whole = begins && t_hi == e;
       if (!whole && begins) {
         const int64_t reach = start + (e + BT - 1) / BT * BT - 1;
@@ -454,27 +503,27 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void rows_kernel(RowsAr
         cut.cols = cols;
         cut.head = head;
       }
-      if (col < cols) {
+      if (col < cols && tok == 0) {
         if (whole) {
           // no token: zeros; every score -inf: 0 / 0 = NaN, as softmax gives
           const float f = seen ? a.v_scale / l : 0.0f;
-          const int64_t o = ((int64_t)qrow * a.num_q_heads + qh) * D;
+          const int64_t o = ((int64_t)qrow * a.num_q_heads + qh) * D + dim;
 #pragma unroll
-          for (int d = 0; d < D / 32; ++d)
+          for (int d = 0; d < DN; ++d)
 #pragma unroll
             for (int n = 0; n < 4; ++n) {
               f32x4 x = {acc[d][4 * n], acc[d][4 * n + 1], acc[d][4 * n + 2], acc[d][4 * n + 3]};
               store4(a.out, QT, o + 32 * d + 8 * n + 4 * h, x * f);
             }
         } else {
-          float* p = a.part + ((sh.index * 2 + begins) * kRows + col) * (D + kPartPad);
+          float* p = a.part + ((sh.index * 2 + begins) * kRows + col) * (D + kPartPad) + dim;
 #pragma unroll
-          for (int d = 0; d < D / 32; ++d)
+          for (int d = 0; d < DN; ++d)
 #pragma unroll
             for (int n = 0; n < 4; ++n)
               *reinterpret_cast<f32x4*>(p + 32 * d + 8 * n + 4 * h) =
                   f32x4{acc[d][4 * n], acc[d][4 * n + 1], acc[d][4 * n + 2], acc[d][4 * n + 3]};
-          if (h == 0) {
+          if (h == 0 && dim == 0) {
             p[D] = m_run;
             p[D + 1] = seen && l == 0.0f ? -1.0f : l;  // -1: tokens, all of them -inf
           }
@@ -487,8 +536,8 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void rows_kernel(RowsAr
             if (!mv.there(t)) continue;
             float p = 0.0f;
             bool known = false;
-            for (int i = 0; i < D / 2; ++i) {  // the dims that this lane has stored
-              const int d = i / 4 * 8 + 4 * h + i % 4;
+            for (int i = 0; i < 16 * DN; ++i) {  // the dims that this lane has stored
+              const int d = dim + i / 4 * 8 + 4 * h + i % 4;
               const float v = mv.v_elem(t, d);
               if (fabsf(v) < INFINITY) continue;
               if (!known) {
@@ -509,6 +558,15 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void rows_kernel(RowsAr
           }
         }
       }
+    };
+    if (begins || t_lo < e) {
+      const int used = __builtin_amdgcn_readfirstlane(cols);
+      if (used > 64)
+        piece(std::integral_constant<int, 4>{});
+      else if (used > 32)
+        piece(std::integral_constant<int, 2>{});
+      else
+        piece(std::integral_constant<int, 1>{});
     }
     start += length;
     if (++j == sq.tiles) {
@@ -525,7 +583,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void rows_kernel(RowsAr
     }
   }
   if (tid == 0) a.cuts[blockIdx.x] = cut;
-  if (bad_seen && tid == 0 && a.err_flag) atomicOr(a.err_flag, AMF_ERRFLAG_BLOCK_RANGE);
+  if (bad_seen && lane == 0 && a.err_flag) atomicOr(a.err_flag, AMF_ERRFLAG_BLOCK_RANGE);
 }
 
 // out = v_scale sum_k f_k acc_k / sum_k f_k l_k, f_k = 2^(m_k - M), over the pieces of a
