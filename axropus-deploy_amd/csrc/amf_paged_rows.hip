@@ -51,8 +51,13 @@ constexpr int kThreads = kRowsThreads;
 constexpr int kRows = 32 * kWaves;  // columns of a workgroup
 constexpr int kMaxDim = 256;
 constexpr int kMaxShares = 512;     // two workgroups a CU
-constexpr int kMinShare = 256;      // tokens
-constexpr int kTileCost = 256;      // tokens' worth of a tile's beginning and end, >= BT
+// Lengths of tiles and shares: a token of a tile of more than 64 columns counts kWide,
+// of a narrower one, whose turns are bound by what they load beside others that are not,
+// kNarrow.
+constexpr int kWide = 4, kNarrow = 3;
+constexpr int kMinShare = 256 * kWide;
+constexpr int kTileCost = 256 * kWide;  // a tile's beginning and end; at least BT tokens
+constexpr int kCusXcd = 32;
 constexpr int kMaxContext = 1 << 30;
 
 // ---- sequences and shares ------------------------------------------------------
@@ -63,6 +68,7 @@ struct Seq {
   int lim;         // tokens that the block table holds of its context
   int base;        // pos0, or more where the table is too short, at least 0
   int tiles;
+  int weight;      // of a token of its tiles
 };
 
 __device__ __forceinline__ Seq get_seq(const RowsArgs& a, int s, int* flags) {
@@ -77,23 +83,29 @@ __device__ __forceinline__ Seq get_seq(const RowsArgs& a, int s, int* flags) {
   r.lim = min(ctx, cap);
   r.base = ctx > cap ? cap : max(r.pos0, 0);
   r.tiles = (r.rows + a.tile_rows - 1) / a.tile_rows;
+  r.weight = min(r.rows, a.tile_rows) * a.group > 64 ? kWide : kNarrow;
   if (!ok || (ctx > cap && r.rows > 0)) *flags |= AMF_ERRFLAG_CONTEXT;
   return r;
 }
 
-// Tile j is base + min((j + 1) tile_rows, rows) + kTileCost long.
+// Tile j is weight (base + min((j + 1) tile_rows, rows)) + kTileCost long.
 __device__ __forceinline__ int64_t tiles_before(const RowsArgs& a, const Seq& s, int64_t j) {
-  return j * ((int64_t)s.base + kTileCost) + a.tile_rows * (j * (j + 1) / 2);
+  return j * ((int64_t)s.weight * s.base + kTileCost) +
+         (int64_t)s.weight * a.tile_rows * (j * (j + 1) / 2);
 }
 __device__ __forceinline__ int64_t seq_length(const RowsArgs& a, const Seq& s) {
-  return s.tiles ? tiles_before(a, s, s.tiles - 1) + s.base + kTileCost + s.rows : 0;
+  return s.tiles ? tiles_before(a, s, s.tiles - 1) + s.weight * ((int64_t)s.base + s.rows) +
+                       kTileCost
+                 : 0;
 }
 
 struct Share {
-  int64_t index, length;  // of every share
+  int64_t index;
+  int64_t length;         // of every share
   int64_t first, end;     // of this one
   int64_t seq_start;      // where the sequence starts that `first` lies in
   int32_t head, seq;      // seq -1: nothing to do
+  bool young;             // not the first of its CU's workgroups
 };
 
 // The same in every thread; workgroup 0 flags.
@@ -124,6 +136,7 @@ __device__ __forceinline__ Share find_share(const RowsArgs& a) {
   if (slot >= per || r.index >= n) return r;
   r.first = r.index * r.length;
   r.end = min(all, r.first + r.length);
+  r.young = slot >= kCusXcd;
   r.head = (int32_t)(r.first / total);
   const int64_t at = r.first - r.head * total;
   if (a.num_seqs <= kThreads) {
@@ -240,14 +253,14 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void rows_kernel(RowsAr
     const int row_lo = j * a.tile_rows;
     const int rows = min(a.tile_rows, sq.rows - row_lo);
     const int pos0 = sq.pos0 + row_lo;  // position of the tile's first row
-    const int length = sq.base + row_lo + rows + kTileCost;
+    const int64_t length = (int64_t)sq.weight * (sq.base + row_lo + rows) + kTileCost;
     const int e = max(min(sq.lim, pos0 + rows), 0);
     // the share's part of [0, length)
     const bool begins = sh.first <= start;
-    const int lo = begins ? 0 : (int)(sh.first - start);
-    const int hi = (int)min(sh.end - start, (int64_t)length);
-    const int t_lo = min(e, lo / BT * BT);
-    const int t_hi = hi == length ? e : min(e, hi / BT * BT);
+    const int64_t lo = begins ? 0 : sh.first - start, hi = min(sh.end - start, length);
+    const int unit = sq.weight * BT;
+    const int t_lo = (int)min((int64_t)e, lo / unit * BT);
+    const int t_hi = hi == length ? e : (int)min((int64_t)e, hi / unit * BT);
     const int cols = rows * G;
     // CG groups of 32 columns.  With fewer groups than waves, several waves work on one:
     // TS of them on 32 tokens of a tile each, DS on parts of V's dims.
@@ -293,6 +306,12 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void rows_kernel(RowsAr
       int m0 = 0, m1 = 1, m2 = 2;  // marks of K tiles i + 2, i + 3, i + 1
       auto move = [&](int i) __attribute__((always_inline)) {
         const int t2 = t_lo + (i + 2) * BT, t1 = t2 - BT;
+        if (sh.young) {
+          if (i & 1)
+            __builtin_amdgcn_s_setprio(1);
+          else
+            __builtin_amdgcn_s_setprio(0);
+        }
         marks[m1][tid & 1] = 0;
         // tokens that some rows see and others do not: V has to be finite there, as
         // 0 * inf is not 0
@@ -496,7 +515,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void rows_kernel(RowsAr
       }
       const bool whole = begins && t_hi == e;
       if (!whole && begins) {
-        const int64_t reach = start + (e + BT - 1) / BT * BT - 1;
+        const int64_t reach = start + (int64_t)(e + BT - 1) / BT * unit - 1;
         cut.more = (int32_t)(reach / sh.length - sh.index);
         cut.share = (int32_t)sh.index;
         cut.row0 = sq.row0 + row_lo;
@@ -842,10 +861,13 @@ void finish_args(RowsArgs* a, void* workspace, float softmax_scale, float k_scal
   a->score_scale = scale * k_scale * kLog2e;
   // shares of kMinShare that the longest contexts of the tables could fill
   const int64_t tiles = a->n_rows / a->tile_rows + std::min<int64_t>(a->num_seqs, a->n_rows);
-  const int64_t cap = (int64_t)a->table_pages * a->block_size + a->tile_rows + kTileCost;
+  const int64_t cap =
+      kWide * ((int64_t)a->table_pages * a->block_size + a->tile_rows) + kTileCost;
+  // a workgroup's registers and LDS: two to a CU, at the largest head_dim one
+  const int64_t fit = a->head_dim == 256 ? kMaxShares / 2 : kMaxShares;
   const int64_t most = (tiles * a->num_kv_heads * cap + kMinShare - 1) / kMinShare;
   // whole rounds of the XCDs
-  a->shares = (int)std::min<int64_t>(kMaxShares, (most + kXcds - 1) / kXcds * kXcds);
+  a->shares = (int)std::min<int64_t>(fit, (most + kXcds - 1) / kXcds * kXcds);
   a->cuts = static_cast<Cut*>(workspace);
   a->part = reinterpret_cast<float*>(a->cuts + kMaxShares);
 }
