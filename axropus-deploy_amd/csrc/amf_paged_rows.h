@@ -43,6 +43,7 @@ struct RowsArgs {
   const uint32_t* vp;
   int64_t page_stride, token_stride, head_stride;  // bytes
   int64_t pool_pages;
+  uint32_t pages;  // pool_pages, or 2^31: every id from 0 on
   const int32_t* block_tables;
   int64_t bt_stride;
   int32_t table_pages;
@@ -93,12 +94,6 @@ __device__ __forceinline__ uint32_t pair16(float a, float b) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), f16x2_t));
 }
 
-// Read by the scalar unit: nothing that a launch writes.
-typedef const __attribute__((address_space(4))) int32_t scalar_i32;
-__device__ __forceinline__ int32_t scalar_load(const int32_t* p, int i) {
-  return ((scalar_i32*)(uintptr_t)p)[i];
-}
-
 // Sets values that are not finite to 0; whether there were any.
 template <int T, int N>
 __device__ __forceinline__ bool clean(uint32_t (&v)[N]) {
@@ -140,7 +135,8 @@ __device__ __forceinline__ void mark_row(uint32_t* marks, int r, bool is) {
 // (they are hidden), V rows zeros.  Rows whose page is none are marked by store_k, and
 // are zeros in V.  check: V values that are not finite become 0, *wild != 0 then.
 //
-// KEEP: there are registers for addresses.  Branches in next() and the stores are the same for all lanes of a wave, or select.
+// KEEP: there are registers for addresses.  Branches in next() and the stores are the same
+// for all lanes of a wave, or select.
 
 // What movers of caches (EB bytes an element) share.  Wave w of the workgroup takes rows
 // RPW w .. of a tile, which lie in one aligned group of 16: with pages of 16, 32, 64 ..
@@ -148,7 +144,7 @@ __device__ __forceinline__ void mark_row(uint32_t* marks, int r, bool is) {
 // rows spread over the tile's pages each looked up them all: 420 scalar instructions
 // a tile, which the CU's one scalar unit takes longer for than the matrix cores for the
 // products.)  A lane takes 16 bytes of a row, CH rows RPI apart.
-template <int EB, int D>
+template <int EB, int D, bool BY16>
 struct CacheMover {
   static constexpr int BT = tile_tokens(D);
   static constexpr int CPR = D * EB / 16;          // 16-byte chunks of a row
@@ -164,6 +160,7 @@ struct CacheMover {
   const uint8_t *kb, *vb;  // the KV head's
   int32_t k_id, v_id;      // by16: pages of the wave's rows; -1 behind `end`
   uint32_t k_off, v_off;   // and their place, in units of 16 bytes
+  int32_t ahead;           // by16: the table's entry for the tile after K's
 
   __device__ __forceinline__ CacheMover(const RowsArgs& args) : a(args) {}
   static __device__ __forceinline__ int wave_row() {
@@ -175,7 +172,7 @@ struct CacheMover {
   static __device__ __forceinline__ int row(int i, int tid = threadIdx.x) {
     return tid / 64 * RPW + lane_row(i, tid);
   }
-  __device__ __forceinline__ bool good(int32_t id) const { return id >= 0 && id < a.pool_pages; }
+  __device__ __forceinline__ bool good(int32_t id) const { return (uint32_t)id < a.pages; }
   // Byte offset of token t's row in page id, of any block size.
   __device__ __forceinline__ int page_of(int t) const {
     return (int)((uint32_t)t / (uint32_t)a.block_size);
@@ -183,7 +180,7 @@ struct CacheMover {
   __device__ __forceinline__ int64_t place(int32_t id, int t) const {
     return id * a.page_stride + (t - page_of(t) * a.block_size) * a.token_stride;
   }
-  __device__ __forceinline__ void start(int seq, int head, int, int e) {
+  __device__ __forceinline__ void start(int seq, int head, int t0, int e) {
     table = a.block_tables + seq * a.bt_stride;
     end = e;
     id = opaque(threadIdx.x);
@@ -191,13 +188,22 @@ struct CacheMover {
     vb = a.v + head * a.head_stride;
     k_id = -1;
     k_off = 0;
+    if (BY16 && e > 0) look_up(t0);
   }
-  __device__ __forceinline__ void found(int t0, int32_t id) {
+  // by16: goes on to the K tile at t0.  The table's entry was asked for a turn before, as
+  // the tile's loads depend on it, by a vector load: reads of LDS behind a scalar one
+  // wait for it.
+  __device__ __forceinline__ void advance(int t0) {
     v_id = k_id;
     v_off = k_off;
     const int t = t0 + wave_row();
-    k_id = __builtin_amdgcn_readfirstlane(t < end ? id : -1);
-    k_off = (uint32_t)k_id * a.page_units + (uint32_t)(t & (a.block_size - 1)) * a.token_units;
+    const int32_t page = __builtin_amdgcn_readfirstlane(ahead);
+    k_id = t < end ? page : -1;
+    k_off = (uint32_t)page * a.page_units + (uint32_t)(t & (a.block_size - 1)) * a.token_units;
+    look_up(t0 + BT);
+  }
+  __device__ __forceinline__ void look_up(int t0) {
+    ahead = table[opaque(min(t0 + wave_row(), end - 1) >> a.block_shift)];
   }
   // The wave's rows behind `off`, and a lane's bytes of row i behind that.
   static __device__ __forceinline__ const uint8_t* base(const uint8_t* plane, uint32_t off) {
@@ -227,75 +233,71 @@ struct CacheMover {
 };
 
 // 16-bit rows go to LDS directly (no registers; a lane's 16 bytes land at its place, so
-// it loads the chunk that belongs there); V rows that need a check, and pages of other
-// sizes, pass through registers.
-template <int QT, int KV, int D>
-struct Mover : CacheMover<2, D> {
-  using Base = CacheMover<2, D>;
+// it loads the chunk that belongs there), in kParts loads that the caller spreads over its
+// products: all at once they hold up the wave, as the CU takes 16 cycles for each.  They
+// are issued for tiles and pages that are not there as well, from page 0, and what they
+// bring is hidden or made zeros.  Pages of other sizes pass through registers.
+template <int QT, int KV, int D, bool BY16>
+struct Mover : CacheMover<2, D, BY16> {
+  using Base = CacheMover<2, D, BY16>;
   using Base::a, Base::id, Base::row, Base::end, Base::kb, Base::vb, Base::k_id, Base::v_id;
-  static constexpr int VT = QT, BT = Base::BT;
+  static constexpr int VT = QT, BT = Base::BT, CH = Base::CH, RB = 2 * D;
   static constexpr bool kInRegisters = false;
+  static constexpr int kParts = 2 * CH;
+
+  uint32_t row_off, k_chunk, v_chunk;  // of the lane's bytes of row(0)
+  const uint8_t *k_src, *v_src;        // the wave's rows
+  uint32_t k_dst, v_dst;
+  // V rows of this wave that are to be looked at when they are there.
+  bool look;
+  int look_t;
 
   __device__ __forceinline__ Mover(const RowsArgs& args) : Base(args), look(false) {}
-  template <bool KEEP>
-  __device__ __forceinline__ void next(int t0) {
-    const int t = t0 + Base::wave_row();
-    if (a.by16) this->found(t0, t < end ? scalar_load(this->table, t >> a.block_shift) : -1);
+  __device__ __forceinline__ void start(int seq, int head, int t0, int e) {
+    Base::start(seq, head, t0, e);
+    const int r = row(0, id), c = id % Base::CPR;
+    row_off = (Base::lane_row(0, id) * a.token_units) << 4;
+    k_chunk = (c ^ k_swizzle<D>(r)) << 4;
+    v_chunk = (c ^ v_swizzle<D>(r)) << 4;
   }
-  // 16 bytes of each lane, at base + off, to 16 lane bytes behind `lds`.  In assembly, as
+  // 16 bytes of each lane, at base + off, to 16 lane bytes behind `lds` + further.  In
+  // assembly, as
   // the compiler waits for all loads in flight before LDS reads that it cannot tell from
   // what they write; settle() does that.
   static __device__ __forceinline__ void load_lds(const uint8_t* base, uint32_t off,
-                                                  uint8_t* lds) {
-    const uint32_t at = __builtin_amdgcn_readfirstlane(lds_address(lds));
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
-                 : : "v"(off), "s"(base), "s"(at) : "memory", "m0");
+                                                  uint32_t lds, int further) {
+    asm volatile("s_add_u32 m0, %2, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+                 : : "v"(off), "s"(base), "s"(lds), "i"(further) : "memory", "m0", "scc");
   }
-  // What store_v() has left to be looked at, once it is there: rows of this wave.
-  bool look;
-  int look_t;
-  uint8_t* look_lds;
-  __device__ __forceinline__ void settle(uint32_t* wild) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    if (!look) return;
-    look = false;
-    const int tid = opaque(threadIdx.x);
-    const bool ok = this->good(__builtin_amdgcn_readfirstlane(look_page));
-    uint8_t* p = look_lds + Base::wave_row() * 2 * D + tid % 64 * 16;
-    bool found = false;
-#pragma unroll
-    for (int i = 0; i < Base::CH; ++i) {
-      const bool in = ok && look_t + row(i, tid) < end;
-      const u32x4 x = *reinterpret_cast<const u32x4*>(p + i * 1024);
-      uint32_t w[4] = {in ? x[0] : 0u, in ? x[1] : 0u, in ? x[2] : 0u, in ? x[3] : 0u};
-      found |= clean<VT>(w);
-      *reinterpret_cast<u32x4*>(p + i * 1024) = u32x4{w[0], w[1], w[2], w[3]};
-    }
-    mark_row(wild, 0, found);
-  }
-  int32_t look_page;
   template <bool KEEP>
-  __device__ __forceinline__ void store_k(int t0, uint8_t* lds, uint32_t* bad) const {
-    if (a.by16) {
+  __device__ __forceinline__ void next(int t0) {
+    if (BY16) this->advance(t0);
+  }
+  // Part p: the wave's K rows, then its V rows, from row(p) on.
+  __device__ __forceinline__ void part(int p) const {
+    if (!BY16) return;
+    const int i = p % CH;  // rows RPI i further on: bits of the swizzles of their own
+    const uint8_t* src = (p < CH ? k_src : v_src) + (uint32_t)(i * Base::RPI * 16) * a.token_units;
+    const uint32_t chunk = p < CH ? k_chunk ^ k_swizzle<D>(i * Base::RPI) << 4
+                                  : v_chunk ^ v_swizzle<D>(i * Base::RPI) << 4;
+    load_lds(src, chunk + row_off, p < CH ? k_dst : v_dst, i * Base::RPI * RB);
+  }
+  template <bool KEEP>
+  __device__ __forceinline__ void store_k(int t0, uint8_t* lds, bool wanted, uint32_t* bad) {
+    if (BY16) {
       const int32_t page = __builtin_amdgcn_readfirstlane(k_id);
       const int wr = Base::wave_row();
-      if (this->good(page)) {
-        const uint8_t* b = Base::base(kb, this->k_off);
-        // (offsets made here, not kept in registers over the loop)
-        const int tid = thread<KEEP>(id), c = tid % Base::CPR;
-#pragma unroll
-        for (int i = 0; i < Base::CH; ++i)
-          load_lds(b, this->lane_off(i, c ^ k_swizzle<D>(row(i, tid)), tid),
-                   lds + (wr + i * Base::RPI) * 2 * D);
-      } else if (t0 + wr < end) {
-#pragma unroll
-        for (int i = 0; i < Base::CH; ++i) mark_row(bad, row(i, thread<KEEP>(id)), true);
-      }
+      const bool ok = this->good(page);
+      k_src = Base::base(kb, ok ? this->k_off : 0u);
+      k_dst = __builtin_amdgcn_readfirstlane(lds_address(lds) + wr * RB);
+      if (wanted && !ok && t0 + wr < end)
+        for (int i = 0; i < CH; ++i) mark_row(bad, row(i, opaque(threadIdx.x)), true);
       return;
     }
+    if (!wanted) return;
     const int tid = thread<KEEP>(id), c = tid % Base::CPR;
 #pragma unroll 1
-    for (int i = 0; i < Base::CH; ++i) {
+    for (int i = 0; i < CH; ++i) {
       const int r = row(i, tid);
       bool none;
       const u32x4 k = this->lane_row_of(kb, t0 + r, 16 * c, &none);
@@ -304,26 +306,20 @@ struct Mover : CacheMover<2, D> {
     }
   }
   template <bool KEEP>
-  __device__ __forceinline__ void store_v(int t0, uint8_t* lds, bool check, uint32_t* wild) {
-    if (a.by16) {
-      const int32_t page = __builtin_amdgcn_readfirstlane(v_id);
-      const int wr = Base::wave_row();
-      look = check || !this->good(page) || t0 + BT > end;
-      look_t = t0;
-      look_lds = lds;
-      look_page = page;
-      if (!this->good(page)) return;
-      const uint8_t* b = Base::base(vb, this->v_off);
-      const int tid = thread<KEEP>(id), c = tid % Base::CPR;
-#pragma unroll
-      for (int i = 0; i < Base::CH; ++i)
-        load_lds(b, this->lane_off(i, c ^ v_swizzle<D>(row(i, tid)), tid),
-                 lds + (wr + i * Base::RPI) * 2 * D);
+  __device__ __forceinline__ void store_v(int t0, uint8_t* lds, bool wanted, bool check,
+                                          uint32_t* wild) {
+    if (BY16) {
+      const bool ok = this->good(__builtin_amdgcn_readfirstlane(v_id));
+      look = wanted && (check || !ok || t0 + BT > end);
+      look_t = ok ? t0 : end;
+      v_src = Base::base(vb, ok ? this->v_off : 0u);
+      v_dst = __builtin_amdgcn_readfirstlane(lds_address(lds) + Base::wave_row() * RB);
       return;
     }
+    if (!wanted) return;
     const int tid = thread<KEEP>(id), c = tid % Base::CPR;
 #pragma unroll 1
-    for (int i = 0; i < Base::CH; ++i) {
+    for (int i = 0; i < CH; ++i) {
       const int r = row(i, tid);
       bool none;
       const u32x4 x = this->lane_row_of(vb, t0 + r, 16 * c, &none);
@@ -335,6 +331,23 @@ struct Mover : CacheMover<2, D> {
       *reinterpret_cast<u32x4*>(lds + v_place<D>(r, c)) = u32x4{w[0], w[1], w[2], w[3]};
     }
   }
+  __device__ __forceinline__ void settle(uint32_t* wild) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if (!look) return;
+    look = false;
+    const int tid = opaque(threadIdx.x);
+    lds_u32x4* p = (lds_u32x4*)(v_dst + tid % 64 * 16);
+    bool found = false;
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      const bool in = look_t + row(i, tid) < end;
+      const u32x4 x = p[64 * i];
+      uint32_t w[4] = {in ? x[0] : 0u, in ? x[1] : 0u, in ? x[2] : 0u, in ? x[3] : 0u};
+      found |= clean<VT>(w);
+      p[64 * i] = u32x4{w[0], w[1], w[2], w[3]};
+    }
+    mark_row(wild, 0, found);
+  }
   __device__ __forceinline__ float k_elem(int t, int d) const {
     return this->template elem<KV>(kb, t, d);
   }
@@ -345,36 +358,25 @@ struct Mover : CacheMover<2, D> {
 
 // FP8 rows: 16 values a chunk, converted on their way from registers to LDS.  V becomes
 // fp16, which holds its values exactly as bf16 does.
-template <int QT, int D>
-struct Mover<QT, AMF_DTYPE_E4M3, D> : CacheMover<1, D> {
-  using Base = CacheMover<1, D>;
+template <int QT, int D, bool BY16>
+struct Mover<QT, AMF_DTYPE_E4M3, D, BY16> : CacheMover<1, D, BY16> {
+  using Base = CacheMover<1, D, BY16>;
   using Base::a, Base::id, Base::row, Base::end, Base::kb, Base::vb, Base::k_id, Base::v_id;
   static constexpr int VT = AMF_DTYPE_F16, BT = Base::BT;
   static constexpr bool kInRegisters = true;
   u32x4 kr[Base::CH], vr[Base::CH];
   int bad;    // bits of the lane's K rows whose pages are none
   bool none;  // by16: no page for the wave's V rows
-  int32_t ahead;  // by16: the table's entry for the tile after K's
 
   __device__ __forceinline__ Mover(const RowsArgs& args) : Base(args) {}
   static __device__ __forceinline__ void settle(uint32_t*) {}
-  __device__ __forceinline__ void start(int seq, int head, int t0, int e) {
-    Base::start(seq, head, t0, e);
-    if (a.by16 && e > 0) look_up(t0);
-  }
-  // The entry is asked for a turn before it is used, as the tile's loads depend on it.  A
-  // vector load: reads of LDS behind a scalar one wait for it.
-  __device__ __forceinline__ void look_up(int t0) {
-    ahead = this->table[opaque(min(t0 + Base::wave_row(), end - 1) >> a.block_shift)];
-  }
   // As many loads on every way, so that a wait for the tile before is not one for this.
   // Where no page is, any is read.
   template <bool KEEP>
   __device__ __forceinline__ void next(int t0) {
     bad = 0;
-    if (a.by16) {
-      this->found(t0, ahead);
-      look_up(t0 + BT);
+    if (BY16) {
+      this->advance(t0);
       const int32_t ki = __builtin_amdgcn_readfirstlane(k_id);
       const int32_t vi = __builtin_amdgcn_readfirstlane(v_id);
       const int tid = thread<KEEP>(id), c = tid % Base::CPR;
@@ -460,7 +462,7 @@ struct Mover<QT, AMF_DTYPE_E4M3, D> : CacheMover<1, D> {
 // by 8 tokens (16 bytes, 8 params), dequantised on their way from registers to LDS.  At
 // head_dim 64 half the threads move K, half V.
 template <int QT, int D>
-struct Mover<QT, kInt4, D> {
+struct Mover<QT, kInt4, D, true> {
   static constexpr int BT = tile_tokens(D);
   static constexpr int VT = QT, G = D / 32, N = BT * G;  // items of K, and of V
   static constexpr bool HALF = N * 2 == kRowsThreads;
@@ -495,7 +497,7 @@ struct Mover<QT, kInt4, D> {
     const int x = item(tid) / (D / 2) * 16;
     return HALF ? x : __builtin_amdgcn_readfirstlane(x);
   }
-  __device__ __forceinline__ bool good(int32_t id) const { return id >= 0 && id < a.pool_pages; }
+  __device__ __forceinline__ bool good(int32_t id) const { return (uint32_t)id < a.pages; }
   __device__ __forceinline__ void start(int seq, int h, int t0, int e) {
     table = a.block_tables + seq * a.bt_stride;
     head = h;

@@ -195,9 +195,9 @@ __device__ __forceinline__ float max_of_halves(float x) {
   return fmaxf(u2f(r[0]), u2f(r[1]));
 }
 
-template <int QT, int KV, int D>
+template <int QT, int KV, int D, bool BY16>
 __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void rows_kernel(RowsArgs a) {
-  using Move = Mover<QT, KV, D>;
+  using Move = Mover<QT, KV, D, BY16>;
   constexpr int BT = Move::BT, VT = Move::VT, RB = 2 * D;
   // Two buffers each: while the values of a tile and the keys of the next are multiplied,
   // the next values and the keys after are on their way, with one barrier a tile.
@@ -324,14 +324,19 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void rows_kernel(RowsAr
           if (more_k) now.template store_k<KEEP>(t2, k_to, marks[m0]);
           if (more_v) now.template store_v<KEEP>(t1, v_to, check, marks[3]);
         } else {
-          if (more_k) mv.template store_k<KEEP>(t2, k_to, marks[m0]);
-          if (more_v) mv.template store_v<KEEP>(t1, v_to, check, marks[3]);
-          if (more_k) mv.template next<KEEP>(t2 + BT);
+          mv.template next<KEEP>(t2);
+          mv.template store_k<KEEP>(t2, k_to, more_k, marks[m0]);
+          mv.template store_v<KEEP>(t1, v_to, more_v, check, marks[3]);
         }
         const int m = m2;
         m2 = m0;
         m0 = m1;
         m1 = m;
+      };
+      // What of move() is spread: every second of 2 kParts calls issues a load.
+      auto load = [&](int p) __attribute__((always_inline)) {
+        if constexpr (!Move::kInRegisters)
+          if (p % 2 == 0 && p / 2 < Move::kParts) mv.part(p / 2);
       };
       // K fragment q of a tile: dims 16 (q % KS) .. of tokens 32 (q / KS) ..
       auto read_k = [&](uint32_t at, int q) __attribute__((always_inline)) {
@@ -340,12 +345,16 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void rows_kernel(RowsAr
       // Whether tile i holds tokens that some of the wave's rows do not see; then they
       // are hidden.  Token of score element e of block tb: t0 + tok + 32 tb + 8 (e / 4) + 4 h
       // + e % 4.
-      auto hide = [&](int i) __attribute__((always_inline)) {
+      auto get_marks = [&](uint32_t(&x)[NB]) __attribute__((always_inline)) {  // m1's
+#pragma unroll
+        for (int tb = 0; tb < NB; ++tb) x[tb] = marks[m1][tok / 32 + tb];
+      };
+      auto hide = [&](int i, const uint32_t(&marked)[NB]) __attribute__((always_inline)) {
         const int t0 = t_lo + i * BT;
         uint32_t bad[NB], any = 0;
 #pragma unroll
         for (int tb = 0; tb < NB; ++tb)
-          any |= bad[tb] = __builtin_amdgcn_readfirstlane(marks[m1][tok / 32 + tb]);
+          any |= bad[tb] = __builtin_amdgcn_readfirstlane(marked[tb]);
         if (t0 + BT <= t_hi && t0 + BT - 1 <= pos0 + wave_first && !any) {
           seen = true;
           return false;
@@ -376,9 +385,11 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void rows_kernel(RowsAr
       auto scaled = [&](float x) { return max_of_halves(x) * c2 - weight_shift<VT>(); };
       float mx = -INFINITY;
       if (n > 0) {
-        mv.template next<KEEP>(t_lo);
+        if constexpr (Move::kInRegisters) mv.template next<KEEP>(t_lo);
         for (int i = -2; i < (wave_on ? 0 : n); ++i) {
           move(i);
+#pragma unroll
+          for (int p = 0; p < 24; ++p) load(p);
           if (wave_on && i == -1) {
             // q is waited for here, not before the first product of every tile, where that
             // would be for the next tiles' loads as well
@@ -392,7 +403,9 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void rows_kernel(RowsAr
               for (int ks = 0; ks < KS; ++ks)
                 s[tb] = mfma32<QT>(read_k(k_wave, tb * KS + ks), qb[ks], s[tb]);
             }
-            hide(0);
+            uint32_t marked[NB];
+            get_marks(marked);
+            hide(0, marked);
             mx = scaled(largest());
           }
           mv.settle(marks[3]);
@@ -415,6 +428,8 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void rows_kernel(RowsAr
           bool over;
           do {
             move(i);
+            uint32_t marked[NB];
+            get_marks(marked);
             const uint32_t k_rd = k_wave + (~i & 1) * TB, v_rd = v_wave + (i & 1) * TB;
             u32x4 pb[2 * NB];  // weights of 16 tokens each, 8 per lane
             float l2 = 0.0f;
@@ -436,7 +451,10 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void rows_kernel(RowsAr
             for (int q = 0; q < AHEAD; ++q) kf[q] = read_k(k_rd, q);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) weigh(0, e);
+            for (int e = 0; e < 8; ++e) {
+              load(e);
+              weigh(0, e);
+            }
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int q = 0; q < QN; ++q) {
@@ -446,6 +464,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void rows_kernel(RowsAr
                 for (int e = 0; e < 16; ++e) s[tb][e] = 0.0f;
               s[tb] = mfma32<QT>(kf[q % AHEAD], qb[ks], s[tb]);
               if (q + AHEAD < QN) kf[q % AHEAD] = read_k(k_rd, q + AHEAD);
+              load(8 + q);
               if (tb + 1 < NB)
 #pragma unroll
                 for (int e = ks * 8 / KS; e < (ks + 1) * 8 / KS; ++e) weigh(tb + 1, e);
@@ -465,12 +484,14 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void rows_kernel(RowsAr
                 big = fmaxf(big, s[e / 16][e % 16]);
               __builtin_amdgcn_sched_barrier(0);
             }
+            // (not put off to where they are used: the scores would be held twice)
+            asm volatile("" : "+v"(big), "+v"(l_run), "+v"(l2));
             l_run += l2;
             // (behind the last tile the scores are of what lies in LDS, and not used)
             ++i;
             over = false;
             if (i < n) {
-              if (hide(i)) big = largest();
+              if (hide(i, marked)) big = largest();
               mx = scaled(big);
               over = __any(mx > m_run + slack<VT>());
             }
@@ -796,8 +817,13 @@ int64_t part_floats(int D) { return (int64_t)2 * kRows * (D + kPartPad); }
 template <int QT, int KV>
 void launch_matrix(const RowsArgs& a, hipStream_t st) {
   const dim3 grid(a.shares), merge(a.shares, kMergeParts);
-#define AMF_ROWS(DD)                                       \
-  rows_kernel<QT, KV, DD><<<grid, kThreads, 0, st>>>(a);   \
+#define AMF_ROWS(DD)                                                                  \
+  if constexpr (KV == kInt4) {                                                        \
+    rows_kernel<QT, KV, DD, true><<<grid, kThreads, 0, st>>>(a);                      \
+  } else {                                                                            \
+    a.by16 ? rows_kernel<QT, KV, DD, true><<<grid, kThreads, 0, st>>>(a)              \
+           : rows_kernel<QT, KV, DD, false><<<grid, kThreads, 0, st>>>(a);            \
+  }                                                                                   \
   rows_merge_kernel<QT, DD><<<merge, kThreads, 0, st>>>(a)
   if (a.head_dim == 64) {
     AMF_ROWS(64);
@@ -906,6 +932,7 @@ extern "C" int amf_paged_attn_rows(
   a.token_stride = token_stride * es;
   a.head_stride = head_stride * es;
   a.pool_pages = pool_pages;
+  a.pages = (uint32_t)std::min<int64_t>(std::max<int64_t>(pool_pages, 0), 1ll << 31);
   a.block_tables = block_tables;
   a.bt_stride = bt_stride;
   a.table_pages = table_pages;
@@ -970,6 +997,7 @@ extern "C" int amf_int4_paged_attn_rows(
   a.kp = static_cast<const uint32_t*>(k_params);
   a.vp = static_cast<const uint32_t*>(v_params);
   a.pool_pages = pool_pages;
+  a.pages = (uint32_t)std::min<int64_t>(std::max<int64_t>(pool_pages, 0), 1ll << 31);
   a.block_tables = block_tables;
   a.bt_stride = bt_stride;
   a.table_pages = table_pages;
