@@ -26,6 +26,23 @@ using namespace amf;
 
 constexpr int kThreads = 256;
 
+// Division by a number that a launch has once: the quotient from floor((2^32 - 1) / d) is
+// one too small at most (n below 2^31).
+struct Div {
+  uint32_t d, m;
+  Div() = default;
+  explicit Div(uint32_t x) : d(x), m(x ? 0xFFFFFFFFu / x : 0) {}
+  __device__ __forceinline__ uint32_t operator()(uint32_t n, uint32_t& rest) const {
+    uint32_t q = __umulhi(n, m);
+    rest = n - q * d;
+    if (rest >= d) {
+      ++q;
+      rest -= d;
+    }
+    return q;
+  }
+};
+
 struct alignas(16) Turn {
   double c, s;
 };
@@ -122,12 +139,24 @@ __device__ __forceinline__ void emit(uint8_t* p, const float* x, float scale) {
   }
 }
 
-// Items of a head: pairs first (VEC: 8 pairs, else one), then what is not
-// rotated (VEC: 8 elements, else one).
-template <bool VEC>
-__host__ __device__ __forceinline__ int head_items(int dim, int pairs) {
-  return VEC ? pairs / 8 + (dim - 2 * pairs) / 8 : dim - pairs;
-}
+// Items of a head: pairs (VEC: 8 pairs, else one), and what is not rotated (VEC: 8
+// elements, else one).
+struct Items {
+  Div rot, rest;
+  Items() = default;
+  Items(int dim, int pairs, bool vec)
+      : rot(pairs / (vec ? 8 : 1)), rest((dim - 2 * pairs) / (vec ? 8 : 1)) {}
+  // Item i of n heads (head, item of it): pairs of all heads first, so that the lanes of a
+  // wave do the same (rotating 64 of 256 dims, half the time went to waves that did both).
+  __device__ __forceinline__ uint32_t head(uint32_t i, uint32_t n, uint32_t& item) const {
+    const uint32_t turned = n * rot.d;
+    if (i < turned) return rot(i, item);
+    const uint32_t h = rest(i - turned, item);
+    item += rot.d;
+    return h;
+  }
+  __device__ __forceinline__ uint32_t each() const { return rot.d + rest.d; }
+};
 
 // Item `it` of the head at p: out(dim, values) for its one or two chunks.
 template <int DT, bool VEC, class Out>
@@ -176,6 +205,8 @@ struct StepArgs {
   int64_t n_rows;
   int dim;
   int tile;  // rows of a workgroup, at most kTile
+  Items items, v_items;  // of heads of q and k, and of v
+  Div q_heads, k_heads, v_heads;
 };
 constexpr int kTile = 8;
 
@@ -200,17 +231,17 @@ __global__ __launch_bounds__(kThreads) void step_kernel(StepArgs a) {
   __syncthreads();
   constexpr int ES = elem_bytes<DT>(), OS = TO == TO_FP8 ? 1 : ES;
   const int pairs = a.rot.pairs;
-  const uint32_t per = head_items<VEC>(a.dim, pairs), vper = head_items<VEC>(a.dim, 0);
-  const uint32_t nq = rows * a.q.heads * per, nk = rows * a.k.heads * per;
-  const uint32_t nv = TO == TO_ROWS ? 0 : rows * a.v.heads * vper;
-  for (uint32_t i = blockIdx.y * kThreads + threadIdx.x; i < nq + nk + nv;
+  const uint32_t hq = rows * a.q.heads, hk = rows * a.k.heads;
+  const uint32_t nqk = (hq + hk) * a.items.each();
+  const uint32_t nv = TO == TO_ROWS ? 0 : rows * a.v.heads * a.v_items.rest.d;
+  for (uint32_t i = blockIdx.y * kThreads + threadIdx.x; i < nqk + nv;
        i += gridDim.y * kThreads) {
-    if (i < nq + nk) {
-      const bool key = i >= nq;
-      const uint32_t j = key ? i - nq : i;
-      const uint32_t hr = j / per, it = j - hr * per;
-      const uint32_t heads = key ? a.k.heads : a.q.heads;
-      const uint32_t r = hr / heads, h = hr - r * heads;
+    if (i < nqk) {
+      uint32_t it, h;
+      const uint32_t hr = a.items.head(i, hq + hk, it);
+      const bool key = hr >= hq;
+      const Div heads = key ? a.k_heads : a.q_heads;
+      const uint32_t r = heads(key ? hr - hq : hr, h);
       const int64_t row = row0 + r;
       const uint8_t* p = key ? a.k.p + row * a.k.row + h * a.k.head
                              : a.q.p + row * a.q.row + h * a.q.head;
@@ -230,9 +261,9 @@ __global__ __launch_bounds__(kThreads) void step_kernel(StepArgs a) {
             [&](int dim, const float* x) { emit<DT, false, VEC>(o + dim * ES, x, 1.0f); });
       }
     } else {
-      const uint32_t j = i - nq - nk;
-      const uint32_t hr = j / vper, it = j - hr * vper;
-      const uint32_t r = hr / a.v.heads, h = hr - r * a.v.heads;
+      uint32_t it, h;
+      const uint32_t hr = a.v_items.rest(i - nqk, it);
+      const uint32_t r = a.v_heads(hr, h);
       const int64_t off = at[r];
       if (off < 0) continue;
       uint8_t* o = a.cache.v + off + h * a.cache.head;
@@ -321,6 +352,8 @@ struct PoolStepArgs {
   int dim;
   int kv_blocks;   // workgroups of a row tile that take KV heads (the others take q)
   int head_block;  // KV heads of such a workgroup
+  Items items;     // of a head
+  Div q_heads;
 };
 
 // Codes of 8 of a group's values, from the group's extremes.
@@ -354,16 +387,15 @@ __global__ __launch_bounds__(kThreads) void int4_step_kernel(PoolStepArgs a) {
   const int64_t row0 = (int64_t)blockIdx.x * kTile;
   const int rows = (int)min((int64_t)kTile, a.n_rows - row0);
   const int D = a.dim, pairs = a.rot.pairs;
-  const uint32_t per = head_items<VEC>(D, pairs);
   constexpr int ES = elem_bytes<DT>();
   fill_turns(a.rot, row0, rows, turns);
   if ((int)blockIdx.y >= a.kv_blocks) {
     __syncthreads();
-    const uint32_t n = rows * a.q.heads * per;
+    const uint32_t hq = rows * a.q.heads, n = hq * a.items.each();
     for (uint32_t i = (blockIdx.y - a.kv_blocks) * kThreads + tid; i < n;
          i += (gridDim.y - a.kv_blocks) * kThreads) {
-      const uint32_t hr = i / per, it = i - hr * per;
-      const uint32_t r = hr / a.q.heads, h = hr - r * a.q.heads;
+      uint32_t it, h;
+      const uint32_t r = a.q_heads(a.items.head(i, hq, it), h);
       uint8_t* o = a.q_out.p + (row0 + r) * a.q_out.row + h * a.q_out.head;
       head_item<DT, VEC>(
           a.q.p + (row0 + r) * a.q.row + h * a.q.head, it, pairs, a.rot.interleaved,
@@ -378,8 +410,9 @@ __global__ __launch_bounds__(kThreads) void int4_step_kernel(PoolStepArgs a) {
   __syncthreads();
   const int H = a.k.heads, h0 = blockIdx.y * a.head_block, nh = min(a.head_block, H - h0);
   const int G = D / 32, C = D / 8;
-  for (uint32_t i = tid; i < rows * nh * per; i += kThreads) {
-    const uint32_t hr = i / per, it = i - hr * per;
+  for (uint32_t i = tid; i < rows * nh * a.items.each(); i += kThreads) {
+    uint32_t it;
+    const uint32_t hr = a.items.head(i, rows * nh, it);
     const uint32_t r = hr / nh, h = hr - r * nh;
     float* o = kx + hr * D;
     head_item<DT, VEC>(a.k.p + (row0 + r) * a.k.row + (h0 + h) * a.k.head, it, pairs,
@@ -633,7 +666,12 @@ unsigned splits(int64_t tiles, int64_t items) {
 bool pairs_in_chunks(int pairs, int dim) { return pairs % 8 == 0 && dim % 8 == 0; }
 
 template <int TO>
-void launch_step(const StepArgs& a, int32_t dtype, bool vec, hipStream_t st) {
+void launch_step(StepArgs a, int32_t dtype, bool vec, hipStream_t st) {
+  a.items = Items(a.dim, a.rot.pairs, vec);
+  a.v_items = Items(a.dim, 0, vec);
+  a.q_heads = Div(a.q.heads);
+  a.k_heads = Div(a.k.heads);
+  a.v_heads = Div(a.v.heads);
   const int64_t tiles = (a.n_rows + a.tile - 1) / a.tile;
   const int64_t heads = a.q.heads + a.k.heads + (TO == TO_ROWS ? 0 : a.v.heads);
   const int64_t items = a.tile * heads * (a.dim - a.rot.pairs) / (vec ? 8 : 1);
@@ -770,6 +808,8 @@ extern "C" int amf_int4_kv_write(
   a.dim = head_dim;
   const bool vec = pairs_in_chunks(n_pairs, head_dim) && chunks(a.k, es) && chunks(a.v, es) &&
                    (num_q_heads == 0 || (chunks(a.q, es) && chunks(a.q_out, es)));
+  a.items = Items(head_dim, n_pairs, vec);
+  a.q_heads = Div(num_q_heads);
   const int64_t tiles = (n_rows + kTile - 1) / kTile;
   // rotated keys of a workgroup's heads in 32 KB of LDS at most
   const int most = std::max(1, (32 << 10) / (kTile * head_dim * 4));
