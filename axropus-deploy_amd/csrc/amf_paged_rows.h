@@ -140,10 +140,9 @@ __device__ __forceinline__ void mark_row(uint32_t* marks, int r, bool is) {
 
 // What movers of caches (EB bytes an element) share.  Wave w of the workgroup takes rows
 // RPW w .. of a tile, which lie in one aligned group of 16: with pages of 16, 32, 64 ..
-// tokens (by16) it looks up one page a tile, on the scalar unit.  (With every wave's
-// rows spread over the tile's pages each looked up them all: 420 scalar instructions
-// a tile, which the CU's one scalar unit takes longer for than the matrix cores for the
-// products.)  A lane takes 16 bytes of a row, CH rows RPI apart.
+// tokens (BY16) it looks up one page a tile (with every wave's rows spread over the tile's
+// pages each looked up them all, in 420 scalar instructions: more than the products
+// take).  A lane takes 16 bytes of a row, CH rows RPI apart.
 template <int EB, int D, bool BY16>
 struct CacheMover {
   static constexpr int BT = tile_tokens(D);
@@ -158,9 +157,9 @@ struct CacheMover {
   int end;
   int id;                  // of the thread
   const uint8_t *kb, *vb;  // the KV head's
-  int32_t k_id, v_id;      // by16: pages of the wave's rows; -1 behind `end`
+  int32_t k_id, v_id;      // BY16: pages of the wave's rows; -1 behind `end`
   uint32_t k_off, v_off;   // and their place, in units of 16 bytes
-  int32_t ahead;           // by16: the table's entry for the tile after K's
+  int32_t ahead;           // BY16: the table's entry for the tile after K's
 
   __device__ __forceinline__ CacheMover(const RowsArgs& args) : a(args) {}
   static __device__ __forceinline__ int wave_row() {
@@ -190,7 +189,7 @@ struct CacheMover {
     k_off = 0;
     if (BY16 && e > 0) look_up(t0);
   }
-  // by16: goes on to the K tile at t0.  The table's entry was asked for a turn before, as
+  // BY16: goes on to the K tile at t0.  The table's entry was asked for a turn before, as
   // the tile's loads depend on it, by a vector load: reads of LDS behind a scalar one
   // wait for it.
   __device__ __forceinline__ void advance(int t0) {
@@ -310,7 +309,8 @@ struct Mover : CacheMover<2, D, BY16> {
                                           uint32_t* wild) {
     if (BY16) {
       const bool ok = this->good(__builtin_amdgcn_readfirstlane(v_id));
-      look = wanted && (check || !ok || t0 + BT > end);
+      // (in other tiles `end` is a page's, so a wave's rows lie all before it or all behind)
+      look = wanted && (check || !ok);
       look_t = ok ? t0 : end;
       v_src = Base::base(vb, ok ? this->v_off : 0u);
       v_dst = __builtin_amdgcn_readfirstlane(lds_address(lds) + Base::wave_row() * RB);
@@ -366,7 +366,7 @@ struct Mover<QT, AMF_DTYPE_E4M3, D, BY16> : CacheMover<1, D, BY16> {
   static constexpr bool kInRegisters = true;
   u32x4 kr[Base::CH], vr[Base::CH];
   int bad;    // bits of the lane's K rows whose pages are none
-  bool none;  // by16: no page for the wave's V rows
+  bool none;  // BY16: no page for the wave's V rows
 
   __device__ __forceinline__ Mover(const RowsArgs& args) : Base(args) {}
   static __device__ __forceinline__ void settle(uint32_t*) {}

@@ -14,6 +14,18 @@
 // lane holds one column (lane % 32) and 16 of 32 tokens, so the softmax statistics are
 // per lane (one exchange with lane ^ 32 for the maximum) and the weights are in the
 // B layout of O^T = V^T P^T as they are.  V^T comes out of LDS by the transposing read.
+// Tiles of 64 columns and fewer (decoded and drafted rows, short ends) are shared: two or
+// four waves take parts of the tokens and of V's dims (with one wave at work 32 x 5 drafted
+// rows over INT4 took 240 us, so 204).
+//
+// What bounds it.  With two workgroups of four waves a CU, a SIMD has two waves, and each
+// issues an instruction every five cycles or so: a turn's time goes with its number of
+// instructions of all kinds, more than with its products (32 of 32 cycles in a turn of 2000).
+// So the turn is written out: weights, loads and maxima stand between the products, the
+// accumulators are changed by products alone, one wave looks up one page, and what can be
+// known before the turns is.  Prompt of 12000 rows, 32 / 8 heads of 128, bf16: 1330 us,
+// 0.89 PFLOP/s (a library product reaches 1.2); 48 decoded rows beside a chunk, 64 x 32 rows
+// of 8192 tokens: 409 us, 5.25 TB/s; one row each: 393 us, 5.5 TB/s, bound by the reads.
 //
 // Shares.  Tile j of a sequence reads its first e_j tokens; the tiles of all
 // (KV head, sequence, tile) one after the other, each as long as it reads plus a
@@ -21,7 +33,12 @@
 // single rows fills the chip.  e_j grows linearly in j, so a workgroup finds its
 // place from sums over the sequences alone.  A tile inside one share is finished
 // there; one that several share leaves partials (acc, m, l), joined by a second
-// launch.
+// launch.  The constant is what a tile's beginning and end take, 256 tokens' time (with 64,
+// shares of many short tiles ran half as long again: 8 prompts of 2048 519 us, so 466).
+// The older of a CU's two workgroups goes first wherever both could and ends at 4/5 of the
+// other's time, which then is alone; the younger has a higher priority in every second turn
+// (prompt 1480 -> 1409 us, and no loss where the reads bind; longer shares for the older gave
+// the same here and lost 10 % there).
 //
 // Precision.  Products of Q and K are exact and summed in fp32; maximum, sum and
 // accumulators are fp32.  The weights enter the second product in one term: bf16 (8
@@ -51,9 +68,8 @@ constexpr int kThreads = kRowsThreads;
 constexpr int kRows = 32 * kWaves;  // columns of a workgroup
 constexpr int kMaxDim = 256;
 constexpr int kMaxShares = 512;     // two workgroups a CU
-// Lengths of tiles and shares: a token of a tile of more than 64 columns counts kWide,
-// of a narrower one, whose turns are bound by what they load beside others that are not,
-// kNarrow.
+// Lengths of tiles and shares.  A token of a tile of more than 64 columns counts kWide, of a
+// narrower one kNarrow: beside chunks, whose turns take 4/3 of its time.
 constexpr int kWide = 4, kNarrow = 3;
 constexpr int kMinShare = 256 * kWide;
 constexpr int kTileCost = 256 * kWide;  // a tile's beginning and end; at least BT tokens

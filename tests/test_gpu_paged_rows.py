@@ -275,6 +275,52 @@ def test_rows_of_nobody_stay(D):
     assert (out == 7.0).all()
 
 
+@pytest.mark.parametrize("heads,D", [((8, 2), 64), ((8, 2), 128), ((64, 2), 128), ((4, 1), 256)])
+def test_infinite_values_before_the_end_of_a_short_table(heads, D):
+    """Every row sees all that the table holds, which ends inside a tile."""
+    g = _gen(heads[0] + D)
+    rows, ctx = [2, 1], [100, 333]
+    table, pool = make_tables([48, 48], 16, g)
+    kv = make_cache(pool, 16, heads[1], D, BF16, g)
+    kv[1, int(table[0, 2]), 8, 0, 3] = float("inf")   # token 40
+    kv[1, int(table[1, 0]), 5, -1, 1] = -float("inf")
+    q = torch.randn(3, heads[0], D, generator=g).to(BF16).to(DEV)
+    flag = torch.zeros(1, dtype=torch.int32, device=DEV)
+    got = _check(q, kv, kv, table, rows, ctx, 16, BF16, err_flag=flag)
+    assert torch.isinf(got[:2, 0, 3]).all() and torch.isinf(got[2, -1, 1]) and int(flag) == 2
+
+
+@pytest.mark.parametrize("cache", [BF16, FP8, "int4"])
+@pytest.mark.parametrize("n,group", [(1, 4), (5, 4), (12, 4), (20, 4), (3, 16)])
+def test_few_columns(cache, n, group):
+    """Tiles of 4 to 80 columns: waves share tokens and dims; bad pages in either half of a tile,
+    values that are not finite beside the diagonal, contexts that shares cut."""
+    from korith_vllm_ext.codecs import get_codec
+
+    g = _gen(n * group)
+    ctx = [n, 40 + n, 2500, 7001]
+    rows, H = [n] * 4, 2
+    for D in (64, 128, 256):
+        table, pool = make_tables(ctx, 16, g, extra=1)
+        q = torch.randn(4 * n, H * group, D, generator=g).to(BF16).to(DEV)
+        if cache == "int4":
+            kv = _pool(make_cache(pool, 16, H, D, BF16, g))
+            values = get_codec("int4_asym_g32").decompress_to(kv, BF16)
+        else:
+            kv = values = make_cache(pool, 16, H, D, cache, g)
+            if cache is BF16:
+                t = ctx[1] - 1 - n // 2
+                kv[1, int(table[1, t // 16]), t % 16, 1, D - 1] = float("inf")
+            else:
+                values = values.cpu().float()
+        weight = F16 if cache is FP8 else BF16
+        _check(q, kv, values, table, rows, ctx, 16, weight)
+        table[2, 3], table[2, 5], table[3, 100] = -1, pool, -7
+        flag = torch.zeros(1, dtype=torch.int32, device=DEV)
+        _check(q, kv, values, table, rows, ctx, 16, weight, err_flag=flag)
+        assert int(flag) == 1
+
+
 def test_strided_rows_and_planes():
     g = _gen(31)
     rows, ctx = [9, 30], [100, 64]
