@@ -473,11 +473,11 @@ struct Mover<QT, kInt4, D, true> {
   const int32_t* table;
   int head;
   int end;
+  const uint8_t *kc, *vc, *kp, *vp;  // the head's codes and parameters in page 0
   int id;  // of the thread
   u32x4 kr, vr, vs[2];
   uint32_t ks;
-  int bad;             // the lane's K row has no page
-  bool none;           // its V items have none
+  bool k_none, v_none; // no page for the items of K (or not in the context), of V
   int32_t k_id, ahead; // the items' page, of K, and in the tile after
 
   __device__ __forceinline__ Mover(const RowsArgs& args) : a(args) {}
@@ -502,6 +502,10 @@ struct Mover<QT, kInt4, D, true> {
     table = a.block_tables + seq * a.bt_stride;
     head = h;
     end = e;
+    kc = a.k + h * 8 * D;
+    vc = a.v + h * 8 * D;
+    kp = reinterpret_cast<const uint8_t*>(a.kp) + h * 2 * D;
+    vp = reinterpret_cast<const uint8_t*>(a.vp) + h * 2 * D;
     id = opaque(threadIdx.x);
     k_id = -1;
     if (e > 0) look_up(t0);
@@ -510,10 +514,11 @@ struct Mover<QT, kInt4, D, true> {
   __device__ __forceinline__ void look_up(int t0) {
     ahead = table[opaque(min(t0 + page_row(), end - 1) / 16)];
   }
-  __device__ __forceinline__ int64_t block(int32_t id) const {
-    int32_t x = good(id) ? id : 0;
+  // Bytes of parameters before page id's, a quarter of those of codes.
+  __device__ __forceinline__ uint64_t page_off(int32_t id) const {
+    uint32_t x = good(id) ? id : 0;
     if constexpr (!HALF) x = __builtin_amdgcn_readfirstlane(x);
-    return (int64_t)x * a.num_kv_heads + head;
+    return (uint64_t)x * (uint32_t)(a.num_kv_heads * 2 * D);
   }
   template <bool KEEP>
   __device__ __forceinline__ void next(int t0) {
@@ -522,21 +527,20 @@ struct Mover<QT, kInt4, D, true> {
     const int32_t v_id = k_id;
     k_id = t0 + page_row(tid) < end ? ahead : -1;
     look_up(t0 + BT);
-    bad = !good(k_id) && t0 + k_row(tid) < end;
-    none = !good(v_id);
+    k_none = !good(k_id);
+    v_none = !good(v_id);
     if (has_k()) {  // items of a (page, head) block follow each other
-      const int64_t b = block(k_id);
+      const uint64_t off = page_off(k_id);
       const uint32_t at = i % (16 * G);
-      kr = *reinterpret_cast<const u32x4*>(a.k + b * 8 * D + 16 * at);
-      ks = (a.kp + b * 16 * G)[at];
+      kr = *reinterpret_cast<const u32x4*>(kc + 4 * off + 16 * at);
+      ks = *reinterpret_cast<const uint32_t*>(kp + off + 4 * at);
     }
     if (has_v()) {
-      const int64_t b = block(v_id);
+      const uint64_t off = page_off(v_id);
       const uint32_t x = i % (D / 2), q = x / 16 * 4 + x / 2 % 2 * 2;
-      vr = *reinterpret_cast<const u32x4*>(a.v + b * 8 * D + 16 * x);
-      const u32x4* p = reinterpret_cast<const u32x4*>(a.vp + b * 16 * G);
-      vs[0] = p[q];
-      vs[1] = p[q + 1];
+      vr = *reinterpret_cast<const u32x4*>(vc + 4 * off + 16 * x);
+      vs[0] = *reinterpret_cast<const u32x4*>(vp + off + 16 * q);
+      vs[1] = *reinterpret_cast<const u32x4*>(vp + off + 16 * q + 16);
     }
   }
   // Codes as fp16 numbers, two an instruction: a code u in the low bits of an fp16 is
@@ -560,10 +564,10 @@ struct Mover<QT, kInt4, D, true> {
     return __builtin_fmaf((float)u[i / 4], s, z);
   }
   template <bool KEEP>
-  __device__ __forceinline__ void store_k(int, uint8_t* lds, uint32_t* marks) const {
+  __device__ __forceinline__ void store_k(int t0, uint8_t* lds, uint32_t* marks) const {
     if (!has_k()) return;
     const int tid = thread<KEEP>(id);
-    if (__any(bad)) mark_row(marks, k_row(tid), bad);
+    if (__any(k_none)) mark_row(marks, k_row(tid), k_none && t0 + k_row(tid) < end);
     const float z = param_zero(ks), s[2] = {param_scale(ks) * unit(0), param_scale(ks) * unit(1)};
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
@@ -592,9 +596,9 @@ struct Mover<QT, kInt4, D, true> {
       y[2 * t] = pair16<QT>(value(x[0], t, s, z), value(x[1], t, s, z));
       y[2 * t + 1] = pair16<QT>(value(x[2], t, s, z), value(x[3], t, s, z));
     }
-    if (check || __any(none)) {
+    if (check || __any(v_none)) {
 #pragma unroll
-      for (int t = 0; t < 16; ++t) y[t] = !none && t0 + r0 + t / 2 < end ? y[t] : 0u;
+      for (int t = 0; t < 16; ++t) y[t] = !v_none && t0 + r0 + t / 2 < end ? y[t] : 0u;
       const bool found = clean<VT>(y);
       mark_row(wild, 0, found);
     }
