@@ -23,9 +23,11 @@
 // instructions of all kinds, more than with its products (32 of 32 cycles in a turn of 2000).
 // So the turn is written out: weights, loads and maxima stand between the products, the
 // accumulators are changed by products alone, one wave looks up one page, and what can be
-// known before the turns is.  Prompt of 12000 rows, 32 / 8 heads of 128, bf16: 1330 us,
-// 0.89 PFLOP/s (a library product reaches 1.2); 48 decoded rows beside a chunk, 64 x 32 rows
-// of 8192 tokens: 409 us, 5.25 TB/s; one row each: 393 us, 5.5 TB/s, bound by the reads.
+// known before the turns is.  32 / 8 heads of 128: prompt of 12000 rows 1230 us, 0.96
+// PFLOP/s (a library product reaches 1.2 to 1.3); 64 x 32 rows of 8192 tokens 406 us, 5.3
+// TB/s; one row each 391 us, 5.5 TB/s, bound by the reads; 48 decoded rows beside a chunk of
+// 2048 rows of 8192 tokens 400 us, 0.6 PFLOP/s and 2.2 TB/s; 32 x 5 drafted rows over INT4
+// 150 us, 2.4 TB/s, where taking out the codes is a third of a turn's instructions.
 //
 // Shares.  Tile j of a sequence reads its first e_j tokens; the tiles of all
 // (KV head, sequence, tile) one after the other, each as long as it reads plus a
@@ -643,7 +645,9 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void rows_kernel(RowsAr
 }
 
 // out = v_scale sum_k f_k acc_k / sum_k f_k l_k, f_k = 2^(m_k - M), over the pieces of a
-// cut tile; D / 4 lanes a column, kMergeParts workgroups a tile.
+// cut tile; D / 4 lanes a column, kMergeParts workgroups a tile.  Bound by the pieces' bytes,
+// up to 69 MB: 15 to 22 us at 128 columns, 6 at few (eight parts, and accumulators loaded
+// with the statistics, gained nothing).
 constexpr int kMergeParts = 4;
 
 template <int QT, int D>
