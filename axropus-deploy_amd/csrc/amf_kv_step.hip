@@ -146,59 +146,118 @@ __device__ __forceinline__ void emit(uint8_t* p, const float* x, float scale) {
 }
 
 // Items of a head: pairs (VEC: 8 pairs, else one), and what is not rotated (VEC: 8
-// elements, else one).
+// elements, else one).  A kernel takes the pairs of all heads first, so that the lanes of a
+// wave do the same (rotating 64 of 256 dims, a third of the time went to waves that did
+// both).
 struct Items {
   Div rot, rest;
   Items() = default;
   Items(int dim, int pairs, bool vec)
       : rot(pairs / (vec ? 8 : 1)), rest((dim - 2 * pairs) / (vec ? 8 : 1)) {}
-  // Item i of n heads (head, item of it): pairs of all heads first, so that the lanes of a
-  // wave do the same (rotating 64 of 256 dims, half the time went to waves that did both).
-  __device__ __forceinline__ uint32_t head(uint32_t i, uint32_t n, uint32_t& item) const {
-    const uint32_t turned = n * rot.d;
-    if (i < turned) return rot(i, item);
-    const uint32_t h = rest(i - turned, item);
-    item += rot.d;
-    return h;
-  }
-  __device__ __forceinline__ uint32_t each() const { return rot.d + rest.d; }
 };
 
-// Item `it` of the head at p: out(dim, values) for its one or two chunks.
-template <int DT, bool VEC, class Out>
-__device__ __forceinline__ void head_item(const uint8_t* p, int it, int pairs, bool interleaved,
-                                          const Turn* turns, Out out) {
-  constexpr int ES = elem_bytes<DT>(), N = VEC ? 8 : 1;
-  const int rot = pairs / N;
-  float a[8], b[8];
-  auto get = [&](int dim, float* x) {
-    if constexpr (VEC)
-      load8<DT>(p + dim * ES, x);
-    else
-      x[0] = kv_elem<DT>(p + dim * ES);
-  };
-  if (it >= rot) {
-    const int dim = 2 * pairs + (it - rot) * N;
-    get(dim, a);
-    out(dim, a);
-    return;
-  }
-  const Turn* t = turns + it * N;
-  const int da = interleaved ? 2 * it * N : it * N, db = interleaved ? da + N : da + pairs;
-  get(da, a);
-  get(db, b);
-  if (VEC && interleaved) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      turn(t[i], a[2 * i], a[2 * i + 1]);
-      turn(t[4 + i], b[2 * i], b[2 * i + 1]);
+// A chunk of a row as it lies in memory: 8 elements (VEC) or one.
+template <int DT, bool VEC>
+struct Chunk {
+  u32x4 w[VEC && DT == AMF_DTYPE_F32 ? 2 : 1];
+  __device__ __forceinline__ void load(const uint8_t* p) {
+    if constexpr (!VEC) {
+      w[0][0] = f2u(kv_elem<DT>(p));
+    } else {
+      w[0] = reinterpret_cast<const u32x4*>(p)[0];
+      if constexpr (DT == AMF_DTYPE_F32) w[1] = reinterpret_cast<const u32x4*>(p)[1];
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i) turn(t[i], a[i], b[i]);
   }
-  out(da, a);
-  out(db, b);
+  __device__ __forceinline__ void get(float* x) const {
+    if constexpr (!VEC) {
+      x[0] = u2f(w[0][0]);
+    } else if constexpr (DT == AMF_DTYPE_F32) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = u2f(w[i / 4][i % 4]);
+    } else {
+      unpack8<DT == AMF_DTYPE_BF16>(w[0], x);
+    }
+  }
+};
+
+// A head of a row; kind: of q (0), k (1) or v (2), or a number of the caller's.
+struct Head {
+  int kind;
+  uint32_t r, h;
+  const uint8_t* p;
+};
+
+// Chunks are loaded kAhead, or pairs of them kAhead / 2, at a time before the first is stored
+// (stores may be to what is read, for all that the compiler knows; one at a time, too few
+// bytes are on their way).
+constexpr int kAhead = 4;
+
+// The pairs of n heads: find(head) gives its Head, put(Head, dim, values) takes the results.
+template <int DT, bool VEC, class Find, class Put>
+__device__ __forceinline__ void each_pair(const RotaryArgs& rot, const Items& items, uint32_t n,
+                                          uint32_t at, uint32_t step, const Turn* turns,
+                                          Find find, Put put) {
+  constexpr int B = kAhead / 2, N = VEC ? 8 : 1, ES = elem_bytes<DT>();
+  const uint32_t all = n * items.rot.d;
+  const int second = rot.interleaved ? N : rot.pairs;
+  for (uint32_t i0 = at; i0 < all; i0 += B * step) {
+    Chunk<DT, VEC> x[B], y[B];
+    Head head[B];
+    uint32_t it[B];
+#pragma unroll
+    for (int j = 0; j < B; ++j) {
+      if (i0 - threadIdx.x + j * step >= all) break;
+      head[j] = find(items.rot(min(i0 + j * step, all - 1), it[j]));
+      const uint8_t* p = head[j].p + it[j] * (rot.interleaved ? 2 * N : N) * ES;
+      x[j].load(p);
+      y[j].load(p + second * ES);
+    }
+#pragma unroll
+    for (int j = 0; j < B; ++j) {
+      if (i0 + j * step >= all) break;
+      const Turn* t = turns + head[j].r * rot.pairs + it[j] * N;
+      float a[8], b[8];
+      x[j].get(a);
+      y[j].get(b);
+      if (VEC && rot.interleaved) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          turn(t[i], a[2 * i], a[2 * i + 1]);
+          turn(t[4 + i], b[2 * i], b[2 * i + 1]);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) turn(t[i], a[i], b[i]);
+      }
+      const int dim = it[j] * (rot.interleaved ? 2 * N : N);
+      put(head[j], dim, a);
+      put(head[j], dim + second, b);
+    }
+  }
+}
+
+// `all` chunks that are not rotated: find(i, dim) gives chunk i's head and first dim.
+template <int DT, bool VEC, class Find, class Put>
+__device__ __forceinline__ void each_chunk(uint32_t all, uint32_t at, uint32_t step, Find find,
+                                           Put put) {
+  for (uint32_t i0 = at; i0 < all; i0 += kAhead * step) {
+    Chunk<DT, VEC> x[kAhead];
+    Head head[kAhead];
+    uint32_t dim[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      if (i0 - threadIdx.x + j * step >= all) break;
+      head[j] = find(min(i0 + j * step, all - 1), dim[j]);
+      x[j].load(head[j].p + dim[j] * elem_bytes<DT>());
+    }
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      if (i0 + j * step >= all) break;
+      float a[8];
+      x[j].get(a);
+      put(head[j], dim[j], a);
+    }
+  }
 }
 
 struct StepArgs {
@@ -235,50 +294,50 @@ __global__ __launch_bounds__(kThreads) void step_kernel(StepArgs a) {
       atomicOr(a.err_flag, AMF_ERRFLAG_BLOCK_RANGE);
   }
   __syncthreads();
-  constexpr int ES = elem_bytes<DT>(), OS = TO == TO_FP8 ? 1 : ES;
+  constexpr int ES = elem_bytes<DT>(), OS = TO == TO_FP8 ? 1 : ES, N = VEC ? 8 : 1;
   const int pairs = a.rot.pairs;
   const uint32_t hq = rows * a.q.heads, hk = rows * a.k.heads;
-  const uint32_t nqk = (hq + hk) * a.items.each();
-  const uint32_t nv = TO == TO_ROWS ? 0 : rows * a.v.heads * a.v_items.rest.d;
-  for (uint32_t i = blockIdx.y * kThreads + threadIdx.x; i < nqk + nv;
-       i += gridDim.y * kThreads) {
-    if (i < nqk) {
-      uint32_t it, h;
-      const uint32_t hr = a.items.head(i, hq + hk, it);
-      const bool key = hr >= hq;
-      const Div heads = key ? a.k_heads : a.q_heads;
-      const uint32_t r = heads(key ? hr - hq : hr, h);
-      const int64_t row = row0 + r;
-      const uint8_t* p = key ? a.k.p + row * a.k.row + h * a.k.head
-                             : a.q.p + row * a.q.row + h * a.q.head;
-      if (TO != TO_ROWS && key) {
-        const int64_t off = at[r];
-        if (off < 0) continue;
-        uint8_t* o = a.cache.k + off + h * a.cache.head;
-        head_item<DT, VEC>(p, it, pairs, a.rot.interleaved, turns + r * pairs,
-                           [&](int dim, const float* x) {
-                             emit<DT, TO == TO_FP8, VEC>(o + dim * OS, x, a.cache.k_scale);
-                           });
-      } else {
-        const Rows& to = key ? a.k_out : a.q_out;
-        uint8_t* o = to.p + row * to.row + h * to.head;
-        head_item<DT, VEC>(
-            p, it, pairs, a.rot.interleaved, turns + r * pairs,
-            [&](int dim, const float* x) { emit<DT, false, VEC>(o + dim * ES, x, 1.0f); });
-      }
+  const uint32_t first = blockIdx.y * kThreads + threadIdx.x, step = gridDim.y * kThreads;
+  auto find = [&](uint32_t n) {  // heads of q, then of k
+    Head x;
+    x.kind = n >= hq;
+    const Div heads = x.kind ? a.k_heads : a.q_heads;
+    x.r = heads(x.kind ? n - hq : n, x.h);
+    const Rows& from = x.kind ? a.k : a.q;
+    x.p = from.p + (row0 + x.r) * from.row + x.h * from.head;
+    return x;
+  };
+  auto put = [&](const Head& x, int dim, const float* v) {
+    if (TO != TO_ROWS && x.kind) {
+      if (at[x.r] < 0) return;
+      uint8_t* o = (x.kind == 1 ? a.cache.k : a.cache.v) + at[x.r] + x.h * a.cache.head;
+      emit<DT, TO == TO_FP8, VEC>(o + dim * OS, v, x.kind == 1 ? a.cache.k_scale : a.cache.v_scale);
     } else {
-      uint32_t it, h;
-      const uint32_t hr = a.v_items.rest(i - nqk, it);
-      const uint32_t r = a.v_heads(hr, h);
-      const int64_t off = at[r];
-      if (off < 0) continue;
-      uint8_t* o = a.cache.v + off + h * a.cache.head;
-      head_item<DT, VEC>(a.v.p + (row0 + r) * a.v.row + h * a.v.head, it, 0, false, turns,
-                         [&](int dim, const float* x) {
-                           emit<DT, TO == TO_FP8, VEC>(o + dim * OS, x, a.cache.v_scale);
-                         });
+      const Rows& to = x.kind ? a.k_out : a.q_out;
+      emit<DT, false, VEC>(to.p + (row0 + x.r) * to.row + x.h * to.head + dim * ES, v, 1.0f);
     }
-  }
+  };
+  each_pair<DT, VEC>(a.rot, a.items, hq + hk, first, step, turns, find, put);
+  const uint32_t rest = (hq + hk) * a.items.rest.d;
+  const uint32_t nv = TO == TO_ROWS ? 0 : rows * a.v.heads * a.v_items.rest.d;
+  each_chunk<DT, VEC>(
+      rest + nv, first, step,
+      [&](uint32_t i, uint32_t& dim) {
+        uint32_t c;
+        Head x;
+        if (i < rest) {
+          x = find(a.items.rest(i, c));
+          dim = 2 * pairs + c * N;
+        } else {
+          const uint32_t n = a.v_items.rest(i - rest, c);
+          x.kind = 2;
+          x.r = a.v_heads(n, x.h);
+          x.p = a.v.p + (row0 + x.r) * a.v.row + x.h * a.v.head;
+          dim = c * N;
+        }
+        return x;
+      },
+      put);
 }
 
 // ------------------------------------------------------------ INT4 pools ----
@@ -397,17 +456,29 @@ __global__ __launch_bounds__(kThreads) void int4_step_kernel(PoolStepArgs a) {
   fill_turns(a.rot, row0, rows, turns);
   if ((int)blockIdx.y >= a.kv_blocks) {
     __syncthreads();
-    const uint32_t hq = rows * a.q.heads, n = hq * a.items.each();
-    for (uint32_t i = (blockIdx.y - a.kv_blocks) * kThreads + tid; i < n;
-         i += (gridDim.y - a.kv_blocks) * kThreads) {
-      uint32_t it, h;
-      const uint32_t r = a.q_heads(a.items.head(i, hq, it), h);
-      uint8_t* o = a.q_out.p + (row0 + r) * a.q_out.row + h * a.q_out.head;
-      head_item<DT, VEC>(
-          a.q.p + (row0 + r) * a.q.row + h * a.q.head, it, pairs, a.rot.interleaved,
-          turns + r * pairs,
-          [&](int dim, const float* x) { emit<DT, false, VEC>(o + dim * ES, x, 1.0f); });
-    }
+    const uint32_t hq = rows * a.q.heads;
+    const uint32_t first = (blockIdx.y - a.kv_blocks) * kThreads + tid;
+    const uint32_t step = (gridDim.y - a.kv_blocks) * kThreads;
+    auto find = [&](uint32_t n) {
+      Head x;
+      x.kind = 0;
+      x.r = a.q_heads(n, x.h);
+      x.p = a.q.p + (row0 + x.r) * a.q.row + x.h * a.q.head;
+      return x;
+    };
+    auto put = [&](const Head& x, int dim, const float* v) {
+      uint8_t* o = a.q_out.p + (row0 + x.r) * a.q_out.row + x.h * a.q_out.head;
+      emit<DT, false, VEC>(o + dim * ES, v, 1.0f);
+    };
+    each_pair<DT, VEC>(a.rot, a.items, hq, first, step, turns, find, put);
+    each_chunk<DT, VEC>(
+        hq * a.items.rest.d, first, step,
+        [&](uint32_t i, uint32_t& dim) {
+          const uint32_t n = a.items.rest(i, dim);
+          dim = 2 * pairs + dim * (VEC ? 8 : 1);
+          return find(n);
+        },
+        put);
     return;
   }
   float* kx = reinterpret_cast<float*>(turns + kTile * pairs);  // [rows][heads][dim]
@@ -416,17 +487,27 @@ __global__ __launch_bounds__(kThreads) void int4_step_kernel(PoolStepArgs a) {
   __syncthreads();
   const int H = a.k.heads, h0 = blockIdx.y * a.head_block, nh = min(a.head_block, H - h0);
   const int G = D / 32, C = D / 8;
-  for (uint32_t i = tid; i < rows * nh * a.items.each(); i += kThreads) {
-    uint32_t it;
-    const uint32_t hr = a.items.head(i, rows * nh, it);
-    const uint32_t r = hr / nh, h = hr - r * nh;
-    float* o = kx + hr * D;
-    head_item<DT, VEC>(a.k.p + (row0 + r) * a.k.row + (h0 + h) * a.k.head, it, pairs,
-                       a.rot.interleaved, turns + r * pairs, [&](int dim, const float* x) {
+  auto find = [&](uint32_t n) {
+    Head x;
+    x.kind = (int)n;
+    x.r = n / nh;
+    x.h = h0 + (n - x.r * nh);
+    x.p = a.k.p + (row0 + x.r) * a.k.row + x.h * a.k.head;
+    return x;
+  };
+  auto put = [&](const Head& x, int dim, const float* v) {
 #pragma unroll
-                         for (int n = 0; n < (VEC ? 8 : 1); ++n) o[dim + n] = round_to<DT>(x[n]);
-                       });
-  }
+    for (int n = 0; n < (VEC ? 8 : 1); ++n) kx[x.kind * D + dim + n] = round_to<DT>(v[n]);
+  };
+  each_pair<DT, VEC>(a.rot, a.items, rows * nh, tid, kThreads, turns, find, put);
+  each_chunk<DT, VEC>(
+      rows * nh * a.items.rest.d, tid, kThreads,
+      [&](uint32_t i, uint32_t& dim) {
+        const uint32_t n = a.items.rest(i, dim);
+        dim = 2 * pairs + dim * (VEC ? 8 : 1);
+        return find(n);
+      },
+      put);
   __syncthreads();
   // K: a chunk of 8 dims per lane, four lanes a group
   for (uint32_t i = tid; i < rows * nh * C; i += kThreads) {
@@ -506,7 +587,6 @@ struct ReadArgs {
   int dim;
   Div heads, chunks;  // of a row, of a head (of 8 elements, or one)
 };
-constexpr int kAhead = 4;
 
 // Elements of rows, 8 (VEC) or one a lane; rows without a slot become zeros.
 template <int KV, int DT, bool VEC>
