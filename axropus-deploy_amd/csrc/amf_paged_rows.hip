@@ -72,9 +72,9 @@ constexpr int kMaxDim = 256;
 constexpr int kMaxShares = 512;     // two workgroups a CU
 // Lengths of tiles and shares.  A token of a tile of more than 64 columns counts kWide, of a
 // narrower one kNarrow: beside chunks, whose turns take 4/3 of its time.
-constexpr int kWide = 4, kNarrow = 3;
+constexpr int kWide = 6, kNarrow = 5;
 constexpr int kMinShare = 256 * kWide;
-constexpr int kTileCost = 256 * kWide;  // a tile's beginning and end; at least BT tokens
+constexpr int kTileCost = 448 * kWide;  // a tile's beginning and end; at least BT tokens
 constexpr int kCusXcd = 32;
 constexpr int kMaxContext = 1 << 30;
 
