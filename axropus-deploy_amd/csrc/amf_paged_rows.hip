@@ -35,8 +35,8 @@
 // single rows fills the chip.  e_j grows linearly in j, so a workgroup finds its
 // place from sums over the sequences alone.  A tile inside one share is finished
 // there; one that several share leaves partials (acc, m, l), joined by a second
-// launch.  The constant is what a tile's beginning and end take, 256 tokens' time (with 64,
-// shares of many short tiles ran half as long again: 8 prompts of 2048 519 us, so 466).
+// launch.  The constant is what a tile's beginning and end take, 448 tokens' time (8 prompts of
+// 2048: with 256 tokens 430 us, 448 389, 576 400).
 // The older of a CU's two workgroups goes first wherever both could and ends at 4/5 of the
 // other's time, which then is alone; the younger has a higher priority in every second turn
 // (prompt 1480 -> 1409 us, and no loss where the reads bind; longer shares for the older gave
@@ -71,7 +71,7 @@ constexpr int kRows = 32 * kWaves;  // columns of a workgroup
 constexpr int kMaxDim = 256;
 constexpr int kMaxShares = 512;     // two workgroups a CU
 // Lengths of tiles and shares.  A token of a tile of more than 64 columns counts kWide, of a
-// narrower one kNarrow: beside chunks, whose turns take 4/3 of its time.
+// narrower one kNarrow (48 decoded rows beside a chunk: 3/4 407 us, 5/6 384).
 constexpr int kWide = 6, kNarrow = 5;
 constexpr int kMinShare = 256 * kWide;
 constexpr int kTileCost = 448 * kWide;  // a tile's beginning and end; at least BT tokens
