@@ -13,10 +13,10 @@
 //
 // All kernels move bytes: each value is read once and written once, in chunks of
 // 8 elements where addresses allow (else one at a time), and the rest is hidden.  Steps of
-// many rows are bound by HBM (10500 rows of 18 heads of 256, 64 dims rotated: 44 us, 4.5
-// TB/s; 11000 rows of 64 + 8 heads of 128, rotated, K and V written as FP8: 92 us, 4.7; 6700
-// rows into an INT4 pool 45 us, 52000 rows read from one 76, 3.7; 24000 FP8 rows read 38,
-// 3.9), steps of one row a sequence by the latency of a launch (4 to 10 us).  The angles of a
+// many rows are bound by HBM (10500 rows of 18 heads of 256, 64 dims rotated: 40 us, 4.9
+// TB/s; 11000 rows of 64 + 8 heads of 128, rotated, K and V written as FP8: 86 us, 4.9; 6700
+// rows into an INT4 pool 44 us, 52000 rows read from one 64, 4.4; 24000 FP8 rows read 27,
+// 5.5), steps of one row a sequence by the latency of a launch (4 to 10 us).  The angles of a
 // tile of rows are one set-up (a load, a sine, a barrier): with four times as many
 // workgroups, of a quarter of the items each, the 10500 rows took 54 us.
 #include <algorithm>

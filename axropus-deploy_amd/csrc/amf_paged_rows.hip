@@ -23,10 +23,10 @@
 // instructions of all kinds, more than with its products (32 of 32 cycles in a turn of 2000).
 // So the turn is written out: weights, loads and maxima stand between the products, the
 // accumulators are changed by products alone, one wave looks up one page, and what can be
-// known before the turns is.  32 / 8 heads of 128: prompt of 12000 rows 1230 us, 0.96
-// PFLOP/s (a library product reaches 1.2 to 1.3); 64 x 32 rows of 8192 tokens 406 us, 5.3
+// known before the turns is.  32 / 8 heads of 128: prompt of 12000 rows 1200 us, 0.98
+// PFLOP/s (a library product reaches 1.2 to 1.3); 64 x 32 rows of 8192 tokens 411 us, 5.2
 // TB/s; one row each 391 us, 5.5 TB/s, bound by the reads; 48 decoded rows beside a chunk of
-// 2048 rows of 8192 tokens 400 us, 0.6 PFLOP/s and 2.2 TB/s; 32 x 5 drafted rows over INT4
+// 2048 rows of 8192 tokens 383 us, 0.64 PFLOP/s and 2.3 TB/s; 32 x 5 drafted rows over INT4
 // 150 us, 2.4 TB/s, where taking out the codes is a third of a turn's instructions.
 //
 // Shares.  Tile j of a sequence reads its first e_j tokens; the tiles of all
