@@ -20,7 +20,7 @@
 //
 // What bounds it.  With two workgroups of four waves a CU, a SIMD has two waves, and each
 // issues an instruction every five cycles or so: a turn's time goes with its number of
-// instructions of all kinds, more than with its products (32 of 32 cycles in a turn of 2000).
+// instructions of all kinds, more than with its products (1024 of a SIMD's 2200 cycles a turn).
 // So the turn is written out: weights, loads and maxima stand between the products, the
 // accumulators are changed by products alone, one wave looks up one page, and what can be
 // known before the turns is.  32 / 8 heads of 128: prompt of 12000 rows 1200 us, 0.98
