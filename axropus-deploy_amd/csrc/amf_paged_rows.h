@@ -94,6 +94,32 @@ __device__ __forceinline__ uint32_t pair16(float a, float b) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), f16x2_t));
 }
 
+// Two fp32 numbers a, b >= 0 as pairs hi + lo of type T.  lo is above 0, so that an infinite
+// factor stays one (a zero or negative lo would make it NaN): bf16, the number cut to 8 bits and
+// what is left with 2^-23 of the number; fp16, a step less than the number cut to 11 bits and
+// what is left.  That is at most 2^-7 (2^-9) of the number's leading bit and rounded to 8 (11)
+// bits: hi + lo is within 2^-16 + 2^-23 (2^-21) of the number, or in fp16 2^-25 of it.  (fp16
+// numbers below 2^-23 have hi = 0.)
+struct TwoTerms {
+  uint32_t hi, lo;
+};
+template <int T>
+__device__ __forceinline__ TwoTerms two_terms(float a, float b) {
+  if constexpr (T == AMF_DTYPE_BF16) {
+    constexpr float up = 1.0f + 0x1p-23f;
+    const uint32_t x = f2u(a), y = f2u(b);
+    return {__builtin_amdgcn_perm(y, x, 0x07060302u),
+            pair16<T>(__builtin_fmaf(a, up, -u2f(x & 0xFFFF0000u)),
+                      __builtin_fmaf(b, up, -u2f(y & 0xFFFF0000u)))};
+  } else {
+    typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+    const u16x2 cut = __builtin_bit_cast(u16x2, __builtin_amdgcn_cvt_pkrtz(a, b));
+    const u16x2 x = __builtin_elementwise_sub_sat(cut, (u16x2){1, 1});
+    const f16x2_t h = __builtin_bit_cast(f16x2_t, x);
+    return {__builtin_bit_cast(uint32_t, x), pair16<T>(a - (float)h[0], b - (float)h[1])};
+  }
+}
+
 // Sets values that are not finite to 0; whether there were any.
 template <int T, int N>
 __device__ __forceinline__ bool clean(uint32_t (&v)[N]) {

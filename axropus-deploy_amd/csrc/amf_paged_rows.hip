@@ -43,11 +43,13 @@
 // the same here and lost 10 % there).
 //
 // Precision.  Products of Q and K are exact and summed in fp32; maximum, sum and
-// accumulators are fp32.  The weights enter the second product in one term: bf16 (8
-// bits) beside a bf16 V, which adds to the result what its own rounding to bf16 does
-// (their sum is within 2^-7 of the weighted |v|), fp16 (11 bits) beside an fp16 or an
-// FP8 one, whose values fp16 holds exactly; three bf16 terms would cost twice the
-// matrix time of the whole for bits that the result's type drops.
+// accumulators are fp32.  A weight enters the second product as two terms of the type
+// beside it: bf16 beside a bf16 V (16 bits of the weight), fp16 beside an fp16 or an FP8
+// one (21 bits; fp16 holds FP8 values exactly).  The result is then off by 2^-16 of the weighted |v|,
+// where rounding it to bf16 takes 2^-8 (2^-21 and 2^-11 for fp16).  With one term it was
+// off by as much again as that rounding, in values that cancel by more (prompt of 12000 rows
+// 1209 us, so 1632; 64 single rows of 8192 tokens 392, so 402); a third bf16 term would cost
+// another 16 products to the turn's 48, for bits that the result's type drops.
 #include <algorithm>
 #include <type_traits>
 
@@ -449,7 +451,8 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void rows_kernel(RowsAr
             uint32_t marked[NB];
             get_marks(marked);
             const uint32_t k_rd = k_wave + (~i & 1) * TB, v_rd = v_wave + (i & 1) * TB;
-            u32x4 pb[2 * NB];  // weights of 16 tokens each, 8 per lane
+            // weights of 16 tokens each, 8 per lane: both terms
+            u32x4 pb[2][2 * NB];
             float l2 = 0.0f;
             // weights of elements 2 e, 2 e + 1 of block tb
             auto weigh = [&](int tb, int e) __attribute__((always_inline)) {
@@ -457,14 +460,20 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void rows_kernel(RowsAr
               const float p1 = __builtin_amdgcn_exp2f(s[tb][2 * e + 1] * c2 - m_use);
               l_run += p0;
               l2 += p1;
-              pb[2 * tb + e / 4][e % 4] = pair16<VT>(p0, p1);
+              const auto [hi, lo] = two_terms<VT>(p0, p1);
+              pb[0][2 * tb + e / 4][e % 4] = hi;
+              pb[1][2 * tb + e / 4][e % 4] = lo;
             };
             // The order of the products and of what is done in their shadow: weights of the
             // first 32 tokens; scores of the next tile's first 32 over them, beside the
             // other weights; the other scores, beside the first reads of V; then V's
             // products, beside the maximum.  Reads are four products and more ahead.
-            constexpr int AHEAD = 4;
-            u32x4 kf[AHEAD], vf[2][DN];
+            constexpr int AHEAD = 4, VR = DN > 2 ? DN : 2, VW = DN > 1 ? 2 : 1;
+            // V fragment p of the tile: 16 tokens p / DN, dims 32 (p % DN) ..
+            auto read_v_of = [&](int p) __attribute__((always_inline)) {
+              return read_v((v_rd ^ (64 * (p % DN))) + 16 * (p / DN) * RB);
+            };
+            u32x4 kf[AHEAD], vf[VR];
 #pragma unroll
             for (int q = 0; q < AHEAD; ++q) kf[q] = read_k(k_rd, q);
             __builtin_amdgcn_sched_barrier(0);
@@ -486,19 +495,19 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void rows_kernel(RowsAr
               if (tb + 1 < NB)
 #pragma unroll
                 for (int e = ks * 8 / KS; e < (ks + 1) * 8 / KS; ++e) weigh(tb + 1, e);
-              else if (ks < DN)
-                vf[0][ks] = read_v(v_rd ^ (64 * ks));
+              else if (ks < VR)
+                vf[ks] = read_v_of(ks);
               __builtin_amdgcn_sched_barrier(0);
             }
             float big = -INFINITY;
 #pragma unroll
-            for (int p = 0; p < PN; ++p) {
-              const int st = p / DN, d = p % DN;
-              acc[d] = mfma32<VT>(vf[st & 1][d], pb[st], acc[d]);
-              if (st + 1 < 2 * NB)
-                vf[(st + 1) & 1][d] = read_v((v_rd ^ (64 * d)) + 16 * (st + 1) * RB);
+            for (int q = 0; q < 2 * PN; ++q) {
+              // both terms of VW fragments in turn: no product waits for the one before it
+              const int p = q / (2 * VW) * VW + q % VW, st = p / DN, d = p % DN, term = q / VW % 2;
+              acc[d] = mfma32<VT>(vf[p % VR], pb[term][st], acc[d]);
+              if (term == 1 && p + VR < PN) vf[p % VR] = read_v_of(p + VR);
 #pragma unroll
-              for (int e = p * (16 * NB) / PN; e < (p + 1) * (16 * NB) / PN; ++e)
+              for (int e = q * (8 * NB) / PN; e < (q + 1) * (8 * NB) / PN; ++e)
                 big = fmaxf(big, s[e / 16][e % 16]);
               __builtin_amdgcn_sched_barrier(0);
             }

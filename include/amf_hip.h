@@ -572,8 +572,9 @@ int amf_int4_kv_read(const void* k_codes, const void* k_params, const void* v_co
  * writes it; context_lens counts them): row j of n, at position
  * p = context_lens[s] - n + j, gets
  *   out[row][h] = v_scale * softmax_{t <= p}(q[row][h] . K[t] * softmax_scale * k_scale) V
- * in fp32 but for the weights (bf16 beside a bf16 V, else fp16 scaled by the row's
- * largest), rounded to out, of q's type, contiguous [n_rows][num_q_heads][head_dim].
+ * in fp32 but for the weights (two terms each: bf16 beside a bf16 V, 16 bits; else fp16,
+ * scaled by the row's largest, 21 bits), rounded to out, of q's type, contiguous
+ * [n_rows][num_q_heads][head_dim].
  * Rows that belong to no sequence are left as they are.  q's rows, heads, the
  * cache's strides, block tables, page ids and the end of a table as in
  * amf_paged_decode_attn; a row without tokens gives zeros, scores that are all
