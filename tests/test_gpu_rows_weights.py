@@ -74,3 +74,26 @@ def test_one_row_is_as_exact_as_the_decode_attention():
         tol = (b.abs() * torch.finfo(dtype).eps / 2 * 1.01 + step_ref.HALF_STEP[TWO[dtype]]
                + 2 * (2 * 132 * 2.0 ** -24 * top + 2.0 ** -21 + 2 * (2048 / 32 + 64) * 2.0 ** -24))
         assert ((a - b).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("rows", [1, 9, 40])
+@pytest.mark.parametrize("rise", [5.0, 29.0, 60.0])
+def test_large_finite_values_and_rising_scores(rows, rise):
+    """Weights are at most 1 whatever tile the largest score lies in: values of 1e30 to 1e35 stay
+    finite where their average is."""
+    ctx = [448, 6000]
+    g = _gen(3)
+    table, pool = make_tables(ctx, 16, g)
+    for D in (64, 128, 256):
+        kv = make_cache(pool, 16, 1, D, BF16, g)
+        kv[0] = 0.0
+        for s, c in enumerate(ctx):  # scores in powers of two: flat, then higher by `rise`
+            for t in range(c):
+                kv[0, int(table[s, t // 16]), t % 16, 0, 0] = rise if t % 448 >= 128 else 0.0
+        for big in (1e30, 1e35):
+            kv[1].normal_().mul_(big)
+            q = torch.zeros(2 * rows, 4, D)
+            q[..., 0] = 1.0
+            got = _check(q.to(BF16).to(DEV), kv, kv, table, [rows, rows], ctx, 16, TWO[BF16],
+                         scale=0.6931471805599453)
+            assert torch.isfinite(got).all()
