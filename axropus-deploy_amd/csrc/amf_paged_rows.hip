@@ -727,6 +727,11 @@ __global__ __launch_bounds__(kThreads) void rows_general_kernel(RowsArgs a) {
   int seq = -1;
   int64_t ctx = 0, pos = -1;
   int flags = 0;
+  if (blockIdx.x == 0 && a.err_flag) {  // what only the sequences show
+    for (int s = threadIdx.x; s < a.num_seqs; s += kThreads) get_seq(a, s, &flags);
+    if (flags) atomicOr(a.err_flag, flags);
+    flags = 0;
+  }
   if (row < a.n_rows && a.num_seqs > 0) {  // the last sequence that starts at or before it
     int lo = 0, hi = a.num_seqs;
     while (hi - lo > 1) {
@@ -747,7 +752,6 @@ __global__ __launch_bounds__(kThreads) void rows_general_kernel(RowsArgs a) {
   __syncthreads();
   if (seq < 0) return;
   const int64_t cap = (int64_t)a.table_pages * a.block_size;
-  if (ctx > cap) flags |= AMF_ERRFLAG_CONTEXT;
   const int64_t n = min(min(pos + 1, ctx), cap);
   const int32_t* table = a.block_tables + seq * a.bt_stride;
   constexpr int EB = KV == kInt4 ? 0 : KV == AMF_DTYPE_E4M3 ? 1 : elem_bytes<KV == kInt4 ? 0 : KV>();

@@ -1,0 +1,53 @@
+"""Attention of several rows on both of its kernels: what query_start may hold, and limits."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from paged_ref import DEV, make_cache, make_tables
+from test_gpu_paged_rows import _i32
+
+pytestmark = pytest.mark.gpu
+
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def _call(D, dtype, start, ctx, rows=40):
+    from korith_vllm_ext.kernels import paged_attention
+
+    g = _gen(D)
+    table, pool = make_tables(ctx, 16, g)
+    kv = make_cache(pool, 16, 2, D, dtype, g)
+    q = torch.randn(rows, 4, D, generator=g).to(dtype).to(DEV)
+    out = torch.full_like(q, 7.0)
+    flag = torch.zeros(1, dtype=torch.int32, device=DEV)
+    paged_attention(q, kv, query_start=_i32(start), block_tables=table.to(DEV),
+                    context_lens=_i32(ctx), out=out, err_flag=flag)
+    return q, kv, table, out, int(flag)
+
+
+@pytest.mark.parametrize("D,dtype", [(64, F16), (48, F16), (64, F32), (7, F32)])
+@pytest.mark.parametrize("start,ctx", [([3, 9, 41], [20, 50]), ([-1, 9, 29], [20, 50]),
+                                       ([9, 3, 29], [20, 50])])
+def test_malformed_starts_are_flagged(D, dtype, start, ctx):
+    """Rows outside the step, or that end before they begin."""
+    assert _call(D, dtype, start, ctx)[-1] == 2
+
+
+@pytest.mark.parametrize("D,dtype", [(64, F16), (48, F16), (64, F32)])
+def test_short_tables_are_flagged_and_rows_of_nobody_are_not(D, dtype):
+    assert _call(D, dtype, [0, 6, 26], [20, 50])[-1] == 0
+    # no rows, so nothing is asked of the table
+    from korith_vllm_ext.kernels import paged_attention
+
+    q, kv, table, _, _ = _call(D, dtype, [0, 6, 26], [20, 50])
+    for start, want in (([0, 6, 6], 0), ([0, 6, 7], 2)):
+        flag = torch.zeros(1, dtype=torch.int32, device=DEV)
+        paged_attention(q, kv, query_start=_i32(start), block_tables=table.to(DEV),
+                        context_lens=_i32([20, 500]), err_flag=flag)
+        assert int(flag) == want
