@@ -732,17 +732,25 @@ __global__ __launch_bounds__(kThreads) void rows_general_kernel(RowsArgs a) {
     if (flags) atomicOr(a.err_flag, flags);
     flags = 0;
   }
-  if (row < a.n_rows && a.num_seqs > 0) {  // the last sequence that starts at or before it
-    int lo = 0, hi = a.num_seqs;
+  if (row < a.n_rows && a.num_seqs > 0) {
+    auto holds = [&](int s) {
+      const int64_t first = a.query_start[s], end = a.query_start[s + 1];
+      return first >= 0 && first <= row && row < end && end <= a.n_rows;
+    };
+    int lo = 0, hi = a.num_seqs;  // the last sequence that starts at or before the row
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
       if (a.query_start[mid] <= row) lo = mid; else hi = mid;
     }
-    const int64_t first = a.query_start[lo], end = a.query_start[lo + 1];
-    if (first >= 0 && first <= row && row < end && end <= a.n_rows) {
-      seq = lo;
-      ctx = max(a.context_lens[lo], 0);
-      pos = ctx - (end - row);
+    if (holds(lo)) seq = lo;
+    // a row of nobody, or of a sequence beside a malformed one
+    for (int s0 = 0; seq < 0 && s0 < a.num_seqs; s0 += 64) {
+      const uint64_t on = __ballot(s0 + lane < a.num_seqs && holds(s0 + lane));
+      if (on) seq = s0 + __ffsll((unsigned long long)on) - 1;
+    }
+    if (seq >= 0) {
+      ctx = max(a.context_lens[seq], 0);
+      pos = ctx - (a.query_start[seq + 1] - row);
     }
   }
   if (seq >= 0) {

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from paged_ref import DEV, make_cache, make_tables
-from test_gpu_paged_rows import _i32
+from test_gpu_paged_rows import _check, _i32
 
 pytestmark = pytest.mark.gpu
 
@@ -51,3 +51,16 @@ def test_short_tables_are_flagged_and_rows_of_nobody_are_not(D, dtype):
         paged_attention(q, kv, query_start=_i32(start), block_tables=table.to(DEV),
                         context_lens=_i32([20, 500]), err_flag=flag)
         assert int(flag) == want
+
+
+@pytest.mark.parametrize("D,dtype", [(64, F16), (48, F16), (64, F32)])
+def test_sequences_behind_a_malformed_one_get_their_rows(D, dtype):
+    """Starts that do not ascend: the sequences whose own two are in order have their rows."""
+    start, ctx = [0, 5, 41, 20, 30], [9, 50, 70, 33]
+    q, kv, table, out, flag = _call(D, dtype, start, ctx)
+    assert flag == 2
+    assert (out[5:20] == 7.0).all() and (out[30:] == 7.0).all()
+    w = F16 if dtype is F16 and D == 64 else F32
+    got = _check(q[20:30], kv, kv, table[3:], [10], [33], 16, w)
+    assert torch.equal(out[20:30], got)
+    assert torch.equal(out[:5], _check(q[:5], kv, kv, table[:1], [5], [9], 16, w))
