@@ -721,13 +721,14 @@ template <int KV, int QT>
 __global__ __launch_bounds__(kThreads) void rows_general_kernel(RowsArgs a) {
   __shared__ float q_lds[kWaves][kMaxDim];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, D = a.head_dim;
-  const int64_t id = (int64_t)blockIdx.x * kWaves + wave;
+  const int64_t block = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
+  const int64_t id = block * kWaves + wave;
   const int64_t row = id / a.num_q_heads;
   const int qh = (int)(id - row * a.num_q_heads), head = qh / a.group;
   int seq = -1;
   int64_t ctx = 0, pos = -1;
   int flags = 0;
-  if (blockIdx.x == 0 && a.err_flag) {  // what only the sequences show
+  if (block == 0 && a.err_flag) {  // what only the sequences show
     for (int s = threadIdx.x; s < a.num_seqs; s += kThreads) get_seq(a, s, &flags);
     if (flags) atomicOr(a.err_flag, flags);
     flags = 0;
@@ -878,9 +879,11 @@ void launch_matrix(const RowsArgs& a, hipStream_t st) {
 
 template <int QT, int KV>
 void launch_general(const RowsArgs& a, hipStream_t st) {
-  const int64_t waves = a.n_rows * a.num_q_heads;
+  // (2^26 rows of one head are 2^32 threads, one more than a dimension of a grid holds)
+  const int64_t blocks = (a.n_rows * a.num_q_heads + kWaves - 1) / kWaves;
+  const int64_t x = std::min<int64_t>(blocks, 1 << 20);
   rows_general_kernel<KV, QT>
-      <<<dim3((unsigned)((waves + kWaves - 1) / kWaves)), kThreads, 0, st>>>(a);
+      <<<dim3((unsigned)x, (unsigned)((blocks + x - 1) / x)), kThreads, 0, st>>>(a);
 }
 
 int check(const char* who, const RowsArgs& a, int32_t q_dtype, const void* workspace,

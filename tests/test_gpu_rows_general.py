@@ -64,3 +64,23 @@ def test_sequences_behind_a_malformed_one_get_their_rows(D, dtype):
     got = _check(q[20:30], kv, kv, table[3:], [10], [33], 16, w)
     assert torch.equal(out[20:30], got)
     assert torch.equal(out[:5], _check(q[:5], kv, kv, table[:1], [5], [9], 16, w))
+
+
+def test_the_most_rows_that_a_call_takes():
+    """2^26 rows of one head on the general kernel: more waves than one dimension of a grid has."""
+    from korith_vllm_ext.kernels import paged_attention
+
+    n = 1 << 26
+    g = _gen(2)
+    table, pool = make_tables([n], 1 << 20, g, spare=0)
+    kv = torch.randn(2, pool, 1 << 20, 1, 1, generator=g).to(DEV)
+    q = torch.zeros(n, 1, 1, device=DEV)  # scores of 0: averages of the values
+    seqs = n // 2  # two rows each, of two tokens
+    start = torch.arange(0, n + 1, 2, dtype=torch.int32, device=DEV)
+    bt = torch.randint(0, pool, (seqs, 1), dtype=torch.int32, device=DEV)
+    lens = torch.full((seqs,), 2, dtype=torch.int32, device=DEV)
+    out = paged_attention(q, kv, query_start=start, block_tables=bt, context_lens=lens)
+    v = kv[1][bt[:, 0].long(), :2, 0, 0]
+    want = torch.stack((v[:, 0], v.double().mean(1).float()), 1).view(-1)
+    # halves are exact: one rounding of the sum, one of the quotient
+    assert ((out.view(-1) - want).abs() <= 2.0 ** -22 * v.abs().max()).all()
