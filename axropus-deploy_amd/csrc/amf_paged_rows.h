@@ -625,8 +625,10 @@ struct Mover<QT, kInt4, D, true> {
     if (check || __any(v_none)) {
 #pragma unroll
       for (int t = 0; t < 16; ++t) y[t] = !v_none && t0 + r0 + t / 2 < end ? y[t] : 0u;
-      const bool found = clean<VT>(y);
-      mark_row(wild, 0, found);
+      if (!HALF || check) {  // (HALF: half of the wave's items may have a page)
+        const bool found = clean<VT>(y);
+        mark_row(wild, 0, found);
+      }
     }
 #pragma unroll
     for (int t = 0; t < 8; ++t)

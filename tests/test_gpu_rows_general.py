@@ -84,3 +84,26 @@ def test_the_most_rows_that_a_call_takes():
     want = torch.stack((v[:, 0], v.double().mean(1).float()), 1).view(-1)
     # halves are exact: one rounding of the sum, one of the quotient
     assert ((out.view(-1) - want).abs() <= 2.0 ** -22 * v.abs().max()).all()
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("bad,wild", [(0, 1), (1, 0), (2, 3), (3, 2), (0, 4)])
+def test_int4_infinite_values_beside_a_bad_page(D, bad, wild):
+    """Pages that one wave takes out of their codes together: one is none, all rows see an infinite
+    zero point of the other, far from the diagonal."""
+    from korith_vllm_ext.codecs import get_codec
+    from test_gpu_paged_rows import _pool
+
+    g = _gen(D)
+    for rows in (1, 20):
+        table, pool = make_tables([200], 16, g)
+        kv = _pool(make_cache(pool, 16, 2, D, BF16, g))
+        # V params [page][head][groups][16 tokens]
+        words = kv.scales[1, int(table[0, wild])].view(2, D // 32, 16)
+        words[1, 1, 3] = (0x7C00 << 16) | (int(words[1, 1, 3]) & 0xFFFF)
+        values = get_codec("int4_asym_g32").decompress_to(kv, BF16)
+        table[0, bad] = -1
+        q = torch.randn(rows, 4, D, generator=g).to(BF16).to(DEV)
+        flag = torch.zeros(1, dtype=torch.int32, device=DEV)
+        got = _check(q, kv, values, table, [rows], [200], 16, BF16, err_flag=flag)
+        assert torch.isinf(got[:, 2:, 32:64]).all() and int(flag) == 1
