@@ -419,8 +419,9 @@ def hip_decode_attention(q: torch.Tensor, k: Any, v: Any = None, scale: Optional
     block_tables and context_lens may be lists, of other integer types or on
     the host with either, at the cost of a copy; int32 tensors on the device
     are taken as they are, tables with rows apart too.  query_start (int32
-    [seqs + 1] on the device) makes it the attention of several rows per sequence
-    (paged_attention) over either, q then [rows, heads, head_dim]."""
+    [seqs + 1], given as those may be) makes it the attention of several rows per
+    sequence (paged_attention) over either, q then [rows, heads, head_dim];
+    max_context_len, which sizes the other forms' work, has no effect on it."""
     if query_start is not None:
         if block_tables is None or context_lens is None:
             raise ValueError("query_start needs block_tables and context_lens")
@@ -430,6 +431,12 @@ def hip_decode_attention(q: torch.Tensor, k: Any, v: Any = None, scale: Optional
             raise ValueError(f"attention of several rows gives q's type, not {out_dtype}")
         from .rows import paged_attention  # it imports what imports this module
 
+        at = k.meta.get("_blob") if isinstance(k, CompressedKV) else k
+        if isinstance(at, torch.Tensor):
+            if not _rows_apart(block_tables, at.get_device()):
+                block_tables = _index_tensor(block_tables, at.device)
+            context_lens = _index_tensor(context_lens, at.device)
+            query_start = _index_tensor(query_start, at.device)
         return paged_attention(q, k, v, query_start=query_start, block_tables=block_tables,
                                context_lens=context_lens, scale=scale, k_scale=k_scale,
                                v_scale=v_scale, out=out, workspace=workspace, err_flag=err_flag)
