@@ -23,6 +23,8 @@ from .paged import (_HALVES, _KV_TAGS, _ROWS_WS, _TAGS, _cache, _flag, _int32, _
                     _raw_stream, _table, _workspace)
 from .step import _extent, _pool, _scales
 
+_TILE_DIMS = (64, 128, 256)  # of the matrix kernel
+
 
 def paged_attention(q: torch.Tensor, k_cache: Union[torch.Tensor, CompressedKV],
                     v_cache: Optional[torch.Tensor] = None, *, query_start: torch.Tensor,
@@ -44,9 +46,10 @@ def paged_attention(q: torch.Tensor, k_cache: Union[torch.Tensor, CompressedKV],
     an INT4 pool (int4_page_pool, or the int4_asym_g32 CompressedKV of a page
     tensor), attended in the values that read_kv_cache gives in q's type.
     block_tables int32 [seqs, max_pages].  A row without tokens gives zeros.
-    16-byte aligned rows of 64, 128 or 256 dims take matrix tiles; other calls
-    and fp32 a slower kernel.  out: contiguous, of q's shape and type, otherwise
-    a new one; rows that belong to no sequence are not written."""
+    64, 128 or 256 dims take matrix tiles where the cache's rows and out are
+    16-byte aligned (q is copied where it is not); other calls and fp32 a slower
+    kernel.  out: contiguous, of q's shape and type, otherwise a new one; rows
+    that belong to no sequence are not written."""
     pool = isinstance(k_cache, CompressedKV)
     if pool:
         if v_cache is not None and v_cache is not k_cache:
@@ -73,8 +76,12 @@ def paged_attention(q: torch.Tensor, k_cache: Union[torch.Tensor, CompressedKV],
     N, Hq, _ = q.shape
     if Hq == 0 or Hq % H:
         raise ValueError(f"{Hq} query heads is not a multiple of {H} KV heads")
-    if q.stride(2) != 1 and D > 1:
+    qs, qh, one = q.stride()
+    if one != 1 and D > 1:
         q = q.contiguous()
+    elif D in _TILE_DIMS and qdt in _HALVES and (
+            q.data_ptr() % 16 or (N > 1 and qs % 8) or (Hq > 1 and qh % 8)):
+        q = q.contiguous() if not q.is_contiguous() else q.clone()  # little beside the tiles' gain
     bt, row, S, width = _table(block_tables, idx, None)
     cl = _int32(context_lens, "context_lens", idx, (S,))
     start = _int32(query_start, "query_start", idx, (S + 1,))

@@ -49,3 +49,38 @@ def test_lists_and_host_tensors(kind):
             call(q, k, v, **kw)
     with pytest.raises(TypeError):
         call(q, "cache", block_tables=table.tolist(), context_lens=ctx, query_start=start)
+
+
+@pytest.mark.parametrize("D,kind", [(64, BF16), (128, F16), (256, BF16), (128, FP8),
+                                    (128, "pool")])
+def test_misaligned_queries_take_the_same_kernel(D, kind):
+    """Rows that are not of whole 16-byte vectors are copied: the same bits as aligned ones."""
+    from korith_vllm_ext.kernels import paged_attention
+
+    g = _gen(D)
+    ctx, start = [400, 100, 7], [0, 50, 51, 54]
+    table, pool = make_tables(ctx, 16, g)
+    dtype = BF16 if kind in (FP8, "pool") else kind
+    kv = make_cache(pool, 16, 2, D, dtype if kind == "pool" else kind, g)
+    kv = _pool(kv) if kind == "pool" else kv
+    q = torch.randn(54, 4, D, generator=g).to(dtype).to(DEV)
+    kw = dict(query_start=_i32(start), block_tables=table.to(DEV), context_lens=_i32(ctx))
+    want = paged_attention(q, kv, **kw)
+    n = q.numel()
+    shifted = torch.empty(n + 3, dtype=dtype, device=DEV)[3:].view(q.shape)
+    rows = torch.empty(54, 4 * D + 4, dtype=dtype, device=DEV)[:, :4 * D].view(54, 4, D)
+    heads = torch.empty(54, 4, D + 2, dtype=dtype, device=DEV)[..., :D]
+    for x in (shifted, rows, heads):
+        x.copy_(q)
+        assert torch.equal(paged_attention(x, kv, **kw), want)
+    one = torch.empty(4 * D + 3, dtype=dtype, device=DEV)[3:].view(1, 4, D)
+    one.copy_(q[50:51])
+    kw = dict(query_start=_i32([0, 1]), block_tables=table[1:2].to(DEV), context_lens=_i32([100]))
+    assert torch.equal(paged_attention(one, kv, **kw), paged_attention(q[50:51].clone(), kv, **kw))
+    # an output that is not aligned is written by the other kernel
+    from test_gpu_paged_rows import _check
+
+    out = torch.empty(4 * D + 1, dtype=dtype, device=DEV)[1:].view(1, 4, D)
+    values = kv if kind != "pool" else None
+    if values is not None:
+        _check(one, kv, values.cpu().float(), table[1:2], [1], [100], 16, F32, out=out)
