@@ -21,7 +21,7 @@ import amf_hip
 from ..codecs import CompressedKV
 from .paged import (_HALVES, _KV_TAGS, _ROWS_WS, _TAGS, _cache, _flag, _int32, _launch,
                     _raw_stream, _table, _workspace)
-from .step import _extent, _pool, _scales
+from .step import _apart, _extent, _planes_spans, _pool, _scales, _span
 
 _TILE_DIMS = (64, 128, 256)  # of the matrix kernel
 
@@ -48,8 +48,8 @@ def paged_attention(q: torch.Tensor, k_cache: Union[torch.Tensor, CompressedKV],
     block_tables int32 [seqs, max_pages].  A row without tokens gives zeros.
     64, 128 or 256 dims take matrix tiles where the cache's rows and out are
     16-byte aligned (q is copied where it is not); other calls and fp32 a slower
-    kernel.  out: contiguous, of q's shape and type, otherwise a new one; rows
-    that belong to no sequence are not written."""
+    kernel.  out: contiguous, of q's shape and type, apart from what is read,
+    otherwise a new one; rows that belong to no sequence are not written."""
     pool = isinstance(k_cache, CompressedKV)
     if pool:
         if v_cache is not None and v_cache is not k_cache:
@@ -89,7 +89,8 @@ def paged_attention(q: torch.Tensor, k_cache: Union[torch.Tensor, CompressedKV],
         scale = 0.0
     elif not 1.2e-38 < scale < math.inf:
         raise ValueError(f"scale must be positive, finite and normal in fp32, got {scale}")
-    if out is None:
+    given = out is not None
+    if not given:
         out = torch.empty((N, Hq, D), dtype=qdt, device=q.device)
     elif (not isinstance(out, torch.Tensor) or out.shape != (N, Hq, D) or out.dtype != qdt
           or out.get_device() != idx or not out.is_contiguous()):
@@ -99,11 +100,24 @@ def paged_attention(q: torch.Tensor, k_cache: Union[torch.Tensor, CompressedKV],
         raise ValueError("paged attention: out must not lie in q")  # q is read until the end
     stream = _raw_stream(idx)
     ws, wsb = _workspace(_ROWS_WS, (Hq, H, D), workspace, q.device, stream)
+    ef = _flag(err_flag, idx)
+    if given or workspace is not None:
+        at, n = out.data_ptr(), out.numel() * out.element_size()
+        read = [("block_tables", bt, bt + 4 * ((S - 1) * row + width) if S else bt),
+                ("context_lens", cl, cl + 4 * S), ("query_start", start, start + 4 * S + 4)]
+        if ef is not None:
+            read.append(("err_flag", ef, ef + 4))
+        read += ((("the pool", planes[0], planes[0] + layout.total_bytes),) if pool else
+                 _planes_spans(kp, vp, ps, ts, hs, nb, bs, H, D, kdt.itemsize))
+        _apart((("out", at, at + n),), read)
+        if workspace is not None:
+            wp = ws.data_ptr()
+            _apart((("workspace", wp, wp + wsb),), read + [_span(q, "q"), ("out", at, at + n)])
     qs, qh, _ = q.stride()
     rows = (q.data_ptr(), _TAGS[qdt], qs if N > 1 else 0, qh if Hq > 1 else 0, out.data_ptr(), N,
             start)
     seqs = (bt, row, width, cl, S, Hq, H, D)
-    end = (None if ws is None else ws.data_ptr(), wsb, _flag(err_flag, idx), stream)
+    end = (None if ws is None else ws.data_ptr(), wsb, ef, stream)
     if pool:
         _launch(idx, "amf_int4_paged_attn_rows", *rows, *planes, layout.n_pages, *seqs, scale, *end)
     else:

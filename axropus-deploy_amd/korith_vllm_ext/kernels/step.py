@@ -170,6 +170,31 @@ def _output(t: Any, what: str, like: torch.Tensor, others: Tuple[torch.Tensor, .
         raise ValueError(f"{what} must not overlap what the call reads or writes otherwise")
 
 
+Span = Tuple[str, int, int]  # what, its first byte's address, the one behind its last
+
+
+def _span(t: torch.Tensor, what: str) -> Span:
+    """Of rows."""
+    at = t.data_ptr()
+    return what, at, at + _extent(t) * t.element_size()
+
+
+def _planes_spans(kp: int, vp: int, ps: int, ts: int, hs: int, nb: int, bs: int, H: int, D: int,
+                  es: int) -> Tuple[Span, Span]:
+    """Of a cache's planes, from _cache's addresses and strides."""
+    n = ((nb - 1) * ps + (bs - 1) * ts + (H - 1) * hs + D) * es
+    return ("the cache", kp, kp + n), ("the cache", vp, vp + n)
+
+
+def _apart(written: Sequence[Span], others: Sequence[Span]) -> None:
+    """Refuses a call of which something written lies in what it reads, or
+    writes otherwise: a launch's workgroups have no order."""
+    for what, lo, hi in written:
+        for name, a, b in others:
+            if a < hi and lo < b:
+                raise ValueError(f"{what} must not overlap {name}")
+
+
 def _int64(t: Any, what: str, idx: int, n: int) -> int:
     """The address of t, a contiguous int64 tensor [n] on device idx."""
     if not isinstance(t, torch.Tensor) or t.dtype is not torch.int64:
@@ -245,6 +270,39 @@ def _pool(kv: CompressedKV, what: str) -> tuple:
                                        at + layout.code_offset(1), at + layout.param_offset(1))
 
 
+def _outside(lo: int, hi: int, rows: tuple, qs: tuple, rot: tuple, ef: Optional[int],
+             q_given: bool) -> None:
+    """_apart of a write's cache, at lo .. hi, from the rest of its arguments, and of a
+    q_out that the caller gave (every decode step waits for this: names come last)."""
+    k, k_row, k_head, v, v_row, v_head, tag, n, H, dim, slots = rows
+    q, q_row, q_head, o, o_row, o_head, Hq = qs
+    if not n:
+        return
+    es = 4 if tag == amf_hip.DTYPE_F32 else 2
+    k_end = k + ((n - 1) * k_row + (H - 1) * k_head + dim) * es
+    v_end = v + ((n - 1) * v_row + (H - 1) * v_head + dim) * es
+    q_end = o_end = 0
+    if Hq:
+        q_end = q + ((n - 1) * q_row + (Hq - 1) * q_head + dim) * es
+        o_end = o + ((n - 1) * o_row + (Hq - 1) * o_head + dim) * es
+    pos, freqs, pairs = rot[0] or 0, rot[1] or 0, rot[2]
+    s_end, p_end, f_end = slots + 8 * n, pos + 8 * n, freqs + 8 * pairs
+    if not (slots < hi and lo < s_end or pos < hi and lo < p_end or freqs < hi and lo < f_end
+            or k < hi and lo < k_end or v < hi and lo < v_end or ef and lo <= ef < hi
+            or q_end and (q < hi and lo < q_end or o < hi and lo < o_end)
+            or q_given and (slots < o_end and o < s_end or pos < o_end and o < p_end
+                            or freqs < o_end and o < f_end or ef and o <= ef < o_end)):
+        return
+    read = [("slot_mapping", slots, s_end), ("positions", pos, p_end),
+            ("the frequencies", freqs, f_end), ("err_flag", ef or 0, (ef or -4) + 4)]
+    if q_given:
+        _apart((("q_out", o, o_end),), read)
+    read += [("k", k, k_end), ("v", v, v_end)]
+    if Hq:
+        read += [("q", q, q_end), ("q_out", o, o_end)]
+    _apart((("the cache", lo, hi),), read)
+
+
 # -------------------------------------------------------------- operators --
 
 
@@ -277,6 +335,10 @@ def rotary_embedding(q: torch.Tensor, k: Optional[torch.Tensor], positions: torc
         _output(qo, "out[0]", q, () if k is None else (k, ko))
         if k is not None:
             _output(ko, "out[1]", k, (q, qo))
+        read = (("positions", rot[0], rot[0] + 8 * n),
+                ("the frequencies", rot[1], rot[1] + 8 * rot[2]))
+        _apart([_span(t, what) for t, what in ((qo, "out[0]"), (ko, "out[1]")) if t is not None],
+               read)
     qs, os = qi.stride(), qo.stride()
     ks = (None, 0, 0, None, 0, 0, 0)
     if ki is not None:
@@ -329,11 +391,14 @@ def write_kv_cache(k: torch.Tensor, v: torch.Tensor,
     other tokens stay.  A rotated key is rounded to its type before it is
     quantised: the codes are those of a page saved from an unquantised cache.
     slot_mapping int64 [rows] (build_slot_maps): negative ones are left out.
-    Rows of the same slot leave it any of their values, in a pool a mixture."""
+    Rows of the same slot leave it any of their values, in a pool a mixture.
+    What is read, and q_out, lies outside the cache: rows from it are copied
+    first."""
     idx, n, H, dim, dt = _step_rows(k, "k")
     ki = _rows(k, "k", idx, n, dim, dt)
     vi = _rows(v, "v", idx, n, dim, dt, H)
     slots = _int64(slot_mapping, "slot_mapping", idx, n)
+    q_given = False
     if q is None:
         if q_out is not None:
             raise ValueError("q_out comes with q")
@@ -342,7 +407,8 @@ def write_kv_cache(k: torch.Tensor, v: torch.Tensor,
         if rotary is None:
             raise ValueError("q comes with rotary")
         qi = _rows(q, "q", idx, n, dim, dt)
-        if q_out is None:
+        q_given = q_out is not None
+        if not q_given:
             q_out = torch.empty(q.shape, dtype=dt, device=q.device)
         else:
             _output(q_out, "q_out", q, (k, v))
@@ -360,6 +426,7 @@ def write_kv_cache(k: torch.Tensor, v: torch.Tensor,
         if pidx != idx or layout.num_heads != H or layout.head_dim != dim:
             raise ValueError(f"rows of {H} heads of {dim} on device {idx} do not fit the pool: "
                              f"{layout.num_heads} of {layout.head_dim} on device {pidx}")
+        _outside(planes[0], planes[0] + layout.total_bytes, rows, qs, rot, ef, q_given)
         _launch(idx, "amf_int4_kv_write", *rows, *planes, layout.n_pages, *rot, *qs, ef, stream)
         return q_out
     cidx, kp, vp, ps, ts, hs, nb, bs, ch, cd = _cache(k_cache, v_cache)
@@ -372,6 +439,12 @@ def write_kv_cache(k: torch.Tensor, v: torch.Tensor,
     if kdt is not dt and kdt is not torch.float8_e4m3fn:
         raise TypeError(f"write_kv_cache: rows are {dt}, the cache {kdt}")
     _scales(k_scale, v_scale, kdt is torch.float8_e4m3fn)
+    size = ((nb - 1) * ps + (bs - 1) * ts + (ch - 1) * hs + cd) * kdt.itemsize
+    if kp <= vp <= kp + size or vp <= kp <= vp + size:
+        _outside(min(kp, vp), max(kp, vp) + size, rows, qs, rot, ef, q_given)
+    else:
+        _outside(kp, kp + size, rows, qs, rot, ef, q_given)
+        _outside(vp, vp + size, rows, qs, rot, ef, False)
     _launch(idx, "amf_kv_write", *rows, kp, vp, _KV_TAGS[kdt], ps, ts, hs, nb, bs, k_scale,
             v_scale, *rot, *qs, ef, stream)
     return q_out
@@ -388,7 +461,8 @@ def read_kv_cache(k_cache: Union[torch.Tensor, CompressedKV],
     write_kv_cache takes them): as they are, or of an FP8 cache code * scale, of a
     pool u * s + z, in fp32 and rounded to dtype (bf16, fp16, fp32; by default bf16,
     a cache's own type where it is not FP8).  Rows of negative slots, and of
-    slots outside the pool, become zeros.  out: tensors to write into."""
+    slots outside the pool, become zeros.  out: tensors to write into, outside
+    the cache."""
     pool = isinstance(k_cache, CompressedKV)
     if pool:
         if v_cache is not None and v_cache is not k_cache:
@@ -414,6 +488,7 @@ def read_kv_cache(k_cache: Union[torch.Tensor, CompressedKV],
     if dt not in _TAGS or (own is not None and dt is not own):
         raise TypeError(f"read_kv_cache: rows of {dt} from a cache of "
                         f"{'INT4 pages' if pool else k_cache.dtype}")
+    ef = _flag(err_flag, idx)
     if out is None:
         ko = torch.empty((n, H, dim), dtype=dt, device=slot_mapping.device)
         vo = torch.empty_like(ko)
@@ -425,9 +500,15 @@ def read_kv_cache(k_cache: Union[torch.Tensor, CompressedKV],
                 raise ValueError(f"{what} must be {(n, H, dim)} of {dt} on device {idx}")
         _output(ko, "out[0]", ko, (vo,))
         _output(vo, "out[1]", vo, ())
+        read = [("slot_mapping", slots, slots + 8 * n)]
+        if ef is not None:
+            read.append(("err_flag", ef, ef + 4))
+        read += ((("the pool", planes[0], planes[0] + layout.total_bytes),) if pool else
+                 _planes_spans(kp, vp, ps, ts, hs, nb, bs, H, dim, k_cache.dtype.itemsize))
+        _apart((_span(ko, "out[0]"), _span(vo, "out[1]")), read)
     a, b = ko.stride(), vo.stride()
-    rows = (slots, ko.data_ptr(), a[0], a[1], vo.data_ptr(), b[0], b[1], _TAGS[dt], n, H, dim,
-            _flag(err_flag, idx), _raw_stream(idx))
+    rows = (slots, ko.data_ptr(), a[0], a[1], vo.data_ptr(), b[0], b[1], _TAGS[dt], n, H, dim, ef,
+            _raw_stream(idx))
     if pool:
         _launch(idx, "amf_int4_kv_read", *planes, layout.n_pages, *rows)
     else:

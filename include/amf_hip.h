@@ -497,7 +497,8 @@ int amf_build_slot_maps(const int32_t* context_lens, const int32_t* new_tokens,
  * head_dim at most 512, n_rows at most 2^25.  n_rows = 0 does nothing.  Chunks of
  * 8 elements are moved where n_pairs and head_dim are multiples of 8 and every
  * pointer and stride is 16-byte aligned (FP8 caches: 8), single ones elsewhere.
- * No counterpart in the reference.
+ * What a call writes lies apart from all that it reads (but for rotations in place) and
+ * writes otherwise; callers see to it.  No counterpart in the reference.
  *
  * Rotary positions: pair i of a head, dims (i, i + n_pairs) or, interleaved,
  * (2i, 2i + 1), turns by the angle positions[row] * freqs[i] (device int64 of
@@ -587,7 +588,8 @@ int amf_int4_kv_read(const void* k_codes, const void* k_params, const void* v_co
  * slower kernel.  Rows of one sequence must not be listed under another (their
  * results are either's then).  softmax_scale <= 0 selects 1/sqrt(head_dim).
  * workspace: amf_paged_attn_rows_workspace_bytes() bytes, 16-byte aligned; calls
- * sharing one must be ordered on one stream.  No counterpart in the reference. */
+ * sharing one must be ordered on one stream.  out and workspace lie apart from each other and
+ * from what is read.  No counterpart in the reference. */
 int64_t amf_paged_attn_rows_workspace_bytes(int32_t num_q_heads, int32_t num_kv_heads,
                                             int32_t head_dim);
 

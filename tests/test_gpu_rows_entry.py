@@ -84,3 +84,79 @@ def test_misaligned_queries_take_the_same_kernel(D, kind):
     values = kv if kind != "pool" else None
     if values is not None:
         _check(one, kv, values.cpu().float(), table[1:2], [1], [100], 16, F32, out=out)
+
+
+def test_what_lies_in_the_cache_is_refused():
+    """Rows, outputs and indices that lie in what the call writes otherwise, or reads."""
+    from korith_vllm_ext.kernels import (int4_page_pool, paged_attention, read_kv_cache,
+                                         rotary_embedding, rotary_frequencies, write_kv_cache)
+
+    g = _gen(5)
+    kv, pool = make_cache(8, 16, 2, 64, BF16, g), int4_page_pool(8, 2, 64)
+    blob = pool.meta["_blob"]
+    k, q = (torch.randn(4, h, 64, generator=g).to(BF16).to(DEV) for h in (2, 4))
+    slots = torch.arange(4, device=DEV)
+    r = rotary_frequencies(64)
+    inside = kv[0, 3, :4]                                   # rows of the cache
+    wide = kv[1, 2].reshape(4, 8, 64)[:, :4]                # [4, 4, 64] there, a view
+    assert wide.data_ptr() == kv[1, 2].data_ptr()
+    tokens = blob[:4 * 4 * 64 * 2].view(BF16).view(4, 4, 64)
+    ints = blob[:32].view(torch.int64)
+    at = dict(slot_mapping=slots)
+    rot = at | dict(rotary=r, positions=slots)
+    flag = kv[0, 0, 0, 0, :2].view(torch.int32)
+    bad = [
+        lambda: write_kv_cache(inside, k, kv, **at),
+        lambda: write_kv_cache(k, inside, kv[0], kv[1], **at),
+        lambda: write_kv_cache(k, k, kv, q=wide, **rot),
+        lambda: write_kv_cache(k, k, kv, q=q, q_out=wide, **rot),
+        lambda: write_kv_cache(tokens[:, :2], k, pool, **at),
+        lambda: write_kv_cache(k, tokens[:, 2:], pool, **at),
+        lambda: write_kv_cache(k, k, pool, q=q, q_out=tokens, **rot),
+        lambda: write_kv_cache(k, k, pool, slot_mapping=ints),
+        lambda: write_kv_cache(k, k, pool, slot_mapping=slots, rotary=r, positions=ints),
+        lambda: write_kv_cache(k, k, kv, err_flag=flag, **at),
+        lambda: write_kv_cache(k, k, kv, q=q[:, :2], q_out=q.view(-1)[:512].view(4, 2, 64),
+                               **rot),
+        lambda: write_kv_cache(k, k, kv, slot_mapping=q.view(-1)[:16].view(torch.int64), rotary=r,
+                               positions=slots, q=q, q_out=q),
+        lambda: read_kv_cache(kv, out=(inside, k), **at),
+        lambda: read_kv_cache(kv, out=(k, inside), **at),
+        lambda: read_kv_cache(kv[0], kv[1], out=(k, wide[:, :2]), **at),
+        lambda: read_kv_cache(pool, out=(k, tokens[:, 2:]), **at),
+        lambda: read_kv_cache(pool, slot_mapping=k.view(-1)[:16].view(torch.int64),
+                              out=(k, k.clone())),
+        lambda: rotary_embedding(q, None, q.view(-1)[:16].view(torch.int64), r, out=(q, None)),
+    ]
+    a = dict(query_start=_i32([0, 4]), block_tables=_i32([[0, 1]]), context_lens=_i32([20]))
+    ws = torch.empty(140 << 20, dtype=torch.uint8, device=DEV)
+    bad += [
+        lambda: paged_attention(q, kv, out=kv[0, 3].view(-1)[:1024].view(4, 4, 64), **a),
+        lambda: paged_attention(q, pool, out=tokens, **a),
+        lambda: paged_attention(q, kv, out=torch.empty_like(q), workspace=ws, err_flag=ws[:4].view(
+            torch.int32), **a),
+        lambda: paged_attention(q, kv, workspace=ws, out=ws[:2048].view(BF16).view(4, 4, 64), **a),
+        lambda: paged_attention(ws[:2048].view(BF16).view(4, 4, 64), kv, workspace=ws, **a),
+        lambda: paged_attention(q, kv, workspace=ws, **a | dict(
+            block_tables=ws[:8].view(torch.int32).view(1, 2))),
+    ]
+    state = [t.clone() for t in (q, k, kv, blob)]
+    for i, call in enumerate(bad):
+        with pytest.raises(ValueError):
+            call()
+            raise AssertionError(f"call {i} was taken")
+    torch.cuda.synchronize()
+    for x, y in zip(state, (q, k, kv, blob)):
+        assert torch.equal(x, y)
+    # rows beside each other, pages of K and V in turn, and a copy of what lies in the cache
+    pages = torch.zeros(8, 2, 16, 2, 64, dtype=BF16, device=DEV)
+    write_kv_cache(inside.clone(), k, pages[:, 0], pages[:, 1], **at)
+    got = read_kv_cache(pages[:, 0], pages[:, 1], **at)
+    assert torch.equal(got[0], inside) and torch.equal(got[1], k)
+    qkv = torch.randn(4, 8, 64, generator=g).to(BF16).to(DEV)
+    want, _ = rotary_embedding(qkv[:, :4], None, slots, r)
+    write_kv_cache(qkv[:, 4:6], qkv[:, 6:], pages[:, 0], pages[:, 1], q=qkv[:, :4],
+                   q_out=qkv[:, :4], **rot)
+    assert torch.equal(qkv[:, :4], want)
+    out = torch.empty_like(q)
+    assert paged_attention(q, kv, out=out, workspace=ws, **a) is out

@@ -178,3 +178,22 @@ def test_workspace_of_the_attention():
     f = amf_hip.load().amf_paged_attn_rows_workspace_bytes
     assert f(32, 8, 128) % 16 == 0 and f(64, 8, 256) > f(32, 8, 128) > f(32, 8, 64) > 0
     assert f(32, 8, 80) == 16 and f(7, 2, 64) == f(8, 0, 64) == f(8, 8, 300) == 0
+
+
+def test_overlaps():
+    """Address ranges of rows and planes, and which are refused."""
+    from korith_vllm_ext.kernels import step
+
+    x = torch.zeros(5, 6, 8, dtype=torch.bfloat16)
+    what, lo, hi = step._span(x[1:, 2:4], "rows")
+    assert (what, lo - x.data_ptr(), hi - lo) == ("rows", (48 + 16) * 2, (3 * 48 + 8 + 8) * 2)
+    assert step._span(x[:0], "none")[1:] == (0, 0) or step._span(x[:0], "none")[1] == \
+        step._span(x[:0], "none")[2]
+    # planes of 3 pages of 4 tokens of 2 heads of 8 dims, pages of K and V in turn
+    k, v = step._planes_spans(1000, 1128, 128, 16, 8, 3, 4, 2, 8, 2)
+    assert k[1:] == (1000, 1000 + (256 + 48 + 8 + 8) * 2) and v[1] - v[2] == k[1] - k[2]
+    step._apart([("a", 10, 20)], [("b", 20, 30), ("c", 0, 10), ("d", 15, 15 - 15), ("e", 0, 0)])
+    step._apart([], [("b", 20, 30)])
+    for lo, hi in ((0, 11), (19, 25), (12, 13), (0, 100), (10, 20)):
+        with pytest.raises(ValueError, match="a must not overlap b"):
+            step._apart([("z", 200, 300), ("a", 10, 20)], [("c", 0, 5), ("b", lo, hi)][lo < 5:])
