@@ -153,7 +153,9 @@ def _output(t: Any, what: str, like: torch.Tensor, others: Tuple[torch.Tensor, .
         raise ValueError(f"{what}'s dims must be contiguous and its rows and heads apart")
     es = t.element_size()
     for i, x in enumerate((like,) + others):
-        if i == 0 and x.data_ptr() == t.data_ptr() and x.stride() == t.stride():
+        if i == 0 and x.data_ptr() == t.data_ptr() and (
+                x.stride() == t.stride() or all(a == b or m == 1 for a, b, m in
+                                                zip(x.stride(), t.stride(), x.shape))):
             continue  # in place
         lo, hi = t.data_ptr(), t.data_ptr() + _extent(t) * es
         a, b = x.data_ptr(), x.data_ptr() + _extent(x) * x.element_size()

@@ -160,3 +160,17 @@ def test_what_lies_in_the_cache_is_refused():
     assert torch.equal(qkv[:, :4], want)
     out = torch.empty_like(q)
     assert paged_attention(q, kv, out=out, workspace=ws, **a) is out
+
+
+def test_one_row_in_place():
+    from korith_vllm_ext.kernels import rotary_embedding, rotary_frequencies
+
+    g = _gen(6)
+    x = torch.randn(1, 8 * 64, generator=g).to(BF16).to(DEV)
+    pos, r = torch.full((1,), 1234, device=DEV), rotary_frequencies(64)
+    want, _ = rotary_embedding(x[:, :256].view(1, 4, 64), None, pos, r)
+    q, out = x.view(1, 8, 64)[:, :4], x[0, :256].view(1, 4, 64)
+    assert q.stride() != out.stride()
+    rest = x[:, 256:].clone()
+    assert rotary_embedding(q, None, pos, r, out=(out, None))[0] is out
+    assert torch.equal(q, want) and torch.equal(x[:, 256:], rest)

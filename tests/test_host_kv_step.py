@@ -197,3 +197,23 @@ def test_overlaps():
     for lo, hi in ((0, 11), (19, 25), (12, 13), (0, 100), (10, 20)):
         with pytest.raises(ValueError, match="a must not overlap b"):
             step._apart([("z", 200, 300), ("a", 10, 20)], [("c", 0, 5), ("b", lo, hi)][lo < 5:])
+
+
+def test_outputs_in_place():
+    """The same elements at the same places, whatever the strides of dims of one element."""
+    from korith_vllm_ext.kernels import step
+
+    x = torch.zeros(6, 4, 64, dtype=torch.bfloat16)
+    wide = torch.zeros(1, 8 * 64, dtype=torch.bfloat16)
+    for like, out in ((x, x), (x, x.view(6, 4, 64)),
+                      (wide[:, :256].view(1, 4, 64), wide[0, :256].view(1, 4, 64)),
+                      (wide.view(1, 8, 64)[:, :4], wide[0, :256].view(1, 4, 64)),
+                      (x[:1].expand(1, 4, 64), x[:1]), (x[:, 1:2], x[:, 1].unsqueeze(1)),
+                      (x[:, :1], x.as_strided((6, 1, 64), (256, 7, 1)))):
+        step._output(out, "out", like, ())
+        with pytest.raises(ValueError, match="overlap"):
+            step._output(out, "out", like, (like,))
+    for like, out in ((x[:3], x[1:4]), (x[:, :2], x[:, 1:3]), (x[:1], x.view(-1)[1:257].view(1, 4, 64)),
+                      (x[:, :1, :32], x.as_strided((6, 1, 32), (32, 32, 1)))):
+        with pytest.raises(ValueError, match="overlap"):
+            step._output(out, "out", like, ())
