@@ -11,7 +11,6 @@ kernels/paged.py.
 
 from __future__ import annotations
 
-import math
 from typing import Optional, Union
 
 import torch
@@ -87,7 +86,7 @@ def paged_attention(q: torch.Tensor, k_cache: Union[torch.Tensor, CompressedKV],
     start = _int32(query_start, "query_start", idx, (S + 1,))
     if scale is None:
         scale = 0.0
-    elif not 1.2e-38 < scale < math.inf:
+    elif not 1.2e-38 < scale < 3.4e38:
         raise ValueError(f"scale must be positive, finite and normal in fp32, got {scale}")
     given = out is not None
     if not given:

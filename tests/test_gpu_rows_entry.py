@@ -174,3 +174,16 @@ def test_one_row_in_place():
     rest = x[:, 256:].clone()
     assert rotary_embedding(q, None, pos, r, out=(out, None))[0] is out
     assert torch.equal(q, want) and torch.equal(x[:, 256:], rest)
+
+
+def test_scales_that_fp32_does_not_hold_are_refused():
+    from korith_vllm_ext.kernels import paged_attention
+
+    g = _gen(7)
+    kv = make_cache(4, 16, 2, 64, BF16, g)
+    q = torch.randn(2, 4, 64, generator=g).to(BF16).to(DEV)
+    kw = dict(query_start=_i32([0, 2]), block_tables=_i32([[0, 1]]), context_lens=_i32([20]))
+    for bad in (1e39, 1e300, float("inf"), 1e-39, 0.0, -0.1, float("nan")):
+        with pytest.raises(ValueError, match="scale"):
+            paged_attention(q, kv, scale=bad, **kw)
+    paged_attention(q, kv, scale=1e-30, **kw)
