@@ -187,3 +187,29 @@ def test_scales_that_fp32_does_not_hold_are_refused():
         with pytest.raises(ValueError, match="scale"):
             paged_attention(q, kv, scale=bad, **kw)
     paged_attention(q, kv, scale=1e-30, **kw)
+
+
+@pytest.mark.parametrize("dtype,n,H", [(BF16, 4100, 2), (F32, 40, 2), (F16, 4100, 3)])
+def test_int4_rows_of_512_dims(dtype, n, H):
+    """The widest heads, rotated whole: the most LDS that a write asks for, and the codec's bytes."""
+    from korith_vllm_ext.codecs import get_codec
+    from korith_vllm_ext.kernels import (read_kv_cache, rotary_embedding, rotary_frequencies,
+                                         write_kv_cache)
+
+    g = _gen(n)
+    pages, D = -(-n // 16) + 2, 512
+    mirror = make_cache(pages, 16, H, D, dtype, g)
+    slots = torch.arange(5, n + 5, device=DEV)
+    k, v = (torch.randn(n, H, D, generator=g).to(dtype).to(DEV) for _ in range(2))
+    pos = torch.randint(0, 40000, (n,), generator=g).to(DEV)
+    r = rotary_frequencies(D)
+    pool = _pool(mirror)
+    write_kv_cache(k, v, pool, slot_mapping=slots, rotary=r, positions=pos)
+    mirror[0].view(-1, H, D)[slots] = rotary_embedding(k, None, pos, r)[0]
+    mirror[1].view(-1, H, D)[slots] = v
+    want = _pool(mirror)
+    assert torch.equal(pool.meta["_blob"], want.meta["_blob"])
+    got = read_kv_cache(pool, slot_mapping=slots, dtype=dtype)
+    full = get_codec("int4_asym_g32").decompress_to(want, dtype)
+    for i in range(2):
+        assert torch.equal(got[i], full[i].view(-1, H, D)[slots])
