@@ -158,6 +158,7 @@ SIGNATURES = {
          _c_i64, _c_ptr, _c_ptr],
     ),
     "amf_paged_attn_rows_workspace_bytes": (_c_i64, [_c_i32, _c_i32, _c_i32]),
+    "amf_paged_attn_rows_call_bytes": (_c_i64, [_c_i64] + [_c_i32] * 6),
     "amf_paged_attn_rows": (
         _c_i32,
         [_c_ptr, _c_i32, _c_i64, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_ptr, _c_ptr, _c_i32, _c_i64,

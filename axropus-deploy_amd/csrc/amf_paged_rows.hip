@@ -886,8 +886,25 @@ void launch_general(const RowsArgs& a, hipStream_t st) {
       <<<dim3((unsigned)x, (unsigned)((blocks + x - 1) / x)), kThreads, 0, st>>>(a);
 }
 
+// Shares of a call: of kMinShare, that the longest contexts of the tables could fill.
+int call_shares(int64_t n_rows, int num_seqs, int table_pages, int block_size, int num_q_heads,
+                int num_kv_heads, int D) {
+  const int tile_rows = std::max(1, kRows / (num_q_heads / num_kv_heads));
+  const int64_t tiles = n_rows / tile_rows + std::min<int64_t>(num_seqs, n_rows);
+  const int64_t cap = kWide * ((int64_t)table_pages * block_size + tile_rows) + kTileCost;
+  // a workgroup's registers and LDS: two to a CU, at the largest head_dim one
+  const int64_t fit = D == 256 ? kMaxShares / 2 : kMaxShares;
+  const int64_t most = (tiles * num_kv_heads * cap + kMinShare - 1) / kMinShare;
+  // whole rounds of the XCDs
+  return (int)std::min<int64_t>(fit, (most + kXcds - 1) / kXcds * kXcds);
+}
+
+int64_t share_bytes(int D) {
+  return (int64_t)sizeof(Cut) + part_floats(D) * (int64_t)sizeof(float);
+}
+
 int check(const char* who, const RowsArgs& a, int32_t q_dtype, const void* workspace,
-          int64_t workspace_bytes, int64_t need) {
+          int64_t workspace_bytes) {
   if (a.num_seqs < 0 || a.n_rows < 0 || a.num_q_heads <= 0 || a.num_kv_heads <= 0 ||
       a.num_q_heads % a.num_kv_heads || a.head_dim <= 0 || a.block_size <= 0 ||
       a.table_pages < 0 || a.bt_stride < a.table_pages || a.pool_pages <= 0)
@@ -908,6 +925,9 @@ int check(const char* who, const RowsArgs& a, int32_t q_dtype, const void* works
   if (!a.q || !a.out || !a.k || !a.v || !a.query_start || !a.context_lens ||
       (a.table_pages > 0 && !a.block_tables))
     return fail(AMF_ERR_INVALID_ARG, "%s: null pointer", who);
+  const int64_t need = amf_paged_attn_rows_call_bytes(a.n_rows, a.num_seqs, a.table_pages,
+                                                      a.block_size, a.num_q_heads, a.num_kv_heads,
+                                                      a.head_dim);
   if (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16)
     return fail(AMF_ERR_WORKSPACE, "%s: workspace of %lld bytes (16-byte aligned) needed, got %lld",
                 who, (long long)need, (long long)workspace_bytes);
@@ -929,17 +949,10 @@ void finish_args(RowsArgs* a, void* workspace, float softmax_scale, float k_scal
   const float scale =
       softmax_scale > 0.0f ? softmax_scale : 1.0f / __builtin_sqrtf((float)a->head_dim);
   a->score_scale = scale * k_scale * kLog2e;
-  // shares of kMinShare that the longest contexts of the tables could fill
-  const int64_t tiles = a->n_rows / a->tile_rows + std::min<int64_t>(a->num_seqs, a->n_rows);
-  const int64_t cap =
-      kWide * ((int64_t)a->table_pages * a->block_size + a->tile_rows) + kTileCost;
-  // a workgroup's registers and LDS: two to a CU, at the largest head_dim one
-  const int64_t fit = a->head_dim == 256 ? kMaxShares / 2 : kMaxShares;
-  const int64_t most = (tiles * a->num_kv_heads * cap + kMinShare - 1) / kMinShare;
-  // whole rounds of the XCDs
-  a->shares = (int)std::min<int64_t>(fit, (most + kXcds - 1) / kXcds * kXcds);
+  a->shares = call_shares(a->n_rows, a->num_seqs, a->table_pages, b, a->num_q_heads,
+                          a->num_kv_heads, a->head_dim);
   a->cuts = static_cast<Cut*>(workspace);
-  a->part = reinterpret_cast<float*>(a->cuts + kMaxShares);
+  a->part = reinterpret_cast<float*>(a->cuts + a->shares);
 }
 
 }  // namespace
@@ -950,7 +963,22 @@ extern "C" int64_t amf_paged_attn_rows_workspace_bytes(int32_t num_q_heads, int3
       head_dim > kMaxDim)
     return 0;
   if (!matrix_dim(head_dim)) return 16;
-  return kMaxShares * ((int64_t)sizeof(Cut) + part_floats(head_dim) * (int64_t)sizeof(float));
+  return kMaxShares * share_bytes(head_dim);
+}
+
+extern "C" int64_t amf_paged_attn_rows_call_bytes(int64_t n_rows, int32_t num_seqs,
+                                                  int32_t table_pages, int32_t block_size,
+                                                  int32_t num_q_heads, int32_t num_kv_heads,
+                                                  int32_t head_dim) {
+  const int64_t most =
+      amf_paged_attn_rows_workspace_bytes(num_q_heads, num_kv_heads, head_dim);
+  if (most <= 16 || n_rows < 0 || num_seqs < 0 || table_pages < 0 || block_size <= 0 ||
+      n_rows > ((int64_t)1 << 26) / num_q_heads ||
+      (int64_t)table_pages * block_size > kMaxContext)
+    return most;
+  return std::max<int64_t>(16, call_shares(n_rows, num_seqs, table_pages, block_size, num_q_heads,
+                                           num_kv_heads, head_dim) *
+                                   share_bytes(head_dim));
 }
 
 extern "C" int amf_paged_attn_rows(
@@ -988,8 +1016,7 @@ extern "C" int amf_paged_attn_rows(
   a.block_size = block_size;
   a.v_scale = v_scale;
   a.err_flag = err_flag;
-  const int rc = check(who, a, q_dtype, workspace, workspace_bytes,
-                       amf_paged_attn_rows_workspace_bytes(num_q_heads, num_kv_heads, head_dim));
+  const int rc = check(who, a, q_dtype, workspace, workspace_bytes);
   if (rc) return rc;
   const bool fp8 = kv_dtype == AMF_DTYPE_E4M3;
   if (!(fp8 ? q_dtype != AMF_DTYPE_F32 : kv_dtype == q_dtype))
@@ -1053,8 +1080,7 @@ extern "C" int amf_int4_paged_attn_rows(
   a.block_size = 16;
   a.v_scale = 1.0f;
   a.err_flag = err_flag;
-  const int rc = check(who, a, q_dtype, workspace, workspace_bytes,
-                       amf_paged_attn_rows_workspace_bytes(num_q_heads, num_kv_heads, head_dim));
+  const int rc = check(who, a, q_dtype, workspace, workspace_bytes);
   if (rc) return rc;
   if (head_dim % 32 || q_dtype == AMF_DTYPE_F32)
     return fail(AMF_ERR_UNSUPPORTED, "%s: head_dim %d (a multiple of 32), q dtype %d", who,

@@ -39,7 +39,7 @@ _HALVES = (torch.bfloat16, torch.float16)
 _I32 = torch.int32
 _I32_MAX = 0x7FFFFFFF
 _ATTN_WS, _SELECT_WS = "amf_paged_decode_workspace_bytes", "amf_select_pages_workspace_bytes"
-_ROWS_WS = "amf_paged_attn_rows_workspace_bytes"
+_ROWS_WS = "amf_paged_attn_rows_call_bytes"
 _WS: dict = {_ATTN_WS: {}, _SELECT_WS: {}, _ROWS_WS: {}}  # entry point -> {sizes: workspace bytes}
 
 # The checks below run on every call of a decode step, where the host's time is

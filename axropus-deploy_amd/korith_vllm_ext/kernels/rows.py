@@ -98,7 +98,7 @@ def paged_attention(q: torch.Tensor, k_cache: Union[torch.Tensor, CompressedKV],
                 and out.data_ptr() < q.data_ptr() + _extent(q) * q.element_size()):
         raise ValueError("paged attention: out must not lie in q")  # q is read until the end
     stream = _raw_stream(idx)
-    ws, wsb = _workspace(_ROWS_WS, (Hq, H, D), workspace, q.device, stream)
+    ws, wsb = _workspace(_ROWS_WS, (N, S, width, bs, Hq, H, D), workspace, q.device, stream)
     ef = _flag(err_flag, idx)
     if given or workspace is not None:
         at, n = out.data_ptr(), out.numel() * out.element_size()

@@ -587,11 +587,16 @@ int amf_int4_kv_read(const void* k_codes, const void* k_params, const void* v_co
  * head, where q, k, v, out and every stride are 16-byte aligned; all other calls a
  * slower kernel.  Rows of one sequence must not be listed under another (their
  * results are either's then).  softmax_scale <= 0 selects 1/sqrt(head_dim).
- * workspace: amf_paged_attn_rows_workspace_bytes() bytes, 16-byte aligned; calls
+ * workspace: amf_paged_attn_rows_call_bytes() bytes, which grow with the rows and the tables,
+ * 16-byte aligned; amf_paged_attn_rows_workspace_bytes() is enough for any of them.  Calls
  * sharing one must be ordered on one stream.  out and workspace lie apart from each other and
  * from what is read.  No counterpart in the reference. */
 int64_t amf_paged_attn_rows_workspace_bytes(int32_t num_q_heads, int32_t num_kv_heads,
                                             int32_t head_dim);
+
+int64_t amf_paged_attn_rows_call_bytes(int64_t n_rows, int32_t num_seqs, int32_t table_pages,
+                                       int32_t block_size, int32_t num_q_heads,
+                                       int32_t num_kv_heads, int32_t head_dim);
 
 int amf_paged_attn_rows(const void* q, int32_t q_dtype, int64_t q_row_stride,
                         int64_t q_head_stride, void* out, int64_t n_rows,

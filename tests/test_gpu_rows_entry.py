@@ -213,3 +213,29 @@ def test_int4_rows_of_512_dims(dtype, n, H):
     full = get_codec("int4_asym_g32").decompress_to(want, dtype)
     for i in range(2):
         assert torch.equal(got[i], full[i].view(-1, H, D)[slots])
+
+
+@pytest.mark.parametrize("D,kind", [(64, F16), (128, BF16), (256, BF16), (128, FP8), (128, "pool")])
+def test_a_workspace_of_the_call_s_size(D, kind):
+    """No byte behind it is written, and what it held before does not matter."""
+    import amf_hip
+    from korith_vllm_ext.kernels import paged_attention
+
+    g = _gen(D)
+    size = amf_hip.load().amf_paged_attn_rows_call_bytes
+    dtype = BF16 if kind in (FP8, "pool") else kind
+    for rows, ctx in (([1], [1]), ([1], [3000]), ([5] * 3, [40, 900, 5000]), ([200, 1], [700, 9]),
+                      ([1] * 40, [100 + 37 * i for i in range(40)]), ([2500], [2500])):
+        table, pool = make_tables(ctx, 16, g)
+        kv = make_cache(pool, 16, 2, D, dtype if kind == "pool" else kind, g)
+        kv = _pool(kv) if kind == "pool" else kv
+        q = torch.randn(sum(rows), 8, D, generator=g).to(dtype).to(DEV)
+        start = [0] + torch.cumsum(torch.tensor(rows), 0).tolist()
+        kw = dict(query_start=_i32(start), block_tables=table.to(DEV), context_lens=_i32(ctx))
+        need = size(sum(rows), len(rows), table.shape[1], 16, 8, 2, D)
+        ws = torch.full((need + (1 << 20),), 0xFF, dtype=torch.uint8, device=DEV)
+        got = paged_attention(q, kv, workspace=ws[:need], **kw)
+        assert torch.equal(got, paged_attention(q, kv, **kw))
+        assert (ws[need:] == 0xFF).all()
+        with pytest.raises(ValueError, match="workspace"):
+            paged_attention(q, kv, workspace=ws[:need - 16], **kw)

@@ -217,3 +217,29 @@ def test_outputs_in_place():
                       (x[:, :1, :32], x.as_strided((6, 1, 32), (32, 32, 1)))):
         with pytest.raises(ValueError, match="overlap"):
             step._output(out, "out", like, ())
+
+
+def test_workspace_of_a_call():
+    """Grows with rows, sequences and tables up to what is enough for any; too little is refused."""
+    lib = amf_hip.load()
+    f, most = lib.amf_paged_attn_rows_call_bytes, lib.amf_paged_attn_rows_workspace_bytes
+    for heads in ((32, 8, 128), (14, 2, 64), (4, 1, 256)):
+        last = 0
+        for rows, seqs, pages in ((1, 1, 1), (1, 1, 64), (8, 8, 64), (8, 8, 8192),
+                                  (4096, 8, 8192), (1 << 20, 1000, 1 << 20)):
+            n = f(rows, seqs, pages, 16, *heads)
+            assert n % 16 == 0 and last <= n <= most(*heads)
+            last = n
+        # (one workgroup a CU at 256 dims, two otherwise)
+        assert last == most(*heads) // (1 + heads[2] // 256)
+        assert f(1, 1, 1, 16, *heads) * 16 <= last
+    assert f(5, 1, 9, 16, 32, 8, 80) == 16 and f(5, 1, 9, 16, 7, 2, 64) == 0
+    for odd in ((-1, 1, 1, 16), (1, -1, 1, 16), (1, 1, -1, 16), (1, 1, 1, 0), (1 << 40, 1, 1, 16),
+                (1, 1, 1 << 30, 1 << 20)):
+        assert f(*odd, 32, 8, 128) == most(32, 8, 128)
+    for name in ATTEND:
+        at = ATTEND[name]
+        need = f(at["rows"], at["seqs"], at["table"], 16, at["hq"], at["hkv"], at["dim"])
+        with pytest.raises(amf_hip.AmfHipError) as e:
+            amf_hip.call(name, *(at | dict(wsb=need - 16)).values())
+        assert e.value.code == amf_hip.ERR_WORKSPACE and str(need) in e.value.message
