@@ -239,3 +239,35 @@ def test_a_workspace_of_the_call_s_size(D, kind):
         assert (ws[need:] == 0xFF).all()
         with pytest.raises(ValueError, match="workspace"):
             paged_attention(q, kv, workspace=ws[:need - 16], **kw)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("pages", [3, 700])
+def test_int4_rows_of_odd_values_are_the_codec_s(dtype, pages):
+    """Zeros of both signs, constants, subnormals, infinities and NaN in a group of 32."""
+    from korith_vllm_ext.kernels import int4_page_pool, write_kv_cache
+
+    g = _gen(pages)
+    H, D, n = 2, 128, pages * 16
+    x = torch.randn(2, n, H, D // 32, 32, generator=g)
+    kinds = torch.randint(0, 8, (2, n, H, D // 32), generator=g)
+    sign = torch.where(torch.rand(x.shape, generator=g) < 0.5, -1.0, 1.0)
+    x = torch.where((kinds == 1)[..., None], 0.0 * sign, x)
+    x = torch.where((kinds == 2)[..., None], torch.full_like(x, 1.25), x)
+    x = torch.where((kinds == 3)[..., None], x * torch.finfo(dtype).tiny, x)
+    x = torch.where((kinds == 4)[..., None], x * 1e4, x)
+    at = torch.randint(0, 32, kinds.shape, generator=g)[..., None] == torch.arange(32)
+    for k, v in ((5, float("inf")), (6, -float("inf")), (7, float("nan"))):
+        x = torch.where((kinds == k)[..., None] & at, v, x)
+    mirror = x.view(2, pages, 16, H, D).to(dtype).to(DEV)
+    want = _pool(mirror).meta["_blob"]
+    pool = int4_page_pool(pages, H, D)
+    write_kv_cache(mirror[0].view(n, H, D), mirror[1].view(n, H, D), pool,
+                   slot_mapping=torch.arange(n, device=DEV))
+    assert torch.equal(pool.meta["_blob"], want)
+    order = torch.randperm(n, generator=g).to(DEV)
+    one = int4_page_pool(pages, H, D)
+    for part in order.split(n // 3 + 1):
+        write_kv_cache(mirror[0].view(n, H, D)[part], mirror[1].view(n, H, D)[part], one,
+                       slot_mapping=part)
+    assert torch.equal(one.meta["_blob"], want)

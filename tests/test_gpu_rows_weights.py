@@ -97,3 +97,30 @@ def test_large_finite_values_and_rising_scores(rows, rise):
             got = _check(q.to(BF16).to(DEV), kv, kv, table, [rows, rows], ctx, 16, TWO[BF16],
                          scale=0.6931471805599453)
             assert torch.isfinite(got).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("rows", [1, 12, 40])
+def test_infinite_values_of_any_weight(dtype, rows):
+    """An infinite value far from the diagonal stays one, not NaN, whether its token has the largest
+    weight, one that a term holds exactly, or 2^-20 of the largest; NaN, and both infinities, give NaN."""
+    g = _gen(8)
+    ctx = [512]
+    for D in (64, 128, 256):
+        table, pool = make_tables(ctx, 16, g)
+        kv = make_cache(pool, 16, 1, D, dtype, g)
+        kv[0] = 0.0
+        place = lambda t: (int(table[0, t // 16]), t % 16, 0)  # noqa: E731
+        for t, score in ((5, 0.0), (70, -1.0), (140, -7.25), (200, -20.0), (300, 6.0)):
+            kv[(0, *place(t), 0)] = score
+        # (dim, token): each alone; then NaN, and infinities of both signs
+        for d, t in ((0, 5), (1, 70), (2, 140), (3, 200), (4, 300)):
+            kv[(1, *place(t), d)] = float("inf") if d % 2 else -float("inf")
+        kv[(1, *place(140), 5)] = float("nan")
+        kv[(1, *place(5), 6)], kv[(1, *place(300), 6)] = float("inf"), -float("inf")
+        q = torch.zeros(rows, 4, D)
+        q[..., 0] = 1.0
+        got = _check(q.to(dtype).to(DEV), kv, kv, table, [rows], ctx, 16, TWO[dtype],
+                     scale=0.6931471805599453)
+        assert torch.isinf(got[..., :5]).all() and torch.isnan(got[..., 5:7]).all()
+        assert torch.isfinite(got[..., 7:]).all()
