@@ -7,7 +7,7 @@
 // Positions reach 10^6 and more, where an angle in fp32 is off by 0.03 and more,
 // so angle, sine and cosine are 64-bit, once per (row, pair) into LDS, and the
 // heads of the row share them.  The products are 64-bit too (three operations a
-// value, hidden behind the loads) and rounded once, to fp32 and from there to the
+// value, hidden behind the loads) and rounded to fp32 and from there to the
 // type: a key that is quantised afterwards then has the bits that an unquantised
 // cache of its type would hold, and the same codes as a page saved from there.
 //

@@ -16,18 +16,19 @@
 // B layout of O^T = V^T P^T as they are.  V^T comes out of LDS by the transposing read.
 // Tiles of 64 columns and fewer (decoded and drafted rows, short ends) are shared: two or
 // four waves take parts of the tokens and of V's dims (with one wave at work 32 x 5 drafted
-// rows over INT4 took 240 us, so 204).
+// rows over INT4 took 240 us, so 204, before the steps below).
 //
 // What bounds it.  With two workgroups of four waves a CU, a SIMD has two waves, and each
 // issues an instruction every five cycles or so: a turn's time goes with its number of
-// instructions of all kinds, more than with its products (1024 of a SIMD's 2200 cycles a turn).
+// instructions of all kinds, and with its products (1536 of a SIMD's 2800 cycles a turn).
 // So the turn is written out: weights, loads and maxima stand between the products, the
 // accumulators are changed by products alone, one wave looks up one page, and what can be
-// known before the turns is.  32 / 8 heads of 128: prompt of 12000 rows 1200 us, 0.98
-// PFLOP/s (a library product reaches 1.2 to 1.3); 64 x 32 rows of 8192 tokens 411 us, 5.2
-// TB/s; one row each 391 us, 5.5 TB/s, bound by the reads; 48 decoded rows beside a chunk of
-// 2048 rows of 8192 tokens 383 us, 0.64 PFLOP/s and 2.3 TB/s; 32 x 5 drafted rows over INT4
-// 150 us, 2.4 TB/s, where taking out the codes is a third of a turn's instructions.
+// known before the turns is.  32 / 8 heads of 128: prompt of 12000 rows 1525 us, 0.77
+// PFLOP/s in what the formula counts, 1.16 in what is multiplied (a library product reaches 1.2
+// to 1.3); 64 x 32 rows of 8192 tokens 457 us, 4.7 TB/s; one row each 392 us, 5.5 TB/s, bound by
+// the reads (FP8 246, 4.4); 48 decoded rows beside a chunk of 2048 rows of 8192 tokens 449 us,
+// 0.54 PFLOP/s and 2.0 TB/s; 32 x 5 drafted rows over INT4 160 us, 2.2 TB/s, where taking out
+// the codes is a third of a turn's instructions; prompt of 4096 rows over FP8 256, INT4 274.
 //
 // Shares.  Tile j of a sequence reads its first e_j tokens; the tiles of all
 // (KV head, sequence, tile) one after the other, each as long as it reads plus a
@@ -36,11 +37,11 @@
 // place from sums over the sequences alone.  A tile inside one share is finished
 // there; one that several share leaves partials (acc, m, l), joined by a second
 // launch.  The constant is what a tile's beginning and end take, 448 tokens' time (8 prompts of
-// 2048: with 256 tokens 430 us, 448 389, 576 400).
+// 2048: with 256 tokens 478 us, 352 464, 448 455, 576 467).
 // The older of a CU's two workgroups goes first wherever both could and ends at 4/5 of the
 // other's time, which then is alone; the younger has a higher priority in every second turn
-// (prompt 1480 -> 1409 us, and no loss where the reads bind; longer shares for the older gave
-// the same here and lost 10 % there).
+// (prompt of 12000 rows 1684 us without, 1543 with, and no loss where the reads bind; longer
+// shares for the older gave the same here and lost 10 % there).
 //
 // Precision.  Products of Q and K are exact and summed in fp32; maximum, sum and
 // accumulators are fp32.  A weight enters the second product as two terms of the type
@@ -48,8 +49,8 @@
 // one (21 bits; fp16 holds FP8 values exactly).  The result is then off by 2^-16 of the weighted |v|,
 // where rounding it to bf16 takes 2^-8 (2^-21 and 2^-11 for fp16).  With one term it was
 // off by as much again as that rounding, in values that cancel by more (prompt of 12000 rows
-// 1209 us, so 1632; 64 single rows of 8192 tokens 392, so 402); a third bf16 term would cost
-// another 16 products to the turn's 48, for bits that the result's type drops.
+// 1209 us with one, 1525 with two; 64 single rows of 8192 tokens 392, so 402); a third bf16 term
+// would cost another 16 products to the turn's 48, for bits that the result's type drops.
 #include <algorithm>
 #include <type_traits>
 
@@ -73,7 +74,8 @@ constexpr int kRows = 32 * kWaves;  // columns of a workgroup
 constexpr int kMaxDim = 256;
 constexpr int kMaxShares = 512;     // two workgroups a CU
 // Lengths of tiles and shares.  A token of a tile of more than 64 columns counts kWide, of a
-// narrower one kNarrow (48 decoded rows beside a chunk: 3/4 407 us, 5/6 384).
+// narrower one kNarrow (48 decoded rows beside a chunk: 4/6 471 us, 5/6 452, 6/6 477).  Shares
+// are of 256 tokens at least (a prompt of 512 rows: 128 tokens 50 us, 256 47, 2048 68).
 constexpr int kWide = 6, kNarrow = 5;
 constexpr int kMinShare = 256 * kWide;
 constexpr int kTileCost = 448 * kWide;  // a tile's beginning and end; at least BT tokens
@@ -202,7 +204,7 @@ __device__ __forceinline__ f32x16 mfma32(const u32x4& x, const u32x4& y, const f
 // the exact maximum, and weights down to 2^-118 of the largest keep their bits.  Weights in
 // fp16 are held 2^7 times as large, at most 2^15 (values of at most 2^16 cannot exceed fp32):
 // those down to 2^-21 of the largest keep the 11 bits of their first term.  (2^30 for bf16, in
-// the maximum's own size, was no faster: prompt of 12000 rows 1542 us, so 1503.)
+// the maximum's own size, was no faster: prompt of 12000 rows 1542 us, with 2^8 1503.)
 constexpr float kSlack = 8.0f;
 template <int T>
 constexpr float weight_shift() {
@@ -715,8 +717,10 @@ __global__ __launch_bounds__(kThreads) void rows_merge_kernel(RowsArgs a) {
 
 // A wave per (row, query head): 64 tokens at a time, one a lane for the scores, then
 // the dims on the lanes for the values.  For fp32, head dims other than 64, 128 and
-// 256, rows that are not 16-byte aligned and groups of more than kRows heads; every
-// K and V element is read again for each row and head.
+// 256, caches or outputs that are not 16-byte aligned and groups of more than kRows heads;
+// every K and V element is read again for each row and head, and a wave's tokens follow each
+// other: 32 / 8 heads of 96, prompt of 2048 rows 3.9 ms (INT4 7.8; of 128 on the tiles 0.09), 16
+// single rows of 2048 tokens 1.2 ms (0.05); fp32 heads of 128 7.4 and 1.4.
 template <int KV, int QT>
 __global__ __launch_bounds__(kThreads) void rows_general_kernel(RowsArgs a) {
   __shared__ float q_lds[kWaves][kMaxDim];

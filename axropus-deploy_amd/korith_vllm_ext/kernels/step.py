@@ -314,7 +314,7 @@ def rotary_embedding(q: torch.Tensor, k: Optional[torch.Tensor], positions: torc
                      ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """(q, k) with the first 2 * pairs dims of each head rotated by its row's
     position: (a, b) -> factor * (a cos - b sin, b cos + a sin), computed in 64
-    bits and rounded once.
+    bits, rounded to fp32 and then to the type.
 
     q [rows, Hq, D], k [rows, Hkv, D] or None, of one type (bf16, fp16, fp32),
     rows and heads strided as they come (a copy where dims are not contiguous);
