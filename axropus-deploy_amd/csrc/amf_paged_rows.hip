@@ -46,9 +46,10 @@
 // Precision.  Products of Q and K are exact and summed in fp32; maximum, sum and
 // accumulators are fp32.  A weight enters the second product as two terms of the type
 // beside it: bf16 beside a bf16 V (16 bits of the weight), fp16 beside an fp16 or an FP8
-// one (21 bits; fp16 holds FP8 values exactly).  The result is then off by 2^-16 of the weighted |v|,
-// where rounding it to bf16 takes 2^-8 (2^-21 and 2^-11 for fp16).  With one term it was
-// off by as much again as that rounding, in values that cancel by more (prompt of 12000 rows
+// one (21 bits; fp16 holds FP8 values exactly).  The result is then off by 2^-16 of the
+// weighted |v|, where rounding it to bf16 takes 2^-8 of itself (2^-21 and 2^-11 for fp16).
+// With one term it was off by as much again as that rounding, and by more in values that cancel:
+// those rounded weights are what a result near 0 consists of (prompt of 12000 rows
 // 1209 us with one, 1525 with two; 64 single rows of 8192 tokens 392, so 402); a third bf16 term
 // would cost another 16 products to the turn's 48, for bits that the result's type drops.
 #include <algorithm>

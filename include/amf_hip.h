@@ -579,9 +579,9 @@ int amf_int4_kv_read(const void* k_codes, const void* k_params, const void* v_co
  * Rows that belong to no sequence are left as they are.  q's rows, heads, the
  * cache's strides, block tables, page ids and the end of a table as in
  * amf_paged_decode_attn; a row without tokens gives zeros, scores that are all
- * -inf, or hold a NaN or +inf, give NaN.  An infinite V gives an infinity, or NaN where its
- * weight is below 2^-30 of the row's largest (fp16; bf16 2^-118).  A sequence whose rows lie outside
- * [0, n_rows) or end before they begin has none (AMF_ERRFLAG_CONTEXT).
+ * -inf, or hold a NaN or +inf, give NaN.  An infinite V gives an infinity, or NaN where
+ * its weight is below 2^-30 of the row's largest (fp16; bf16 2^-118).  A sequence whose rows
+ * lie outside [0, n_rows) or end before they begin has none (AMF_ERRFLAG_CONTEXT).
  * kv_dtype: q_dtype, or AMF_DTYPE_E4M3 with q bf16 or fp16.  head_dim at most 256;
  * n_rows * num_q_heads at most 2^26, table_pages * block_size at most 2^30.  Matrix
  * tiles take 16-bit q with head_dim 64, 128 or 256 and at most 128 query heads a KV
